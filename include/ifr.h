@@ -353,6 +353,112 @@ int ifr_pad_scores_min_f64(ifr_handle h, double *scores, int64_t n, int64_t ld, 
  * scores: dev [n][ld] whose first n_items columns were written by ifr_score_dense. */
 int ifr_pad_scores_min(ifr_handle h, float *scores, int64_t n, int64_t ld, void *stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * A catalogue in 4 bits, probabilities over the catalogue, and the losses that are taken of them.  (No counterpart in the
+ * reference, which trains BPR's pairwise criterion and WMF's / MF's squared error on the CPU: cornac/models/bpr/
+ * recom_bpr.pyx:208-269.)  These entry points take every operand as a device pointer: no model need be set, the handle
+ * supplies the GPU and the error text.  They are asynchronous on `stream`, allocate nothing and keep nothing: what they
+ * need beside the operands is a workspace of the caller, whose size a ..._workspace call gives (calls that overlap need one
+ * each; its contents mean nothing between calls).  All of them may be captured into a HIP graph.  The device that is
+ * current in the calling thread is the same after the call.  n = 0 is a call that does nothing. */
+
+enum { IFR_F32 = 0, IFR_BF16 = 1, IFR_MXFP4 = 2 };
+
+/* A matrix in 4-bit microscaled floating point: blocks of 32 columns, kb = ceil(k / 32) a row.  codes [n][16 * kb] bytes, 16-byte
+ * aligned: element 2j of a row in the low half of byte j, as E2M1 (0 .5 1 1.5 2 3 4 6 and their negatives); scales [n][kb]:
+ * 127 + the exponent of the block's power of two.  The exponent is floor(log2 max|v|) - 2, at least -127; elements are
+ * v / 2^exponent rounded to the nearest value, ties to the even code, at most 6 in magnitude.  A block that holds a NaN or an
+ * infinity gets scale 255 and stands for NaN.  Columns behind k are zeros.
+ * X: dev [n][ld] of `dtype` (IFR_F32 or IFR_BF16), 1 <= k <= ld. */
+int ifr_mxfp4_quantize(ifr_handle h, const void *X, int dtype, int64_t n, int64_t k, int64_t ld, uint8_t *codes, uint8_t *scales,
+                       void *stream);
+/* The values that codes and scales stand for, exactly: out dev [n][ld] fp32, ld >= k. */
+int ifr_mxfp4_dequantize(ifr_handle h, const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, float *out, int64_t ld,
+                         void *stream);
+/* Score rows of a 4-bit model, beside ifr_score_dense: out[u][i] = (ibase[i] + ubase[u]) + <X[u], V[i]>, sums in fp32, rounded
+ * once to `out_dtype` (IFR_F32 or IFR_BF16).  out: dev [n][ld], ld >= n_items; ibase [n_items], ubase [n]: dev or NULL.
+ * 1 <= k <= IFR_MAX_FACTORS, n and n_items below 2^30. */
+int ifr_mxfp4_scores(ifr_handle h, const uint8_t *x_codes, const uint8_t *x_scales, int64_t n, const uint8_t *v_codes,
+                     const uint8_t *v_scales, int64_t n_items, int k, const float *ubase, const float *ibase, void *out,
+                     int out_dtype, int64_t ld, void *stream);
+
+/* Users (rows of X) and a catalogue (rows of V): z[u][i] = scale * (<X[u], V[i]> + ibase[i]). */
+typedef struct ifr_catalogue {
+    const void *X, *V;           /* dev [n][ldx], [n_items][ldv] of `dtype`; IFR_MXFP4: the codes (ldx, ldv unused)         */
+    const uint8_t *x_scales, *v_scales;   /* IFR_MXFP4: the scales, else NULL                                               */
+    const float *ibase;          /* dev [n_items] or NULL; -inf takes an item out of the catalogue                          */
+    int64_t n, n_items, ldx, ldv;
+    int k, dtype;                /* 1 <= k <= IFR_MAX_FACTORS; n, n_items < 2^30                                            */
+    double scale;                /* > 0: an inverse temperature                                                             */
+} ifr_catalogue;
+
+/* Log-probabilities of items under the softmax over the whole catalogue; the n x n_items scores are never stored.
+ * ids: dev [n][ld_ids], m >= 0 items a user (a slate; an item may stand in it twice).  A negative id is an empty place: its
+ * logp is 0 and nothing flows through it.  An id >= n_items gives NaN.
+ *   lse[u] = log sum_i exp z[u][i] (dev [n] or NULL), logp[u][j] = z[u][ids[u][j]] - lse[u] (dev [n][ld_logp], or NULL where m = 0).
+ * Products of fp32 operands keep 22 bits of each operand (more than the sum of k products in fp32 does); sums are fp32. */
+int ifr_catalogue_logprob_workspace(ifr_handle h, const ifr_catalogue *c, int64_t *bytes);
+int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids, float *logp,
+                          int64_t ld_logp, float *lse, void *ws, int64_t ws_bytes, void *stream);
+/* Its gradient.  dlogp: dev [n][ld_dlogp]; lse as ifr_catalogue_logprob returned it.  With G[u] = the sum of dlogp[u][j] over the
+ * places that hold an item and dz[u][i] = sum_j dlogp[u][j] [ids[u][j] = i] - G[u] exp(z[u][i] - lse[u]):
+ *   dX = scale dz V, dV = scale dz^T X (both of `dtype`, rows ld_dx / ld_dv apart), dibase = scale sum_u dz (fp32).
+ * Any of the three may be NULL.  fp32 or bf16 operands.  No atomics: the same call gives the same bits.  A user whose lse is
+ * -inf (every item taken out) has no probabilities, and only its targets' part of the gradient. */
+int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int want_dx, int want_dv, int want_dibase, int64_t *bytes);
+int ifr_catalogue_logprob_backward(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids,
+                                   const float *lse, const float *dlogp, int64_t ld_dlogp, void *dX, int64_t ld_dx, void *dV,
+                                   int64_t ld_dv, float *dibase, void *ws, int64_t ws_bytes, void *stream);
+
+enum { IFR_PREFERENCE_LOGISTIC = 0, IFR_PREFERENCE_HINGE = 1, IFR_PREFERENCE_SQUARED = 2 };
+
+/* A batch of n pairs (a chosen and a rejected slate) and its loss with its gradient.  Per pair, with C the sum of the chosen
+ * slate's log-probabilities over its mask, R the rejected slate's (`average`: their means; an empty slate has 0), and Cr, Rr
+ * those of a frozen reference model (0 without one):
+ *   h = beta ((C - R) - (Cr - Rr)) - margin
+ *   logistic: (1 - e) log(1 + exp(-h)) + e log(1 + exp(h)), e = label_smoothing;  hinge: max(0, 1 - h);  squared: ((h - 1/2) / beta)^2
+ *   d_chosen = weight dloss/dh beta on the mask (divided by the number of places where `average`), 0 elsewhere; d_rejected = minus that.
+ * What stands in masked places is not looked at.  Sums are fp64.  Slates of one item under the logistic kind, without a
+ * reference and with beta = 1, are BPR's criterion (cornac/models/bpr/recom_bpr.pyx:208-269). */
+typedef struct ifr_preference {
+    int64_t n;
+    int32_t len_chosen, len_rejected;            /* places a row, >= 0                                                 */
+    int32_t kind, average;
+    const float *chosen, *rejected;              /* dev [n][ld]                                                        */
+    const float *ref_chosen, *ref_rejected;      /* dev [n][ld], both or none                                          */
+    const uint8_t *mask_chosen, *mask_rejected;  /* dev [n][ld] 0 / 1, or NULL: every place counts                     */
+    const float *weight;                         /* dev [n]: dL/dloss, or NULL: 1                                      */
+    float *loss, *h, *d_chosen, *d_rejected;     /* dev [n], [n], [n][ld], [n][ld]; any may be NULL                    */
+    int64_t ld_chosen, ld_rejected, ld_ref_chosen, ld_ref_rejected, ld_mask_chosen, ld_mask_rejected, ld_d_chosen, ld_d_rejected;
+    double beta, margin, label_smoothing;        /* beta > 0, 0 <= label_smoothing < 1/2 (logistic only)               */
+} ifr_preference;
+int ifr_preference_loss(ifr_handle h, const ifr_preference *p, void *stream);
+
+enum { IFR_POLICY_SUM = 0, IFR_POLICY_ROW = 1, IFR_POLICY_BATCH = 2 };
+
+/* The clipped policy loss of n rows of `len` choices with its gradient.  Per place of the mask, with d = logp - old_logp in fp32,
+ * r = exp d and A the row's advantage:
+ *   clipped = (A > 0 and d > log(1 + clip_high)) or (A < 0 and d < log(1 - clip_low))     (borders rounded to fp32)
+ *   q = ref_logp - logp, kl = exp(q) - q - 1                                              (0 without a reference)
+ *   term = -A (clipped ? the border's ratio : r) + kl_coef kl
+ *   d_logp = c ((clipped ? 0 : -A r) - kl_coef (exp(q) - 1)), 0 outside the mask
+ * loss[row] = c sum of the terms, c = weight (1 if NULL) times 1 (SUM), 1 / the row's places (ROW) or 1 / the batch's places (BATCH);
+ * kl[row] = the mean of kl over the row's places; clipped[row] = the number of clipped places.  Rows without a place give 0. */
+typedef struct ifr_policy {
+    int64_t n;
+    int32_t len, reduction;
+    const float *logp, *old_logp, *ref_logp;     /* dev [n][ld]; ref_logp may be NULL                                  */
+    const float *advantages, *weight;            /* dev [n]; weight may be NULL                                        */
+    const uint8_t *mask;                         /* dev [n][ld] 0 / 1, or NULL                                         */
+    float *loss, *kl;                            /* dev [n]; any output may be NULL                                    */
+    int32_t *clipped;                            /* dev [n]                                                            */
+    float *d_logp;                               /* dev [n][ld]                                                        */
+    int64_t ld_logp, ld_old, ld_ref, ld_mask, ld_d_logp;
+    double clip_low, clip_high, kl_coef;         /* 0 <= clip_low < 1, clip_high >= 0                                  */
+} ifr_policy;
+int ifr_policy_loss_workspace(ifr_handle h, const ifr_policy *p, int64_t *bytes);
+int ifr_policy_loss(ifr_handle h, const ifr_policy *p, void *ws, int64_t ws_bytes, void *stream);
+
 /* Kernel timing with HIP events on the launch stream (used by bench.py for the roofline
  * figure; no reference counterpart).  After ifr_profile_enable(h, 1) every ifr_rank_topk
  * records events around its fused score+select kernel; ifr_profile_read synchronises those

@@ -22,6 +22,31 @@ class CsrSplit(ctypes.Structure):
     _fields_ = [("indptr", vp), ("indices", vp), ("ratings", vp), ("n_rows", ctypes.c_int64)]
 
 
+class Catalogue(ctypes.Structure):
+    """ifr_catalogue (include/ifr.h)."""
+    _fields_ = [("X", vp), ("V", vp), ("x_scales", vp), ("v_scales", vp), ("ibase", vp),
+                ("n", ctypes.c_int64), ("n_items", ctypes.c_int64), ("ldx", ctypes.c_int64), ("ldv", ctypes.c_int64),
+                ("k", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_double)]
+
+
+class Preference(ctypes.Structure):
+    """ifr_preference (include/ifr.h)."""
+    _fields_ = [("n", ctypes.c_int64)] + [(f, ctypes.c_int32) for f in ("len_chosen", "len_rejected", "kind", "average")] + \
+        [(f, vp) for f in ("chosen", "rejected", "ref_chosen", "ref_rejected", "mask_chosen", "mask_rejected", "weight", "loss", "h", "d_chosen",
+                           "d_rejected")] + \
+        [("ld_" + f, ctypes.c_int64) for f in ("chosen", "rejected", "ref_chosen", "ref_rejected", "mask_chosen", "mask_rejected", "d_chosen",
+                                               "d_rejected")] + \
+        [(f, ctypes.c_double) for f in ("beta", "margin", "label_smoothing")]
+
+
+class Policy(ctypes.Structure):
+    """ifr_policy (include/ifr.h)."""
+    _fields_ = [("n", ctypes.c_int64), ("len", ctypes.c_int32), ("reduction", ctypes.c_int32)] + \
+        [(f, vp) for f in ("logp", "old_logp", "ref_logp", "advantages", "weight", "mask", "loss", "kl", "clipped", "d_logp")] + \
+        [("ld_" + f, ctypes.c_int64) for f in ("logp", "old", "ref", "mask", "d_logp")] + \
+        [(f, ctypes.c_double) for f in ("clip_low", "clip_high", "kl_coef")]
+
+
 # name -> (restype, argtypes); one row per declaration in include/ifr.h
 SIGNATURES = {
     "ifr_version": (ctypes.c_char_p, []),
@@ -68,6 +93,18 @@ SIGNATURES = {
     "ifr_auc_dense": (ctypes.c_int, [vp, vp, ctypes.c_int64, vp, ctypes.c_int64, vp, vp]),
     "ifr_rank_full": (ctypes.c_int, [vp, vp, ctypes.c_int64, vp, ctypes.c_int64, vp, vp, vp]),
     "ifr_pad_scores_min": (ctypes.c_int, [vp, vp, ctypes.c_int64, ctypes.c_int64, vp]),
+    "ifr_mxfp4_quantize": (ctypes.c_int, [vp, vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, vp, vp, vp]),
+    "ifr_mxfp4_dequantize": (ctypes.c_int, [vp, vp, vp, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_int64, vp]),
+    "ifr_mxfp4_scores": (ctypes.c_int, [vp, vp, vp, ctypes.c_int64, vp, vp, ctypes.c_int64, ctypes.c_int, vp, vp, vp, ctypes.c_int, ctypes.c_int64, vp]),
+    "ifr_catalogue_logprob_workspace": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), c_i64p]),
+    "ifr_catalogue_logprob": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), vp, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_int64, vp, vp,
+                                             ctypes.c_int64, vp]),
+    "ifr_catalogue_logprob_backward_workspace": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), ctypes.c_int, ctypes.c_int, ctypes.c_int, c_i64p]),
+    "ifr_catalogue_logprob_backward": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), vp, ctypes.c_int64, ctypes.c_int64, vp, vp, ctypes.c_int64, vp,
+                                                      ctypes.c_int64, vp, ctypes.c_int64, vp, vp, ctypes.c_int64, vp]),
+    "ifr_preference_loss": (ctypes.c_int, [vp, ctypes.POINTER(Preference), vp]),
+    "ifr_policy_loss_workspace": (ctypes.c_int, [vp, ctypes.POINTER(Policy), c_i64p]),
+    "ifr_policy_loss": (ctypes.c_int, [vp, ctypes.POINTER(Policy), vp, ctypes.c_int64, vp]),
     "ifr_profile_enable": (ctypes.c_int, [vp, ctypes.c_int]),
     "ifr_profile_read": (ctypes.c_int, [vp, c_f64p, c_i64p, c_f64p]),
     "ifr_wide_overflows": (ctypes.c_int, [vp, c_i64p]),

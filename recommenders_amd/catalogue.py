@@ -1,0 +1,348 @@
+"""Catalogue operators of `HipScorer`: a 4-bit microscaled model and its score rows, log-probabilities of items under the
+softmax over the whole catalogue with their gradient, and the preference and policy losses (contracts: include/ifr.h).
+
+Operands are torch tensors on the scorer's GPU; a tensor whose last dimension is not contiguous is copied, any row stride is
+taken as it is.  Every call runs on the GPU's current stream, allocates its outputs and its workspace there with torch's
+allocator (so it can be captured into a graph) and does not synchronise.  Gradients are results of their own, not of autograd:
+tensors that require one are refused while autograd records."""
+import ctypes
+from collections import namedtuple
+
+from . import _lib
+
+F32, BF16, MXFP4 = 0, 1, 2
+MAX_FACTORS = 256            # IFR_MAX_FACTORS
+MAX_ROWS, MAX_CATALOGUE = 1 << 25, 1 << 28
+
+PreferenceLoss = namedtuple("PreferenceLoss", "loss h d_chosen d_rejected")
+PolicyLoss = namedtuple("PolicyLoss", "loss kl clipped d_logp")
+
+
+class MxFp4Matrix:
+    """A matrix [n, k] in 4-bit microscaled floating point (OCP MX: E2M1 elements, a power of two per 32 columns): `codes` uint8
+    [n, 16 * ceil(k / 32)], element 2j of a row in the low half of byte j, and `scales` uint8 [n, ceil(k / 32)], exponent + 127
+    (255: the block stands for NaN).  17/32 byte an element."""
+
+    __slots__ = ("codes", "scales", "k")
+
+    def __init__(self, codes, scales, k):
+        import torch
+        k = int(k)
+        kb = (k + 31) // 32
+        if k < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
+            raise ValueError("MxFp4Matrix: codes and scales must be uint8 matrices, k at least 1")
+        if codes.shape[1] != 16 * kb or tuple(scales.shape) != (codes.shape[0], kb):
+            raise ValueError(f"MxFp4Matrix: k = {k} takes codes [n, {16 * kb}] and scales [n, {kb}]")
+        if codes.device != scales.device:
+            raise ValueError("MxFp4Matrix: codes and scales must be on one device")
+        self.codes, self.scales, self.k = codes.contiguous(), scales.contiguous(), k
+        if self.codes.data_ptr() % 16:
+            self.codes = self.codes.clone()
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.k)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _matrix(t, name, dtypes, cols=None, rows=None, device=None):
+    """`t` as a matrix with contiguous rows at least its width apart; ValueError / TypeError where it is not what `name` is."""
+    import torch
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be a matrix, not {t.dim()}-dimensional")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, not {str(t.dtype).replace('torch.', '')}")
+    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {'any' if cols is None else cols}], not {list(t.shape)}")
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise ValueError(f"{name} requires a gradient: autograd does not see this call, pass {name}.detach() and use the gradients it returns")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the scorer on {device}")
+    if t.numel() and (t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _vector(t, name, n, device=None, dtype=None):
+    """None, or `t` as a contiguous vector of n fp32 values."""
+    import torch
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if t.dtype != (dtype or torch.float32):
+        raise TypeError(f"{name} must be {str(dtype or torch.float32).replace('torch.', '')}")
+    if tuple(t.shape) != (n,):
+        raise ValueError(f"{name} must be [{n}], not {list(t.shape)}")
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise ValueError(f"{name} requires a gradient: pass {name}.detach()")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the scorer on {device}")
+    return t.contiguous()
+
+
+def _row_stride(t):
+    """Elements from one row to the next; a single row reaches as far as it is wide."""
+    return 0 if t is None else max(t.stride(0) if t.shape[0] > 1 else 0, t.shape[1])
+
+
+def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
+    """What the log-probability calls take: (X, V, ids, ibase) ready for the library, or the refusal."""
+    import torch
+    if isinstance(X, MxFp4Matrix) != isinstance(V, MxFp4Matrix):
+        raise TypeError("X and V must both be tensors or both be MxFp4Matrix")
+    if isinstance(X, MxFp4Matrix):
+        if X.k != V.k:
+            raise ValueError(f"X has {X.k} factors, V {V.k}")
+        for name, q in (("X", X), ("V", V)):
+            if device is not None and q.device != device:
+                raise ValueError(f"{name} is on {q.device}, the scorer on {device}")
+    else:
+        X = _matrix(X, "X", (torch.float32, torch.bfloat16), device=device)
+        V = _matrix(V, "V", (X.dtype,), cols=X.shape[1], device=device)
+    n, k = X.shape
+    n_items = V.shape[0]
+    if not 1 <= k <= MAX_FACTORS:
+        raise ValueError(f"k must be in [1, {MAX_FACTORS}], not {k}")
+    if n > MAX_ROWS or not 1 <= n_items <= MAX_CATALOGUE:
+        raise ValueError(f"at most {MAX_ROWS} rows of X and 1 ... {MAX_CATALOGUE} rows of V")
+    scale = float(scale)
+    if not 0.0 < scale <= 1e30:
+        raise ValueError("scale must be positive")
+    ids = _matrix(ids, "ids", (torch.int32,), rows=n, device=device)
+    return X, V, ids, _vector(ibase, "ibase", n_items, device)
+
+
+def check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, weight, beta, kind, label_smoothing, margin, device=None):
+    """What `preference_loss` takes, ready for the library, or the refusal."""
+    import torch
+    f32, masks = (torch.float32,), (torch.bool, torch.uint8)
+    chosen = _matrix(chosen, "chosen", f32, device=device)
+    n = chosen.shape[0]
+    rejected = _matrix(rejected, "rejected", f32, rows=n, device=device)
+    if (ref_chosen is None) != (ref_rejected is None):
+        raise ValueError("a reference needs both ref_chosen and ref_rejected")
+    if ref_chosen is not None:
+        ref_chosen = _matrix(ref_chosen, "ref_chosen", f32, rows=n, cols=chosen.shape[1], device=device)
+        ref_rejected = _matrix(ref_rejected, "ref_rejected", f32, rows=n, cols=rejected.shape[1], device=device)
+    if mask_chosen is not None:
+        mask_chosen = _matrix(mask_chosen, "mask_chosen", masks, rows=n, cols=chosen.shape[1], device=device)
+    if mask_rejected is not None:
+        mask_rejected = _matrix(mask_rejected, "mask_rejected", masks, rows=n, cols=rejected.shape[1], device=device)
+    if kind not in ("logistic", "hinge", "squared"):
+        raise ValueError("kind must be 'logistic', 'hinge' or 'squared'")
+    if not 0.0 < float(beta) <= 1e30:
+        raise ValueError("beta must be positive")
+    if not 0.0 <= float(label_smoothing) < 0.5:
+        raise ValueError("label_smoothing must be in [0, 1/2)")
+    if label_smoothing and kind != "logistic":
+        raise ValueError("label_smoothing needs kind='logistic'")
+    if not abs(float(margin)) < 1e30:
+        raise ValueError("margin must be finite")
+    return chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, _vector(weight, "weight", n, device)
+
+
+def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef, reduction, device=None):
+    """What `policy_loss` takes, ready for the library, or the refusal."""
+    import torch
+    f32 = (torch.float32,)
+    logp = _matrix(logp, "logp", f32, device=device)
+    n, width = logp.shape
+    old_logp = _matrix(old_logp, "old_logp", f32, rows=n, cols=width, device=device)
+    if ref_logp is not None:
+        ref_logp = _matrix(ref_logp, "ref_logp", f32, rows=n, cols=width, device=device)
+    if mask is not None:
+        mask = _matrix(mask, "mask", (torch.bool, torch.uint8), rows=n, cols=width, device=device)
+    if advantages is None:
+        raise TypeError("advantages must be a torch tensor")
+    if reduction not in ("sum", "row", "batch"):
+        raise ValueError("reduction must be 'sum', 'row' or 'batch'")
+    if not 0.0 <= float(clip_low) < 1.0 or not 0.0 <= float(clip_high) < 1e30:
+        raise ValueError("clip_low must be in [0, 1) and clip_high at least 0")
+    if not abs(float(kl_coef)) < 1e30:
+        raise ValueError("kl_coef must be finite")
+    if kl_coef and ref_logp is None:
+        raise ValueError("kl_coef needs ref_logp")
+    return logp, old_logp, _vector(advantages, "advantages", n, device), ref_logp, mask, _vector(weight, "weight", n, device)
+
+
+class CatalogueOps:
+    """The catalogue operators of `HipScorer` (engine.py), which supplies `_lib`, `_h`, `device`, `_check` and `_stream`."""
+
+    def _workspace(self, fn, *args):
+        import torch
+        need = ctypes.c_int64(0)
+        self._check(fn(self._h, *args, ctypes.byref(need)))
+        return torch.empty(max(1, need.value), dtype=torch.uint8, device=self.device), need.value
+
+    # ------------------------------------------------------------------ 4-bit model
+    def quantize_mxfp4(self, X):
+        """`X` [n, k] (fp32 or bf16) as an MxFp4Matrix: per block of 32 columns the exponent floor(log2 max|v|) - 2 (at least -127)
+        and elements rounded to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 times it, ties to the even code, at most 6."""
+        import torch
+        X = _matrix(X, "X", (torch.float32, torch.bfloat16), device=self.device)
+        n, k = X.shape
+        if k < 1:
+            raise ValueError("X must have at least one column")
+        kb = (k + 31) // 32
+        codes = torch.empty((n, 16 * kb), dtype=torch.uint8, device=self.device)
+        scales = torch.empty((n, kb), dtype=torch.uint8, device=self.device)
+        self._check(self._lib.ifr_mxfp4_quantize(self._h, _ptr(X), F32 if X.dtype == torch.float32 else BF16, n, k, _row_stride(X),
+                                                 _ptr(codes), _ptr(scales), self._stream()))
+        return MxFp4Matrix(codes, scales, k)
+
+    def dequantize_mxfp4(self, q, out=None):
+        """The fp32 values [n, k] that an MxFp4Matrix stands for."""
+        import torch
+        if not isinstance(q, MxFp4Matrix) or q.device != self.device:
+            raise ValueError(f"dequantize_mxfp4 takes an MxFp4Matrix on {self.device}")
+        out = self._out(out, q.shape, torch.float32)
+        self._check(self._lib.ifr_mxfp4_dequantize(self._h, _ptr(q.codes), _ptr(q.scales), q.shape[0], q.k, _ptr(out), _row_stride(out),
+                                                   self._stream()))
+        return out
+
+    def _out(self, out, shape, dtype):
+        import torch
+        if out is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != self.device or (out.numel() and (
+                out.stride(1) != 1 and out.shape[1] > 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1])):
+            raise ValueError(f"out must be {str(dtype).replace('torch.', '')} {list(shape)} on {self.device} with contiguous rows")
+        return out
+
+    def score_mxfp4(self, X, V, ubase=None, ibase=None, out=None, dtype=None):
+        """Score rows [n, n_items] of a 4-bit model, beside `score_dense`: (ibase + ubase) + <X[u], V[i]>, fp32 sums rounded once to
+        `dtype` (float32, the default, or bfloat16)."""
+        import torch
+        if not isinstance(X, MxFp4Matrix) or not isinstance(V, MxFp4Matrix):
+            raise TypeError("score_mxfp4 takes two MxFp4Matrix (quantize_mxfp4)")
+        if X.k != V.k:
+            raise ValueError(f"X has {X.k} factors, V {V.k}")
+        if X.k > MAX_FACTORS or X.shape[0] > MAX_ROWS or not 1 <= V.shape[0] <= MAX_CATALOGUE:
+            raise ValueError(f"score_mxfp4: at most {MAX_FACTORS} factors, {MAX_ROWS} rows of X, 1 ... {MAX_CATALOGUE} rows of V")
+        if X.device != self.device or V.device != self.device:
+            raise ValueError(f"X and V must be on {self.device}")
+        dtype = torch.float32 if dtype is None and out is None else out.dtype if dtype is None else dtype
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("score_mxfp4 writes float32 or bfloat16")
+        n, n_items = X.shape[0], V.shape[0]
+        ubase, ibase = _vector(ubase, "ubase", n, self.device), _vector(ibase, "ibase", n_items, self.device)
+        out = self._out(out, (n, n_items), dtype)
+        self._check(self._lib.ifr_mxfp4_scores(self._h, _ptr(X.codes), _ptr(X.scales), n, _ptr(V.codes), _ptr(V.scales), n_items, X.k, _ptr(ubase),
+                                               _ptr(ibase), _ptr(out), F32 if dtype == torch.float32 else BF16, _row_stride(out), self._stream()))
+        return out
+
+    # ------------------------------------------------------------------ log-probabilities
+    def _catalogue(self, X, V, ibase, scale):
+        import torch
+        c = _lib.Catalogue()
+        mx = isinstance(X, MxFp4Matrix)
+        c.X, c.V = (_ptr(X.codes), _ptr(V.codes)) if mx else (_ptr(X), _ptr(V))
+        c.x_scales, c.v_scales = (_ptr(X.scales), _ptr(V.scales)) if mx else (None, None)
+        c.ibase = _ptr(ibase)
+        c.n, c.k = X.shape
+        c.n_items = V.shape[0]
+        c.ldx, c.ldv = (0, 0) if mx else (_row_stride(X), _row_stride(V))
+        c.dtype = MXFP4 if mx else F32 if X.dtype == torch.float32 else BF16
+        c.scale = float(scale)
+        return c
+
+    def catalogue_logprob(self, X, V, ids, ibase=None, scale=1.0):
+        """(logp [n, m], lse [n]), fp32: logp[u, j] = z[u, ids[u, j]] - lse[u] with z[u, i] = scale * (<X[u], V[i]> + ibase[i]) and
+        lse[u] = log sum_i exp z[u, i] over the whole catalogue.  X [n, k] and V [n_items, k]: both fp32, both bf16, or both
+        MxFp4Matrix (a frozen model); ids int32 [n, m], negative = an empty place (logp 0; an id past the catalogue gives NaN);
+        an ibase of -inf takes an item out.  The n x n_items scores are not stored."""
+        import torch
+        X, V, ids, ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
+        n, m = ids.shape
+        c = self._catalogue(X, V, ibase, scale)
+        logp = torch.empty((n, m), dtype=torch.float32, device=self.device)
+        lse = torch.empty((n,), dtype=torch.float32, device=self.device)
+        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_workspace, ctypes.byref(c))
+        self._check(self._lib.ifr_catalogue_logprob(self._h, ctypes.byref(c), _ptr(ids), m, _row_stride(ids), _ptr(logp), max(m, 1), _ptr(lse),
+                                                    _ptr(ws), need, self._stream()))
+        return logp, lse
+
+    def catalogue_logprob_backward(self, X, V, ids, lse, dlogp, ibase=None, scale=1.0, want=("X", "V", "ibase")):
+        """(dX, dV, dibase) for the upstream gradient dlogp [n, m] of `catalogue_logprob`'s logp, with its lse: dX and dV in the
+        operands' type, dibase fp32 (None where there is no ibase, or where `want` leaves one out).  The same call gives the
+        same bits."""
+        import torch
+        if isinstance(X, MxFp4Matrix) or isinstance(V, MxFp4Matrix):
+            raise TypeError("a 4-bit model has no gradient")
+        if set(want) - {"X", "V", "ibase"}:
+            raise ValueError("want holds 'X', 'V' and 'ibase'")
+        X, V, ids, ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
+        n, m = ids.shape
+        dlogp = _matrix(dlogp, "dlogp", (torch.float32,), rows=n, cols=m, device=self.device)
+        if lse is None:
+            raise TypeError("lse must be a torch tensor")
+        lse = _vector(lse, "lse", n, self.device)
+        empty = torch.empty if n else torch.zeros
+        dX = empty((n, X.shape[1]), dtype=X.dtype, device=self.device) if "X" in want else None
+        dV = empty((V.shape[0], V.shape[1]), dtype=V.dtype, device=self.device) if "V" in want else None
+        db = empty((V.shape[0],), dtype=torch.float32, device=self.device) if "ibase" in want and ibase is not None else None
+        c = self._catalogue(X, V, ibase, scale)
+        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_backward_workspace, ctypes.byref(c), int(dX is not None), int(dV is not None),
+                                   int(db is not None))
+        self._check(self._lib.ifr_catalogue_logprob_backward(self._h, ctypes.byref(c), _ptr(ids), m, _row_stride(ids), _ptr(lse), _ptr(dlogp), _row_stride(dlogp),
+                                                             _ptr(dX), 0 if dX is None else _row_stride(dX), _ptr(dV), 0 if dV is None else _row_stride(dV),
+                                                             _ptr(db), _ptr(ws), need, self._stream()))
+        return dX, dV, db
+
+    # ------------------------------------------------------------------ losses
+    def preference_loss(self, chosen, rejected, ref_chosen=None, ref_rejected=None, mask_chosen=None, mask_rejected=None, beta=0.1, kind="logistic",
+                        label_smoothing=0.0, margin=0.0, average=False, weight=None):
+        """PreferenceLoss(loss [n], h [n], d_chosen, d_rejected) of n pairs of slates from the log-probabilities of their items
+        [n, places]: h = beta ((C - R) - (Cr - Rr)) - margin with C, R the sums (`average`: means) over the masks of the chosen and
+        the rejected slate and Cr, Rr those of a frozen reference.  kind "logistic": log(1 + exp(-h)), smoothed towards the other
+        order by label_smoothing; "hinge": max(0, 1 - h); "squared": ((h - 1/2) / beta)^2.  d_chosen and d_rejected are the
+        gradients of sum(weight * loss), weight 1 unless given.  Slates of one item with beta = 1 and no reference are BPR's criterion."""
+        import torch
+        chosen, rejected, ref_c, ref_r, mask_c, mask_r, weight = check_preference(
+            chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, weight, beta, kind, label_smoothing, margin, self.device)
+        n = chosen.shape[0]
+        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=self.device)
+        r = PreferenceLoss(new(n), new(n), new(*chosen.shape), new(*rejected.shape))
+        p = _lib.Preference()
+        p.n, p.len_chosen, p.len_rejected = n, chosen.shape[1], rejected.shape[1]
+        p.kind, p.average = ("logistic", "hinge", "squared").index(kind), int(bool(average))
+        p.chosen, p.rejected, p.ref_chosen, p.ref_rejected = _ptr(chosen), _ptr(rejected), _ptr(ref_c), _ptr(ref_r)
+        p.mask_chosen, p.mask_rejected, p.weight = _ptr(mask_c), _ptr(mask_r), _ptr(weight)
+        p.loss, p.h, p.d_chosen, p.d_rejected = (_ptr(t) for t in r)
+        p.ld_chosen, p.ld_rejected, p.ld_ref_chosen, p.ld_ref_rejected = (_row_stride(t) for t in (chosen, rejected, ref_c, ref_r))
+        p.ld_mask_chosen, p.ld_mask_rejected, p.ld_d_chosen, p.ld_d_rejected = (_row_stride(t) for t in (mask_c, mask_r, r.d_chosen, r.d_rejected))
+        p.beta, p.margin, p.label_smoothing = float(beta), float(margin), float(label_smoothing)
+        self._check(self._lib.ifr_preference_loss(self._h, ctypes.byref(p), self._stream()))
+        return r
+
+    def policy_loss(self, logp, old_logp, advantages, ref_logp=None, mask=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="row", weight=None):
+        """PolicyLoss(loss [n], kl [n], clipped int32 [n], d_logp [n, places]) of n rows of choices sampled from an older policy: per
+        place of the mask -A r, r = exp(logp - old_logp) clipped to [1 - clip_low, 1 + clip_high] where that raises the loss, plus
+        kl_coef (exp(q) - q - 1), q = ref_logp - logp.  loss[row] = c * the sum over its places with c = weight (1 unless given) times
+        1 ("sum"), 1 / places of the row ("row") or 1 / places of the batch ("batch"); d_logp is the gradient of sum(loss).  kl is the row's
+        mean (None without ref_logp), clipped its number of clipped places."""
+        import torch
+        logp, old_logp, advantages, ref_logp, mask, weight = check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef,
+                                                                          reduction, self.device)
+        n, width = logp.shape
+        new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=self.device)
+        r = PolicyLoss(new(n), None if ref_logp is None else new(n), new(n, dtype=torch.int32), new(n, width))
+        p = _lib.Policy()
+        p.n, p.len, p.reduction = n, width, ("sum", "row", "batch").index(reduction)
+        p.logp, p.old_logp, p.ref_logp, p.advantages, p.weight, p.mask = (_ptr(t) for t in (logp, old_logp, ref_logp, advantages, weight, mask))
+        p.loss, p.kl, p.clipped, p.d_logp = (_ptr(t) for t in r)
+        p.ld_logp, p.ld_old, p.ld_ref, p.ld_mask, p.ld_d_logp = (_row_stride(t) for t in (logp, old_logp, ref_logp, mask, r.d_logp))
+        p.clip_low, p.clip_high, p.kl_coef = float(clip_low), float(clip_high), float(kl_coef)
+        ws, need = self._workspace(self._lib.ifr_policy_loss_workspace, ctypes.byref(p))
+        self._check(self._lib.ifr_policy_loss(self._h, ctypes.byref(p), _ptr(ws), need, self._stream()))
+        return r

@@ -16,6 +16,9 @@
 #include "ifr_itemitem.h"
 #include "ifr_fit.h"
 #include "ifr_evalcsr.h"
+#include "ifr_mxfp4.h"
+#include "ifr_logprob.h"
+#include "ifr_losses.h"
 
 namespace ifr {
 // implemented in ifr_aux.hip
@@ -1738,6 +1741,242 @@ int ifr_factor_chain_order(ifr_handle h, int32_t *perm, int *n)
         for (int e = 0; e < 4; ++e) { perm[t++] = 8 * g + e; perm[t++] = 8 * g + 4 + e; }
     *n = h->KD;
     return IFR_OK;
+}
+
+/* ---------------------------------------------------------------- catalogue operators (4-bit model, log-probabilities, losses) */
+
+}  // extern "C"
+
+namespace {
+
+// makes the handle's GPU current for the length of a call
+struct DeviceGuard {
+    int before = -1;
+    hipError_t err;
+    explicit DeviceGuard(int device)
+    {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+        else if (err == hipSuccess) before = -1;
+    }
+    ~DeviceGuard() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+// body of an entry point on the handle's GPU; a C++ exception (the error text is a std::string) does not leave it
+template <typename F>
+int guarded(ifr_handle h, F &&body)
+{
+    if (!h) return IFR_ERR_ARG;
+    try {
+        DeviceGuard g(h->device);
+        if (g.err != hipSuccess) return fail(h, IFR_ERR_HIP, std::string("hipSetDevice: ") + hipGetErrorString(g.err));
+        return body();
+    } catch (...) {
+        return IFR_ERR_NOMEM;
+    }
+}
+
+int launched(ifr_handle h, int rc, const char *what)
+{
+    return rc ? fail(h, IFR_ERR_HIP, std::string(what) + ": launch failed") : IFR_OK;
+}
+
+constexpr int64_t MAX_ROWS = (int64_t)1 << 25, MAX_CATALOGUE = (int64_t)1 << 28;
+
+int check_catalogue(ifr_handle h, const char *what, const ifr_catalogue *c)
+{
+    const std::string w(what);
+    if (!c) return fail(h, IFR_ERR_ARG, w + ": null catalogue");
+    if (c->dtype != IFR_F32 && c->dtype != IFR_BF16 && c->dtype != IFR_MXFP4) return fail(h, IFR_ERR_ARG, w + ": unknown dtype");
+    if (c->k < 1 || c->k > IFR_MAX_FACTORS) return fail(h, IFR_ERR_ARG, w + ": k must be in [1, 256]");
+    if (c->n < 0 || c->n > MAX_ROWS) return fail(h, IFR_ERR_ARG, w + ": n must be in [0, 2^25]");
+    if (c->n_items < 1 || c->n_items > MAX_CATALOGUE) return fail(h, IFR_ERR_ARG, w + ": n_items must be in [1, 2^28]");
+    if (!(c->scale > 0.0) || c->scale > 1e30) return fail(h, IFR_ERR_ARG, w + ": scale must be positive");
+    if (c->dtype != IFR_MXFP4 && (c->ldx < c->k || c->ldv < c->k)) return fail(h, IFR_ERR_ARG, w + ": rows shorter than k");
+    return IFR_OK;
+}
+
+int check_operands(ifr_handle h, const char *what, const ifr_catalogue *c)
+{
+    const std::string w(what);
+    if (!c->X || !c->V) return fail(h, IFR_ERR_ARG, w + ": null X or V");
+    if (c->dtype == IFR_MXFP4 && (!c->x_scales || !c->v_scales)) return fail(h, IFR_ERR_ARG, w + ": null scales");
+    if (c->dtype == IFR_MXFP4 && (((uintptr_t)c->X | (uintptr_t)c->V) & 15)) return fail(h, IFR_ERR_ARG, w + ": codes must be 16-byte aligned");
+    return IFR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ifr_mxfp4_quantize(ifr_handle h, const void *X, int dtype, int64_t n, int64_t k, int64_t ld, uint8_t *codes, uint8_t *scales,
+                       void *stream)
+{
+    return guarded(h, [&]() -> int {
+        if (dtype != IFR_F32 && dtype != IFR_BF16) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_quantize: dtype must be fp32 or bf16");
+        if (n < 0 || n > MAX_CATALOGUE || k < 1 || k > ((int64_t)1 << 20) || ld < k) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_quantize: bad n, k or ld");
+        if (n == 0) return IFR_OK;
+        if (!X || !codes || !scales) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_quantize: null argument");
+        if ((uintptr_t)codes & 15) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_quantize: codes must be 16-byte aligned");
+        return launched(h, ifr::launch_mx_quantize(X, dtype == IFR_BF16, n, k, ld, codes, scales, (hipStream_t)stream), "ifr_mxfp4_quantize");
+    });
+}
+
+int ifr_mxfp4_dequantize(ifr_handle h, const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, float *out, int64_t ld,
+                         void *stream)
+{
+    return guarded(h, [&]() -> int {
+        if (n < 0 || n > MAX_CATALOGUE || k < 1 || k > ((int64_t)1 << 20) || ld < k) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_dequantize: bad n, k or ld");
+        if (n == 0) return IFR_OK;
+        if (!codes || !scales || !out) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_dequantize: null argument");
+        if ((uintptr_t)codes & 15) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_dequantize: codes must be 16-byte aligned");
+        return launched(h, ifr::launch_mx_dequantize(codes, scales, n, k, out, ld, (hipStream_t)stream), "ifr_mxfp4_dequantize");
+    });
+}
+
+int ifr_mxfp4_scores(ifr_handle h, const uint8_t *x_codes, const uint8_t *x_scales, int64_t n, const uint8_t *v_codes,
+                     const uint8_t *v_scales, int64_t n_items, int k, const float *ubase, const float *ibase, void *out,
+                     int out_dtype, int64_t ld, void *stream)
+{
+    return guarded(h, [&]() -> int {
+        if (out_dtype != IFR_F32 && out_dtype != IFR_BF16) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_scores: out_dtype must be fp32 or bf16");
+        if (k < 1 || k > IFR_MAX_FACTORS) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_scores: k must be in [1, 256]");
+        if (n < 0 || n > MAX_ROWS || n_items < 1 || n_items > MAX_CATALOGUE || ld < n_items) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_scores: bad n, n_items or ld");
+        if (n == 0) return IFR_OK;
+        if (!x_codes || !x_scales || !v_codes || !v_scales || !out) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_scores: null argument");
+        if (((uintptr_t)x_codes | (uintptr_t)v_codes) & 15) return fail(h, IFR_ERR_ARG, "ifr_mxfp4_scores: codes must be 16-byte aligned");
+        ifr::MxScoreParams p;
+        p.x = {x_codes, x_scales, n};
+        p.v = {v_codes, v_scales, n_items};
+        p.k = k; p.ubase = ubase; p.ibase = ibase; p.out = out; p.ld = ld; p.out_bf16 = out_dtype == IFR_BF16;
+        return launched(h, ifr::launch_mx_scores(p, (hipStream_t)stream), "ifr_mxfp4_scores");
+    });
+}
+
+int ifr_catalogue_logprob_workspace(ifr_handle h, const ifr_catalogue *c, int64_t *bytes)
+{
+    return guarded(h, [&]() -> int {
+        const int rc = check_catalogue(h, "ifr_catalogue_logprob_workspace", c);
+        if (rc) return rc;
+        if (!bytes) return fail(h, IFR_ERR_ARG, "ifr_catalogue_logprob_workspace: null argument");
+        *bytes = c->n ? (int64_t)ifr::logprob_workspace(*c) : 0;
+        return IFR_OK;
+    });
+}
+
+int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids, float *logp,
+                          int64_t ld_logp, float *lse, void *ws, int64_t ws_bytes, void *stream)
+{
+    return guarded(h, [&]() -> int {
+        const char *what = "ifr_catalogue_logprob";
+        int rc = check_catalogue(h, what, c);
+        if (rc) return rc;
+        if (m < 0 || m > ((int64_t)1 << 20) || (m > 0 && (ld_ids < m || ld_logp < m))) return fail(h, IFR_ERR_ARG, std::string(what) + ": bad m or rows shorter than m");
+        if (c->n == 0) return IFR_OK;
+        rc = check_operands(h, what, c);
+        if (rc) return rc;
+        if (m > 0 && (!ids || !logp)) return fail(h, IFR_ERR_ARG, std::string(what) + ": null ids or logp");
+        if (!ws || ((uintptr_t)ws & 255) || ws_bytes < (int64_t)ifr::logprob_workspace(*c))
+            return fail(h, IFR_ERR_ARG, std::string(what) + ": workspace missing, not 256-byte aligned or too small");
+        return launched(h, ifr::launch_logprob(*c, ids, m, ld_ids, logp, ld_logp, lse, ws, (hipStream_t)stream), what);
+    });
+}
+
+int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int want_dx, int want_dv, int want_dibase, int64_t *bytes)
+{
+    return guarded(h, [&]() -> int {
+        const int rc = check_catalogue(h, "ifr_catalogue_logprob_backward_workspace", c);
+        if (rc) return rc;
+        if (!bytes) return fail(h, IFR_ERR_ARG, "ifr_catalogue_logprob_backward_workspace: null argument");
+        if (c->dtype == IFR_MXFP4) return fail(h, IFR_ERR_ARG, "ifr_catalogue_logprob_backward_workspace: a 4-bit model has no gradient");
+        *bytes = c->n ? (int64_t)ifr::logprob_backward_workspace(*c, want_dx, want_dv, want_dibase) : 0;
+        return IFR_OK;
+    });
+}
+
+int ifr_catalogue_logprob_backward(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids,
+                                   const float *lse, const float *dlogp, int64_t ld_dlogp, void *dX, int64_t ld_dx, void *dV,
+                                   int64_t ld_dv, float *dibase, void *ws, int64_t ws_bytes, void *stream)
+{
+    return guarded(h, [&]() -> int {
+        const std::string what = "ifr_catalogue_logprob_backward";
+        int rc = check_catalogue(h, what.c_str(), c);
+        if (rc) return rc;
+        if (c->dtype == IFR_MXFP4) return fail(h, IFR_ERR_ARG, what + ": a 4-bit model has no gradient");
+        if (m < 0 || m > ((int64_t)1 << 20) || (m > 0 && (ld_ids < m || ld_dlogp < m))) return fail(h, IFR_ERR_ARG, what + ": bad m or rows shorter than m");
+        if ((dX && ld_dx < c->k) || (dV && ld_dv < c->k)) return fail(h, IFR_ERR_ARG, what + ": gradient rows shorter than k");
+        if (c->n == 0) return IFR_OK;
+        rc = check_operands(h, what.c_str(), c);
+        if (rc) return rc;
+        if (!lse || (m > 0 && (!ids || !dlogp))) return fail(h, IFR_ERR_ARG, what + ": null lse, ids or dlogp");
+        if (!dX && !dV && !dibase) return IFR_OK;
+        if (!ws || ((uintptr_t)ws & 255) || ws_bytes < (int64_t)ifr::logprob_backward_workspace(*c, dX != nullptr, dV != nullptr, dibase != nullptr))
+            return fail(h, IFR_ERR_ARG, what + ": workspace missing, not 256-byte aligned or too small");
+        ifr::LogprobGrad g = {lse, dlogp, ld_dlogp, dX, dV, ld_dx, ld_dv, dibase};
+        return launched(h, ifr::launch_logprob_backward(*c, ids, m, ld_ids, g, ws, (hipStream_t)stream), what.c_str());
+    });
+}
+
+int ifr_preference_loss(ifr_handle h, const ifr_preference *p, void *stream)
+{
+    return guarded(h, [&]() -> int {
+        const std::string what = "ifr_preference_loss";
+        if (!p) return fail(h, IFR_ERR_ARG, what + ": null argument");
+        if (p->n < 0 || p->len_chosen < 0 || p->len_rejected < 0) return fail(h, IFR_ERR_ARG, what + ": negative size");
+        if (p->kind < IFR_PREFERENCE_LOGISTIC || p->kind > IFR_PREFERENCE_SQUARED) return fail(h, IFR_ERR_ARG, what + ": unknown kind");
+        if (!(p->beta > 0.0) || p->beta > 1e30) return fail(h, IFR_ERR_ARG, what + ": beta must be positive");
+        if (!(p->label_smoothing >= 0.0 && p->label_smoothing < 0.5)) return fail(h, IFR_ERR_ARG, what + ": label_smoothing must be in [0, 1/2)");
+        if (p->label_smoothing != 0.0 && p->kind != IFR_PREFERENCE_LOGISTIC) return fail(h, IFR_ERR_ARG, what + ": label_smoothing needs the logistic kind");
+        if (!(p->margin > -1e30 && p->margin < 1e30)) return fail(h, IFR_ERR_ARG, what + ": margin must be finite");
+        if (p->n == 0) return IFR_OK;
+        if ((p->len_chosen && !p->chosen) || (p->len_rejected && !p->rejected)) return fail(h, IFR_ERR_ARG, what + ": null chosen or rejected");
+        if ((p->len_chosen && p->len_rejected) && !p->ref_chosen != !p->ref_rejected) return fail(h, IFR_ERR_ARG, what + ": a reference needs both slates");
+        if (p->ld_chosen < p->len_chosen || p->ld_rejected < p->len_rejected || (p->ref_chosen && p->ld_ref_chosen < p->len_chosen) ||
+            (p->ref_rejected && p->ld_ref_rejected < p->len_rejected) || (p->mask_chosen && p->ld_mask_chosen < p->len_chosen) ||
+            (p->mask_rejected && p->ld_mask_rejected < p->len_rejected) || (p->d_chosen && p->ld_d_chosen < p->len_chosen) ||
+            (p->d_rejected && p->ld_d_rejected < p->len_rejected))
+            return fail(h, IFR_ERR_ARG, what + ": rows shorter than their slates");
+        return launched(h, ifr::launch_preference(*p, (hipStream_t)stream), what.c_str());
+    });
+}
+
+static int check_policy(ifr_handle h, const std::string &what, const ifr_policy *p)
+{
+    if (!p) return fail(h, IFR_ERR_ARG, what + ": null argument");
+    if (p->n < 0 || p->len < 0) return fail(h, IFR_ERR_ARG, what + ": negative size");
+    if (p->reduction < IFR_POLICY_SUM || p->reduction > IFR_POLICY_BATCH) return fail(h, IFR_ERR_ARG, what + ": unknown reduction");
+    if (!(p->clip_low >= 0.0 && p->clip_low < 1.0) || !(p->clip_high >= 0.0 && p->clip_high < 1e30))
+        return fail(h, IFR_ERR_ARG, what + ": clip_low must be in [0, 1), clip_high at least 0");
+    if (!(p->kl_coef > -1e30 && p->kl_coef < 1e30)) return fail(h, IFR_ERR_ARG, what + ": kl_coef must be finite");
+    return IFR_OK;
+}
+
+int ifr_policy_loss_workspace(ifr_handle h, const ifr_policy *p, int64_t *bytes)
+{
+    return guarded(h, [&]() -> int {
+        const int rc = check_policy(h, "ifr_policy_loss_workspace", p);
+        if (rc) return rc;
+        if (!bytes) return fail(h, IFR_ERR_ARG, "ifr_policy_loss_workspace: null argument");
+        *bytes = (int64_t)ifr::policy_workspace(*p);
+        return IFR_OK;
+    });
+}
+
+int ifr_policy_loss(ifr_handle h, const ifr_policy *p, void *ws, int64_t ws_bytes, void *stream)
+{
+    return guarded(h, [&]() -> int {
+        const std::string what = "ifr_policy_loss";
+        const int rc = check_policy(h, what, p);
+        if (rc) return rc;
+        if (p->n == 0) return IFR_OK;
+        if (!p->advantages || (p->len && (!p->logp || !p->old_logp))) return fail(h, IFR_ERR_ARG, what + ": null logp, old_logp or advantages");
+        if (p->ld_logp < p->len || p->ld_old < p->len || (p->ref_logp && p->ld_ref < p->len) || (p->mask && p->ld_mask < p->len) ||
+            (p->d_logp && p->ld_d_logp < p->len))
+            return fail(h, IFR_ERR_ARG, what + ": rows shorter than len");
+        const int64_t need = (int64_t)ifr::policy_workspace(*p);
+        if (need && (!ws || ((uintptr_t)ws & 255) || ws_bytes < need)) return fail(h, IFR_ERR_ARG, what + ": workspace missing, not 256-byte aligned or too small");
+        return launched(h, ifr::launch_policy(*p, ws, (hipStream_t)stream), what.c_str());
+    });
 }
 
 }  // extern "C"

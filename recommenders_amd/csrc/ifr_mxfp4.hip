@@ -1,0 +1,210 @@
+// ifr_mxfp4.hip -- a catalogue in 4-bit microscaled floating point: quantisation, its inverse and the product that yields
+// score rows (layout: ifr_mxfp4.h).
+#include <hip/hip_runtime.h>
+
+#include "ifr_mxfp4.h"
+
+namespace ifr {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+namespace {
+
+__device__ __forceinline__ float load_f32(const float *p) { return *p; }
+__device__ __forceinline__ float load_f32(const __bf16 *p) { return (float)*p; }
+
+// 8 consecutive elements of a row, zeros behind its end
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *row, int64_t col, int64_t k, float v[8])
+{
+    if (VEC) {                                        // 16-byte aligned rows, k a multiple of 8
+        if (col >= k) {
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        } else if (sizeof(T) == 4) {
+            const float4 a = ((const float4 *)(row + col))[0], b = ((const float4 *)(row + col))[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 a = *(const uint4 *)(row + col);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+            for (int j = 0; j < 4; ++j) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        }
+    } else {
+        for (int j = 0; j < 8; ++j) v[j] = col + j < k ? load_f32(row + col + j) : 0.f;
+    }
+}
+
+}  // namespace
+
+// One lane takes 8 columns of a row, four neighbouring lanes a block: e = floor(log2 max|v|) - 2 is the exponent field of the
+// largest magnitude less 2 (subnormal maxima clamp to 2^-127), v / 2^e is exact, and the conversion rounds to the nearest of the
+// grid, ties to the even code, at most 6 in magnitude.  HBM-bound: 4 bytes read and 17/32 written an element.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *X, int64_t n, int64_t k, int64_t ld, int kb, uint8_t *codes, uint8_t *scales)
+{
+    const int64_t g = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = g / (kb * 4);
+    const int c8 = (int)(g - row * (kb * 4));         // which 8 columns of the row
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row < n) load8<T, VEC>(X + row * ld, (int64_t)c8 * 8, k, v);
+    uint32_t top = 0;
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    if (row >= n) return;
+    const uint32_t field = top >> 23;
+    const uint32_t byte = field == 255 ? 255u : (field > 2 ? field - 2 : 0u);
+    // 2^(127 - byte): byte <= 252, so the exponent field 254 - byte is at least 2
+    const float inv = byte == 255 ? 0.f : __uint_as_float((254u - byte) << 23);
+    uint32_t c = 0;
+    if (byte != 255) {
+        for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j] * inv, -6.f), 6.f);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], 1.0f, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], 1.0f, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], 1.0f, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], 1.0f, 3);
+    }
+    ((uint32_t *)codes)[row * (kb * 4) + c8] = c;
+    if ((c8 & 3) == 0) scales[row * kb + (c8 >> 2)] = (uint8_t)byte;
+}
+
+// 2^(byte - 127), NaN for 255 (2^-127 is the subnormal 0x400000)
+__device__ __forceinline__ float mx_scale(uint32_t byte)
+{
+    return byte == 255 ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+
+__device__ __forceinline__ void mx_values8(uint32_t c, float s, float v[8])
+{
+    v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+    v2f d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+    v[0] = a[0] * s; v[1] = a[1] * s; v[2] = b[0] * s; v[3] = b[1] * s;
+    v[4] = d[0] * s; v[5] = d[1] * s; v[6] = e[0] * s; v[7] = e[1] * s;
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, int kb, float *out, int64_t ld)
+{
+    const int64_t g = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = g / (kb * 4);
+    const int c8 = (int)(g - row * (kb * 4));
+    if (row >= n) return;
+    float v[8];
+    mx_values8(((const uint32_t *)codes)[row * (kb * 4) + c8], mx_scale(scales[row * kb + (c8 >> 2)]), v);
+    float *o = out + row * ld + (int64_t)c8 * 8;
+    if (VEC) {
+        if ((int64_t)c8 * 8 < k) {
+            ((float4 *)o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            ((float4 *)o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    } else {
+        for (int j = 0; j < 8; ++j)
+            if ((int64_t)c8 * 8 + j < k) o[j] = v[j];
+    }
+}
+
+// ---------------------------------------------------------------------------- product
+
+// Score rows: D[query][item] by v_mfma_scale_f32_32x32x64 with both operands in E2M1.  A lane of that instruction holds one
+// block of 32 of one row and that block's scale, which is the layout in memory.  A wave takes 32 queries and walks item tiles
+// of 32; sums are fp32.
+__global__ __launch_bounds__(256) void mx_scores_kernel(MxScoreParams p, int kb, int tiles_per_wave)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    const int64_t q0 = (int64_t)blockIdx.y * 32;
+    const int64_t q = min(q0 + r, p.x.n - 1);
+    const int steps = (kb + 1) / 2;
+    const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * tiles_per_wave;
+    for (int t = 0; t < tiles_per_wave; ++t) {
+        const int64_t i0 = (first + t) * 32;
+        if (i0 >= p.v.n) return;
+        const int64_t item = min(i0 + r, p.v.n - 1);
+        v16f d = {0};
+        for (int s = 0; s < steps; ++s) {
+            const int b = 2 * s + h;
+            v8i a = {0}, w = {0};
+            int sa = 127, sw = 127;
+            if (b < kb) {
+                const uint4 ca = *(const uint4 *)(p.x.codes + (q * kb + b) * 16);
+                const uint4 cw = *(const uint4 *)(p.v.codes + (item * kb + b) * 16);
+                a[0] = ca.x; a[1] = ca.y; a[2] = ca.z; a[3] = ca.w;
+                w[0] = cw.x; w[1] = cw.y; w[2] = cw.z; w[3] = cw.w;
+                sa = p.x.scales[q * kb + b];
+                sw = p.v.scales[item * kb + b];
+            }
+            d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, w, d, 4, 4, 0, sa, 0, sw);
+        }
+        if (i0 + r < p.v.n) {
+            const float ib = p.ibase ? p.ibase[item] : 0.f;
+            for (int e = 0; e < 16; ++e) {
+                const int64_t row = q0 + 8 * (e >> 2) + 4 * h + (e & 3);
+                if (row >= p.x.n) continue;
+                const float v = d[e] + (p.ubase ? ib + p.ubase[row] : ib);
+                if (p.out_bf16) ((__bf16 *)p.out)[row * p.ld + item] = (__bf16)v;
+                else ((float *)p.out)[row * p.ld + item] = v;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- launches
+
+namespace {
+// the grid counts work items in 32 bits: more than 2^22 workgroups go into a second dimension
+dim3 grid_of(int64_t blocks)
+{
+    const int64_t x = blocks < (1 << 22) ? blocks : (1 << 22);
+    return dim3((uint32_t)x, (uint32_t)((blocks + x - 1) / x));
+}
+
+bool aligned16(const void *p, int64_t row_bytes) { return ((uintptr_t)p & 15) == 0 && row_bytes % 16 == 0; }
+}  // namespace
+
+int launch_mx_quantize(const void *X, int bf16, int64_t n, int64_t k, int64_t ld, uint8_t *codes, uint8_t *scales, hipStream_t s)
+{
+    const int kb = (int)((k + 31) / 32);
+    const dim3 grid = grid_of((n * kb * 4 + 255) / 256);
+    const bool vec = k % 8 == 0 && aligned16(X, ld * (bf16 ? 2 : 4));
+    if (bf16) {
+        if (vec) hipLaunchKernelGGL((mx_quantize_kernel<__bf16, true>), grid, dim3(256), 0, s, (const __bf16 *)X, n, k, ld, kb, codes, scales);
+        else hipLaunchKernelGGL((mx_quantize_kernel<__bf16, false>), grid, dim3(256), 0, s, (const __bf16 *)X, n, k, ld, kb, codes, scales);
+    } else {
+        if (vec) hipLaunchKernelGGL((mx_quantize_kernel<float, true>), grid, dim3(256), 0, s, (const float *)X, n, k, ld, kb, codes, scales);
+        else hipLaunchKernelGGL((mx_quantize_kernel<float, false>), grid, dim3(256), 0, s, (const float *)X, n, k, ld, kb, codes, scales);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, float *out, int64_t ld, hipStream_t s)
+{
+    const int kb = (int)((k + 31) / 32);
+    const dim3 grid = grid_of((n * kb * 4 + 255) / 256);
+    if (k % 8 == 0 && aligned16(out, ld * 4)) hipLaunchKernelGGL(mx_dequantize_kernel<true>, grid, dim3(256), 0, s, codes, scales, n, k, kb, out, ld);
+    else hipLaunchKernelGGL(mx_dequantize_kernel<false>, grid, dim3(256), 0, s, codes, scales, n, k, kb, out, ld);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_mx_scores(const MxScoreParams &p, hipStream_t s)
+{
+    const int kb = (p.k + 31) / 32;
+    const int64_t qt = (p.x.n + 31) / 32, it = (p.v.n + 31) / 32;
+    const int per = (int)(it * qt > 65536 ? 8 : 1);
+    for (int64_t y = 0; y < qt; y += 65535) {         // grid.y holds 65535 query tiles
+        MxScoreParams c = p;
+        const int64_t rows = y * 32;
+        c.x.codes += rows * kb * 16; c.x.scales += rows * kb; c.x.n -= rows;
+        if (c.ubase) c.ubase += rows;
+        c.out = (char *)p.out + rows * p.ld * (p.out_bf16 ? 2 : 4);
+        const int64_t ny = qt - y < 65535 ? qt - y : 65535;
+        if (c.x.n > ny * 32) c.x.n = ny * 32;
+        hipLaunchKernelGGL(mx_scores_kernel, dim3((it + 4 * per - 1) / (4 * per), ny), dim3(256), 0, s, c, kb, per);
+        if (hipGetLastError() != hipSuccess) return -1;
+    }
+    return 0;
+}
+
+}  // namespace ifr

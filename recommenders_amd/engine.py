@@ -8,6 +8,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
+from .catalogue import CatalogueOps
 
 
 METRICS_PER_K = 6      # ndcg, recall, precision, hit ratio, f1, ncrr (include/ifr.h IFR_METRICS_PER_K)
@@ -65,7 +66,7 @@ class DeviceCsr:
                    torch.as_tensor(np.ascontiguousarray(data)).to(device), m.shape)
 
 
-class HipScorer:
+class HipScorer(CatalogueOps):
     """Device-resident model + CSR data and the batched rank / metric entry points."""
 
     def __init__(self, device=0):
