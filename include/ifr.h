@@ -377,7 +377,7 @@ int ifr_mxfp4_dequantize(ifr_handle h, const uint8_t *codes, const uint8_t *scal
                          void *stream);
 /* Score rows of a 4-bit model, beside ifr_score_dense: out[u][i] = (ibase[i] + ubase[u]) + <X[u], V[i]>, sums in fp32, rounded
  * once to `out_dtype` (IFR_F32 or IFR_BF16).  out: dev [n][ld], ld >= n_items; ibase [n_items], ubase [n]: dev or NULL.
- * 1 <= k <= IFR_MAX_FACTORS, n and n_items below 2^30. */
+ * 1 <= k <= IFR_MAX_FACTORS, n <= 2^25, 1 <= n_items <= 2^28. */
 int ifr_mxfp4_scores(ifr_handle h, const uint8_t *x_codes, const uint8_t *x_scales, int64_t n, const uint8_t *v_codes,
                      const uint8_t *v_scales, int64_t n_items, int k, const float *ubase, const float *ibase, void *out,
                      int out_dtype, int64_t ld, void *stream);
@@ -386,14 +386,14 @@ int ifr_mxfp4_scores(ifr_handle h, const uint8_t *x_codes, const uint8_t *x_scal
 typedef struct ifr_catalogue {
     const void *X, *V;           /* dev [n][ldx], [n_items][ldv] of `dtype`; IFR_MXFP4: the codes (ldx, ldv unused)         */
     const uint8_t *x_scales, *v_scales;   /* IFR_MXFP4: the scales, else NULL                                               */
-    const float *ibase;          /* dev [n_items] or NULL; -inf takes an item out of the catalogue                          */
+    const float *ibase;          /* dev [n_items] or NULL; -inf, or what overflows to it as scale ibase log2(e), takes an item out */
     int64_t n, n_items, ldx, ldv;
-    int k, dtype;                /* 1 <= k <= IFR_MAX_FACTORS; n, n_items < 2^30                                            */
+    int k, dtype;                /* 1 <= k <= IFR_MAX_FACTORS; n <= 2^25, 1 <= n_items <= 2^28                               */
     double scale;                /* > 0: an inverse temperature                                                             */
 } ifr_catalogue;
 
 /* Log-probabilities of items under the softmax over the whole catalogue; the n x n_items scores are never stored.
- * ids: dev [n][ld_ids], m >= 0 items a user (a slate; an item may stand in it twice).  A negative id is an empty place: its
+ * ids: dev [n][ld_ids], m items a user (0 <= m <= 2^20, n m <= 2^32) (a slate; an item may stand in it twice).  A negative id is an empty place: its
  * logp is 0 and nothing flows through it.  An id >= n_items gives NaN.
  *   lse[u] = log sum_i exp z[u][i] (dev [n] or NULL), logp[u][j] = z[u][ids[u][j]] - lse[u] (dev [n][ld_logp], or NULL where m = 0).
  * Products of fp32 operands keep 22 bits of each operand (more than the sum of k products in fp32 does); sums are fp32. */
@@ -405,7 +405,8 @@ int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *i
  *   dX = scale dz V, dV = scale dz^T X (both of `dtype`, rows ld_dx / ld_dv apart), dibase = scale sum_u dz (fp32).
  * Any of the three may be NULL.  fp32 or bf16 operands.  No atomics: the same call gives the same bits.  A user whose lse is
  * -inf (every item taken out) has no probabilities, and only its targets' part of the gradient. */
-int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int want_dx, int want_dv, int want_dibase, int64_t *bytes);
+int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int64_t m, int want_dx, int want_dv, int want_dibase,
+                                             int64_t *bytes);
 int ifr_catalogue_logprob_backward(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids,
                                    const float *lse, const float *dlogp, int64_t ld_dlogp, void *dX, int64_t ld_dx, void *dV,
                                    int64_t ld_dv, float *dibase, void *ws, int64_t ws_bytes, void *stream);

@@ -99,7 +99,7 @@ SIGNATURES = {
     "ifr_catalogue_logprob_workspace": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), c_i64p]),
     "ifr_catalogue_logprob": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), vp, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_int64, vp, vp,
                                              ctypes.c_int64, vp]),
-    "ifr_catalogue_logprob_backward_workspace": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), ctypes.c_int, ctypes.c_int, ctypes.c_int, c_i64p]),
+    "ifr_catalogue_logprob_backward_workspace": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, c_i64p]),
     "ifr_catalogue_logprob_backward": (ctypes.c_int, [vp, ctypes.POINTER(Catalogue), vp, ctypes.c_int64, ctypes.c_int64, vp, vp, ctypes.c_int64, vp,
                                                       ctypes.c_int64, vp, ctypes.c_int64, vp, vp, ctypes.c_int64, vp]),
     "ifr_preference_loss": (ctypes.c_int, [vp, ctypes.POINTER(Preference), vp]),

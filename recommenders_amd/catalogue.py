@@ -292,7 +292,7 @@ class CatalogueOps:
         dV = empty((V.shape[0], V.shape[1]), dtype=V.dtype, device=self.device) if "V" in want else None
         db = empty((V.shape[0],), dtype=torch.float32, device=self.device) if "ibase" in want and ibase is not None else None
         c = self._catalogue(X, V, ibase, scale)
-        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_backward_workspace, ctypes.byref(c), int(dX is not None), int(dV is not None),
+        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_backward_workspace, ctypes.byref(c), m, int(dX is not None), int(dV is not None),
                                    int(db is not None))
         self._check(self._lib.ifr_catalogue_logprob_backward(self._h, ctypes.byref(c), _ptr(ids), m, _row_stride(ids), _ptr(lse), _ptr(dlogp), _row_stride(dlogp),
                                                              _ptr(dX), 0 if dX is None else _row_stride(dX), _ptr(dV), 0 if dV is None else _row_stride(dV),

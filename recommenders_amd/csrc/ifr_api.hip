@@ -1781,7 +1781,7 @@ int launched(ifr_handle h, int rc, const char *what)
     return rc ? fail(h, IFR_ERR_HIP, std::string(what) + ": launch failed") : IFR_OK;
 }
 
-constexpr int64_t MAX_ROWS = (int64_t)1 << 25, MAX_CATALOGUE = (int64_t)1 << 28;
+constexpr int64_t MAX_ROWS = (int64_t)1 << 25, MAX_CATALOGUE = (int64_t)1 << 28, MAX_PLACES = (int64_t)1 << 20, MAX_LIST = (int64_t)1 << 32;
 
 int check_catalogue(ifr_handle h, const char *what, const ifr_catalogue *c)
 {
@@ -1871,7 +1871,8 @@ int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *i
         const char *what = "ifr_catalogue_logprob";
         int rc = check_catalogue(h, what, c);
         if (rc) return rc;
-        if (m < 0 || m > ((int64_t)1 << 20) || (m > 0 && (ld_ids < m || ld_logp < m))) return fail(h, IFR_ERR_ARG, std::string(what) + ": bad m or rows shorter than m");
+        if (m < 0 || m > MAX_PLACES || c->n * m > MAX_LIST || (m > 0 && (ld_ids < m || ld_logp < m)))
+            return fail(h, IFR_ERR_ARG, std::string(what) + ": bad m (at most 2^20 a user, 2^32 in all) or rows shorter than m");
         if (c->n == 0) return IFR_OK;
         rc = check_operands(h, what, c);
         if (rc) return rc;
@@ -1882,14 +1883,15 @@ int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *i
     });
 }
 
-int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int want_dx, int want_dv, int want_dibase, int64_t *bytes)
+int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int64_t m, int want_dx, int want_dv, int want_dibase, int64_t *bytes)
 {
     return guarded(h, [&]() -> int {
         const int rc = check_catalogue(h, "ifr_catalogue_logprob_backward_workspace", c);
         if (rc) return rc;
         if (!bytes) return fail(h, IFR_ERR_ARG, "ifr_catalogue_logprob_backward_workspace: null argument");
         if (c->dtype == IFR_MXFP4) return fail(h, IFR_ERR_ARG, "ifr_catalogue_logprob_backward_workspace: a 4-bit model has no gradient");
-        *bytes = c->n ? (int64_t)ifr::logprob_backward_workspace(*c, want_dx, want_dv, want_dibase) : 0;
+        if (m < 0 || m > MAX_PLACES || c->n * m > MAX_LIST) return fail(h, IFR_ERR_ARG, "ifr_catalogue_logprob_backward_workspace: bad m (at most 2^20 a user, 2^32 in all)");
+        *bytes = c->n ? (int64_t)ifr::logprob_backward_workspace(*c, m, want_dx, want_dv, want_dibase) : 0;
         return IFR_OK;
     });
 }
@@ -1903,14 +1905,15 @@ int ifr_catalogue_logprob_backward(ifr_handle h, const ifr_catalogue *c, const i
         int rc = check_catalogue(h, what.c_str(), c);
         if (rc) return rc;
         if (c->dtype == IFR_MXFP4) return fail(h, IFR_ERR_ARG, what + ": a 4-bit model has no gradient");
-        if (m < 0 || m > ((int64_t)1 << 20) || (m > 0 && (ld_ids < m || ld_dlogp < m))) return fail(h, IFR_ERR_ARG, what + ": bad m or rows shorter than m");
+        if (m < 0 || m > MAX_PLACES || c->n * m > MAX_LIST || (m > 0 && (ld_ids < m || ld_dlogp < m)))
+            return fail(h, IFR_ERR_ARG, what + ": bad m (at most 2^20 a user, 2^32 in all) or rows shorter than m");
         if ((dX && ld_dx < c->k) || (dV && ld_dv < c->k)) return fail(h, IFR_ERR_ARG, what + ": gradient rows shorter than k");
         if (c->n == 0) return IFR_OK;
         rc = check_operands(h, what.c_str(), c);
         if (rc) return rc;
         if (!lse || (m > 0 && (!ids || !dlogp))) return fail(h, IFR_ERR_ARG, what + ": null lse, ids or dlogp");
         if (!dX && !dV && !dibase) return IFR_OK;
-        if (!ws || ((uintptr_t)ws & 255) || ws_bytes < (int64_t)ifr::logprob_backward_workspace(*c, dX != nullptr, dV != nullptr, dibase != nullptr))
+        if (!ws || ((uintptr_t)ws & 255) || ws_bytes < (int64_t)ifr::logprob_backward_workspace(*c, m, dX != nullptr, dV != nullptr, dibase != nullptr))
             return fail(h, IFR_ERR_ARG, what + ": workspace missing, not 256-byte aligned or too small");
         ifr::LogprobGrad g = {lse, dlogp, ld_dlogp, dX, dV, ld_dx, ld_dv, dibase};
         return launched(h, ifr::launch_logprob_backward(*c, ids, m, ld_ids, g, ws, (hipStream_t)stream), what.c_str());

@@ -19,7 +19,7 @@ struct LogprobGrad {
 size_t logprob_workspace(const ifr_catalogue &c);
 int launch_logprob(const ifr_catalogue &c, const int32_t *ids, int64_t m, int64_t ld_ids, float *logp, int64_t ld_logp, float *lse,
                    void *ws, hipStream_t s);
-size_t logprob_backward_workspace(const ifr_catalogue &c, bool want_dx, bool want_dv, bool want_db);
+size_t logprob_backward_workspace(const ifr_catalogue &c, int64_t m, bool want_dx, bool want_dv, bool want_db);
 int launch_logprob_backward(const ifr_catalogue &c, const int32_t *ids, int64_t m, int64_t ld_ids, const LogprobGrad &g, void *ws,
                             hipStream_t s);
 

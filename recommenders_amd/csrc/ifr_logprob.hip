@@ -11,13 +11,14 @@
 // between lanes, and the block of probabilities already is the B operand of the second product, whose contraction runs over t in
 // the order the block's registers hold (t = 16 c + 8 (j / 4) + 4 (lane / 32) + j % 4 for element j of step c).
 //
-// Operands in 16 bits: bf16 as it is.  fp32 is split into two fp16 parts after scaling by a power of two that brings the largest
-// magnitude to [2^14, 2^15): hi + lo keeps 22 bits of values near the maximum and an absolute step of 2^-39 of the maximum below,
-// and three products (hi hi, hi lo, lo hi) leave out lo lo, at most 2^-24 of a term.  Three fp16 products at 16 times the
-// rate of the fp32 matrix instruction cost a fifth of it.
+// Operands in 16 bits: bf16 as it is.  fp32 is split into two fp16 parts after scaling each tile of 32 rows by the power of two that
+// brings its largest magnitude to [2^14, 2^15): hi + lo keeps 22 bits of values near the maximum and an absolute step of 2^-39 of
+// the maximum below, and three products (hi hi, hi lo, lo hi) leave out lo lo, at most 2^-22 of a term.  Three fp16 products at 16
+// times the rate of the fp32 matrix instruction cost a fifth of it.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
+#include <type_traits>
 
 #include "ifr_logprob.h"
 
@@ -34,10 +35,9 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.6931471805599453;
 constexpr int S_ROWS = 128;            // S rows of a workgroup: 4 waves of 32
-constexpr int AMAX_BLOCKS = 256;
 constexpr int64_t MAX_GRID = 1 << 22;  // workgroups of 256 in one launch (the grid counts work items in 32 bits)
 
-int pad_factors(int k) { return k <= 64 ? 64 : k <= 128 ? 128 : k <= 192 ? 192 : 256; }
+int pad_factors(int k) { return (k + 31) / 32 * 32; }
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 __device__ __forceinline__ float as_f32(float v) { return v; }
@@ -45,74 +45,75 @@ __device__ __forceinline__ float as_f32(__bf16 v) { return (float)v; }
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// exponent e with max * 2^e in [2^14, 2^15) from the partial maxima (bit patterns) of amax_kernel; 0 for an all-zero matrix
-__device__ __forceinline__ int split_exponent(const uint32_t *part)
+// exponent e with max * 2^e in [2^14, 2^15) for a finite maximum (a subnormal one counts as 2^-126: scaled to at most 2^14, which is as
+// exact); a tile of zeros gets the largest, so that it never is the reference of a sum
+__device__ __forceinline__ int split_exponent(float top)
 {
-    uint32_t m = 0;
-    for (int i = 0; i < AMAX_BLOCKS; i += 64) m = max(m, part[i + (threadIdx.x & 63)]);
-    for (int o = 32; o; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    if (m == 0) return 0;
-    // a subnormal maximum counts as 2^-126: it is scaled to at most 2^14, which is as exact
-    const int e = m < 0x00800000u ? -126 : (int)(m >> 23) - 127;
-    return 14 - e;
+    const uint32_t m = __float_as_uint(top);
+    if (m == 0) return 140;
+    return 14 - (m < 0x00800000u ? -126 : (int)(m >> 23) - 127);
 }
 
-// v * 2^e for any e in [-113, 140]
-__device__ __forceinline__ float scale_pow2(float v, int e) { return ldexpf(v, e); }
+// One block of sums d (16 of a lane's own S row) into the running maximum m (of c d) and the sum of 2^(c d - m); c > 0, so the
+// largest d gives the largest exponent.
+__device__ __forceinline__ void online(const v16f &d, float c, float &m, float &sum)
+{
+    float high = d[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) high = fmaxf(high, d[r]);
+    // at least the lowest finite number, so that a block of -inf adds zeros; NaN in d reaches the sum through its own exponential
+    const float top = fmaxf(m, high * c);
+    float add = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) add += exp2_raw(fmaf(d[r], c, -top));
+    sum = fmaf(sum, exp2_raw(m - top), add);
+    m = top;
+}
 
 }  // namespace
 
 // ---------------------------------------------------------------------------- preparation
 
-// Largest finite magnitude of a matrix, one partial maximum a workgroup; `row_factor` multiplies each row (G x).
-template <typename T>
-__global__ __launch_bounds__(256) void amax_kernel(const T *src, int64_t rows, int k, int64_t ld, const float *row_factor, uint32_t *part)
-{
-    __shared__ uint32_t lds[4];
-    uint32_t m = 0;
-    const int lane = threadIdx.x & 63;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    for (int64_t r = wave; r < rows; r += (int64_t)AMAX_BLOCKS * 4) {
-        const float f = row_factor ? row_factor[r] : 1.f;
-        for (int c = lane; c < k; c += 64) {
-            const uint32_t b = __float_as_uint(as_f32(src[r * ld + c]) * f) & 0x7fffffffu;
-            if (b < 0x7f800000u) m = max(m, b);
-        }
-    }
-    for (int o = 32; o; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    if (lane == 0) lds[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = max(max(lds[0], lds[1]), max(lds[2], lds[3]));
-}
-
 // A matrix in the order the matrix instructions read it, 32 rows a workgroup, zeros behind the last row and column:
 //   f1 [tile][part][KP / 16][lane][8]: row lane % 32, columns 16 s + 8 (lane / 32) + 0..7                 (first product)
 //   f2 [tile][part][KP / 32][2][lane][8]: column 32 kb + lane % 32, rows 16 c + 8 (j / 4) + 4 (lane / 32) + j % 4   (second)
+//   exps [tile]: the tile's exponent (split operands); infinities and NaN do not count for it and stay what they are
+// `row_factor` multiplies each row (G x).  Memory-bound: one read, one write for each order.
 template <typename T, int NS>
-__global__ __launch_bounds__(256) void fragments_kernel(const T *src, int64_t rows, int k, int64_t ld, const float *row_factor,
-                                                        const uint32_t *amax, int KP, uint4 *f1, uint4 *f2)
+__global__ __launch_bounds__(256) void fragments_kernel(const T *src, int64_t rows, int k, int64_t ld, const float *row_factor, int KP, int *exps, uint4 *f1,
+                                                        uint4 *f2)
 {
     extern __shared__ float tile[];                   // [32][KP + 1]
-    const int W = KP + 1;
+    __shared__ float tops[4];
+    const int W = KP + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t r0 = (int64_t)blockIdx.x * 32;
-    const int e = NS == 2 ? split_exponent(amax) : 0;
-    for (int i = threadIdx.x; i < 32 * KP; i += 256) {
-        const int r = i / KP, c = i - r * KP;
-        float v = 0.f;
-        if (r0 + r < rows && c < k) {
-            v = as_f32(src[(r0 + r) * ld + c]);
-            if (row_factor) v *= row_factor[r0 + r];
-            if (NS == 2) v = scale_pow2(v, e);
+    float top = 0.f;
+    for (int r = wave; r < 32; r += 4) {
+        const bool in = r0 + r < rows;
+        const float f = in && row_factor ? row_factor[r0 + r] : 1.f;
+        for (int c = lane; c < KP; c += 64) {
+            float v = in && c < k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
+            if (row_factor) v *= f;
+            tile[r * W + c] = v;
+            if (NS == 2 && fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
         }
-        tile[r * W + c] = v;
+    }
+    if (NS == 2) {
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if (lane == 0) tops[wave] = top;
     }
     __syncthreads();
+    int e = 0;
+    if (NS == 2) {
+        e = split_exponent(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+        if (threadIdx.x == 0) exps[blockIdx.x] = e;
+    }
     for (int which = 0; which < 2; ++which) {
         uint4 *f = which ? f2 : f1;
         if (!f) continue;
         const int per = KP / 16 * 64;                 // 16-byte pieces of one part of a tile
         for (int i = threadIdx.x; i < per; i += 256) {
-            const int lane = i & 63, s = i >> 6, q = lane & 31, h = lane >> 5;
+            const int l = i & 63, s = i >> 6, q = l & 31, h = l >> 5;
             float v[8];
             for (int j = 0; j < 8; ++j) {
                 const int r = which ? 16 * (s & 1) + 8 * (j >> 2) + 4 * h + (j & 3) : q;
@@ -126,8 +127,9 @@ __global__ __launch_bounds__(256) void fragments_kernel(const T *src, int64_t ro
             } else {
                 h8 hi, lo;
                 for (int j = 0; j < 8; ++j) {
-                    hi[j] = (_Float16)v[j];
-                    lo[j] = (_Float16)(v[j] - (float)hi[j]);
+                    const float x = ldexpf(v[j], e);
+                    hi[j] = (_Float16)x;
+                    lo[j] = (_Float16)(x - (float)hi[j]);
                 }
                 f[((int64_t)blockIdx.x * 2) * per + i] = __builtin_bit_cast(uint4, hi);
                 f[((int64_t)blockIdx.x * 2 + 1) * per + i] = __builtin_bit_cast(uint4, lo);
@@ -137,9 +139,10 @@ __global__ __launch_bounds__(256) void fragments_kernel(const T *src, int64_t ro
 }
 
 // Per-row terms in powers of two: the item side scale log2(e) b_i, the user side -log2(e) lse_u; -inf behind the last row.
-__global__ __launch_bounds__(256) void item_terms_kernel(const float *ibase, int64_t n, int64_t padded, float c, float *out)
+__global__ __launch_bounds__(256) void item_terms_kernel(const float *ibase, int64_t n, int64_t padded, float c, float *out, uint8_t *named)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (named && i < padded && (i & 63) == 0) named[i >> 6] = 0;
     if (i < padded) out[i] = i < n ? (ibase ? ibase[i] * c : 0.f) : -INFINITY;
 }
 
@@ -159,21 +162,49 @@ __global__ __launch_bounds__(256) void user_terms_kernel(const float *lse, const
     G[u] = g;
 }
 
+// The places as one list in (user, place) order, padded with empty ones: what the gradient of V looks its items up in.  `named` was
+// cleared by item_terms_kernel; whoever sets a byte sets it to the same.
+__global__ __launch_bounds__(256) void places_kernel(const int32_t *ids, int64_t m, int64_t ld_ids, int64_t n, int64_t n_items, int64_t padded, int32_t *list,
+                                                     uint8_t *named)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < padded; i += (int64_t)gridDim.x * 256) {
+        const uint32_t u = (uint32_t)i / (uint32_t)m;                           // at most 2^32 places
+        const int32_t id = i < n * m ? ids[u * ld_ids + (i - u * m)] : -1;
+        list[i] = id;
+        if (id >= 0 && id < n_items) named[id >> 6] = 1;
+    }
+}
+
 // ---------------------------------------------------------------------------- the walk
 
-enum { WALK_STATS = 0, WALK_GRAD = 1 };
+enum { WALK_STATS = 0, WALK_GRAD = 1, WALK_GRAD_BASE = 2 };     // ..._BASE: with the sums for the gradient of the bases
+
+// What the gradient of V needs to finish its rows in the kernel that summed them (one split): see finish_rows.
+struct Finish {
+    const int32_t *places;             // [n_places, padded to 1024]: items named, in (user, place) order
+    const uint8_t *named;              // [n_items / 64]: whether one of 64 items is
+    const void *X;                     // [n][ldx]
+    const float *dlogp;
+    void *dV;                          // [n_items][ld_dv] or null
+    float *db;                         // [n_items] or null
+    int64_t n_places, m, ldx, ld_dlogp, ld_dv, n_items;
+    int k;
+    float scale;
+    int vec_x;                         // rows of X are aligned for loads of four columns, k a multiple of four
+};
 
 struct WalkParams {
     const uint4 *s_f1, *t_f1, *t_f2;
     const float *s_term, *t_term;      // powers of two added to the score (see item_terms_kernel, user_terms_kernel)
-    const float *t_factor;             // WALK_GRAD: sum_t factor P -> out_b, or null
-    const uint32_t *s_amax, *t_amax;   // split operands: their exponents
+    const float *t_factor;             // WALK_GRAD_BASE: sum_t factor P -> out_b
+    const int *s_exp, *t_exp, *t2_exp; // split operands: exponents of their tiles
     float c;                           // scale log2(e)
-    int t_tiles, tiles_per_split;
+    int s_blocks, splits, t_tiles, tiles_per_split;
     int64_t s_padded;
     float *out_m, *out_s;              // WALK_STATS: [splits][s_padded]
-    float *out_acc;                    // WALK_GRAD: [splits][s_padded][KP]
+    float *out_acc;                    // WALK_GRAD: [splits][s_padded][KP], or null: finish
     float *out_b;                      // ... [splits][s_padded]
+    Finish f;
 };
 
 template <int NS>
@@ -183,333 +214,773 @@ __device__ __forceinline__ v16f product(uint4 a, uint4 b, v16f d)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), d, 0, 0, 0);
 }
 
-template <int KP, int NS, int MODE>
-__global__ __launch_bounds__(256, KP * NS <= 256 ? 2 : 1) void walk_kernel(WalkParams p)
+// 64 floats (one wave), and PIECES 16-byte pieces, from memory to LDS without a stop in registers; the caller waits for them
+__device__ __forceinline__ void fetch_row(const float *from, float *to)
 {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + (threadIdx.x & 63)),
+                                     (__attribute__((address_space(3))) void *)to, 4, 0, 0);
+}
+
+template <int PIECES>
+__device__ __forceinline__ void fetch(const uint4 *from, uint4 *to)
+{
+    static_assert(PIECES % 64 == 0, "whole waves");
+#pragma unroll
+    for (int i = 0; i < (PIECES + 255) / 256; ++i) {
+        const int at = i * 256 + (int)(threadIdx.x & ~63u);
+        if (PIECES % 256 == 0 || at < PIECES)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + at + (threadIdx.x & 63)),
+                                             (__attribute__((address_space(3))) void *)(to + at), 16, 0, 0);
+    }
+}
+
+// asks the scheduler for LDS reads six ahead of the matrix instructions that use them
+template <int READS, int PRODUCTS>
+__device__ __forceinline__ void reads_ahead()
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, READS < 6 ? READS : 6, 0);
+#pragma unroll
+    for (int i = 6; i < READS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / READS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+}
+
+// places a workgroup keeps of those it looks through: their list and its sorted order fit a stage of walk_kernel
+constexpr int list_length(int KP) { return KP >= 128 ? 4096 : KP >= 64 ? 2048 : 1024; }
+
+// four columns of a row, zeros behind its end
+template <typename T>
+__device__ __forceinline__ void load4(const T *row, int c, int k, bool vec, float v[4])
+{
+    if (vec) {
+        if (sizeof(T) == 4) {
+            const float4 a = *(const float4 *)(row + c);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        } else {
+            const uint2 a = *(const uint2 *)(row + c);
+            v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
+            v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+        }
+    } else {
+        for (int j = 0; j < 4; ++j) v[j] = c + j < k ? as_f32(row[c + j]) : 0.f;
+    }
+}
+
+// The last steps of dV for 64 S rows, whose sums lie in LDS as rows[local][KP]: adds g x of every place that names one of the
+// items, scales, rounds and stores.  Each wave looks through a quarter of the places in order and lists those it wants, until its list
+// is full or the quarter is done; the lists are sorted by item.  The groups of threads (four columns a thread) take equal parts of
+// the sorted order, so that an item that everybody names does not fall to one group; an item's first run in a part is set aside and
+// added after the others, in the parts' order.  Nothing depends on scheduling.
+template <typename T, int KP>
+__device__ void finish_rows(const Finish &f, float *rows, float *row_b, uint32_t *list, int *counts, float *aside, int *aside_item, int64_t i0)
+{
+    constexpr int LIST = list_length(KP), CAP = LIST / 4, EACH = CAP / 64, ROWS = 64;
+    constexpr int COLS = KP / 4;                      // threads of a row
+    constexpr int GROUPS = 256 / COLS;
+    uint32_t *order = list + LIST;
+    uint8_t *item_of = (uint8_t *)aside;              // free while the lists are made
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int group = tid / COLS, c4 = (tid % COLS) * 4;
+    const bool vec = f.vec_x;
+    const T *X = (const T *)f.X;
+    const int64_t steps = (f.n_places + 64 * EACH - 1) / (64 * EACH);          // of a wave, over all places
+    int64_t step = steps * wave / 4;
+    const int64_t end = steps * (wave + 1) / 4;
+    bool more = f.n_places > 0 && f.named[i0 >> 6];
+    while (more) {
+        int held = 0;
+        int32_t id[EACH], next[EACH];
+        auto load = [&](int64_t at, int32_t *to) {
+            const int4 *src = (const int4 *)f.places + at * 64 * (EACH / 4) + lane;
+#pragma unroll
+            for (int q = 0; q < EACH / 4; ++q) *(int4 *)(to + 4 * q) = src[q * 64];
+        };
+        if (step < end) load(step, id);
+        while (step < end) {
+            if (step + 1 < end) load(step + 1, next);
+            int mine = 0;
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) {
+                if (id[q] >= f.n_items) id[q] = -1;   // behind the catalogue: no row takes it
+                mine += (uint64_t)((int64_t)id[q] - i0) < (uint64_t)ROWS;
+            }
+            if (__ballot(mine)) {
+                int before = mine;
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int v = __shfl_up(before, o);
+                    if (lane >= o) before += v;
+                }
+                const int all = __shfl(before, 63);
+                if (held + all > CAP) break;          // next time: a step alone always fits
+                before += held - mine;
+                if (mine) {
+#pragma unroll
+                    for (int q = 0; q < EACH; ++q) {
+                        const int64_t local = (int64_t)id[q] - i0;
+                        if ((uint64_t)local < (uint64_t)ROWS) {
+                            item_of[wave * CAP + before] = (uint8_t)local;
+                            list[wave * CAP + before++] = (uint32_t)(step * 64 * EACH + (q >> 2) * 256 + lane * 4 + (q & 3));      // at most 2^32 places
+                        }
+                    }
+                }
+                held += all;
+            }
+            ++step;
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) id[q] = next[q];
+        }
+        if (lane == 0) counts[wave] = held;
+        more = __syncthreads_or(step < end);
+        int total = 0, offset = 0;
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) offset += counts[w];
+            total += counts[w];
+        }
+        for (int q = lane; q < held; q += 64) order[offset + q] = (uint32_t)item_of[wave * CAP + q] << 12 | (uint32_t)(wave * CAP + q);
+        int size = 1;
+        while (size < total) size <<= 1;
+        for (int q = total + tid; q < size; q += 256) order[q] = ~0u;
+        __syncthreads();
+        for (int w = 2; w <= size; w <<= 1)           // bitonic: keys are unique (item, position)
+            for (int d = w >> 1; d; d >>= 1) {
+                for (int q = tid; q < size / 2; q += 256) {
+                    const int lo = 2 * q - (q & (d - 1)), hi = lo + d;
+                    const uint32_t x = order[lo], y = order[hi];
+                    if ((x > y) == !(lo & w)) { order[lo] = y; order[hi] = x; }
+                }
+                __syncthreads();
+            }
+        if (total) {
+            const int part = (total + GROUPS - 1) / GROUPS, from = group * part, to = min(from + part, total);
+            if (group < GROUPS) {
+                if (c4 == 0) aside_item[group] = -1;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                float ab = 0.f;
+                int item = -1, first = -1;
+                auto flush = [&]() {
+                    if (item < 0) return;
+                    if (item == first) {
+                        *(float4 *)(aside + group * KP + c4) = a;
+                        if (c4 == 0) { aside_item[group] = item; aside[GROUPS * KP + group] = ab; }
+                    } else {
+                        float4 *r = (float4 *)(rows + item * KP + c4);
+                        float4 v = *r;
+                        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+                        *r = v;
+                        if (c4 == 0) row_b[item] += ab;
+                    }
+                };
+                for (int q0 = from; q0 < to; q0 += 8) {
+                    float x[8][4], g[8];
+                    int at[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        at[q] = -1;
+                        if (q0 + q < to) {
+                            const uint32_t key = order[q0 + q], place = list[key & 4095], u = place / (uint32_t)f.m;
+                            at[q] = (int)(key >> 12);
+                            g[q] = f.dlogp[(int64_t)u * f.ld_dlogp + (place - u * (uint32_t)f.m)];
+                            load4(X + (int64_t)u * f.ldx, c4, f.k, vec && c4 < f.k, x[q]);
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        if (at[q] >= 0) {
+                            if (at[q] != item) {
+                                flush();
+                                if (first < 0) first = at[q];
+                                item = at[q];
+                                a = make_float4(0.f, 0.f, 0.f, 0.f);
+                                ab = 0.f;
+                            }
+                            a.x = fmaf(g[q], x[q][0], a.x); a.y = fmaf(g[q], x[q][1], a.y);
+                            a.z = fmaf(g[q], x[q][2], a.z); a.w = fmaf(g[q], x[q][3], a.w);
+                            ab += g[q];
+                        }
+                }
+                flush();
+            }
+            __syncthreads();
+            for (int g = 0; g < GROUPS; ++g) {
+                const int item = aside_item[g];
+                if (item < 0) continue;
+                for (int c = tid; c < KP; c += 256) rows[item * KP + c] += aside[g * KP + c];
+                if (tid == 0) row_b[item] += aside[GROUPS * KP + g];
+            }
+        }
+        __syncthreads();
+    }
+    if (f.dV) {
+        T *out = (T *)f.dV;
+        for (int i = tid; i < ROWS * KP; i += 256) {
+            const int r = i / KP, c = i - r * KP;
+            if (i0 + r < f.n_items && c < f.k) out[(i0 + r) * f.ld_dv + c] = (T)(f.scale * rows[i]);
+        }
+    }
+    if (f.db)
+        for (int r = tid; r < ROWS; r += 256)
+            if (i0 + r < f.n_items) f.db[i0 + r] = f.scale * row_b[r];
+}
+// memory of the sums set aside (one row and one number a group), or a byte for each place of the lists
+constexpr int aside_floats(int KP)
+{
+    const int sums = 256 / (KP / 4) * (KP + 1), bytes = list_length(KP) / 4;
+    return sums > bytes ? sums : bytes;
+}
+
+template <int KP, int NS, int MODE>
+__global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <= 128) ? 2 : 1) void walk_kernel(WalkParams p)
+{
+    typedef typename std::conditional<NS == 2, float, __bf16>::type T;
     constexpr int STEPS = KP / 16;
     constexpr int PART = STEPS * 64;                  // 16-byte pieces of a part of a tile
-    constexpr int TILE = PART * NS * (MODE == WALK_GRAD ? 2 : 1);
-    __shared__ uint4 lds[TILE];
+    constexpr int SUB = NS == 1 ? 2 : 1;              // tiles of 32 rows a stage
+    constexpr int HALF = PART * NS * SUB;
+    constexpr bool GRAD = MODE != WALK_STATS;
+    constexpr int STAGE = HALF * (GRAD ? 2 : 1);
+    // two stages: one is read while the other arrives (two arrays, so that the compiler sees that they are apart)
+    __shared__ uint4 stage0[STAGE], stage1[STAGE];
+    __shared__ float terms0[GRAD ? 128 : 64], terms1[GRAD ? 128 : 64];      // of the stage's T rows: t_term, t_factor
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int64_t s_tile = (int64_t)blockIdx.x * 4 + wave;
+    // workgroups go to the eight XCDs in turn: splits are dealt so that an XCD's L2 sees each part of T from one split only
+    int s_block, split;
+    {
+        const int id = blockIdx.x, whole = p.splits / 8 * 8 * p.s_blocks;
+        if (id < whole) {
+            s_block = (id >> 3) % p.s_blocks;
+            split = (id >> 3) / p.s_blocks * 8 + (id & 7);
+        } else {
+            s_block = (id - whole) % p.s_blocks;
+            split = p.splits / 8 * 8 + (id - whole) / p.s_blocks;
+        }
+    }
+    const int64_t s_tile = (int64_t)s_block * 4 + wave;
     const int64_t s_row = s_tile * 32 + (lane & 31);
 
     uint4 sf[NS][STEPS];
+#pragma unroll
     for (int q = 0; q < NS; ++q)
+#pragma unroll
         for (int s = 0; s < STEPS; ++s) sf[q][s] = p.s_f1[(s_tile * NS + q) * PART + s * 64 + lane];
-    float c = p.c;
-    if (NS == 2) c = fminf(ldexpf(c, -split_exponent(p.s_amax) - split_exponent(p.t_amax)), 3.402823466e38f);
-    // split probabilities sit at 2^15: fp16 then holds them down to 2^-39 of 1
-    const float s_term = (p.s_term ? p.s_term[s_row] : 0.f) + (MODE == WALK_GRAD && NS == 2 ? 15.f : 0.f);
+    const int s_exp = NS == 2 ? p.s_exp[s_tile] : 0;
+    const float s_term = p.s_term ? p.s_term[s_row] : 0.f;
 
-    v16f acc[MODE == WALK_GRAD ? KP / 32 : 1] = {};
+    v16f acc[GRAD ? KP / 32 : 1] = {};
     float m = -3.402823466e38f, sum = 0.f, b_sum = 0.f;
+    int ref = 140;                                    // exponent of acc (split operands), the least of the tiles so far
 
-    const int first = blockIdx.y * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
-    for (int t = first; t < last; ++t) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < PART * NS; i += 256) lds[i] = p.t_f1[(int64_t)t * PART * NS + i];
-        if (MODE == WALK_GRAD)
-            for (int i = threadIdx.x; i < PART * NS; i += 256) lds[PART * NS + i] = p.t_f2[(int64_t)t * PART * NS + i];
-        __syncthreads();
-        v16f d = {};
-        for (int s = 0; s < STEPS; ++s) {
-            const uint4 a = lds[s * 64 + lane];
-            d = product<NS>(a, sf[0][s], d);
-            if (NS == 2) {
-                d = product<NS>(a, sf[NS - 1][s], d);
-                d = product<NS>(lds[PART + s * 64 + lane], sf[0][s], d);
-            }
-        }
-        float z[16];
-        for (int q = 0; q < 4; ++q) {
-            const float4 tt = *(const float4 *)(p.t_term + (int64_t)t * 32 + 8 * q + 4 * h);
-            z[4 * q] = fmaf(d[4 * q], c, tt.x); z[4 * q + 1] = fmaf(d[4 * q + 1], c, tt.y);
-            z[4 * q + 2] = fmaf(d[4 * q + 2], c, tt.z); z[4 * q + 3] = fmaf(d[4 * q + 3], c, tt.w);
-        }
-        if (MODE == WALK_STATS) {
-            float top = m;
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, z[r]);
-            float add = 0.f;
-            for (int r = 0; r < 16; ++r) add += exp2_raw(z[r] - top);
-            sum = fmaf(sum, exp2_raw(m - top), add);
-            m = top;
-        } else {
-            float P[16];
-            for (int r = 0; r < 16; ++r) P[r] = exp2_raw(z[r] + s_term);
-            if (p.t_factor)
-                for (int q = 0; q < 4; ++q) {
-                    const float4 g = *(const float4 *)(p.t_factor + (int64_t)t * 32 + 8 * q + 4 * h);
-                    b_sum = fmaf(P[4 * q], g.x, b_sum); b_sum = fmaf(P[4 * q + 1], g.y, b_sum);
-                    b_sum = fmaf(P[4 * q + 2], g.z, b_sum); b_sum = fmaf(P[4 * q + 3], g.w, b_sum);
+    const int first = split * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
+
+    auto fetch_stage = [&](int t, uint4 *to, float *terms) {
+        fetch<HALF>(p.t_f1 + (int64_t)t * PART * NS, to);
+        if (GRAD) fetch<HALF>(p.t_f2 + (int64_t)t * PART * NS, to + HALF);
+        if (wave == 0) fetch_row(p.t_term + (int64_t)t * 32, terms);
+        if (MODE == WALK_GRAD_BASE && wave == 1) fetch_row(p.t_factor + (int64_t)t * 32, terms + 64);
+    };
+    auto compute = [&](int t0, const uint4 *lds, const float *terms) {
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub) {
+            const int t = t0 + sub;
+            const uint4 *l1 = lds + sub * PART * NS, *l2 = lds + HALF + sub * PART * NS;
+            float4 tt[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tt[q] = *(const float4 *)(terms + sub * 32 + 8 * q + 4 * h);
+            float c = p.c;
+            if (NS == 2) c = fminf(ldexpf(c, -s_exp - p.t_exp[t]), 3.402823466e38f);
+            v16f d = {};
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const uint4 a = l1[s * 64 + lane];
+                d = product<NS>(a, sf[0][s], d);
+                if (NS == 2) {
+                    d = product<NS>(a, sf[NS - 1][s], d);
+                    d = product<NS>(l1[PART + s * 64 + lane], sf[0][s], d);
                 }
-            uint4 pf[NS][2];
-            for (int e = 0; e < 2; ++e) {
-                if (NS == 1) {
-                    b8 o;
-                    for (int j = 0; j < 8; ++j) o[j] = (__bf16)P[8 * e + j];
-                    pf[0][e] = __builtin_bit_cast(uint4, o);
-                } else {
-                    h8 hi, lo;
-                    for (int j = 0; j < 8; ++j) {
-                        hi[j] = (_Float16)P[8 * e + j];
-                        lo[j] = (_Float16)(P[8 * e + j] - (float)hi[j]);
+            }
+            reads_ahead<STEPS * NS, STEPS * (2 * NS - 1)>();
+            float z[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                z[4 * q] = fmaf(d[4 * q], c, tt[q].x); z[4 * q + 1] = fmaf(d[4 * q + 1], c, tt[q].y);
+                z[4 * q + 2] = fmaf(d[4 * q + 2], c, tt[q].z); z[4 * q + 3] = fmaf(d[4 * q + 3], c, tt[q].w);
+            }
+            if (MODE == WALK_STATS) {
+                float top = m;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, z[r]);
+                float add = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) add += exp2_raw(z[r] - top);
+                sum = fmaf(sum, exp2_raw(m - top), add);
+                m = top;
+            } else {
+                // split probabilities are scaled to 2^15: fp16 then holds them down to 2^-39; tiles of T with a larger exponent than
+                // the reference take that off here, one with a smaller becomes the reference
+                int up = 0;
+                if (NS == 2) {
+                    const int e = p.t2_exp[t];
+                    if (e < ref) {
+                        const float f = ldexpf(1.f, e - ref);
+                        for (int kb = 0; kb < KP / 32; ++kb) acc[kb] *= f;
+                        ref = e;
                     }
-                    pf[0][e] = __builtin_bit_cast(uint4, hi);
-                    pf[NS - 1][e] = __builtin_bit_cast(uint4, lo);
+                    up = 15 - (e - ref);
                 }
-            }
-            const uint4 *l2 = lds + PART * NS;
-            for (int kb = 0; kb < KP / 32; ++kb)
+                const float add = s_term + (float)up;
+                float P[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) P[r] = exp2_raw(z[r] + add);
+                if (MODE == WALK_GRAD_BASE) {
+                    float b = 0.f;
+                    float4 tg[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) tg[q] = *(const float4 *)(terms + 64 + sub * 32 + 8 * q + 4 * h);
+                    if (NS == 2 && up < -20) {        // a tile far below the reference: its probabilities as they are
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float4 g = tg[r >> 2];
+                            b = fmaf(exp2_raw(z[r] + s_term), (r & 3) == 0 ? g.x : (r & 3) == 1 ? g.y : (r & 3) == 2 ? g.z : g.w, b);
+                        }
+                        b_sum += b;
+                    } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        b = fmaf(P[4 * q], tg[q].x, b); b = fmaf(P[4 * q + 1], tg[q].y, b);
+                        b = fmaf(P[4 * q + 2], tg[q].z, b); b = fmaf(P[4 * q + 3], tg[q].w, b);
+                    }
+                    b_sum += NS == 2 ? ldexpf(b, -up) : b;
+                    }
+                }
+                uint4 pf[NS][2];
+#pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint4 a = l2[(kb * 2 + e) * 64 + lane];
-                    acc[kb] = product<NS>(a, pf[0][e], acc[kb]);
-                    if (NS == 2) {
-                        acc[kb] = product<NS>(a, pf[NS - 1][e], acc[kb]);
-                        acc[kb] = product<NS>(l2[PART + (kb * 2 + e) * 64 + lane], pf[0][e], acc[kb]);
+                    if (NS == 1) {
+                        b8 o;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) o[j] = (__bf16)P[8 * e + j];
+                        pf[0][e] = __builtin_bit_cast(uint4, o);
+                    } else {
+                        h8 hi, lo;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            hi[j] = (_Float16)P[8 * e + j];
+                            lo[j] = (_Float16)(P[8 * e + j] - (float)hi[j]);
+                        }
+                        pf[0][e] = __builtin_bit_cast(uint4, hi);
+                        pf[NS - 1][e] = __builtin_bit_cast(uint4, lo);
                     }
                 }
+#pragma unroll
+                for (int kb = 0; kb < KP / 32; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint4 a = l2[(kb * 2 + e) * 64 + lane];
+                        acc[kb] = product<NS>(a, pf[0][e], acc[kb]);
+                        if (NS == 2) {
+                            acc[kb] = product<NS>(a, pf[NS - 1][e], acc[kb]);
+                            acc[kb] = product<NS>(l2[PART + (kb * 2 + e) * 64 + lane], pf[0][e], acc[kb]);
+                        }
+                    }
+            }
         }
+    };
+    auto arrived = [&]() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+
+    if (first < last) fetch_stage(first, stage0, terms0);
+    for (int t = first; t < last; t += 2 * SUB) {
+        arrived();
+        if (t + SUB < last) fetch_stage(t + SUB, stage1, terms1);
+        compute(t, stage0, terms0);
+        if (t + SUB >= last) break;
+        arrived();
+        if (t + 2 * SUB < last) fetch_stage(t + 2 * SUB, stage0, terms0);
+        compute(t + SUB, stage1, terms1);
     }
-    const int64_t at = (int64_t)blockIdx.y * p.s_padded + s_row;
+
+    const int64_t at = (int64_t)split * p.s_padded + s_row;
     if (MODE == WALK_STATS) {
         // lane and lane + 32 hold the same S row
         const float m2 = __shfl_xor(m, 32), s2 = __shfl_xor(sum, 32), top = fmaxf(m, m2);
         sum = sum * exp2_raw(m - top) + s2 * exp2_raw(m2 - top);
         if (h == 0) { p.out_m[at] = top; p.out_s[at] = sum; }
-    } else {
-        float unit = 1.f;
-        if (NS == 2) unit = ldexpf(1.f, -15);
-        if (p.out_b) {
-            b_sum += __shfl_xor(b_sum, 32);
-            if (h == 0) p.out_b[at] = b_sum * unit;
-        }
+        return;
+    }
+    const float unit = NS == 2 ? ldexpf(1.f, -15 - ref) : 1.f;
+    b_sum += __shfl_xor(b_sum, 32);
+    if (p.out_acc) {
+        if (p.out_b && h == 0) p.out_b[at] = b_sum;
         for (int kb = 0; kb < KP / 32; ++kb)
             for (int q = 0; q < 4; ++q)
                 *(float4 *)(p.out_acc + at * KP + kb * 32 + 8 * q + 4 * h) =
                     make_float4(acc[kb][4 * q] * unit, acc[kb][4 * q + 1] * unit, acc[kb][4 * q + 2] * unit, acc[kb][4 * q + 3] * unit);
+        return;
+    }
+    // one split: the rows are finished here, 64 a time (waves 0 and 1, then 2 and 3), their sums in the first stage's memory
+    __shared__ float row_b[64], aside[aside_floats(KP)];
+    __shared__ int counts[4], aside_item[32];
+    static_assert(MODE == WALK_STATS || STAGE * 16 >= 64 * KP * 4, "a stage holds 64 rows of sums");
+    static_assert(MODE == WALK_STATS || STAGE * 16 >= list_length(KP) * 8, "a stage holds a list and its order");
+    float *rows = (float *)stage0;
+    for (int half = 0; half < 2; ++half) {
+        __syncthreads();
+        if ((wave >> 1) == half) {
+            const int r = (wave & 1) * 32 + (lane & 31);
+            for (int kb = 0; kb < KP / 32; ++kb)
+                for (int q = 0; q < 4; ++q)
+                    *(float4 *)(rows + r * KP + kb * 32 + 8 * q + 4 * h) =
+                        make_float4(-acc[kb][4 * q] * unit, -acc[kb][4 * q + 1] * unit, -acc[kb][4 * q + 2] * unit, -acc[kb][4 * q + 3] * unit);
+            if (h == 0) row_b[r] = -b_sum;
+        }
+        __syncthreads();
+        finish_rows<T, KP>(p.f, rows, row_b, (uint32_t *)stage1, counts, aside, aside_item, (int64_t)s_block * S_ROWS + half * 64);
     }
 }
 
-// The same statistics from 4-bit operands: a lane of the instruction reads one block of 32 and its scale from memory.
-__global__ __launch_bounds__(256) void walk_mx_kernel(const uint8_t *xc, const uint8_t *xs, int64_t n, const uint8_t *vc, const uint8_t *vs, int64_t n_items,
-                                                      int kb, const float *t_term, float c, int t_tiles, int tiles_per_split, int64_t s_padded,
-                                                      float *out_m, float *out_s)
+// The statistics for few users, straight from V as it lies in memory: a wave takes 16 items at a time, its lanes 16 rows by four
+// pieces of 16 bytes, which are the A operands of the 16 x 16 instructions (fp32: 16x16x4, a piece feeds four of them; bf16: 16x16x32).
+// The order of the factors is the same in X's operand, so it does not matter.  V is read once for 16 UT users, the next tile's rows
+// are on their way while one is computed: HBM-bound.
+struct DirectParams {
+    const void *X, *V;
+    const float *ibase;
+    int64_t ldx, ldv, n, n_items, s_padded;
+    int k;
+    float c;
+    float *out_m, *out_s;              // [workgroups][s_padded]
+};
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 piece(const T *row, int c, int k)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int64_t s_row = ((int64_t)blockIdx.x * 4 + wave) * 32 + (lane & 31);
-    const int64_t u = min(s_row, n - 1);
-    const int steps = (kb + 1) / 2;
-    float m = -3.402823466e38f, sum = 0.f;
-    const int first = blockIdx.y * tiles_per_split, last = min(first + tiles_per_split, t_tiles);
-    for (int t = first; t < last; ++t) {
-        const int64_t item = min((int64_t)t * 32 + (lane & 31), n_items - 1);
-        v16f d = {};
-        for (int s = 0; s < steps; ++s) {
-            const int b = 2 * s + h;
-            v8i a = {}, w = {};
-            int sa = 127, sw = 127;
-            if (b < kb) {
-                const uint4 ca = *(const uint4 *)(vc + (item * kb + b) * 16), cw = *(const uint4 *)(xc + (u * kb + b) * 16);
-                a[0] = ca.x; a[1] = ca.y; a[2] = ca.z; a[3] = ca.w;
-                w[0] = cw.x; w[1] = cw.y; w[2] = cw.z; w[3] = cw.w;
-                sa = vs[item * kb + b];
-                sw = xs[u * kb + b];
+    constexpr int N = 16 / sizeof(T);
+    if (VEC) return c < k ? *(const uint4 *)(row + c) : make_uint4(0, 0, 0, 0);
+    T v[N];
+    for (int j = 0; j < N; ++j) v[j] = c + j < k ? row[c + j] : (T)0.f;
+    uint4 o;
+    __builtin_memcpy(&o, v, 16);
+    return o;
+}
+
+template <typename T, int KP, int UT, bool VEC>
+__global__ __launch_bounds__(256) void direct_kernel(DirectParams p)
+{
+    constexpr int N = 16 / sizeof(T), STEPS = KP / (4 * N);
+    __shared__ float lm[4][UT * 16], ls[4][UT * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int64_t u0 = (int64_t)blockIdx.y * UT * 16;
+    const T *X = (const T *)p.X, *V = (const T *)p.V;
+    uint4 b[UT][STEPS];
+#pragma unroll
+    for (int t = 0; t < UT; ++t)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) b[t][s] = piece<T, VEC>(X + min(u0 + t * 16 + r, p.n - 1) * p.ldx, (s * 4 + g) * N, p.k);
+    float m[UT], sum[UT];
+    for (int t = 0; t < UT; ++t) { m[t] = -3.402823466e38f; sum[t] = 0.f; }
+    const int64_t tiles = (p.n_items + 15) / 16, stride = (int64_t)gridDim.x * 4;
+    int64_t i = (int64_t)blockIdx.x * 4 + wave;
+    uint4 a[STEPS];
+    float base[4];
+    auto load = [&](int64_t tile, uint4 *to, float *bases) {
+        const T *row = V + min(tile * 16 + r, p.n_items - 1) * p.ldv;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) to[s] = piece<T, VEC>(row, (s * 4 + g) * N, p.k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t item = tile * 16 + 4 * g + e;
+            bases[e] = item < p.n_items ? (p.ibase ? p.ibase[item] * p.c : 0.f) : -INFINITY;
+        }
+    };
+    if (i < tiles) load(i, a, base);
+    for (; i < tiles; i += stride) {
+        uint4 next[STEPS];
+        float next_base[4];
+        if (i + stride < tiles) load(i + stride, next, next_base);
+#pragma unroll
+        for (int t = 0; t < UT; ++t) {
+            v4f d = {};
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                if (sizeof(T) == 4) {
+                    const v4f x = __builtin_bit_cast(v4f, a[s]), y = __builtin_bit_cast(v4f, b[t][s]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], d, 0, 0, 0);
+                } else {
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a[s]), __builtin_bit_cast(b8, b[t][s]), d, 0, 0, 0);
+                }
             }
-            d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, w, d, 4, 4, 0, sa, 0, sw);
+            float z[4], top = m[t];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { z[e] = fmaf(d[e], p.c, base[e]); top = fmaxf(top, z[e]); }
+            float add = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add += exp2_raw(z[e] - top);
+            sum[t] = fmaf(sum[t], exp2_raw(m[t] - top), add);
+            m[t] = top;
         }
-        float z[16], top = m;
-        for (int q = 0; q < 4; ++q) {
-            const float4 tt = *(const float4 *)(t_term + (int64_t)t * 32 + 8 * q + 4 * h);
-            z[4 * q] = fmaf(d[4 * q], c, tt.x); z[4 * q + 1] = fmaf(d[4 * q + 1], c, tt.y);
-            z[4 * q + 2] = fmaf(d[4 * q + 2], c, tt.z); z[4 * q + 3] = fmaf(d[4 * q + 3], c, tt.w);
-        }
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, z[r]);
-        float add = 0.f;
-        for (int r = 0; r < 16; ++r) add += exp2_raw(z[r] - top);
-        sum = fmaf(sum, exp2_raw(m - top), add);
-        m = top;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) a[s] = next[s];
+        for (int e = 0; e < 4; ++e) base[e] = next_base[e];
     }
-    const float m2 = __shfl_xor(m, 32), s2 = __shfl_xor(sum, 32), top = fmaxf(m, m2);
-    sum = sum * exp2_raw(m - top) + s2 * exp2_raw(m2 - top);
-    if (h == 0) { out_m[(int64_t)blockIdx.y * s_padded + s_row] = top; out_s[(int64_t)blockIdx.y * s_padded + s_row] = sum; }
+#pragma unroll
+    for (int t = 0; t < UT; ++t) {
+        for (int o = 16; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(m[t], o), s2 = __shfl_xor(sum[t], o), top = fmaxf(m[t], m2);
+            sum[t] = sum[t] * exp2_raw(m[t] - top) + s2 * exp2_raw(m2 - top);
+            m[t] = top;
+        }
+        if (g == 0) { lm[wave][t * 16 + r] = m[t]; ls[wave][t * 16 + r] = sum[t]; }
+    }
+    __syncthreads();
+    if (threadIdx.x < UT * 16) {
+        const int q = threadIdx.x;
+        const float top = fmaxf(fmaxf(lm[0][q], lm[1][q]), fmaxf(lm[2][q], lm[3][q]));
+        const float all = (ls[0][q] * exp2_raw(lm[0][q] - top) + ls[1][q] * exp2_raw(lm[1][q] - top)) +
+                          (ls[2][q] * exp2_raw(lm[2][q] - top) + ls[3][q] * exp2_raw(lm[3][q] - top));
+        p.out_m[blockIdx.x * p.s_padded + u0 + q] = top;
+        p.out_s[blockIdx.x * p.s_padded + u0 + q] = all;
+    }
+}
+
+// The same statistics from 4-bit operands: a lane of the instruction holds one block of 32 of a row and its scale, as it lies in
+// memory.  A wave keeps UT tiles of 32 users (B operand) and walks item tiles of 32, the next one's codes on their way; the bases are
+// the initial value of the sums.  Bound by the exponentials (v_exp_f32 at a quarter of the rate of the rest).
+struct MxWalkParams {
+    const uint8_t *xc, *xs, *vc, *vs;
+    const float *base;                 // [t_tiles * 32]: ibase, -inf behind the last item
+    int64_t n, n_items, s_padded;
+    int kb, t_tiles, tiles_per_split;
+    float c;
+    float *out_m, *out_s;
+};
+
+template <int STEPS, int UT>
+__global__ __launch_bounds__(256) void walk_mx_kernel(MxWalkParams p)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    const int64_t s0 = (int64_t)blockIdx.x * 32 * UT;
+    v8i x[UT][STEPS];
+    int sx[UT][STEPS];
+    auto block_of = [&](const uint8_t *codes, const uint8_t *scales, int64_t row, int s, uint4 *c, int *scale) {
+        const int b = 2 * s + h;
+        *c = make_uint4(0, 0, 0, 0);
+        *scale = 127;
+        if (b < p.kb) {
+            *c = *(const uint4 *)(codes + (row * p.kb + b) * 16);
+            *scale = scales[row * p.kb + b];
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < UT; ++t)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            uint4 c;
+            block_of(p.xc, p.xs, min(s0 + t * 32 + r, p.n - 1), s, &c, &sx[t][s]);
+            x[t][s] = v8i{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
+        }
+    float m[UT], sum[UT];
+#pragma unroll
+    for (int t = 0; t < UT; ++t) { m[t] = -3.402823466e38f; sum[t] = 0.f; }
+    const int split = blockIdx.y * 4 + wave;          // each wave walks items of its own
+    const int first = split * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
+    uint4 a[STEPS];
+    int sa[STEPS];
+    float4 base[4];
+    auto load = [&](int t, uint4 *to, int *scale, float4 *bases) {
+        const int64_t item = min((int64_t)t * 32 + r, p.n_items - 1);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) block_of(p.vc, p.vs, item, s, &to[s], &scale[s]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) bases[q] = *(const float4 *)(p.base + (int64_t)t * 32 + 8 * q + 4 * h);
+    };
+    if (first < last) load(first, a, sa, base);
+    for (int t = first; t < last; ++t) {
+        uint4 a2[STEPS];
+        int sa2[STEPS];
+        float4 base2[4];
+        if (t + 1 < last) load(t + 1, a2, sa2, base2);
+        v8i w[STEPS];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) w[s] = v8i{(int)a[s].x, (int)a[s].y, (int)a[s].z, (int)a[s].w, 0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < UT; ++u) {
+            v16f d;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { d[4 * q] = base[q].x; d[4 * q + 1] = base[q].y; d[4 * q + 2] = base[q].z; d[4 * q + 3] = base[q].w; }
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[s], x[u][s], d, 4, 4, 0, sa[s], 0, sx[u][s]);
+            online(d, p.c, m[u], sum[u]);
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) { a[s] = a2[s]; sa[s] = sa2[s]; }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) base[q] = base2[q];
+    }
+#pragma unroll
+    for (int u = 0; u < UT; ++u) {
+        const float top0 = m[u] , m2 = __shfl_xor(top0, 32), s2 = __shfl_xor(sum[u], 32), top = fmaxf(top0, m2);
+        const float all = sum[u] * exp2_raw(top0 - top) + s2 * exp2_raw(m2 - top);
+        const int64_t at = (int64_t)split * p.s_padded + s0 + u * 32 + r;
+        if (h == 0) { p.out_m[at] = top; p.out_s[at] = all; }
+    }
 }
 
 // ---------------------------------------------------------------------------- joins
 
-// lse from the splits' maxima and sums
-__global__ __launch_bounds__(256) void join_lse_kernel(const float *m, const float *s, int splits, int64_t n, int64_t s_padded, float *lse)
-{
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (u >= n) return;
-    float top = -3.402823466e38f, sum = 0.f;
-    bool nan = false;
-    for (int q = 0; q < splits; ++q) {
-        const float b = s[q * s_padded + u];
-        nan |= b != b;
-        top = fmaxf(top, m[q * s_padded + u]);
-    }
-    for (int q = 0; q < splits; ++q) sum += s[q * s_padded + u] * exp2f(m[q * s_padded + u] - top);
-    lse[u] = nan ? __uint_as_float(0x7fc00000u) : (float)(((double)top + (double)log2f(sum)) * LN2);
-}
-
-// logp of the named items: 16 lanes a place, the score as one fp32 sum over the factors
-template <typename T>
-__global__ __launch_bounds__(256) void targets_kernel(const T *X, int64_t ldx, const T *V, int64_t ldv, const float *ibase, int k, int64_t n_items, float scale,
-                                                      const int32_t *ids, int64_t n, int64_t m, int64_t ld_ids, const float *lse, float *logp, int64_t ld_logp)
-{
-    const int l = threadIdx.x & 15;
-    for (int64_t g = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4; g < n * m; g += (int64_t)gridDim.x * 16) {
-        const int64_t u = g / m, j = g - u * m;
-        const int32_t id = ids[u * ld_ids + j];
-        float out = 0.f;
-        if (id >= n_items) out = __uint_as_float(0x7fc00000u);
-        else if (id >= 0) {
-            float d = 0.f;
-            for (int c = l; c < k; c += 16) d = fmaf(as_f32(X[u * ldx + c]), as_f32(V[id * ldv + c]), d);
-            for (int o = 8; o; o >>= 1) d += __shfl_xor(d, o);
-            const float z = scale * (d + (ibase ? ibase[id] : 0.f));
-            const float l0 = lse[u];
-            out = z == -INFINITY && l0 == -INFINITY ? z : z - l0;
-        }
-        if (l == 0) logp[u * ld_logp + j] = out;
-    }
-}
+// What the last kernel of the forward pass reads: the splits' maxima and sums, and the model for the scores of the named items.
+struct Targets {
+    const float *m, *s;
+    int64_t s_padded;
+    int splits, k, kb;
+    const void *X, *V;                 // fp32, bf16, or the codes
+    const uint8_t *xs, *vs;
+    int64_t ldx, ldv, n_items;
+    const float *ibase;
+    float scale;
+    const int32_t *ids;
+    int64_t places, ld_ids, ld_logp;
+    float *lse, *logp;
+};
 
 __device__ __forceinline__ float mx_unit(uint32_t byte)
 {
     return byte == 255 ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
 }
 
-// ... of a 4-bit model: 8 columns a lane and step
-__global__ __launch_bounds__(256) void targets_mx_kernel(const uint8_t *xc, const uint8_t *xs, const uint8_t *vc, const uint8_t *vs, const float *ibase, int kb,
-                                                         int64_t n_items, float scale, const int32_t *ids, int64_t n, int64_t m, int64_t ld_ids,
-                                                         const float *lse, float *logp, int64_t ld_logp)
+// lane l of 16: its share of <x, v>
+template <typename T>
+__device__ __forceinline__ float dot_share(const Targets &t, int64_t u, int64_t id, int l)
 {
-    const int l = threadIdx.x & 15;
-    for (int64_t g = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4; g < n * m; g += (int64_t)gridDim.x * 16) {
-        const int64_t u = g / m, j = g - u * m;
-        const int32_t id = ids[u * ld_ids + j];
+    const T *x = (const T *)t.X + u * t.ldx, *v = (const T *)t.V + id * t.ldv;
+    float d = 0.f;
+#pragma unroll 4
+    for (int c = l; c < t.k; c += 16) d = fmaf(as_f32(x[c]), as_f32(v[c]), d);
+    return d;
+}
+
+// ... of a 4-bit model: 8 columns a lane and step.  Sums of products of the grid are exact, the scales powers of two.
+struct Mx {};
+template <>
+__device__ __forceinline__ float dot_share<Mx>(const Targets &t, int64_t u, int64_t id, int l)
+{
+    const uint32_t *x = (const uint32_t *)t.X + u * t.kb * 4, *v = (const uint32_t *)t.V + id * t.kb * 4;
+    float d = 0.f;
+#pragma unroll 2
+    for (int c = l; c < t.kb * 4; c += 16) {
+        const uint32_t a = x[c], b = v[c];
+        const v2f a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 0), b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 0);
+        const v2f a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 1), b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 1);
+        const v2f a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 2), b2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 2);
+        const v2f a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 3), b3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 3);
+        const float e = a0[0] * b0[0] + a0[1] * b0[1] + a1[0] * b1[0] + a1[1] * b1[1] + a2[0] * b2[0] + a2[1] * b2[1] + a3[0] * b3[0] + a3[1] * b3[1];
+        d += e * mx_unit(t.xs[u * t.kb + (c >> 2)]) * mx_unit(t.vs[id * t.kb + (c >> 2)]);
+    }
+    return d;
+}
+
+// A workgroup a user: lse from the splits, then logp of the named items, 16 lanes a place (the score as one fp32 sum over the
+// factors).  Bound by the latency of its gathers.
+template <typename T>
+__global__ __launch_bounds__(256) void targets_kernel(Targets t)
+{
+    __shared__ float lm[4], ls[4];
+    const int64_t u = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = threadIdx.x & 15;
+    float top = -3.402823466e38f, sum = 0.f;
+    for (int q = threadIdx.x; q < t.splits; q += 256) {
+        const float a = t.m[q * t.s_padded + u], both = fmaxf(top, a);
+        sum = sum * exp2f(top - both) + t.s[q * t.s_padded + u] * exp2f(a - both);
+        top = both;
+    }
+    for (int o = 32; o; o >>= 1) {
+        const float a = __shfl_xor(top, o), r = __shfl_xor(sum, o), both = fmaxf(top, a);
+        sum = sum * exp2f(top - both) + r * exp2f(a - both);
+        top = both;
+    }
+    if (lane == 0) { lm[wave] = top; ls[wave] = sum; }
+    __syncthreads();
+    top = fmaxf(fmaxf(lm[0], lm[1]), fmaxf(lm[2], lm[3]));
+    sum = (ls[0] * exp2f(lm[0] - top) + ls[1] * exp2f(lm[1] - top)) + (ls[2] * exp2f(lm[2] - top) + ls[3] * exp2f(lm[3] - top));
+    const float lse = (float)(((double)top + (double)log2f(sum)) * LN2);
+    if (threadIdx.x == 0 && t.lse) t.lse[u] = lse;
+    for (int64_t j = threadIdx.x >> 4; j < t.places; j += 16) {
+        const int32_t id = t.ids[u * t.ld_ids + j];
         float out = 0.f;
-        if (id >= n_items) out = __uint_as_float(0x7fc00000u);
-        else if (id >= 0) {
-            float d = 0.f;
-            for (int c = l; c < kb * 4; c += 16) {
-                const uint32_t a = ((const uint32_t *)xc)[u * kb * 4 + c], b = ((const uint32_t *)vc)[(int64_t)id * kb * 4 + c];
-                const v2f a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 0), b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 0);
-                const v2f a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 1), b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 1);
-                const v2f a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 2), b2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 2);
-                const v2f a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 3), b3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 3);
-                // sums of products of the grid are exact; the scales are powers of two
-                const float e = a0[0] * b0[0] + a0[1] * b0[1] + a1[0] * b1[0] + a1[1] * b1[1] + a2[0] * b2[0] + a2[1] * b2[1] + a3[0] * b3[0] + a3[1] * b3[1];
-                d += e * mx_unit(xs[u * kb + (c >> 2)]) * mx_unit(vs[(int64_t)id * kb + (c >> 2)]);
-            }
+        if (id >= t.n_items) {
+            out = __uint_as_float(0x7fc00000u);
+        } else if (id >= 0) {
+            float d = dot_share<T>(t, u, id, l);
             for (int o = 8; o; o >>= 1) d += __shfl_xor(d, o);
-            const float z = scale * (d + (ibase ? ibase[id] : 0.f));
-            const float l0 = lse[u];
-            out = z == -INFINITY && l0 == -INFINITY ? z : z - l0;
+            const float z = t.scale * (d + (t.ibase ? t.ibase[id] : 0.f));
+            out = lse == -INFINITY ? -INFINITY : z - lse;
         }
-        if (l == 0) logp[u * ld_logp + j] = out;
+        if (l == 0) t.logp[u * t.ld_logp + j] = out;
     }
 }
 
-// dX = scale (sum over the places of g v - G acc 2^-e): a wave a user
+// dX = scale (sum over the places of g v - G acc): four columns a thread
 template <typename T>
-__global__ __launch_bounds__(256) void join_dx_kernel(const float *acc, int splits, int64_t s_padded, int KP, const uint32_t *v_amax, const float *G,
-                                                      const T *V, int64_t ldv, int64_t n_items, int k, float scale, const int32_t *ids, int64_t m,
-                                                      int64_t ld_ids, const float *dlogp, int64_t ld_dlogp, int64_t n, T *dX, int64_t ld_dx)
+__global__ __launch_bounds__(256) void join_dx_kernel(const float *acc, int splits, int64_t s_padded, int KP, const float *G, const T *V, int64_t ldv,
+                                                      int64_t n_items, int k, float scale, const int32_t *ids, int64_t m, int64_t ld_ids,
+                                                      const float *dlogp, int64_t ld_dlogp, int64_t n, T *dX, int64_t ld_dx)
 {
-    const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int e = v_amax ? split_exponent(v_amax) : 0;
-    if (u >= n) return;
-    for (int c = lane; c < k; c += 64) {
-        float a = 0.f;
-        for (int q = 0; q < splits; ++q) a += acc[((int64_t)q * s_padded + u) * KP + c];
-        float r = -G[u] * ldexpf(a, -e);
-        for (int64_t j = 0; j < m; ++j) {
-            const int32_t id = ids[u * ld_ids + j];
-            if (id >= 0 && id < n_items) r = fmaf(dlogp[u * ld_dlogp + j], as_f32(V[id * ldv + c]), r);
-        }
-        dX[u * ld_dx + c] = (T)(scale * r);
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t u = at / (KP / 4);
+    const int c = (int)(at - u * (KP / 4)) * 4;
+    if (u >= n || c >= k) return;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = 0; q < splits; ++q) {
+        const float4 v = *(const float4 *)(acc + ((int64_t)q * s_padded + u) * KP + c);
+        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
+    const float g0 = -G[u];
+    float r[4] = {g0 * a.x, g0 * a.y, g0 * a.z, g0 * a.w};
+#pragma unroll 4
+    for (int64_t j = 0; j < m; ++j) {
+        const int32_t id = ids[u * ld_ids + j];
+        const bool in = id >= 0 && id < n_items;
+        const float g = in ? dlogp[u * ld_dlogp + j] : 0.f;
+        const T *v = V + (int64_t)(in ? id : 0) * ldv + c;
+        for (int e = 0; e < 4; ++e)
+            if (in && c + e < k) r[e] = fmaf(g, as_f32(v[e]), r[e]);
+    }
+    for (int e = 0; e < 4; ++e)
+        if (c + e < k) dX[u * ld_dx + c + e] = (T)(scale * r[e]);
 }
 
-// dV = scale (sum over the places that name the item of g x - acc 2^-e), db likewise: 32 items a workgroup.  The workgroup scans
-// all places in order and keeps those that name one of its items; each column of an item is summed by one thread in that order,
-// so no sum depends on scheduling.
-constexpr int JOIN_ITEMS = 32, JOIN_LIST = 1024;
-
-template <typename T>
-__global__ __launch_bounds__(256) void join_dv_kernel(const float *acc, const float *acc_b, int splits, int64_t s_padded, int KP, const uint32_t *x_amax,
-                                                      const T *X, int64_t ldx, int64_t n_items, int k, float scale, const int32_t *ids, int64_t n, int64_t m,
-                                                      int64_t ld_ids, const float *dlogp, int64_t ld_dlogp, T *dV, int64_t ld_dv, float *db)
+// dV and db where the walk was split: the splits' sums of 64 items, then the same last steps
+template <typename T, int KP>
+__global__ __launch_bounds__(256) void join_dv_kernel(const float *acc, const float *acc_b, int splits, int64_t s_padded, Finish f)
 {
-    extern __shared__ float tile[];                   // [32][KP], then [32] for db
-    __shared__ int list_at[JOIN_LIST];                // item of the tile in the low 5 bits, place above ... row kept apart
-    __shared__ int list_row[JOIN_LIST];
-    __shared__ float list_g[JOIN_LIST];
-    __shared__ int wave_hits[4];
-    const int64_t i0 = (int64_t)blockIdx.x * JOIN_ITEMS;
-    const int e = x_amax ? split_exponent(x_amax) : 0;
-    float *tile_b = tile + JOIN_ITEMS * KP;
-    for (int i = threadIdx.x; i < JOIN_ITEMS * KP + JOIN_ITEMS; i += 256) tile[i] = 0.f;
-    __syncthreads();
-    const int64_t places = n * m;
-    const int groups = 256 / KP > 0 ? 256 / KP : 1;
-    const int col = threadIdx.x % KP, group = threadIdx.x / KP;
-    int held = 0;
-    for (int64_t b = 0; b < places || held; b += 256) {
-        bool hit = false;
-        int local = 0, row = 0;
-        float g = 0.f;
-        if (b < places) {
-            const int64_t at = b + threadIdx.x;
-            if (at < places) {
-                const int64_t u = at / m, j = at - u * m;
-                const int64_t id = (int64_t)ids[u * ld_ids + j] - i0;
-                hit = id >= 0 && id < JOIN_ITEMS && i0 + id < n_items;
-                if (hit) { local = (int)id; row = (int)u; g = dlogp[u * ld_dlogp + j]; }
-            }
+    __shared__ float rows[64 * KP];
+    __shared__ uint32_t list[list_length(KP) * 2];
+    __shared__ float row_b[64], aside[aside_floats(KP)];
+    __shared__ int counts[4], aside_item[32];
+    const int64_t i0 = (int64_t)blockIdx.x * 64;
+    for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int q = 0; q < splits; ++q) {
+            const float4 v = ((const float4 *)(acc + ((int64_t)q * s_padded + i0) * KP))[i];
+            a.x -= v.x; a.y -= v.y; a.z -= v.z; a.w -= v.w;
         }
-        const unsigned long long votes = __ballot(hit);
-        if ((threadIdx.x & 63) == 0) wave_hits[threadIdx.x >> 6] = __popcll(votes);
-        __syncthreads();
-        int at = held;
-        for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) at += wave_hits[w];
-        at += __popcll(votes & ((1ull << (threadIdx.x & 63)) - 1));
-        if (hit) { list_at[at] = local; list_row[at] = row; list_g[at] = g; }
-        held += wave_hits[0] + wave_hits[1] + wave_hits[2] + wave_hits[3];
-        __syncthreads();
-        if (held > JOIN_LIST - 256 || b + 256 >= places) {
-            if (group < groups) {
-                for (int q = 0; q < held; ++q) {
-                    const int li = list_at[q];
-                    if (li % groups != group) continue;
-                    if (col < k) tile[li * KP + col] = fmaf(list_g[q], as_f32(X[(int64_t)list_row[q] * ldx + col]), tile[li * KP + col]);
-                    if (col == 0) tile_b[li] += list_g[q];
-                }
-            }
-            held = 0;
-            __syncthreads();
-        }
+        ((float4 *)rows)[i] = a;
+    }
+    if (threadIdx.x < 64) {
+        float b = 0.f;
+        if (acc_b)
+            for (int q = 0; q < splits; ++q) b -= acc_b[(int64_t)q * s_padded + i0 + threadIdx.x];
+        row_b[threadIdx.x] = b;
     }
     __syncthreads();
-    if (dV)
-        for (int i = threadIdx.x; i < JOIN_ITEMS * k; i += 256) {
-            const int li = i / k, c = i - li * k;
-            if (i0 + li >= n_items) break;
-            float a = 0.f;
-            for (int q = 0; q < splits; ++q) a += acc[((int64_t)q * s_padded + i0 + li) * KP + c];
-            dV[(i0 + li) * ld_dv + c] = (T)(scale * (tile[li * KP + c] - ldexpf(a, -e)));
-        }
-    if (db)
-        for (int li = threadIdx.x; li < JOIN_ITEMS; li += 256) {
-            if (i0 + li >= n_items) break;
-            float a = 0.f;
-            for (int q = 0; q < splits; ++q) a += acc_b[(int64_t)q * s_padded + i0 + li];
-            db[i0 + li] = scale * (tile_b[li] - a);
-        }
+    finish_rows<T, KP>(f, rows, row_b, list, counts, aside, aside_item, i0);
 }
 
 // ---------------------------------------------------------------------------- launches
@@ -530,19 +1001,29 @@ struct Pieces {
     }
 };
 
-// splits of the T axis: enough workgroups for the chip, none shorter than 4 tiles
-int split_count(int64_t s_blocks, int64_t t_tiles)
+// Splits of the T axis: the count with the shortest plan, in stages: rounds of resident workgroups times (a split's stages + what a
+// workgroup costs besides), plus what joining costs where there is more than one.
+struct Split { int count, per; };
+
+Split split_plan(int64_t s_blocks, int64_t t_tiles, int unit, int64_t resident, double join)
 {
-    const int64_t want = (1024 + s_blocks - 1) / s_blocks;
-    const int64_t most = t_tiles / 4 > 0 ? t_tiles / 4 : 1;
-    const int64_t n = want < most ? want : most;
-    const int64_t per = (t_tiles + n - 1) / n;
-    return (int)((t_tiles + per - 1) / per);
+    const int64_t stages = (t_tiles + unit - 1) / unit;
+    int64_t best = 1;
+    double best_cost = 0;
+    for (int64_t c = 1; c <= stages && c <= 4096; c = c < 16 ? c + 1 : c + c / 8) {
+        const int64_t per = (stages + c - 1) / c;
+        const double cost = (double)((s_blocks * c + resident - 1) / resident) * ((double)per + 4.0) + (c > 1 ? join * (double)c : 0.0);
+        if (c == 1 || cost < best_cost) { best = c; best_cost = cost; }
+    }
+    Split s;
+    s.per = (int)((stages + best - 1) / best) * unit;
+    s.count = (int)((t_tiles + s.per - 1) / s.per);
+    return s;
 }
 
 struct Side {                          // one matrix in fragment order
     int64_t rows, tiles, padded;       // tiles of 32 rows; padded: rows up to whole S blocks
-    uint32_t *amax;
+    int *exps;
     uint4 *f1, *f2;
 };
 
@@ -552,7 +1033,7 @@ Side side(Pieces &w, int64_t rows, int KP, int NS, bool want1, bool want2)
     s.rows = rows;
     s.padded = up(rows, S_ROWS);
     s.tiles = s.padded / 32;
-    s.amax = w.take<uint32_t>(NS == 2 ? AMAX_BLOCKS : 0);
+    s.exps = w.take<int>(NS == 2 ? s.tiles : 0);
     const int64_t n = s.tiles * NS * (KP / 16) * 64;
     s.f1 = want1 ? w.take<uint4>(n) : nullptr;
     s.f2 = want2 ? w.take<uint4>(n) : nullptr;
@@ -563,25 +1044,44 @@ template <typename T>
 void fill_side(const Side &d, const T *src, int k, int64_t ld, const float *row_factor, int KP, hipStream_t s)
 {
     constexpr int NS = sizeof(T) == 4 ? 2 : 1;
-    if (NS == 2) hipLaunchKernelGGL((amax_kernel<T>), dim3(AMAX_BLOCKS), dim3(256), 0, s, src, d.rows, k, ld, row_factor, d.amax);
-    hipLaunchKernelGGL((fragments_kernel<T, NS>), dim3((uint32_t)d.tiles), dim3(256), 32 * (KP + 1) * sizeof(float), s, src, d.rows, k, ld, row_factor,
-                       d.amax, KP, d.f1, d.f2);
+    hipLaunchKernelGGL((fragments_kernel<T, NS>), dim3((uint32_t)d.tiles), dim3(256), 32 * (KP + 1) * sizeof(float), s, src, d.rows, k, ld, row_factor, KP,
+                       d.exps, d.f1, d.f2);
 }
+
+#define IFR_FOR_FACTORS(KP, CALL)                                                                                     \
+    switch (KP) {                                                                                                     \
+    case 32: CALL(32); break;                                                                                         \
+    case 64: CALL(64); break;                                                                                         \
+    case 96: CALL(96); break;                                                                                         \
+    case 128: CALL(128); break;                                                                                       \
+    case 160: CALL(160); break;                                                                                       \
+    case 192: CALL(192); break;                                                                                       \
+    case 224: CALL(224); break;                                                                                       \
+    default: CALL(256); break;                                                                                        \
+    }
 
 template <int NS, int MODE>
-void launch_walk(const WalkParams &p, int KP, dim3 grid, hipStream_t s)
+void launch_walk(const WalkParams &p, int KP, hipStream_t s)
 {
-    if (KP == 64) hipLaunchKernelGGL((walk_kernel<64, NS, MODE>), grid, dim3(256), 0, s, p);
-    else if (KP == 128) hipLaunchKernelGGL((walk_kernel<128, NS, MODE>), grid, dim3(256), 0, s, p);
-    else if (KP == 192) hipLaunchKernelGGL((walk_kernel<192, NS, MODE>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((walk_kernel<256, NS, MODE>), grid, dim3(256), 0, s, p);
+    const dim3 grid((uint32_t)(p.s_blocks * p.splits));
+#define IFR_WALK(K) hipLaunchKernelGGL((walk_kernel<K, NS, MODE>), grid, dim3(256), 0, s, p)
+    IFR_FOR_FACTORS(KP, IFR_WALK)
+#undef IFR_WALK
 }
 
+int resident_blocks(int KP, int NS, int mode) { return 256 * (mode != WALK_STATS && (KP * NS > 256 || KP > 128) ? 1 : 2); }
+
+// Users one pass over V serves (their operand stays in registers: at most 128 of them), and up to how many users the direct kernel is taken.
+int direct_tiles(int KP, int64_t n) { return n <= 16 ? 1 : n <= 32 || KP > 128 ? 2 : 4; }
+constexpr int64_t DIRECT_USERS = 64;
+
 struct ForwardPlan {
+    bool direct;
     Side x, v;
-    float *term, *lse, *out_m, *out_s;
-    int splits, per;
-    int64_t s_padded, t_tiles;
+    float *term, *out_m, *out_s;
+    Split split;
+    int64_t s_padded, t_padded;
+    int mx_users;                      // user tiles of a wave, 4-bit model
 };
 
 ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c)
@@ -589,44 +1089,64 @@ ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c)
     ForwardPlan p = {};
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
     p.s_padded = up(c.n, S_ROWS);
-    p.t_tiles = (c.n_items + 31) / 32;
+    p.t_padded = up(c.n_items, S_ROWS);
+    p.direct = c.dtype != IFR_MXFP4 && c.n <= DIRECT_USERS;
+    if (p.direct) {
+        const int64_t want = (c.n_items + 63) / 64;
+        p.split.count = (int)(want < 1024 ? want : 1024);      // workgroups of four waves
+        p.out_m = w.take<float>(p.split.count * p.s_padded);
+        p.out_s = w.take<float>(p.split.count * p.s_padded);
+        return p;
+    }
     if (c.dtype != IFR_MXFP4) {
         p.x = side(w, c.n, KP, NS, true, false);
         p.v = side(w, c.n_items, KP, NS, true, false);
     }
-    p.splits = split_count(p.s_padded / S_ROWS, p.t_tiles);
-    p.per = (int)((p.t_tiles + p.splits - 1) / p.splits);
-    p.term = w.take<float>(p.t_tiles * 32);
-    p.lse = w.take<float>(c.n);
-    p.out_m = w.take<float>(p.splits * p.s_padded);
-    p.out_s = w.take<float>(p.splits * p.s_padded);
+    if (c.dtype == IFR_MXFP4) {                       // waves walk alone: 16 a compute unit, none with fewer than two tiles
+        p.mx_users = c.n > 64 ? 4 : c.n > 32 ? 2 : 1;
+        const int64_t s_tiles = (c.n + 32 * p.mx_users - 1) / (32 * p.mx_users), tiles = p.t_padded / 32;
+        int64_t waves = (4096 + s_tiles - 1) / s_tiles;
+        waves = waves < tiles / 2 ? waves : (tiles / 2 > 0 ? tiles / 2 : 1);
+        p.split.per = (int)((tiles + waves - 1) / waves);
+        p.split.count = (int)up((tiles + p.split.per - 1) / p.split.per, 4);
+    } else {
+        p.split = split_plan(p.s_padded / S_ROWS, p.t_padded / 32, 2, resident_blocks(KP, NS, WALK_STATS), 0.0);
+    }
+    p.term = w.take<float>(p.t_padded + 32);
+    p.out_m = w.take<float>(p.split.count * p.s_padded);
+    p.out_s = w.take<float>(p.split.count * p.s_padded);
     return p;
 }
 
 struct BackwardPlan {
     Side x, v, xg;                     // xg: rows times G, second product of dV
     float *item_term, *user_term, *G, *acc, *acc_b;
-    int splits_x, per_x, splits_v, per_v;
+    int32_t *places;
+    uint8_t *named;
+    int64_t places_padded;
+    Split split_x, split_v;
 };
 
-BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, bool dx, bool dv, bool db)
+BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx, bool dv, bool db)
 {
     BackwardPlan p = {};
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
     p.x = side(w, c.n, KP, NS, true, false);
     p.v = side(w, c.n_items, KP, NS, true, dx);
     p.xg = side(w, c.n, KP, NS, false, dv || db);
-    p.item_term = w.take<float>(p.v.padded);
-    p.user_term = w.take<float>(p.x.padded);
-    p.G = w.take<float>(p.x.padded);
-    const int64_t tv = (c.n_items + 31) / 32, tx = (c.n + 31) / 32;
-    p.splits_x = split_count(p.x.padded / S_ROWS, tv);
-    p.per_x = (int)((tv + p.splits_x - 1) / p.splits_x);
-    p.splits_v = split_count(p.v.padded / S_ROWS, tx);
-    p.per_v = (int)((tx + p.splits_v - 1) / p.splits_v);
-    const int64_t ax = dx ? p.splits_x * p.x.padded * KP : 0, av = dv || db ? p.splits_v * p.v.padded * KP : 0;
+    p.item_term = w.take<float>(p.v.padded + 32);     // a stage fetches 64 terms, also where it holds 32 rows
+    p.user_term = w.take<float>(p.x.padded + 32);
+    p.G = w.take<float>(p.x.padded + 32);
+    p.places_padded = dv || db ? up(c.n * m, 1024) : 0;
+    p.places = w.take<int32_t>(p.places_padded);
+    p.named = w.take<uint8_t>(p.places_padded ? p.v.padded / 64 : 0);
+    const int resident = resident_blocks(KP, NS, WALK_GRAD);
+    p.split_x = split_plan(p.x.padded / S_ROWS, p.v.tiles, 2, resident, 0.05);
+    p.split_v = split_plan(p.v.padded / S_ROWS, p.x.tiles, 2, resident, 0.5);
+    const int64_t ax = dx ? p.split_x.count * p.x.padded * KP : 0;
+    const int64_t av = (dv || db) && p.split_v.count > 1 ? p.split_v.count * p.v.padded * KP : 0;
     p.acc = w.take<float>(ax > av ? ax : av);         // dX is joined before dV is begun
-    p.acc_b = w.take<float>(db ? p.splits_v * p.v.padded : 0);
+    p.acc_b = w.take<float>(db && p.split_v.count > 1 ? p.split_v.count * p.v.padded : 0);
     return p;
 }
 
@@ -639,10 +1159,10 @@ size_t logprob_workspace(const ifr_catalogue &c)
     return w.used;
 }
 
-size_t logprob_backward_workspace(const ifr_catalogue &c, bool want_dx, bool want_dv, bool want_db)
+size_t logprob_backward_workspace(const ifr_catalogue &c, int64_t m, bool want_dx, bool want_dv, bool want_db)
 {
     Pieces w{nullptr};
-    backward_plan(w, c, want_dx, want_dv, want_db);
+    backward_plan(w, c, m, want_dx, want_dv, want_db);
     return w.used;
 }
 
@@ -654,10 +1174,51 @@ static void forward_typed(const ifr_catalogue &c, const ForwardPlan &p, hipStrea
     fill_side<T>(p.x, (const T *)c.X, c.k, c.ldx, nullptr, KP, s);
     fill_side<T>(p.v, (const T *)c.V, c.k, c.ldv, nullptr, KP, s);
     WalkParams w = {};
-    w.s_f1 = p.x.f1; w.t_f1 = p.v.f1; w.t_term = p.term; w.s_amax = p.x.amax; w.t_amax = p.v.amax;
-    w.c = (float)(c.scale / LN2); w.t_tiles = (int)p.t_tiles; w.tiles_per_split = p.per; w.s_padded = p.s_padded;
+    w.s_f1 = p.x.f1; w.t_f1 = p.v.f1; w.t_term = p.term; w.s_exp = p.x.exps; w.t_exp = p.v.exps;
+    w.c = (float)(c.scale / LN2); w.t_tiles = (int)p.v.tiles; w.tiles_per_split = p.split.per; w.splits = p.split.count;
+    w.s_blocks = (int)(p.s_padded / S_ROWS); w.s_padded = p.s_padded;
     w.out_m = p.out_m; w.out_s = p.out_s;
-    launch_walk<NS, WALK_STATS>(w, KP, dim3((uint32_t)(p.s_padded / S_ROWS), p.splits), s);
+    launch_walk<NS, WALK_STATS>(w, KP, s);
+}
+
+template <int STEPS>
+static void launch_mx_users(const MxWalkParams &w, int users, dim3 grid, hipStream_t s)
+{
+    if (users == 1) hipLaunchKernelGGL((walk_mx_kernel<STEPS, 1>), grid, dim3(256), 0, s, w);
+    else if (users == 2) hipLaunchKernelGGL((walk_mx_kernel<STEPS, 2>), grid, dim3(256), 0, s, w);
+    else hipLaunchKernelGGL((walk_mx_kernel<STEPS, 4>), grid, dim3(256), 0, s, w);
+}
+
+static void launch_mx_walk(const ifr_catalogue &c, const ForwardPlan &p, hipStream_t s)
+{
+    const int kb = (c.k + 31) / 32;
+    const MxWalkParams w = {(const uint8_t *)c.X, c.x_scales, (const uint8_t *)c.V, c.v_scales, p.term, c.n, c.n_items, p.s_padded, kb, (int)(p.t_padded / 32),
+                            p.split.per, (float)(c.scale / LN2), p.out_m, p.out_s};
+    const dim3 grid((uint32_t)((c.n + 32 * p.mx_users - 1) / (32 * p.mx_users)), (uint32_t)(p.split.count / 4));
+    if (kb <= 2) launch_mx_users<1>(w, p.mx_users, grid, s);
+    else if (kb <= 4) launch_mx_users<2>(w, p.mx_users, grid, s);
+    else if (kb <= 6) launch_mx_users<3>(w, p.mx_users, grid, s);
+    else launch_mx_users<4>(w, p.mx_users, grid, s);
+}
+
+template <typename T, int KP, bool VEC>
+static void launch_direct_tiles(const DirectParams &d, int tiles, int grid, hipStream_t s)
+{
+    const dim3 g((uint32_t)grid, (uint32_t)((d.n + tiles * 16 - 1) / (tiles * 16)));
+    if (tiles == 1) hipLaunchKernelGGL((direct_kernel<T, KP, 1, VEC>), g, dim3(256), 0, s, d);
+    else if (tiles == 2) hipLaunchKernelGGL((direct_kernel<T, KP, 2, VEC>), g, dim3(256), 0, s, d);
+    else hipLaunchKernelGGL((direct_kernel<T, KP, (KP > 128 ? 2 : 4), VEC>), g, dim3(256), 0, s, d);
+}
+
+template <typename T>
+static void launch_direct(const ifr_catalogue &c, const ForwardPlan &p, hipStream_t s)
+{
+    const int KP = pad_factors(c.k), tiles = direct_tiles(KP, c.n), N = 16 / sizeof(T);
+    const bool vec = c.k % N == 0 && c.ldx % N == 0 && c.ldv % N == 0 && (((uintptr_t)c.X | (uintptr_t)c.V) & 15) == 0;
+    const DirectParams d = {c.X, c.V, c.ibase, c.ldx, c.ldv, c.n, c.n_items, p.s_padded, c.k, (float)(c.scale / LN2), p.out_m, p.out_s};
+#define IFR_DIRECT(K) vec ? launch_direct_tiles<T, K, true>(d, tiles, p.split.count, s) : launch_direct_tiles<T, K, false>(d, tiles, p.split.count, s)
+    IFR_FOR_FACTORS(KP, IFR_DIRECT)
+#undef IFR_DIRECT
 }
 
 int launch_logprob(const ifr_catalogue &c, const int32_t *ids, int64_t m, int64_t ld_ids, float *logp, int64_t ld_logp, float *lse,
@@ -666,29 +1227,22 @@ int launch_logprob(const ifr_catalogue &c, const int32_t *ids, int64_t m, int64_
     Pieces w{(char *)ws};
     const ForwardPlan p = forward_plan(w, c);
     const float cc = (float)(c.scale / LN2);
-    hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.t_tiles * 32 + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.t_tiles * 32, cc, p.term);
     const int kb = (c.k + 31) / 32;
-    if (c.dtype == IFR_MXFP4)
-        hipLaunchKernelGGL(walk_mx_kernel, dim3((uint32_t)(p.s_padded / S_ROWS), p.splits), dim3(256), 0, s, (const uint8_t *)c.X, c.x_scales, c.n,
-                           (const uint8_t *)c.V, c.v_scales, c.n_items, kb, p.term, cc, (int)p.t_tiles, p.per, p.s_padded, p.out_m, p.out_s);
-    else if (c.dtype == IFR_F32) forward_typed<float>(c, p, s);
-    else forward_typed<__bf16>(c, p, s);
-    float *l = lse ? lse : p.lse;
-    hipLaunchKernelGGL(join_lse_kernel, dim3((uint32_t)((c.n + 255) / 256)), dim3(256), 0, s, p.out_m, p.out_s, p.splits, c.n, p.s_padded, l);
-    if (m > 0) {
-        const int64_t want = (c.n * m + 15) / 16;
-        const dim3 grid((uint32_t)(want < MAX_GRID ? want : MAX_GRID));
-        const float sc = (float)c.scale;
-        if (c.dtype == IFR_MXFP4)
-            hipLaunchKernelGGL(targets_mx_kernel, grid, dim3(256), 0, s, (const uint8_t *)c.X, c.x_scales, (const uint8_t *)c.V, c.v_scales, c.ibase, kb,
-                               c.n_items, sc, ids, c.n, m, ld_ids, l, logp, ld_logp);
-        else if (c.dtype == IFR_F32)
-            hipLaunchKernelGGL((targets_kernel<float>), grid, dim3(256), 0, s, (const float *)c.X, c.ldx, (const float *)c.V, c.ldv, c.ibase, c.k, c.n_items, sc,
-                               ids, c.n, m, ld_ids, l, logp, ld_logp);
-        else
-            hipLaunchKernelGGL((targets_kernel<__bf16>), grid, dim3(256), 0, s, (const __bf16 *)c.X, c.ldx, (const __bf16 *)c.V, c.ldv, c.ibase, c.k, c.n_items,
-                               sc, ids, c.n, m, ld_ids, l, logp, ld_logp);
+    if (p.direct) {
+        if (c.dtype == IFR_F32) launch_direct<float>(c, p, s);
+        else launch_direct<__bf16>(c, p, s);
+    } else {
+        hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.t_padded + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.t_padded, c.dtype == IFR_MXFP4 ? 1.f : cc, p.term, nullptr);
+        if (c.dtype == IFR_MXFP4) launch_mx_walk(c, p, s);
+        else if (c.dtype == IFR_F32) forward_typed<float>(c, p, s);
+        else forward_typed<__bf16>(c, p, s);
     }
+    Targets t = {p.out_m, p.out_s, p.s_padded, p.split.count, c.k, kb, c.X, c.V, c.x_scales, c.v_scales, c.ldx, c.ldv, c.n_items, c.ibase, (float)c.scale,
+                 ids, m, ld_ids, ld_logp, lse, logp};
+    const dim3 grid((uint32_t)c.n);
+    if (c.dtype == IFR_MXFP4) hipLaunchKernelGGL((targets_kernel<Mx>), grid, dim3(256), 0, s, t);
+    else if (c.dtype == IFR_F32) hipLaunchKernelGGL((targets_kernel<float>), grid, dim3(256), 0, s, t);
+    else hipLaunchKernelGGL((targets_kernel<__bf16>), grid, dim3(256), 0, s, t);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
@@ -699,7 +1253,7 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     const int KP = pad_factors(c.k);
     const float cc = (float)(c.scale / LN2), sc = (float)c.scale;
     const T *X = (const T *)c.X, *V = (const T *)c.V;
-    hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.v.padded + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.v.padded, cc, p.item_term);
+    hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.v.padded + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.v.padded, cc, p.item_term, p.named);
     hipLaunchKernelGGL(user_terms_kernel, dim3((uint32_t)((p.x.padded + 255) / 256)), dim3(256), 0, s, g.lse, ids, m, ld_ids, g.dlogp, g.ld_dlogp, c.n,
                        p.x.padded, p.user_term, p.G);
     fill_side<T>(p.x, X, c.k, c.ldx, nullptr, KP, s);
@@ -708,21 +1262,37 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     w.c = cc;
     if (g.dX) {
         w.s_f1 = p.x.f1; w.t_f1 = p.v.f1; w.t_f2 = p.v.f2; w.s_term = p.user_term; w.t_term = p.item_term;
-        w.s_amax = p.x.amax; w.t_amax = p.v.amax;
-        w.t_tiles = (int)((c.n_items + 31) / 32); w.tiles_per_split = p.per_x; w.s_padded = p.x.padded; w.out_acc = p.acc;
-        launch_walk<NS, WALK_GRAD>(w, KP, dim3((uint32_t)(p.x.padded / S_ROWS), p.splits_x), s);
-        hipLaunchKernelGGL((join_dx_kernel<T>), dim3((uint32_t)((c.n + 3) / 4)), dim3(256), 0, s, p.acc, p.splits_x, p.x.padded, KP, p.v.amax, p.G, V, c.ldv,
+        w.s_exp = p.x.exps; w.t_exp = w.t2_exp = p.v.exps;
+        w.t_tiles = (int)p.v.tiles; w.tiles_per_split = p.split_x.per; w.splits = p.split_x.count;
+        w.s_blocks = (int)(p.x.padded / S_ROWS); w.s_padded = p.x.padded; w.out_acc = p.acc;
+        launch_walk<NS, WALK_GRAD>(w, KP, s);
+        const int64_t threads = c.n * (KP / 4);
+        hipLaunchKernelGGL((join_dx_kernel<T>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, s, p.acc, p.split_x.count, p.x.padded, KP, p.G, V, c.ldv,
                            c.n_items, c.k, sc, ids, m, ld_ids, g.dlogp, g.ld_dlogp, c.n, (T *)g.dX, g.ld_dx);
     }
     if (g.dV || g.dibase) {
         fill_side<T>(p.xg, X, c.k, c.ldx, p.G, KP, s);
+        if (p.places_padded) {
+            const int64_t want = p.places_padded / 256;
+            hipLaunchKernelGGL(places_kernel, dim3((uint32_t)(want < MAX_GRID ? want : MAX_GRID)), dim3(256), 0, s, ids, m, ld_ids, c.n, c.n_items,
+                               p.places_padded, p.places, p.named);
+        }
+        const bool whole = p.split_v.count == 1;
         w.s_f1 = p.v.f1; w.t_f1 = p.x.f1; w.t_f2 = p.xg.f2; w.s_term = p.item_term; w.t_term = p.user_term;
-        w.s_amax = p.v.amax; w.t_amax = p.x.amax; w.t_factor = g.dibase ? p.G : nullptr;
-        w.t_tiles = (int)((c.n + 31) / 32); w.tiles_per_split = p.per_v; w.s_padded = p.v.padded; w.out_acc = p.acc; w.out_b = g.dibase ? p.acc_b : nullptr;
-        launch_walk<NS, WALK_GRAD>(w, KP, dim3((uint32_t)(p.v.padded / S_ROWS), p.splits_v), s);
-        hipLaunchKernelGGL((join_dv_kernel<T>), dim3((uint32_t)((c.n_items + JOIN_ITEMS - 1) / JOIN_ITEMS)), dim3(256), (JOIN_ITEMS * KP + JOIN_ITEMS) * sizeof(float), s,
-                           p.acc, p.acc_b, p.splits_v, p.v.padded, KP, p.xg.amax, X, c.ldx, c.n_items, c.k, sc, ids, c.n, m, ld_ids, g.dlogp, g.ld_dlogp,
-                           (T *)g.dV, g.ld_dv, g.dibase);
+        w.s_exp = p.v.exps; w.t_exp = p.x.exps; w.t2_exp = p.xg.exps; w.t_factor = g.dibase ? p.G : nullptr;
+        w.t_tiles = (int)p.x.tiles; w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
+        w.s_blocks = (int)(p.v.padded / S_ROWS); w.s_padded = p.v.padded;
+        w.out_acc = whole ? nullptr : p.acc; w.out_b = whole || !g.dibase ? nullptr : p.acc_b;
+        w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc,
+               c.k % 4 == 0 && c.ldx % 4 == 0 && ((uintptr_t)X & (4 * sizeof(T) - 1)) == 0};
+        if (g.dibase) launch_walk<NS, WALK_GRAD_BASE>(w, KP, s);
+        else launch_walk<NS, WALK_GRAD>(w, KP, s);
+        if (!whole) {
+            const dim3 grid((uint32_t)(p.v.padded / 64));
+#define IFR_JOIN(K) hipLaunchKernelGGL((join_dv_kernel<T, K>), grid, dim3(256), 0, s, p.acc, g.dibase ? p.acc_b : nullptr, p.split_v.count, p.v.padded, w.f)
+            IFR_FOR_FACTORS(KP, IFR_JOIN)
+#undef IFR_JOIN
+        }
     }
 }
 
@@ -730,7 +1300,7 @@ int launch_logprob_backward(const ifr_catalogue &c, const int32_t *ids, int64_t 
                             hipStream_t s)
 {
     Pieces w{(char *)ws};
-    const BackwardPlan p = backward_plan(w, c, g.dX != nullptr, g.dV != nullptr, g.dibase != nullptr);
+    const BackwardPlan p = backward_plan(w, c, m, g.dX != nullptr, g.dV != nullptr, g.dibase != nullptr);
     if (c.dtype == IFR_F32) backward_typed<float>(c, ids, m, ld_ids, g, p, s);
     else backward_typed<__bf16>(c, ids, m, ld_ids, g, p, s);
     return hipGetLastError() == hipSuccess ? 0 : -1;

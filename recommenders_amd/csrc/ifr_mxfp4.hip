@@ -109,44 +109,74 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *codes
 
 // ---------------------------------------------------------------------------- product
 
-// Score rows: D[query][item] by v_mfma_scale_f32_32x32x64 with both operands in E2M1.  A lane of that instruction holds one
-// block of 32 of one row and that block's scale, which is the layout in memory.  A wave takes 32 queries and walks item tiles
-// of 32; sums are fp32.
-__global__ __launch_bounds__(256) void mx_scores_kernel(MxScoreParams p, int kb, int tiles_per_wave)
+// Score rows by v_mfma_scale_f32_32x32x64 with both operands in E2M1.  A lane of that instruction holds one block of 32 of one row and
+// that block's scale, which is the layout in memory, so nothing is rearranged.  A wave keeps IT tiles of 32 items in registers (A
+// operand) and walks query tiles of 32 (B operand): D[item][query], four neighbouring items of one query a lane and quad, which go
+// through a strip of LDS of the wave's own so that rows are stored in long pieces.  Bound by the store of the scores for k <= 256.
+template <int STEPS, int IT, typename OUT>
+__global__ __launch_bounds__(256) void mx_scores_kernel(MxScoreParams p, int kb, int64_t q_tiles, int64_t q_per_block, int vec)
 {
+    constexpr int COLS = IT * 32, PITCH = COLS + 16 / sizeof(OUT);      // a row further by one 16-byte piece: fewer bank conflicts
+    __shared__ __align__(16) OUT strips[4][32 * PITCH];
+    __shared__ __align__(16) float bases[4][COLS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
-    const int64_t q0 = (int64_t)blockIdx.y * 32;
-    const int64_t q = min(q0 + r, p.x.n - 1);
-    const int steps = (kb + 1) / 2;
-    const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * tiles_per_wave;
-    for (int t = 0; t < tiles_per_wave; ++t) {
-        const int64_t i0 = (first + t) * 32;
-        if (i0 >= p.v.n) return;
-        const int64_t item = min(i0 + r, p.v.n - 1);
-        v16f d = {0};
-        for (int s = 0; s < steps; ++s) {
-            const int b = 2 * s + h;
-            v8i a = {0}, w = {0};
-            int sa = 127, sw = 127;
-            if (b < kb) {
-                const uint4 ca = *(const uint4 *)(p.x.codes + (q * kb + b) * 16);
-                const uint4 cw = *(const uint4 *)(p.v.codes + (item * kb + b) * 16);
-                a[0] = ca.x; a[1] = ca.y; a[2] = ca.z; a[3] = ca.w;
-                w[0] = cw.x; w[1] = cw.y; w[2] = cw.z; w[3] = cw.w;
-                sa = p.x.scales[q * kb + b];
-                sw = p.v.scales[item * kb + b];
-            }
-            d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, w, d, 4, 4, 0, sa, 0, sw);
+    OUT *strip = strips[wave];
+    const int64_t i0 = ((int64_t)blockIdx.x * 4 + wave) * COLS;
+    if (i0 >= p.v.n) return;                          // waves work alone: no barrier below
+    v8i a[IT][STEPS];
+    int sa[IT][STEPS];
+    auto block_of = [&](const MxMatrix &m, int64_t row, int s, v8i *to, int *scale) {
+        const int b = 2 * s + h;
+        v8i v = {0};
+        *scale = 127;
+        if (b < kb) {
+            const uint4 c = *(const uint4 *)(m.codes + (row * kb + b) * 16);
+            v[0] = c.x; v[1] = c.y; v[2] = c.z; v[3] = c.w;
+            *scale = m.scales[row * kb + b];
         }
-        if (i0 + r < p.v.n) {
-            const float ib = p.ibase ? p.ibase[item] : 0.f;
-            for (int e = 0; e < 16; ++e) {
-                const int64_t row = q0 + 8 * (e >> 2) + 4 * h + (e & 3);
-                if (row >= p.x.n) continue;
-                const float v = d[e] + (p.ubase ? ib + p.ubase[row] : ib);
-                if (p.out_bf16) ((__bf16 *)p.out)[row * p.ld + item] = (__bf16)v;
-                else ((float *)p.out)[row * p.ld + item] = v;
+        *to = v;
+    };
+#pragma unroll
+    for (int t = 0; t < IT; ++t)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) block_of(p.v, min(i0 + t * 32 + r, p.v.n - 1), s, &a[t][s], &sa[t][s]);
+    for (int c = lane; c < COLS; c += 64) bases[wave][c] = p.ibase && i0 + c < p.v.n ? p.ibase[i0 + c] : 0.f;
+    const int64_t first = (int64_t)blockIdx.y * q_per_block, last = min(first + q_per_block, q_tiles);
+    const int cols = (int)min((int64_t)COLS, p.v.n - i0);
+    for (int64_t qt = first; qt < last; ++qt) {
+        const int64_t q = min(qt * 32 + r, p.x.n - 1);
+        v8i x[STEPS];
+        int sx[STEPS];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) block_of(p.x, q, s, &x[s], &sx[s]);
+        const float ub = p.ubase ? p.ubase[q] : 0.f;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < IT; ++t) {
+            v16f d = {0};
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[t][s], x[s], d, 4, 4, 0, sa[t][s], 0, sx[s]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 b = *(const float4 *)&bases[wave][t * 32 + 8 * e + 4 * h];
+                const float v0 = d[4 * e] + (b.x + ub), v1 = d[4 * e + 1] + (b.y + ub), v2 = d[4 * e + 2] + (b.z + ub), v3 = d[4 * e + 3] + (b.w + ub);
+                OUT *to = strip + r * PITCH + t * 32 + 8 * e + 4 * h;
+                to[0] = (OUT)v0; to[1] = (OUT)v1; to[2] = (OUT)v2; to[3] = (OUT)v3;
             }
+        }
+        __builtin_amdgcn_wave_barrier();
+        OUT *out = (OUT *)p.out + qt * 32 * p.ld + i0;
+        const int rows = (int)min((int64_t)32, p.x.n - qt * 32);
+        if (vec && cols == COLS) {
+            constexpr int PIECE = 16 / sizeof(OUT), ROW = COLS / PIECE;          // 16-byte pieces of a row
+#pragma unroll
+            for (int i = 0; i < 32 * ROW / 64; ++i) {
+                const int at = i * 64 + lane, row = at / ROW, c = (at - row * ROW) * PIECE;
+                if (row < rows) *(uint4 *)(out + row * p.ld + c) = *(const uint4 *)(strip + row * PITCH + c);
+            }
+        } else {
+            for (int row = 0; row < rows; ++row)
+                for (int c = lane; c < cols; c += 64) out[row * p.ld + c] = strip[row * PITCH + c];
         }
     }
 }
@@ -188,23 +218,34 @@ int launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n,
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
+template <int STEPS, typename OUT>
+static void launch_mx_scores_typed(const MxScoreParams &p, int kb, hipStream_t s)
+{
+    const int64_t qt = (p.x.n + 31) / 32, it = (p.v.n + 31) / 32;
+    const int vec = aligned16(p.out, p.ld * (int64_t)sizeof(OUT));
+    // few scores: 32 items a wave fill the chip; many: 128, which reads X a quarter as often and stores rows of 256 bytes or more
+    const bool wide = it * qt >= 16384;
+    const int64_t gx = wide ? (it + 15) / 16 : (it + 3) / 4;
+    int64_t gy = (4096 + gx - 1) / gx;
+    gy = gy < qt ? gy : qt;
+    const int64_t per = (qt + gy - 1) / gy;
+    gy = (qt + per - 1) / per;
+    const dim3 grid((uint32_t)gx, (uint32_t)gy);
+    if (wide) hipLaunchKernelGGL((mx_scores_kernel<STEPS, 4, OUT>), grid, dim3(256), 0, s, p, kb, qt, per, vec);
+    else hipLaunchKernelGGL((mx_scores_kernel<STEPS, 1, OUT>), grid, dim3(256), 0, s, p, kb, qt, per, vec);
+}
+
 int launch_mx_scores(const MxScoreParams &p, hipStream_t s)
 {
     const int kb = (p.k + 31) / 32;
-    const int64_t qt = (p.x.n + 31) / 32, it = (p.v.n + 31) / 32;
-    const int per = (int)(it * qt > 65536 ? 8 : 1);
-    for (int64_t y = 0; y < qt; y += 65535) {         // grid.y holds 65535 query tiles
-        MxScoreParams c = p;
-        const int64_t rows = y * 32;
-        c.x.codes += rows * kb * 16; c.x.scales += rows * kb; c.x.n -= rows;
-        if (c.ubase) c.ubase += rows;
-        c.out = (char *)p.out + rows * p.ld * (p.out_bf16 ? 2 : 4);
-        const int64_t ny = qt - y < 65535 ? qt - y : 65535;
-        if (c.x.n > ny * 32) c.x.n = ny * 32;
-        hipLaunchKernelGGL(mx_scores_kernel, dim3((it + 4 * per - 1) / (4 * per), ny), dim3(256), 0, s, c, kb, per);
-        if (hipGetLastError() != hipSuccess) return -1;
-    }
-    return 0;
+#define IFR_SCORES(STEPS)                                                                                  \
+    p.out_bf16 ? launch_mx_scores_typed<STEPS, __bf16>(p, kb, s) : launch_mx_scores_typed<STEPS, float>(p, kb, s)
+    if (kb <= 2) IFR_SCORES(1);
+    else if (kb <= 4) IFR_SCORES(2);
+    else if (kb <= 6) IFR_SCORES(3);
+    else IFR_SCORES(4);
+#undef IFR_SCORES
+    return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
 }  // namespace ifr

@@ -233,6 +233,27 @@ def test_logprob_and_gradient(torch, sc, n, items, k, m, dtype, bias, scale):
     assert all(a is None and c is None or torch.equal(a, c) for a, c in zip((dX, dV, db), again))
 
 
+@pytest.mark.parametrize("n,items,k,m", [(600, 150, 40, 40), (700, 3, 128, 30), (300, 70001, 32, 20), (90, 66000, 200, 3), (200, 40000, 128, 64)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_logprob_gradient_of_items_that_everybody_names(torch, sc, n, items, k, m, dtype):
+    """More places than one pass over them holds, one item in half of them, catalogues of few and of many rows."""
+    X, V, b, ids, dlogp = _case(torch, n, items, k, m, dtype, True, 21, spread=0.2)
+    g = _gen(torch, 22)
+    pick = torch.rand((n, m), generator=g, device="cuda")
+    ids = torch.where(pick < 0.5, torch.full_like(ids, items // 2), torch.where(pick < 0.6, torch.full_like(ids, items - 1), ids))
+    dlogp /= n
+    _, lse = sc.catalogue_logprob(X, V, ids, ibase=b)
+    r = _reference(torch, X, V, b, ids, dlogp, 1.0)
+    got = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp, ibase=b)
+    # the norm of the error: rounding of the result, operands and probabilities in 16 bits (their errors are independent and add up
+    # like at most sqrt(3) steps), or 22 bits and up to n m additions of one item's places, errors again independent
+    bound = 3 * B if dtype == "bfloat16" else 8 * 2.0 ** -22 + math.sqrt(n * m) * U
+    for a, ref in zip(got, (r["dX"], r["dV"], r["db"])):
+        assert float((a.double() - ref).norm() / ref.norm()) <= (bound if a.dtype != torch.float32 or dtype == "float32" else 2.0 ** -18)
+    again = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp, ibase=b)
+    assert all(torch.equal(a, c) for a, c in zip(got, again))
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_logprob_parts_that_are_not_wanted(torch, sc, dtype):
     X, V, b, ids, dlogp = _case(torch, 50, 300, 70, 3, dtype, True, 5)
@@ -294,6 +315,9 @@ def test_logprob_masks_and_awkward_places(torch, sc):
         assert float((got.double() - ref).abs().max()) < 1e-4 * max(1.0, float(ref.abs().max()))
     assert (dX[0] == 0).all()
     # every item out: no probabilities, -inf, and a gradient through the named items alone
+    out = torch.full_like(b, torch.finfo(torch.float32).min)
+    _, lse = sc.catalogue_logprob(X, V, ids, ibase=out, scale=2.0)
+    assert (lse == float("-inf")).all()
     out = torch.full_like(b, float("-inf"))
     logp, lse = sc.catalogue_logprob(X, V, ids, ibase=out)
     assert (lse == float("-inf")).all() and (logp[ids >= 0] == float("-inf")).all() and (logp[ids < 0] == 0).all()
