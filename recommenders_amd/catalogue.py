@@ -14,6 +14,9 @@ F32, BF16, MXFP4 = 0, 1, 2
 MAX_FACTORS = 256            # IFR_MAX_FACTORS
 MAX_ROWS, MAX_CATALOGUE = 1 << 25, 1 << 28
 
+_KINDS = {"logistic": 0, "hinge": 1, "squared": 2}
+_REDUCTIONS = {"sum": 0, "row": 1, "batch": 2}
+
 PreferenceLoss = namedtuple("PreferenceLoss", "loss h d_chosen d_rejected")
 PolicyLoss = namedtuple("PolicyLoss", "loss kl clipped d_logp")
 
@@ -39,6 +42,12 @@ class MxFp4Matrix:
         if self.codes.data_ptr() % 16:
             self.codes = self.codes.clone()
 
+    @classmethod
+    def _of(cls, codes, scales, k):
+        q = cls.__new__(cls)                     # fresh from quantize_mxfp4: nothing to check
+        q.codes, q.scales, q.k = codes, scales, k
+        return q
+
     @property
     def shape(self):
         return (self.codes.shape[0], self.k)
@@ -52,47 +61,64 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _matrix(t, name, dtypes, cols=None, rows=None, device=None):
-    """`t` as a matrix with contiguous rows at least its width apart; ValueError / TypeError where it is not what `name` is."""
+def _name(dtype):
+    return str(dtype).replace("torch.", "")
+
+
+def _refuse(t, name, dtypes, shape, device):
+    """The refusal of a tensor that `_matrix` or `_vector` does not take."""
     import torch
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be a matrix, not {t.dim()}-dimensional")
     if t.dtype not in dtypes:
-        raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, not {str(t.dtype).replace('torch.', '')}")
-    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {'any' if cols is None else cols}], not {list(t.shape)}")
-    if torch.is_grad_enabled() and t.requires_grad:
-        raise ValueError(f"{name} requires a gradient: autograd does not see this call, pass {name}.detach() and use the gradients it returns")
+        raise TypeError(f"{name} must be {' or '.join(_name(d) for d in dtypes)}, not {_name(t.dtype)}")
+    if t.dim() != len(shape) and len(shape) == 2:
+        raise ValueError(f"{name} must be a matrix, not {t.dim()}-dimensional")
+    if t.dim() != len(shape) or any(w is not None and w != h for w, h in zip(shape, t.shape)):
+        raise ValueError(f"{name} must be [{', '.join('any' if w is None else str(w) for w in shape)}], not {list(t.shape)}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the scorer on {device}")
-    if t.numel() and (t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    raise ValueError(f"{name} requires a gradient: autograd does not see this call, pass {name}.detach() and use the gradients it returns")
+
+
+def _recorded(t):
+    if not t.requires_grad:
+        return False
+    import torch
+    return torch.is_grad_enabled()
+
+
+def _matrix(t, name, dtypes, cols=None, rows=None, device=None):
+    """`t` as a matrix with contiguous rows at least its width apart; ValueError / TypeError where it is not what `name` is."""
+    try:
+        n, w = t.shape
+        fine = t.dtype in dtypes and (rows is None or n == rows) and (cols is None or w == cols) and (device is None or t.device == device)
+        n, stride = n, t.stride()
+    except (AttributeError, TypeError, ValueError):
+        fine = False
+    if not fine or _recorded(t):
+        _refuse(t, name, dtypes, (rows, cols), device)
+    if (stride[1] != 1 and w > 1 or stride[0] < w and n > 1) and n * w:
         t = t.contiguous()
     return t
 
 
-def _vector(t, name, n, device=None, dtype=None):
+def _vector(t, name, n, device=None):
     """None, or `t` as a contiguous vector of n fp32 values."""
-    import torch
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch tensor")
-    if t.dtype != (dtype or torch.float32):
-        raise TypeError(f"{name} must be {str(dtype or torch.float32).replace('torch.', '')}")
-    if tuple(t.shape) != (n,):
-        raise ValueError(f"{name} must be [{n}], not {list(t.shape)}")
-    if torch.is_grad_enabled() and t.requires_grad:
-        raise ValueError(f"{name} requires a gradient: pass {name}.detach()")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the scorer on {device}")
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.shape != (n,) or (device is not None and t.device != device) or _recorded(t):
+        _refuse(t, name, (torch.float32,), (n,), device)
     return t.contiguous()
 
 
 def _row_stride(t):
     """Elements from one row to the next; a single row reaches as far as it is wide."""
-    return 0 if t is None else max(t.stride(0) if t.shape[0] > 1 else 0, t.shape[1])
+    if t is None:
+        return 0
+    n, w = t.shape
+    return max(t.stride(0), w) if n > 1 else w
 
 
 def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
@@ -138,7 +164,7 @@ def check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, ma
         mask_chosen = _matrix(mask_chosen, "mask_chosen", masks, rows=n, cols=chosen.shape[1], device=device)
     if mask_rejected is not None:
         mask_rejected = _matrix(mask_rejected, "mask_rejected", masks, rows=n, cols=rejected.shape[1], device=device)
-    if kind not in ("logistic", "hinge", "squared"):
+    if kind not in _KINDS:
         raise ValueError("kind must be 'logistic', 'hinge' or 'squared'")
     if not 0.0 < float(beta) <= 1e30:
         raise ValueError("beta must be positive")
@@ -164,7 +190,7 @@ def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, c
         mask = _matrix(mask, "mask", (torch.bool, torch.uint8), rows=n, cols=width, device=device)
     if advantages is None:
         raise TypeError("advantages must be a torch tensor")
-    if reduction not in ("sum", "row", "batch"):
+    if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'sum', 'row' or 'batch'")
     if not 0.0 <= float(clip_low) < 1.0 or not 0.0 <= float(clip_high) < 1e30:
         raise ValueError("clip_low must be in [0, 1) and clip_high at least 0")
@@ -176,13 +202,26 @@ def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, c
 
 
 class CatalogueOps:
-    """The catalogue operators of `HipScorer` (engine.py), which supplies `_lib`, `_h`, `device`, `_check` and `_stream`."""
+    """The catalogue operators of `HipScorer` (engine.py), which supplies `_lib`, `_h`, `device` and `_check`."""
 
-    def _workspace(self, fn, *args):
+    def _workspace(self, fn, key, *args):
+        """(workspace, bytes) of a call; `key`: the sizes its length depends on, remembered."""
         import torch
-        need = ctypes.c_int64(0)
-        self._check(fn(self._h, *args, ctypes.byref(need)))
-        return torch.empty(max(1, need.value), dtype=torch.uint8, device=self.device), need.value
+        known = self.__dict__.setdefault("_workspace_bytes", {})
+        need = known.get(key)
+        if need is None:
+            value = ctypes.c_int64(0)
+            self._check(fn(self._h, *args, ctypes.byref(value)))
+            need = value.value
+            if len(known) >= 256:
+                known.clear()
+            known[key] = need
+        return torch.empty(max(1, need), dtype=torch.uint8, device=self.device), need
+
+    def _stream_of(self):
+        """The current stream's handle (the call behind torch.cuda.current_stream, without the object around it)."""
+        import torch
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     # ------------------------------------------------------------------ 4-bit model
     def quantize_mxfp4(self, X):
@@ -197,8 +236,8 @@ class CatalogueOps:
         codes = torch.empty((n, 16 * kb), dtype=torch.uint8, device=self.device)
         scales = torch.empty((n, kb), dtype=torch.uint8, device=self.device)
         self._check(self._lib.ifr_mxfp4_quantize(self._h, _ptr(X), F32 if X.dtype == torch.float32 else BF16, n, k, _row_stride(X),
-                                                 _ptr(codes), _ptr(scales), self._stream()))
-        return MxFp4Matrix(codes, scales, k)
+                                                 _ptr(codes), _ptr(scales), self._stream_of()))
+        return MxFp4Matrix._of(codes, scales, k)
 
     def dequantize_mxfp4(self, q, out=None):
         """The fp32 values [n, k] that an MxFp4Matrix stands for."""
@@ -207,7 +246,7 @@ class CatalogueOps:
             raise ValueError(f"dequantize_mxfp4 takes an MxFp4Matrix on {self.device}")
         out = self._out(out, q.shape, torch.float32)
         self._check(self._lib.ifr_mxfp4_dequantize(self._h, _ptr(q.codes), _ptr(q.scales), q.shape[0], q.k, _ptr(out), _row_stride(out),
-                                                   self._stream()))
+                                                   self._stream_of()))
         return out
 
     def _out(self, out, shape, dtype):
@@ -238,23 +277,18 @@ class CatalogueOps:
         ubase, ibase = _vector(ubase, "ubase", n, self.device), _vector(ibase, "ibase", n_items, self.device)
         out = self._out(out, (n, n_items), dtype)
         self._check(self._lib.ifr_mxfp4_scores(self._h, _ptr(X.codes), _ptr(X.scales), n, _ptr(V.codes), _ptr(V.scales), n_items, X.k, _ptr(ubase),
-                                               _ptr(ibase), _ptr(out), F32 if dtype == torch.float32 else BF16, _row_stride(out), self._stream()))
+                                               _ptr(ibase), _ptr(out), F32 if dtype == torch.float32 else BF16, _row_stride(out), self._stream_of()))
         return out
 
     # ------------------------------------------------------------------ log-probabilities
     def _catalogue(self, X, V, ibase, scale):
         import torch
-        c = _lib.Catalogue()
         mx = isinstance(X, MxFp4Matrix)
-        c.X, c.V = (_ptr(X.codes), _ptr(V.codes)) if mx else (_ptr(X), _ptr(V))
-        c.x_scales, c.v_scales = (_ptr(X.scales), _ptr(V.scales)) if mx else (None, None)
-        c.ibase = _ptr(ibase)
-        c.n, c.k = X.shape
-        c.n_items = V.shape[0]
-        c.ldx, c.ldv = (0, 0) if mx else (_row_stride(X), _row_stride(V))
-        c.dtype = MXFP4 if mx else F32 if X.dtype == torch.float32 else BF16
-        c.scale = float(scale)
-        return c
+        n, k = X.shape
+        if mx:
+            return _lib.Catalogue(X.codes.data_ptr(), V.codes.data_ptr(), X.scales.data_ptr(), V.scales.data_ptr(), _ptr(ibase), n, V.shape[0], 0, 0, k, MXFP4, float(scale))
+        return _lib.Catalogue(X.data_ptr(), V.data_ptr(), None, None, _ptr(ibase), n, V.shape[0], _row_stride(X), _row_stride(V), k,
+                              F32 if X.dtype is torch.float32 else BF16, float(scale))
 
     def catalogue_logprob(self, X, V, ids, ibase=None, scale=1.0):
         """(logp [n, m], lse [n]), fp32: logp[u, j] = z[u, ids[u, j]] - lse[u] with z[u, i] = scale * (<X[u], V[i]> + ibase[i]) and
@@ -267,9 +301,9 @@ class CatalogueOps:
         c = self._catalogue(X, V, ibase, scale)
         logp = torch.empty((n, m), dtype=torch.float32, device=self.device)
         lse = torch.empty((n,), dtype=torch.float32, device=self.device)
-        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_workspace, ctypes.byref(c))
+        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_workspace, (c.n, c.n_items, c.k, c.dtype), ctypes.byref(c))
         self._check(self._lib.ifr_catalogue_logprob(self._h, ctypes.byref(c), _ptr(ids), m, _row_stride(ids), _ptr(logp), max(m, 1), _ptr(lse),
-                                                    _ptr(ws), need, self._stream()))
+                                                    _ptr(ws), need, self._stream_of()))
         return logp, lse
 
     def catalogue_logprob_backward(self, X, V, ids, lse, dlogp, ibase=None, scale=1.0, want=("X", "V", "ibase")):
@@ -292,11 +326,11 @@ class CatalogueOps:
         dV = empty((V.shape[0], V.shape[1]), dtype=V.dtype, device=self.device) if "V" in want else None
         db = empty((V.shape[0],), dtype=torch.float32, device=self.device) if "ibase" in want and ibase is not None else None
         c = self._catalogue(X, V, ibase, scale)
-        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_backward_workspace, ctypes.byref(c), m, int(dX is not None), int(dV is not None),
-                                   int(db is not None))
+        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_backward_workspace, (c.n, c.n_items, c.k, c.dtype, m, dX is None, dV is None, db is None),
+                                   ctypes.byref(c), m, int(dX is not None), int(dV is not None), int(db is not None))
         self._check(self._lib.ifr_catalogue_logprob_backward(self._h, ctypes.byref(c), _ptr(ids), m, _row_stride(ids), _ptr(lse), _ptr(dlogp), _row_stride(dlogp),
                                                              _ptr(dX), 0 if dX is None else _row_stride(dX), _ptr(dV), 0 if dV is None else _row_stride(dV),
-                                                             _ptr(db), _ptr(ws), need, self._stream()))
+                                                             _ptr(db), _ptr(ws), need, self._stream_of()))
         return dX, dV, db
 
     # ------------------------------------------------------------------ losses
@@ -307,22 +341,15 @@ class CatalogueOps:
         the rejected slate and Cr, Rr those of a frozen reference.  kind "logistic": log(1 + exp(-h)), smoothed towards the other
         order by label_smoothing; "hinge": max(0, 1 - h); "squared": ((h - 1/2) / beta)^2.  d_chosen and d_rejected are the
         gradients of sum(weight * loss), weight 1 unless given.  Slates of one item with beta = 1 and no reference are BPR's criterion."""
-        import torch
         chosen, rejected, ref_c, ref_r, mask_c, mask_r, weight = check_preference(
             chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, weight, beta, kind, label_smoothing, margin, self.device)
         n = chosen.shape[0]
-        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=self.device)
-        r = PreferenceLoss(new(n), new(n), new(*chosen.shape), new(*rejected.shape))
-        p = _lib.Preference()
-        p.n, p.len_chosen, p.len_rejected = n, chosen.shape[1], rejected.shape[1]
-        p.kind, p.average = ("logistic", "hinge", "squared").index(kind), int(bool(average))
-        p.chosen, p.rejected, p.ref_chosen, p.ref_rejected = _ptr(chosen), _ptr(rejected), _ptr(ref_c), _ptr(ref_r)
-        p.mask_chosen, p.mask_rejected, p.weight = _ptr(mask_c), _ptr(mask_r), _ptr(weight)
-        p.loss, p.h, p.d_chosen, p.d_rejected = (_ptr(t) for t in r)
-        p.ld_chosen, p.ld_rejected, p.ld_ref_chosen, p.ld_ref_rejected = (_row_stride(t) for t in (chosen, rejected, ref_c, ref_r))
-        p.ld_mask_chosen, p.ld_mask_rejected, p.ld_d_chosen, p.ld_d_rejected = (_row_stride(t) for t in (mask_c, mask_r, r.d_chosen, r.d_rejected))
-        p.beta, p.margin, p.label_smoothing = float(beta), float(margin), float(label_smoothing)
-        self._check(self._lib.ifr_preference_loss(self._h, ctypes.byref(p), self._stream()))
+        r = PreferenceLoss(chosen.new_empty(n), chosen.new_empty(n), chosen.new_empty(chosen.shape), chosen.new_empty(rejected.shape))
+        p = _lib.Preference(n, chosen.shape[1], rejected.shape[1], _KINDS[kind], int(bool(average)), chosen.data_ptr(), rejected.data_ptr(), _ptr(ref_c),
+                            _ptr(ref_r), _ptr(mask_c), _ptr(mask_r), _ptr(weight), r[0].data_ptr(), r[1].data_ptr(), r[2].data_ptr(), r[3].data_ptr(),
+                            _row_stride(chosen), _row_stride(rejected), _row_stride(ref_c), _row_stride(ref_r), _row_stride(mask_c), _row_stride(mask_r),
+                            chosen.shape[1], rejected.shape[1], float(beta), float(margin), float(label_smoothing))
+        self._check(self._lib.ifr_preference_loss(self._h, ctypes.byref(p), self._stream_of()))
         return r
 
     def policy_loss(self, logp, old_logp, advantages, ref_logp=None, mask=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="row", weight=None):
@@ -335,14 +362,10 @@ class CatalogueOps:
         logp, old_logp, advantages, ref_logp, mask, weight = check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef,
                                                                           reduction, self.device)
         n, width = logp.shape
-        new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=self.device)
-        r = PolicyLoss(new(n), None if ref_logp is None else new(n), new(n, dtype=torch.int32), new(n, width))
-        p = _lib.Policy()
-        p.n, p.len, p.reduction = n, width, ("sum", "row", "batch").index(reduction)
-        p.logp, p.old_logp, p.ref_logp, p.advantages, p.weight, p.mask = (_ptr(t) for t in (logp, old_logp, ref_logp, advantages, weight, mask))
-        p.loss, p.kl, p.clipped, p.d_logp = (_ptr(t) for t in r)
-        p.ld_logp, p.ld_old, p.ld_ref, p.ld_mask, p.ld_d_logp = (_row_stride(t) for t in (logp, old_logp, ref_logp, mask, r.d_logp))
-        p.clip_low, p.clip_high, p.kl_coef = float(clip_low), float(clip_high), float(kl_coef)
-        ws, need = self._workspace(self._lib.ifr_policy_loss_workspace, ctypes.byref(p))
-        self._check(self._lib.ifr_policy_loss(self._h, ctypes.byref(p), _ptr(ws), need, self._stream()))
+        r = PolicyLoss(logp.new_empty(n), None if ref_logp is None else logp.new_empty(n), torch.empty(n, dtype=torch.int32, device=self.device), logp.new_empty((n, width)))
+        p = _lib.Policy(n, width, _REDUCTIONS[reduction], logp.data_ptr(), old_logp.data_ptr(), _ptr(ref_logp), advantages.data_ptr(), _ptr(weight), _ptr(mask),
+                        r[0].data_ptr(), _ptr(r[1]), r[2].data_ptr(), r[3].data_ptr(), _row_stride(logp), _row_stride(old_logp), _row_stride(ref_logp),
+                        _row_stride(mask), width, float(clip_low), float(clip_high), float(kl_coef))
+        ws, need = (None, 0) if mask is None or reduction != "batch" else self._workspace(self._lib.ifr_policy_loss_workspace, "policy", ctypes.byref(p))
+        self._check(self._lib.ifr_policy_loss(self._h, ctypes.byref(p), _ptr(ws), need, self._stream_of()))
         return r

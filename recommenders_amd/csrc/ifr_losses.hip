@@ -1,5 +1,8 @@
 // ifr_losses.hip -- what a factor model learns from: the preference loss on paired log ratios and the clipped policy loss with
 // a KL term, each with its gradient in the same call (contracts: include/ifr.h).
+//
+// Both are bound by memory: every element is read once, its gradient written once.  A row belongs to a group of 16, 64, 256 or 1024
+// threads by its length (short rows would leave most of a workgroup idle), which takes it four elements a thread at a time.
 #include <hip/hip_runtime.h>
 
 #include "ifr_losses.h"
@@ -8,28 +11,78 @@ namespace ifr {
 
 namespace {
 
-dim3 grid_of_rows(int64_t n) { return dim3((uint32_t)(n < (1 << 22) ? n : (1 << 22))); }
+constexpr int64_t MAX_GRID = 1 << 20;  // workgroups of one launch; rows beyond come round again
 
-__device__ __forceinline__ double wave_sum(double v)
+// sum over the GROUP threads of a row, the same bits in each of them (GROUP <= 64: lanes of one wave)
+template <int GROUP, typename T>
+__device__ __forceinline__ T group_sum(T v, T *lds)
 {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ __forceinline__ int wave_sum(int v)
-{
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-// sum over the 256 threads, the same bits in every thread
-template <typename T>
-__device__ __forceinline__ T block_sum(T v, T *lds)
-{
-    v = wave_sum(v);
+    for (int o = (GROUP < 64 ? GROUP : 64) / 2; o; o >>= 1) v += __shfl_xor(v, o);
+    if (GROUP <= 64) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    T s = lds[0];
+    for (int w = 1; w < GROUP / 64; ++w) s += lds[w];
+    return s;
+}
+
+// Four neighbouring elements of rows of several arrays at once.  Where all rows begin at the same place modulo four elements, the
+// pieces lie at 16-byte borders (the first and the last may be partial); otherwise, and at the ends, elements are taken one by one.
+struct Pieces {
+    int phase, len;                    // elements of the first piece before the row
+    bool whole;                        // pieces may be taken at once
+    __device__ int count() const { return (len + phase + 3) >> 2; }
+    __device__ int at(int piece) const { return 4 * piece - phase; }
+    __device__ bool full(int t) const { return whole && t >= 0 && t + 4 <= len; }
+};
+
+__device__ __forceinline__ int phase_of(const float *p) { return (int)(((uintptr_t)p >> 2) & 3); }
+__device__ __forceinline__ int phase_of(const uint8_t *p) { return (int)((uintptr_t)p & 3); }
+
+template <typename... P>
+__device__ __forceinline__ Pieces pieces_of(int len, const float *first, P... others)
+{
+    Pieces r;
+    r.len = len;
+    const int f = phase_of(first);
+    r.whole = ((others == nullptr || phase_of(others) == f) && ...);
+    r.phase = r.whole ? f : 0;
+    return r;
+}
+
+__device__ __forceinline__ void take(const Pieces &r, const float *row, int t, float v[4])
+{
+    if (r.full(t)) {
+        const float4 a = *(const float4 *)(row + t);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    } else {
+        for (int j = 0; j < 4; ++j) v[j] = t + j >= 0 && t + j < r.len ? row[t + j] : 0.f;
+    }
+}
+
+// bit j: element j lies in the row and its mask (null: every place) is set
+__device__ __forceinline__ uint32_t take_mask(const Pieces &r, const uint8_t *row, int t)
+{
+    if (r.full(t)) {
+        if (!row) return 15u;
+        const uint32_t w = *(const uint32_t *)(row + t);
+        return (w & 0xffu ? 1u : 0u) | (w & 0xff00u ? 2u : 0u) | (w & 0xff0000u ? 4u : 0u) | (w & 0xff000000u ? 8u : 0u);
+    }
+    uint32_t m = 0;
+    for (int j = 0; j < 4; ++j)
+        if (t + j >= 0 && t + j < r.len && (!row || row[t + j])) m |= 1u << j;
+    return m;
+}
+
+__device__ __forceinline__ void put(const Pieces &r, float *row, int t, const float v[4])
+{
+    if (r.full(t)) {
+        *(float4 *)(row + t) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        for (int j = 0; j < 4; ++j)
+            if (t + j >= 0 && t + j < r.len) row[t + j] = v[j];
+    }
 }
 
 __device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
@@ -60,66 +113,104 @@ __device__ __forceinline__ void preference_of(const ifr_preference &p, float h, 
 
 }  // namespace
 
-// One workgroup a pair: sums of both slates in 64 bits (without a reference the two sums are large and near each other), the
-// loss, and the gradient, which is one number per slate.
-__global__ __launch_bounds__(256) void preference_kernel(ifr_preference p)
+// A group of threads a pair: the sums of both slates in 64 bits (without a reference the two are large and near each other), the loss, and
+// the gradient, which is one number per slate.
+template <int GROUP>
+__global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP) void preference_kernel(ifr_preference p)
 {
-    __shared__ double lds[4];
-    __shared__ int ldsn[4];
-    for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x) {
+    constexpr int BLOCK = GROUP < 256 ? 256 : GROUP, ROWS = BLOCK / GROUP;
+    __shared__ double lds[16];
+    __shared__ int ldsn[16];
+    const int me = threadIdx.x % GROUP;
+    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < p.n; first += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = first + threadIdx.x / GROUP;
+        if (row >= p.n) return;                       // groups within a wave or whole workgroups: nobody waits for this one
         double sum[2];
         int count[2];
+#pragma unroll
         for (int side = 0; side < 2; ++side) {
             const float *x = side ? p.rejected + row * p.ld_rejected : p.chosen + row * p.ld_chosen;
             const float *ref = side ? p.ref_rejected : p.ref_chosen;
             if (ref) ref += row * (side ? p.ld_ref_rejected : p.ld_ref_chosen);
             const uint8_t *mask = side ? p.mask_rejected : p.mask_chosen;
             if (mask) mask += row * (side ? p.ld_mask_rejected : p.ld_mask_chosen);
-            const int len = side ? p.len_rejected : p.len_chosen;
+            const Pieces r = pieces_of(side ? p.len_rejected : p.len_chosen, x, ref, mask);
             double s = 0.0;
             int c = 0;
-            for (int t = threadIdx.x; t < len; t += 256) {
-                if (mask && !mask[t]) continue;
-                s += (double)x[t] - (ref ? (double)ref[t] : 0.0);
-                ++c;
+#pragma unroll 2
+            for (int q = me; q < r.count(); q += GROUP) {
+                const int t = r.at(q);
+                const uint32_t m = take_mask(r, mask, t);
+                float a[4], b[4] = {0.f, 0.f, 0.f, 0.f};
+                take(r, x, t, a);
+                if (ref) take(r, ref, t, b);
+                for (int j = 0; j < 4; ++j)
+                    if (m >> j & 1) s += (double)a[j] - (double)b[j];
+                c += __popc(m);
             }
-            sum[side] = block_sum(s, lds);
-            count[side] = p.average ? max(block_sum(c, ldsn), 1) : 1;
+            sum[side] = group_sum<GROUP>(s, lds);
+            count[side] = p.average ? max(group_sum<GROUP>(c, ldsn), 1) : 1;
         }
         const float h = (float)(p.beta * (sum[0] / count[0] - sum[1] / count[1]) - p.margin);
         float loss, slope;
         preference_of(p, h, &loss, &slope);
         const float g = (p.weight ? p.weight[row] : 1.f) * slope * (float)p.beta;
-        if (threadIdx.x == 0) {
+        if (me == 0) {
             if (p.loss) p.loss[row] = loss;
             if (p.h) p.h[row] = h;
         }
+#pragma unroll
         for (int side = 0; side < 2; ++side) {
             float *out = side ? p.d_rejected : p.d_chosen;
             if (!out) continue;
             out += row * (side ? p.ld_d_rejected : p.ld_d_chosen);
             const uint8_t *mask = side ? p.mask_rejected : p.mask_chosen;
             if (mask) mask += row * (side ? p.ld_mask_rejected : p.ld_mask_chosen);
-            const int len = side ? p.len_rejected : p.len_chosen;
+            const Pieces r = pieces_of(side ? p.len_rejected : p.len_chosen, out, mask);
             const float v = (side ? -g : g) / (float)count[side];
-            for (int t = threadIdx.x; t < len; t += 256) out[t] = mask && !mask[t] ? 0.f : v;
+            for (int q = me; q < r.count(); q += GROUP) {
+                const int t = r.at(q);
+                const uint32_t m = take_mask(r, mask, t);
+                const float o[4] = {m & 1 ? v : 0.f, m & 2 ? v : 0.f, m & 4 ? v : 0.f, m & 8 ? v : 0.f};
+                put(r, out, t, o);
+            }
         }
     }
 }
 
+namespace {
+
+// threads of a row
+int group_of(int64_t len) { return len <= 64 ? 16 : len <= 2048 ? 64 : len <= 8192 ? 256 : 1024; }
+
+dim3 grid_of(int64_t n, int group)
+{
+    const int64_t rows = group < 256 ? 256 / group : 1, want = (n + rows - 1) / rows;
+    return dim3((uint32_t)(want < MAX_GRID ? want : MAX_GRID));
+}
+
+}  // namespace
+
 int launch_preference(const ifr_preference &p, hipStream_t s)
 {
-    hipLaunchKernelGGL(preference_kernel, grid_of_rows(p.n), dim3(256), 0, s, p);
+    const int group = group_of(p.len_chosen > p.len_rejected ? p.len_chosen : p.len_rejected);
+    const dim3 grid = grid_of(p.n, group);
+    if (group == 16) hipLaunchKernelGGL(preference_kernel<16>, grid, dim3(256), 0, s, p);
+    else if (group == 64) hipLaunchKernelGGL(preference_kernel<64>, grid, dim3(256), 0, s, p);
+    else if (group == 256) hipLaunchKernelGGL(preference_kernel<256>, grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(preference_kernel<1024>, grid, dim3(1024), 0, s, p);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
 // ---------------------------------------------------------------------------- policy
 
-// exp(q) - q - 1: the series where the difference would cancel
-__device__ __forceinline__ float kl_term(float q)
+// exp(q) - 1 and exp(q) - 1 - q: below 1 by the series of the second, where the difference would cancel
+__device__ __forceinline__ void exp_terms(float q, float *m1, float *kl)
 {
-    if (fabsf(q) < 0.5f) {
-        float s = 2.7557319e-7f;                      // 1 / 10!
+    if (fabsf(q) < 1.f) {
+        float s = 2.0876757e-9f;                      // 1 / 12!
+        s = fmaf(s, q, 2.5052108e-8f);
+        s = fmaf(s, q, 2.7557319e-7f);
         s = fmaf(s, q, 2.7557319e-6f);
         s = fmaf(s, q, 2.4801587e-5f);
         s = fmaf(s, q, 1.9841270e-4f);
@@ -128,90 +219,123 @@ __device__ __forceinline__ float kl_term(float q)
         s = fmaf(s, q, 4.1666667e-2f);
         s = fmaf(s, q, 1.6666667e-1f);
         s = fmaf(s, q, 0.5f);
-        return s * q * q;
+        *kl = s * q * q;
+        *m1 = *kl + q;
+    } else {
+        *m1 = expm1f(q);
+        *kl = *m1 - q;
     }
-    return expm1f(q) - q;
 }
 
 enum { COUNT_BLOCKS = 1024 };
 
-// masked elements of the batch, one partial count a workgroup (whole numbers: any order gives the same total)
+__device__ __forceinline__ int set_bytes(uint32_t w) { return __popc((((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) & 0x80808080u); }
+
+// places of the batch, one partial count a workgroup (whole numbers: any order gives the same total)
 __global__ __launch_bounds__(256) void policy_count_kernel(ifr_policy p, int64_t *part)
 {
-    __shared__ int lds[4];
+    __shared__ int64_t lds[4];
     int64_t total = 0;
-    for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x) {
-        const uint8_t *mask = p.mask + row * p.ld_mask;
-        int c = 0;
-        for (int t = threadIdx.x; t < p.len; t += 256) c += mask[t] != 0;
-        total += block_sum(c, lds);
+    const int64_t me = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
+    if (p.ld_mask == p.len || p.n == 1) {             // one row of bytes
+        const int64_t bytes = p.n * p.len;
+        const int64_t head = min((int64_t)((16 - ((uintptr_t)p.mask & 15)) & 15), bytes), body = (bytes - head) / 16;
+        for (int64_t i = me; i < body; i += all) {
+            const uint4 w = ((const uint4 *)(p.mask + head))[i];
+            total += set_bytes(w.x) + set_bytes(w.y) + set_bytes(w.z) + set_bytes(w.w);
+        }
+        if (me < head) total += p.mask[me] != 0;
+        if (me < bytes - head - body * 16) total += p.mask[head + body * 16 + me] != 0;
+    } else {
+        for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x)
+            for (int t = threadIdx.x; t < p.len; t += 256) total += p.mask[row * p.ld_mask + t] != 0;
     }
+    total = group_sum<256>(total, lds);
     if (threadIdx.x == 0) part[blockIdx.x] = total;
 }
 
-__global__ __launch_bounds__(256) void policy_kernel(ifr_policy p, const int64_t *part, int n_part, float hi, float lo)
+template <int GROUP>
+__global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP) void policy_kernel(ifr_policy p, const int64_t *part, int n_part, float hi, float lo)
 {
-    __shared__ double lds[4];
-    __shared__ int ldsn[4];
-    for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x) {
+    constexpr int BLOCK = GROUP < 256 ? 256 : GROUP, ROWS = BLOCK / GROUP;
+    __shared__ double lds[16];
+    __shared__ int ldsn[16];
+    __shared__ int64_t ldsl[16];
+    const int me = threadIdx.x % GROUP;
+    const float most = (float)(1.0 + p.clip_high), least = (float)(1.0 - p.clip_low), kl_coef = (float)p.kl_coef;
+    double all = 1.0;
+    if (p.reduction == IFR_POLICY_BATCH) {
+        int64_t c = (int64_t)p.n * p.len;
+        if (part) {
+            c = 0;
+            for (int i = threadIdx.x; i < n_part; i += BLOCK) c += part[i];
+            c = group_sum<BLOCK>(c, ldsl);
+        }
+        all = c > 1 ? (double)c : 1.0;
+    }
+    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < p.n; first += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = first + threadIdx.x / GROUP;
+        if (row >= p.n) return;
         const uint8_t *mask = p.mask ? p.mask + row * p.ld_mask : nullptr;
-        int count = p.len;
-        if (mask) {
-            int c = 0;
-            for (int t = threadIdx.x; t < p.len; t += 256) c += mask[t] != 0;
-            count = block_sum(c, ldsn);
-        }
-        float scale = p.weight ? p.weight[row] : 1.f;
-        if (p.reduction == IFR_POLICY_ROW) scale /= (float)max(count, 1);
-        else if (p.reduction == IFR_POLICY_BATCH) {
-            double all = 0.0;                             // counts below 2^53: exact
-            if (part) {
-                for (int i = threadIdx.x; i < n_part; i += 256) all += (double)part[i];
-                all = block_sum(all, lds);
-            } else {
-                all = (double)p.n * p.len;
-            }
-            scale = (float)((double)scale / (all > 1.0 ? all : 1.0));
-        }
-        const float A = p.advantages[row], kl_coef = (float)p.kl_coef;
-        const float most = (float)(1.0 + p.clip_high), least = (float)(1.0 - p.clip_low);
         const float *logp = p.logp + row * p.ld_logp, *old = p.old_logp + row * p.ld_old;
         const float *ref = p.ref_logp ? p.ref_logp + row * p.ld_ref : nullptr;
         float *out = p.d_logp ? p.d_logp + row * p.ld_d_logp : nullptr;
+        const Pieces r = pieces_of(p.len, logp, old, ref, (const float *)out, mask);
+        const float weight = p.weight ? p.weight[row] : 1.f, A = p.advantages[row];
+        int count = p.len;
+        if (mask && p.reduction == IFR_POLICY_ROW) {
+            int c = 0;
+            for (int q = me; q < r.count(); q += GROUP) c += __popc(take_mask(r, mask, r.at(q)));
+            count = group_sum<GROUP>(c, ldsn);
+        }
+        const float scale = p.reduction == IFR_POLICY_SUM ? weight : p.reduction == IFR_POLICY_ROW ? weight / (float)max(count, 1) : (float)(weight / all);
         double loss = 0.0, kl = 0.0;
-        int clipped = 0;
-        for (int t = threadIdx.x; t < p.len; t += 256) {
-            float g = 0.f;
-            if (!mask || mask[t]) {
-                const float d = logp[t] - old[t];
+        int clipped = 0, places = 0;
+        for (int q = me; q < r.count(); q += GROUP) {
+            const int t = r.at(q);
+            const uint32_t m = take_mask(r, mask, t);
+            float a[4], b[4], c[4], g[4];
+            take(r, logp, t, a);
+            take(r, old, t, b);
+            if (ref) take(r, ref, t, c);
+            float loss4 = 0.f, kl4 = 0.f;
+            for (int j = 0; j < 4; ++j) {
+                g[j] = 0.f;
+                if (!(m >> j & 1)) continue;
+                const float d = a[j] - b[j];
                 const bool over = A > 0.f && d > hi, under = A < 0.f && d < lo;
                 float term;
                 if (over || under) {
                     term = -A * (over ? most : least);
                     ++clipped;
                 } else {
-                    g = -A * expf(d);
-                    term = g;
+                    g[j] = -A * expf(d);
+                    term = g[j];
                 }
                 if (ref) {
-                    const float q = ref[t] - logp[t], m = kl_term(q);
-                    kl += m;
-                    term += kl_coef * m;
-                    g -= kl_coef * expm1f(q);
+                    float m1, k;
+                    exp_terms(c[j] - a[j], &m1, &k);
+                    kl4 += k;
+                    term = fmaf(kl_coef, k, term);
+                    g[j] -= kl_coef * m1;
                 }
-                loss += term;
-                g *= scale;
+                loss4 += term;
+                g[j] *= scale;
             }
-            if (out) out[t] = g;
+            loss += loss4;
+            kl += kl4;
+            places += __popc(m);
+            if (out) put(r, out, t, g);
         }
-        loss = block_sum(loss, lds);
-        if (threadIdx.x == 0 && p.loss) p.loss[row] = (float)(loss * scale);
+        loss = group_sum<GROUP>(loss, lds);
+        if (me == 0 && p.loss) p.loss[row] = (float)(loss * scale);
         if (p.kl) {
-            kl = block_sum(kl, lds);
-            if (threadIdx.x == 0) p.kl[row] = (float)(kl / max(count, 1));
+            kl = group_sum<GROUP>(kl, lds);
+            places = group_sum<GROUP>(places, ldsn);
+            if (me == 0) p.kl[row] = (float)(kl / max(places, 1));
         }
-        clipped = block_sum(clipped, ldsn);
-        if (threadIdx.x == 0 && p.clipped) p.clipped[row] = clipped;
+        clipped = group_sum<GROUP>(clipped, ldsn);
+        if (me == 0 && p.clipped) p.clipped[row] = clipped;
     }
 }
 
@@ -222,13 +346,19 @@ int launch_policy(const ifr_policy &p, void *ws, hipStream_t s)
     int64_t *part = nullptr;
     int n_part = 0;
     if (policy_workspace(p)) {
+        const int64_t want = (p.n * p.len + 4095) / 4096;
         part = (int64_t *)ws;
-        n_part = (int)(p.n < COUNT_BLOCKS ? p.n : COUNT_BLOCKS);
+        n_part = (int)(want < 1 ? 1 : want < COUNT_BLOCKS ? want : COUNT_BLOCKS);
         hipLaunchKernelGGL(policy_count_kernel, dim3(n_part), dim3(256), 0, s, p, part);
     }
     // the clip borders as logarithms, rounded once: log p - log p_old is compared with them
-    hipLaunchKernelGGL(policy_kernel, grid_of_rows(p.n), dim3(256), 0, s, p, part, n_part, (float)log1p(p.clip_high),
-                       (float)log1p(-p.clip_low));
+    const float hi = (float)log1p(p.clip_high), lo = (float)log1p(-p.clip_low);
+    const int group = group_of(p.len);
+    const dim3 grid = grid_of(p.n, group);
+    if (group == 16) hipLaunchKernelGGL(policy_kernel<16>, grid, dim3(256), 0, s, p, part, n_part, hi, lo);
+    else if (group == 64) hipLaunchKernelGGL(policy_kernel<64>, grid, dim3(256), 0, s, p, part, n_part, hi, lo);
+    else if (group == 256) hipLaunchKernelGGL(policy_kernel<256>, grid, dim3(256), 0, s, p, part, n_part, hi, lo);
+    else hipLaunchKernelGGL(policy_kernel<1024>, grid, dim3(1024), 0, s, p, part, n_part, hi, lo);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
