@@ -74,105 +74,161 @@ __device__ __forceinline__ void online(const v16f &d, float c, float &m, float &
 
 // ---------------------------------------------------------------------------- preparation
 
-// A matrix in the order the matrix instructions read it, 32 rows a workgroup, zeros behind the last row and column:
+// A matrix in the order the matrix instructions read it, by tiles of 32 rows, zeros behind the last row and column:
 //   f1 [tile][part][KP / 16][lane][8]: row lane % 32, columns 16 s + 8 (lane / 32) + 0..7                 (first product)
 //   f2 [tile][part][KP / 32][2][lane][8]: column 32 kb + lane % 32, rows 16 c + 8 (j / 4) + 4 (lane / 32) + j % 4   (second)
 //   exps [tile]: the tile's exponent (split operands); infinities and NaN do not count for it and stay what they are
-// `row_factor` multiplies each row (G x).  Memory-bound: one read, one write for each order.
+struct PrepParams {
+    const void *V, *X;
+    int64_t ldv, ldx, n_items, n, v_tiles;
+    int k, KP;
+    int *v_exp, *x_exp, *g_exp;
+    uint4 *v_f1, *v_f2, *x_f1, *g_f2;  // any may be null; g: rows of X times G
+    const float *ibase;
+    float base_unit;                   // item_term = base_unit ibase, -inf behind the last item
+    float *item_term;
+    // gradient only (lse null otherwise)
+    const float *lse, *dlogp;
+    const int32_t *ids;
+    int64_t m, ld_ids, ld_dlogp, places_padded;
+    float *user_term, *G;              // -log2(e) lse, -inf behind the last user; the sum of a user's upstream gradients
+    int32_t *places;                   // the items named in (user, place) order, -1 behind the last place; null: not wanted
+    uint8_t *named;                    // [items / 64], cleared before: set where an item is named; or null
+};
+
+// LDS tile -> fragments; `factor` (of the tile's rows) and the exponent are applied on the way
+template <int NS>
+__device__ __forceinline__ void store_fragments(const float *tile, int W, int KP, const float *factor, int e, bool second, int64_t at, uint4 *f)
+{
+    const int per = KP / 16 * 64;                     // 16-byte pieces of one part of a tile
+    for (int i = threadIdx.x; i < per; i += 256) {
+        const int l = i & 63, s = i >> 6, q = l & 31, h = l >> 5;
+        float v[8];
+        for (int j = 0; j < 8; ++j) {
+            const int r = second ? 16 * (s & 1) + 8 * (j >> 2) + 4 * h + (j & 3) : q;
+            const int c = second ? 32 * (s >> 1) + q : 16 * s + 8 * h + j;
+            v[j] = tile[r * W + c];
+            if (factor) v[j] *= factor[r];
+        }
+        if (NS == 1) {
+            b8 o;
+            for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
+            f[at * per + i] = __builtin_bit_cast(uint4, o);
+        } else {
+            h8 hi, lo;
+            for (int j = 0; j < 8; ++j) {
+                const float x = ldexpf(v[j], e);
+                hi[j] = (_Float16)x;
+                lo[j] = (_Float16)(x - (float)hi[j]);
+            }
+            f[at * 2 * per + i] = __builtin_bit_cast(uint4, hi);
+            f[(at * 2 + 1) * per + i] = __builtin_bit_cast(uint4, lo);
+        }
+    }
+}
+
+// Everything the walks read, a workgroup a tile of 32 rows of V (first) or X.  Memory-bound: one read, one write for each order.
 template <typename T, int NS>
-__global__ __launch_bounds__(256) void fragments_kernel(const T *src, int64_t rows, int k, int64_t ld, const float *row_factor, int KP, int *exps, uint4 *f1,
-                                                        uint4 *f2)
+__global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
 {
     extern __shared__ float tile[];                   // [32][KP + 1]
-    __shared__ float tops[4];
-    const int W = KP + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r0 = (int64_t)blockIdx.x * 32;
+    __shared__ float tops[4], sums[256], factor[32];
+    const int W = p.KP + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool of_v = blockIdx.x < p.v_tiles;
+    const int64_t at = of_v ? blockIdx.x : blockIdx.x - p.v_tiles, r0 = at * 32;
+    const T *src = (const T *)(of_v ? p.V : p.X);
+    const int64_t rows = of_v ? p.n_items : p.n, ld = of_v ? p.ldv : p.ldx;
+    uint4 *f1 = of_v ? p.v_f1 : p.x_f1;
+    auto highest = [&](float v) {                     // over the workgroup
+        for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+        __syncthreads();
+        if (lane == 0) tops[wave] = v;
+        __syncthreads();
+        return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    };
     float top = 0.f;
-    for (int r = wave; r < 32; r += 4) {
-        const bool in = r0 + r < rows;
-        const float f = in && row_factor ? row_factor[r0 + r] : 1.f;
-        for (int c = lane; c < KP; c += 64) {
-            float v = in && c < k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
-            if (row_factor) v *= f;
+    for (int r = wave; r < 32; r += 4)
+        for (int c = lane; c < p.KP; c += 64) {
+            const float v = r0 + r < rows && c < p.k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
             tile[r * W + c] = v;
             if (NS == 2 && fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
         }
-    }
-    if (NS == 2) {
-        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        if (lane == 0) tops[wave] = top;
-    }
-    __syncthreads();
     int e = 0;
     if (NS == 2) {
-        e = split_exponent(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-        if (threadIdx.x == 0) exps[blockIdx.x] = e;
+        e = split_exponent(highest(top));
+        int *exps = of_v ? p.v_exp : p.x_exp;
+        if (threadIdx.x == 0 && exps) exps[at] = e;
     }
-    for (int which = 0; which < 2; ++which) {
-        uint4 *f = which ? f2 : f1;
-        if (!f) continue;
-        const int per = KP / 16 * 64;                 // 16-byte pieces of one part of a tile
-        for (int i = threadIdx.x; i < per; i += 256) {
-            const int l = i & 63, s = i >> 6, q = l & 31, h = l >> 5;
-            float v[8];
-            for (int j = 0; j < 8; ++j) {
-                const int r = which ? 16 * (s & 1) + 8 * (j >> 2) + 4 * h + (j & 3) : q;
-                const int c = which ? 32 * (s >> 1) + q : 16 * s + 8 * h + j;
-                v[j] = tile[r * W + c];
-            }
-            if (NS == 1) {
-                b8 o;
-                for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
-                f[(int64_t)blockIdx.x * per + i] = __builtin_bit_cast(uint4, o);
-            } else {
-                h8 hi, lo;
-                for (int j = 0; j < 8; ++j) {
-                    const float x = ldexpf(v[j], e);
-                    hi[j] = (_Float16)x;
-                    lo[j] = (_Float16)(x - (float)hi[j]);
+    __syncthreads();
+    if (f1) store_fragments<NS>(tile, W, p.KP, nullptr, e, false, at, f1);
+    if (of_v) {
+        if (p.v_f2) store_fragments<NS>(tile, W, p.KP, nullptr, e, true, at, p.v_f2);
+        if (threadIdx.x < 32) {
+            const int64_t i = r0 + threadIdx.x;
+            p.item_term[i] = i < p.n_items ? (p.ibase ? p.ibase[i] * p.base_unit : 0.f) : -INFINITY;
+        }
+        return;
+    }
+    if (!p.lse) return;
+    {   // G over the places that hold an item: eight threads a user, their sums added in their order
+        const int r = threadIdx.x >> 3;
+        const int64_t u = r0 + r;
+        float g = 0.f;
+        if (u < p.n)
+            for (int64_t j = threadIdx.x & 7; j < p.m; j += 8)
+                if (p.ids[u * p.ld_ids + j] >= 0) g += p.dlogp[u * p.ld_dlogp + j];
+        sums[threadIdx.x] = g;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int64_t u = r0 + threadIdx.x;
+        float g = 0.f;
+        for (int q = 0; q < 8; ++q) g += sums[threadIdx.x * 8 + q];
+        factor[threadIdx.x] = g;
+        p.G[u] = g;
+        // no probabilities where lse is -inf: every exponential is 0
+        p.user_term[u] = u < p.n && p.lse[u] != -INFINITY ? -p.lse[u] * LOG2E : -INFINITY;
+    }
+    __syncthreads();
+    if (p.g_f2) {
+        int eg = 0;
+        if (NS == 2) {
+            float t = 0.f;
+            for (int r = wave; r < 32; r += 4)
+                for (int c = lane; c < p.KP; c += 64) {
+                    const float v = fabsf(tile[r * W + c] * factor[r]);
+                    if (v < INFINITY) t = fmaxf(t, v);
                 }
-                f[((int64_t)blockIdx.x * 2) * per + i] = __builtin_bit_cast(uint4, hi);
-                f[((int64_t)blockIdx.x * 2 + 1) * per + i] = __builtin_bit_cast(uint4, lo);
+            eg = split_exponent(highest(t));
+            if (threadIdx.x == 0) p.g_exp[at] = eg;
+        }
+        store_fragments<NS>(tile, W, p.KP, factor, eg, true, at, p.g_f2);
+    }
+    if (p.places) {
+        const int64_t all = p.n * p.m;
+        const int64_t from = min(r0 * p.m, all), to = r0 + 32 >= p.n ? (r0 < p.n ? p.places_padded : from) : (r0 + 32) * p.m;
+        for (int64_t i = from + threadIdx.x; i < to; i += 256) {
+            int32_t id = -1;
+            if (i < all) {
+                const int32_t r = (int32_t)((i - from) / (int32_t)p.m);          // below 32 m, at most 2^25
+                id = p.ids[(r0 + r) * p.ld_ids + (i - from - (int64_t)r * p.m)];
+                if (p.named && id >= 0 && id < p.n_items) p.named[id >> 6] = 1;
             }
+            p.places[i] = id;
         }
     }
 }
 
-// Per-row terms in powers of two: the item side scale log2(e) b_i, the user side -log2(e) lse_u; -inf behind the last row.
-__global__ __launch_bounds__(256) void item_terms_kernel(const float *ibase, int64_t n, int64_t padded, float c, float *out, uint8_t *named)
+__global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+// the terms alone, for the 4-bit walk
+__global__ __launch_bounds__(256) void item_terms_kernel(const float *ibase, int64_t n, int64_t padded, float *out)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (named && i < padded && (i & 63) == 0) named[i >> 6] = 0;
-    if (i < padded) out[i] = i < n ? (ibase ? ibase[i] * c : 0.f) : -INFINITY;
-}
-
-// ... and G, the sum of a user's upstream gradients over the places that hold an item (in place order)
-__global__ __launch_bounds__(256) void user_terms_kernel(const float *lse, const int32_t *ids, int64_t m, int64_t ld_ids, const float *dlogp,
-                                                         int64_t ld_dlogp, int64_t n, int64_t padded, float *term, float *G)
-{
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (u >= padded) return;
-    float t = -INFINITY, g = 0.f;
-    if (u < n) {
-        t = lse[u] == -INFINITY ? -INFINITY : -lse[u] * LOG2E;      // no probabilities: every exponential is 0
-        for (int64_t j = 0; j < m; ++j)
-            if (ids[u * ld_ids + j] >= 0) g += dlogp[u * ld_dlogp + j];
-    }
-    term[u] = t;
-    G[u] = g;
-}
-
-// The places as one list in (user, place) order, padded with empty ones: what the gradient of V looks its items up in.  `named` was
-// cleared by item_terms_kernel; whoever sets a byte sets it to the same.
-__global__ __launch_bounds__(256) void places_kernel(const int32_t *ids, int64_t m, int64_t ld_ids, int64_t n, int64_t n_items, int64_t padded, int32_t *list,
-                                                     uint8_t *named)
-{
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < padded; i += (int64_t)gridDim.x * 256) {
-        const uint32_t u = (uint32_t)i / (uint32_t)m;                           // at most 2^32 places
-        const int32_t id = i < n * m ? ids[u * ld_ids + (i - u * m)] : -1;
-        list[i] = id;
-        if (id >= 0 && id < n_items) named[id >> 6] = 1;
-    }
+    if (i < padded) out[i] = i < n ? (ibase ? ibase[i] : 0.f) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------- the walk
@@ -182,7 +238,7 @@ enum { WALK_STATS = 0, WALK_GRAD = 1, WALK_GRAD_BASE = 2 };     // ..._BASE: wit
 // What the gradient of V needs to finish its rows in the kernel that summed them (one split): see finish_rows.
 struct Finish {
     const int32_t *places;             // [n_places, padded to 1024]: items named, in (user, place) order
-    const uint8_t *named;              // [n_items / 64]: whether one of 64 items is
+    const uint8_t *named;              // [n_items / 64]: whether one of 64 items is, or null
     const void *X;                     // [n][ldx]
     const float *dlogp;
     void *dV;                          // [n_items][ld_dv] or null
@@ -195,7 +251,7 @@ struct Finish {
 
 struct WalkParams {
     const uint4 *s_f1, *t_f1, *t_f2;
-    const float *s_term, *t_term;      // powers of two added to the score (see item_terms_kernel, user_terms_kernel)
+    const float *s_term, *t_term;      // powers of two added to the score (item_term, user_term of prepare_kernel)
     const float *t_factor;             // WALK_GRAD_BASE: sum_t factor P -> out_b
     const int *s_exp, *t_exp, *t2_exp; // split operands: exponents of their tiles
     float c;                           // scale log2(e)
@@ -288,7 +344,7 @@ __device__ void finish_rows(const Finish &f, float *rows, float *row_b, uint32_t
     const int64_t steps = (f.n_places + 64 * EACH - 1) / (64 * EACH);          // of a wave, over all places
     int64_t step = steps * wave / 4;
     const int64_t end = steps * (wave + 1) / 4;
-    bool more = f.n_places > 0 && f.named[i0 >> 6];
+    bool more = f.n_places > 0 && (!f.named || f.named[i0 >> 6]);
     while (more) {
         int held = 0;
         int32_t id[EACH], next[EACH];
@@ -925,45 +981,63 @@ __global__ __launch_bounds__(256) void targets_kernel(Targets t)
 }
 
 // dX = scale (sum over the places of g v - G acc): four columns a thread
+struct JoinDx {
+    const float *acc, *G;
+    const void *V;
+    const int32_t *ids;
+    const float *dlogp;
+    void *dX;
+    int64_t s_padded, ldv, n_items, m, ld_ids, ld_dlogp, n, ld_dx;
+    int splits, KP, k, vec_v;
+    float scale;
+    int64_t blocks;                    // workgroups it takes
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void join_dx_kernel(const float *acc, int splits, int64_t s_padded, int KP, const float *G, const T *V, int64_t ldv,
-                                                      int64_t n_items, int k, float scale, const int32_t *ids, int64_t m, int64_t ld_ids,
-                                                      const float *dlogp, int64_t ld_dlogp, int64_t n, T *dX, int64_t ld_dx)
+__device__ __forceinline__ void join_dx(const JoinDx &p, int64_t block)
 {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t u = at / (KP / 4);
-    const int c = (int)(at - u * (KP / 4)) * 4;
-    if (u >= n || c >= k) return;
+    const int64_t at = block * 256 + threadIdx.x;
+    const int64_t u = at / (p.KP / 4);
+    const int c = (int)(at - u * (p.KP / 4)) * 4;
+    if (u >= p.n || c >= p.k) return;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int q = 0; q < splits; ++q) {
-        const float4 v = *(const float4 *)(acc + ((int64_t)q * s_padded + u) * KP + c);
+    for (int q = 0; q < p.splits; ++q) {
+        const float4 v = *(const float4 *)(p.acc + ((int64_t)q * p.s_padded + u) * p.KP + c);
         a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
-    const float g0 = -G[u];
+    const float g0 = -p.G[u];
     float r[4] = {g0 * a.x, g0 * a.y, g0 * a.z, g0 * a.w};
 #pragma unroll 4
-    for (int64_t j = 0; j < m; ++j) {
-        const int32_t id = ids[u * ld_ids + j];
-        const bool in = id >= 0 && id < n_items;
-        const float g = in ? dlogp[u * ld_dlogp + j] : 0.f;
-        const T *v = V + (int64_t)(in ? id : 0) * ldv + c;
-        for (int e = 0; e < 4; ++e)
-            if (in && c + e < k) r[e] = fmaf(g, as_f32(v[e]), r[e]);
+    for (int64_t j = 0; j < p.m; ++j) {
+        const int32_t id = p.ids[u * p.ld_ids + j];
+        if (id < 0 || id >= p.n_items) continue;
+        const float g = p.dlogp[u * p.ld_dlogp + j];
+        float v[4];
+        load4((const T *)p.V + (int64_t)id * p.ldv, c, p.k, p.vec_v, v);
+        for (int e = 0; e < 4; ++e) r[e] = fmaf(g, v[e], r[e]);
     }
+    T *out = (T *)p.dX + u * p.ld_dx;
     for (int e = 0; e < 4; ++e)
-        if (c + e < k) dX[u * ld_dx + c + e] = (T)(scale * r[e]);
+        if (c + e < p.k) out[c + e] = (T)(p.scale * r[e]);
 }
 
-// dV and db where the walk was split: the splits' sums of 64 items, then the same last steps
+template <typename T>
+__global__ __launch_bounds__(256) void join_dx_kernel(JoinDx p) { join_dx<T>(p, blockIdx.x); }
+
+// dV and db where the walk was split: the splits' sums of 64 items, then the same last steps.  The first x.blocks workgroups do dX.
 template <typename T, int KP>
-__global__ __launch_bounds__(256) void join_dv_kernel(const float *acc, const float *acc_b, int splits, int64_t s_padded, Finish f)
+__global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, const float *acc_b, int splits, int64_t s_padded, Finish f)
 {
     __shared__ float rows[64 * KP];
     __shared__ uint32_t list[list_length(KP) * 2];
     __shared__ float row_b[64], aside[aside_floats(KP)];
     __shared__ int counts[4], aside_item[32];
-    const int64_t i0 = (int64_t)blockIdx.x * 64;
+    if (blockIdx.x < x.blocks) {
+        join_dx<T>(x, blockIdx.x);
+        return;
+    }
+    const int64_t i0 = (blockIdx.x - x.blocks) * 64;
     for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -1041,11 +1115,10 @@ Side side(Pieces &w, int64_t rows, int KP, int NS, bool want1, bool want2)
 }
 
 template <typename T>
-void fill_side(const Side &d, const T *src, int k, int64_t ld, const float *row_factor, int KP, hipStream_t s)
+void launch_prepare(const PrepParams &p, int64_t x_tiles, hipStream_t s)
 {
     constexpr int NS = sizeof(T) == 4 ? 2 : 1;
-    hipLaunchKernelGGL((fragments_kernel<T, NS>), dim3((uint32_t)d.tiles), dim3(256), 32 * (KP + 1) * sizeof(float), s, src, d.rows, k, ld, row_factor, KP,
-                       d.exps, d.f1, d.f2);
+    hipLaunchKernelGGL((prepare_kernel<T, NS>), dim3((uint32_t)(p.v_tiles + x_tiles)), dim3(256), 32 * (p.KP + 1) * sizeof(float), s, p);
 }
 
 #define IFR_FOR_FACTORS(KP, CALL)                                                                                     \
@@ -1120,7 +1193,7 @@ ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c)
 
 struct BackwardPlan {
     Side x, v, xg;                     // xg: rows times G, second product of dV
-    float *item_term, *user_term, *G, *acc, *acc_b;
+    float *item_term, *user_term, *G, *acc_x, *acc_v, *acc_b;
     int32_t *places;
     uint8_t *named;
     int64_t places_padded;
@@ -1131,22 +1204,24 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
 {
     BackwardPlan p = {};
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
+    const bool items = dv || db;
     p.x = side(w, c.n, KP, NS, true, false);
     p.v = side(w, c.n_items, KP, NS, true, dx);
-    p.xg = side(w, c.n, KP, NS, false, dv || db);
+    p.xg = side(w, c.n, KP, NS, false, items);
     p.item_term = w.take<float>(p.v.padded + 32);     // a stage fetches 64 terms, also where it holds 32 rows
     p.user_term = w.take<float>(p.x.padded + 32);
     p.G = w.take<float>(p.x.padded + 32);
-    p.places_padded = dv || db ? up(c.n * m, 1024) : 0;
+    p.places_padded = items ? up(c.n * m, 1024) : 0;
     p.places = w.take<int32_t>(p.places_padded);
-    p.named = w.take<uint8_t>(p.places_padded ? p.v.padded / 64 : 0);
+    // flags save the search where most groups of 64 items are not named; where the places are as many as the groups, none is saved
+    p.named = w.take<uint8_t>(p.places_padded && c.n_items > 64 * c.n * m ? up(p.v.padded / 64, 4) : 0);
     const int resident = resident_blocks(KP, NS, WALK_GRAD);
     p.split_x = split_plan(p.x.padded / S_ROWS, p.v.tiles, 2, resident, 0.05);
     p.split_v = split_plan(p.v.padded / S_ROWS, p.x.tiles, 2, resident, 0.5);
-    const int64_t ax = dx ? p.split_x.count * p.x.padded * KP : 0;
-    const int64_t av = (dv || db) && p.split_v.count > 1 ? p.split_v.count * p.v.padded * KP : 0;
-    p.acc = w.take<float>(ax > av ? ax : av);         // dX is joined before dV is begun
-    p.acc_b = w.take<float>(db && p.split_v.count > 1 ? p.split_v.count * p.v.padded : 0);
+    const bool parts = items && p.split_v.count > 1;
+    p.acc_x = w.take<float>(dx ? p.split_x.count * p.x.padded * KP : 0);
+    p.acc_v = w.take<float>(parts ? p.split_v.count * p.v.padded * KP : 0);
+    p.acc_b = w.take<float>(db && parts ? p.split_v.count * p.v.padded : 0);
     return p;
 }
 
@@ -1166,19 +1241,27 @@ size_t logprob_backward_workspace(const ifr_catalogue &c, int64_t m, bool want_d
     return w.used;
 }
 
+static PrepParams prepare_sides(const ifr_catalogue &c, const Side &x, const Side &v, float *item_term)
+{
+    PrepParams p = {};
+    p.V = c.V; p.X = c.X; p.ldv = c.ldv; p.ldx = c.ldx; p.n_items = c.n_items; p.n = c.n; p.v_tiles = v.tiles;
+    p.k = c.k; p.KP = pad_factors(c.k);
+    p.v_exp = v.exps; p.x_exp = x.exps; p.v_f1 = v.f1; p.v_f2 = v.f2; p.x_f1 = x.f1;
+    p.ibase = c.ibase; p.base_unit = (float)(c.scale / LN2); p.item_term = item_term;
+    return p;
+}
+
 template <typename T>
 static void forward_typed(const ifr_catalogue &c, const ForwardPlan &p, hipStream_t s)
 {
     constexpr int NS = sizeof(T) == 4 ? 2 : 1;
-    const int KP = pad_factors(c.k);
-    fill_side<T>(p.x, (const T *)c.X, c.k, c.ldx, nullptr, KP, s);
-    fill_side<T>(p.v, (const T *)c.V, c.k, c.ldv, nullptr, KP, s);
+    launch_prepare<T>(prepare_sides(c, p.x, p.v, p.term), p.x.tiles, s);
     WalkParams w = {};
     w.s_f1 = p.x.f1; w.t_f1 = p.v.f1; w.t_term = p.term; w.s_exp = p.x.exps; w.t_exp = p.v.exps;
     w.c = (float)(c.scale / LN2); w.t_tiles = (int)p.v.tiles; w.tiles_per_split = p.split.per; w.splits = p.split.count;
     w.s_blocks = (int)(p.s_padded / S_ROWS); w.s_padded = p.s_padded;
     w.out_m = p.out_m; w.out_s = p.out_s;
-    launch_walk<NS, WALK_STATS>(w, KP, s);
+    launch_walk<NS, WALK_STATS>(w, pad_factors(c.k), s);
 }
 
 template <int STEPS>
@@ -1226,14 +1309,15 @@ int launch_logprob(const ifr_catalogue &c, const int32_t *ids, int64_t m, int64_
 {
     Pieces w{(char *)ws};
     const ForwardPlan p = forward_plan(w, c);
-    const float cc = (float)(c.scale / LN2);
     const int kb = (c.k + 31) / 32;
     if (p.direct) {
         if (c.dtype == IFR_F32) launch_direct<float>(c, p, s);
         else launch_direct<__bf16>(c, p, s);
     } else {
-        hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.t_padded + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.t_padded, c.dtype == IFR_MXFP4 ? 1.f : cc, p.term, nullptr);
-        if (c.dtype == IFR_MXFP4) launch_mx_walk(c, p, s);
+        if (c.dtype == IFR_MXFP4) {
+            hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.t_padded + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.t_padded, p.term);
+            launch_mx_walk(c, p, s);
+        }
         else if (c.dtype == IFR_F32) forward_typed<float>(c, p, s);
         else forward_typed<__bf16>(c, p, s);
     }
@@ -1251,48 +1335,51 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
 {
     constexpr int NS = sizeof(T) == 4 ? 2 : 1;
     const int KP = pad_factors(c.k);
-    const float cc = (float)(c.scale / LN2), sc = (float)c.scale;
+    const float sc = (float)c.scale;
     const T *X = (const T *)c.X, *V = (const T *)c.V;
-    hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.v.padded + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.v.padded, cc, p.item_term, p.named);
-    hipLaunchKernelGGL(user_terms_kernel, dim3((uint32_t)((p.x.padded + 255) / 256)), dim3(256), 0, s, g.lse, ids, m, ld_ids, g.dlogp, g.ld_dlogp, c.n,
-                       p.x.padded, p.user_term, p.G);
-    fill_side<T>(p.x, X, c.k, c.ldx, nullptr, KP, s);
-    fill_side<T>(p.v, V, c.k, c.ldv, nullptr, KP, s);
+    auto fours = [&](const void *rows, int64_t ld) { return c.k % 4 == 0 && ld % 4 == 0 && ((uintptr_t)rows & (4 * sizeof(T) - 1)) == 0; };
+    const bool items = g.dV || g.dibase;
+    if (p.named) {
+        const int64_t words = up(p.v.padded / 64, 4) / 4, want = (words + 255) / 256;
+        hipLaunchKernelGGL(clear_kernel, dim3((uint32_t)(want < MAX_GRID ? want : MAX_GRID)), dim3(256), 0, s, (uint32_t *)p.named, words);
+    }
+    PrepParams pp = prepare_sides(c, p.x, p.v, p.item_term);
+    pp.lse = g.lse; pp.dlogp = g.dlogp; pp.ids = ids; pp.m = m; pp.ld_ids = ld_ids; pp.ld_dlogp = g.ld_dlogp; pp.places_padded = p.places_padded;
+    pp.user_term = p.user_term; pp.G = p.G; pp.places = p.places; pp.named = p.named;
+    pp.g_exp = p.xg.exps; pp.g_f2 = p.xg.f2;
+    launch_prepare<T>(pp, p.x.tiles, s);
     WalkParams w = {};
-    w.c = cc;
+    w.c = (float)(c.scale / LN2);
+    JoinDx x = {};
     if (g.dX) {
         w.s_f1 = p.x.f1; w.t_f1 = p.v.f1; w.t_f2 = p.v.f2; w.s_term = p.user_term; w.t_term = p.item_term;
         w.s_exp = p.x.exps; w.t_exp = w.t2_exp = p.v.exps;
         w.t_tiles = (int)p.v.tiles; w.tiles_per_split = p.split_x.per; w.splits = p.split_x.count;
-        w.s_blocks = (int)(p.x.padded / S_ROWS); w.s_padded = p.x.padded; w.out_acc = p.acc;
+        w.s_blocks = (int)(p.x.padded / S_ROWS); w.s_padded = p.x.padded; w.out_acc = p.acc_x;
         launch_walk<NS, WALK_GRAD>(w, KP, s);
-        const int64_t threads = c.n * (KP / 4);
-        hipLaunchKernelGGL((join_dx_kernel<T>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, s, p.acc, p.split_x.count, p.x.padded, KP, p.G, V, c.ldv,
-                           c.n_items, c.k, sc, ids, m, ld_ids, g.dlogp, g.ld_dlogp, c.n, (T *)g.dX, g.ld_dx);
+        x = {p.acc_x, p.G, V, ids, g.dlogp, g.dX, p.x.padded, c.ldv, c.n_items, m, ld_ids, g.ld_dlogp, c.n, g.ld_dx, p.split_x.count, KP, c.k, fours(V, c.ldv), sc,
+             (c.n * (KP / 4) + 255) / 256};
     }
-    if (g.dV || g.dibase) {
-        fill_side<T>(p.xg, X, c.k, c.ldx, p.G, KP, s);
-        if (p.places_padded) {
-            const int64_t want = p.places_padded / 256;
-            hipLaunchKernelGGL(places_kernel, dim3((uint32_t)(want < MAX_GRID ? want : MAX_GRID)), dim3(256), 0, s, ids, m, ld_ids, c.n, c.n_items,
-                               p.places_padded, p.places, p.named);
-        }
-        const bool whole = p.split_v.count == 1;
+    const bool parts = items && p.split_v.count > 1;
+    if (items) {
         w.s_f1 = p.v.f1; w.t_f1 = p.x.f1; w.t_f2 = p.xg.f2; w.s_term = p.item_term; w.t_term = p.user_term;
-        w.s_exp = p.v.exps; w.t_exp = p.x.exps; w.t2_exp = p.xg.exps; w.t_factor = g.dibase ? p.G : nullptr;
+        w.s_exp = p.v.exps; w.t_exp = p.x.exps; w.t2_exp = p.xg.exps; w.t_factor = p.G;
         w.t_tiles = (int)p.x.tiles; w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.s_blocks = (int)(p.v.padded / S_ROWS); w.s_padded = p.v.padded;
-        w.out_acc = whole ? nullptr : p.acc; w.out_b = whole || !g.dibase ? nullptr : p.acc_b;
-        w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc,
-               c.k % 4 == 0 && c.ldx % 4 == 0 && ((uintptr_t)X & (4 * sizeof(T) - 1)) == 0};
+        w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
+        w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx)};
         if (g.dibase) launch_walk<NS, WALK_GRAD_BASE>(w, KP, s);
         else launch_walk<NS, WALK_GRAD>(w, KP, s);
-        if (!whole) {
-            const dim3 grid((uint32_t)(p.v.padded / 64));
-#define IFR_JOIN(K) hipLaunchKernelGGL((join_dv_kernel<T, K>), grid, dim3(256), 0, s, p.acc, g.dibase ? p.acc_b : nullptr, p.split_v.count, p.v.padded, w.f)
-            IFR_FOR_FACTORS(KP, IFR_JOIN)
+    }
+    // the joins as one launch where dX's is short (its workgroups hold the memory of the other's)
+    const bool together = parts && x.blocks <= 512;
+    if (g.dX && !together) hipLaunchKernelGGL((join_dx_kernel<T>), dim3((uint32_t)x.blocks), dim3(256), 0, s, x);
+    if (parts) {
+        if (!together) x.blocks = 0;
+        const dim3 grid((uint32_t)(x.blocks + p.v.padded / 64));
+#define IFR_JOIN(K) hipLaunchKernelGGL((join_kernel<T, K>), grid, dim3(256), 0, s, x, p.acc_v, p.acc_b, p.split_v.count, p.v.padded, w.f)
+        IFR_FOR_FACTORS(KP, IFR_JOIN)
 #undef IFR_JOIN
-        }
     }
 }
 
