@@ -74,16 +74,16 @@ __device__ __forceinline__ void online(const v16f &d, float c, float &m, float &
 
 // ---------------------------------------------------------------------------- preparation
 
-// A matrix in the order the matrix instructions read it, by tiles of 32 rows, zeros behind the last row and column:
-//   f1 [tile][part][KP / 16][lane][8]: row lane % 32, columns 16 s + 8 (lane / 32) + 0..7                 (first product)
-//   f2 [tile][part][KP / 32][2][lane][8]: column 32 kb + lane % 32, rows 16 c + 8 (j / 4) + 4 (lane / 32) + j % 4   (second)
+// A matrix in the order the walks read it, by tiles of 32 rows, zeros behind the last row and column:
+//   frag [tile][part][KP / 16][row][2][8]: columns 16 s + 8 h + 0..7 of a row are the 16-byte piece 64 s + 2 row + h
 //   exps [tile]: the tile's exponent (split operands); infinities and NaN do not count for it and stay what they are
+// bf16 matrices whose rows are whole, aligned pieces (k = KP) are read as they lie: frag is null then.
 struct PrepParams {
     const void *V, *X;
-    int64_t ldv, ldx, n_items, n, v_tiles;
+    int64_t ldv, ldx, n_items, n, v_blocks, v_padded, x_padded;
     int k, KP;
     int *v_exp, *x_exp, *g_exp;
-    uint4 *v_f1, *v_f2, *x_f1, *g_f2;  // any may be null; g: rows of X times G
+    uint4 *v_frag, *x_frag;
     const float *ibase;
     float base_unit;                   // item_term = base_unit ibase, -inf behind the last item
     float *item_term;
@@ -91,25 +91,18 @@ struct PrepParams {
     const float *lse, *dlogp;
     const int32_t *ids;
     int64_t m, ld_ids, ld_dlogp, places_padded;
-    float *user_term, *G;              // -log2(e) lse, -inf behind the last user; the sum of a user's upstream gradients
+    float *user_term, *G, *G_scaled;   // -log2(e) lse, -inf behind the last user; the sum of a user's upstream gradients; split: times 2^g_exp
     int32_t *places;                   // the items named in (user, place) order, -1 behind the last place; null: not wanted
     uint8_t *named;                    // [items / 64], cleared before: set where an item is named; or null
 };
 
-// LDS tile -> fragments; `factor` (of the tile's rows) and the exponent are applied on the way
+// LDS tile [32][W] -> pieces
 template <int NS>
-__device__ __forceinline__ void store_fragments(const float *tile, int W, int KP, const float *factor, int e, bool second, int64_t at, uint4 *f)
+__device__ __forceinline__ void store_fragments(const float *tile, int W, int KP, int e, int64_t at, uint4 *f)
 {
     const int per = KP / 16 * 64;                     // 16-byte pieces of one part of a tile
     for (int i = threadIdx.x; i < per; i += 256) {
-        const int l = i & 63, s = i >> 6, q = l & 31, h = l >> 5;
-        float v[8];
-        for (int j = 0; j < 8; ++j) {
-            const int r = second ? 16 * (s & 1) + 8 * (j >> 2) + 4 * h + (j & 3) : q;
-            const int c = second ? 32 * (s >> 1) + q : 16 * s + 8 * h + j;
-            v[j] = tile[r * W + c];
-            if (factor) v[j] *= factor[r];
-        }
+        const float *v = tile + ((i >> 1) & 31) * W + (i >> 6) * 16 + (i & 1) * 8;
         if (NS == 1) {
             b8 o;
             for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
@@ -127,46 +120,48 @@ __device__ __forceinline__ void store_fragments(const float *tile, int W, int KP
     }
 }
 
-// Everything the walks read, a workgroup a tile of 32 rows of V (first) or X.  Memory-bound: one read, one write for each order.
+// Everything the walks read, a workgroup a tile of 32 rows of V (or 256 of its terms, where it needs no other order) or X.
+// Memory-bound: one read, one write.
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
 {
     extern __shared__ float tile[];                   // [32][KP + 1]
-    __shared__ float tops[4], sums[256], factor[32];
+    __shared__ float tops[4], sums[256];
     const int W = p.KP + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool of_v = blockIdx.x < p.v_tiles;
-    const int64_t at = of_v ? blockIdx.x : blockIdx.x - p.v_tiles, r0 = at * 32;
-    const T *src = (const T *)(of_v ? p.V : p.X);
-    const int64_t rows = of_v ? p.n_items : p.n, ld = of_v ? p.ldv : p.ldx;
-    uint4 *f1 = of_v ? p.v_f1 : p.x_f1;
-    auto highest = [&](float v) {                     // over the workgroup
-        for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-        __syncthreads();
-        if (lane == 0) tops[wave] = v;
-        __syncthreads();
-        return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const bool of_v = blockIdx.x < p.v_blocks;
+    const int64_t at = of_v ? blockIdx.x : blockIdx.x - p.v_blocks, r0 = at * 32;
+    uint4 *frag = of_v ? p.v_frag : p.x_frag;
+    auto item_term = [&](int64_t i) {
+        if (i < p.v_padded) p.item_term[i] = i < p.n_items ? (p.ibase ? p.ibase[i] * p.base_unit : 0.f) : -INFINITY;
     };
-    float top = 0.f;
-    for (int r = wave; r < 32; r += 4)
-        for (int c = lane; c < p.KP; c += 64) {
-            const float v = r0 + r < rows && c < p.k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
-            tile[r * W + c] = v;
-            if (NS == 2 && fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
-        }
-    int e = 0;
-    if (NS == 2) {
-        e = split_exponent(highest(top));
-        int *exps = of_v ? p.v_exp : p.x_exp;
-        if (threadIdx.x == 0 && exps) exps[at] = e;
+    if (of_v && !frag) {
+        item_term(at * 256 + threadIdx.x);
+        return;
     }
-    __syncthreads();
-    if (f1) store_fragments<NS>(tile, W, p.KP, nullptr, e, false, at, f1);
-    if (of_v) {
-        if (p.v_f2) store_fragments<NS>(tile, W, p.KP, nullptr, e, true, at, p.v_f2);
-        if (threadIdx.x < 32) {
-            const int64_t i = r0 + threadIdx.x;
-            p.item_term[i] = i < p.n_items ? (p.ibase ? p.ibase[i] * p.base_unit : 0.f) : -INFINITY;
+    if (frag) {
+        const T *src = (const T *)(of_v ? p.V : p.X);
+        const int64_t rows = of_v ? p.n_items : p.n, ld = of_v ? p.ldv : p.ldx;
+        float top = 0.f;
+        for (int r = wave; r < 32; r += 4)
+            for (int c = lane; c < p.KP; c += 64) {
+                const float v = r0 + r < rows && c < p.k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
+                tile[r * W + c] = v;
+                if (NS == 2 && fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
+            }
+        if (NS == 2) {
+            for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+            if (lane == 0) tops[wave] = top;
         }
+        __syncthreads();
+        int e = 0;
+        if (NS == 2) {
+            e = split_exponent(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+            if (threadIdx.x == 0) (of_v ? p.v_exp : p.x_exp)[at] = e;
+        }
+        store_fragments<NS>(tile, W, p.KP, e, at, frag);
+    }
+    if (of_v) {
+        if (threadIdx.x < 32) item_term(r0 + threadIdx.x);
         return;
     }
     if (!p.lse) return;
@@ -180,29 +175,20 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
         sums[threadIdx.x] = g;
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int64_t u = r0 + threadIdx.x;
+    if (threadIdx.x < 64) {
+        const int64_t u = r0 + (threadIdx.x & 31);
         float g = 0.f;
-        for (int q = 0; q < 8; ++q) g += sums[threadIdx.x * 8 + q];
-        factor[threadIdx.x] = g;
-        p.G[u] = g;
-        // no probabilities where lse is -inf: every exponential is 0
-        p.user_term[u] = u < p.n && p.lse[u] != -INFINITY ? -p.lse[u] * LOG2E : -INFINITY;
-    }
-    __syncthreads();
-    if (p.g_f2) {
-        int eg = 0;
-        if (NS == 2) {
-            float t = 0.f;
-            for (int r = wave; r < 32; r += 4)
-                for (int c = lane; c < p.KP; c += 64) {
-                    const float v = fabsf(tile[r * W + c] * factor[r]);
-                    if (v < INFINITY) t = fmaxf(t, v);
-                }
-            eg = split_exponent(highest(t));
-            if (threadIdx.x == 0) p.g_exp[at] = eg;
+        for (int q = 0; q < 8; ++q) g += sums[(threadIdx.x & 31) * 8 + q];
+        float top = fabsf(g) < INFINITY ? fabsf(g) : 0.f;
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const int e = split_exponent(top);
+        if (threadIdx.x < 32) {
+            p.G[u] = g;
+            if (NS == 2) p.G_scaled[u] = ldexpf(g, e);
+            if (NS == 2 && threadIdx.x == 0) p.g_exp[at] = e;
+            // no probabilities where lse is -inf: every exponential is 0
+            p.user_term[u] = u < p.n && p.lse[u] != -INFINITY ? -p.lse[u] * LOG2E : -INFINITY;
         }
-        store_fragments<NS>(tile, W, p.KP, factor, eg, true, at, p.g_f2);
     }
     if (p.places) {
         const int64_t all = p.n * p.m;
@@ -233,7 +219,7 @@ __global__ __launch_bounds__(256) void item_terms_kernel(const float *ibase, int
 
 // ---------------------------------------------------------------------------- the walk
 
-enum { WALK_STATS = 0, WALK_GRAD = 1, WALK_GRAD_BASE = 2 };     // ..._BASE: with the sums for the gradient of the bases
+enum { WALK_STATS = 0, WALK_USERS = 1, WALK_ITEMS = 2 };     // lse; the sums of dX (S users, T items); those of dV and db (S items, T users)
 
 // What the gradient of V needs to finish its rows in the kernel that summed them (one split): see finish_rows.
 struct Finish {
@@ -250,18 +236,30 @@ struct Finish {
 };
 
 struct WalkParams {
-    const uint4 *s_f1, *t_f1, *t_f2;
+    const uint4 *s_frag, *t_frag;      // null: rows of bf16 as they lie
+    const __bf16 *s_rows, *t_rows;
+    int64_t s_ld, t_ld, s_n, t_n;
     const float *s_term, *t_term;      // powers of two added to the score (item_term, user_term of prepare_kernel)
-    const float *t_factor;             // WALK_GRAD_BASE: sum_t factor P -> out_b
-    const int *s_exp, *t_exp, *t2_exp; // split operands: exponents of their tiles
+    const float *t_factor;             // WALK_ITEMS: G (split: scaled by t_factor_exp)
+    const int *s_exp, *t_exp, *t_factor_exp;     // split operands: exponents of their tiles
     float c;                           // scale log2(e)
     int s_blocks, splits, t_tiles, tiles_per_split;
     int64_t s_padded;
     float *out_m, *out_s;              // WALK_STATS: [splits][s_padded]
-    float *out_acc;                    // WALK_GRAD: [splits][s_padded][KP], or null: finish
-    float *out_b;                      // ... [splits][s_padded]
+    float *out_acc;                    // else: [splits][s_padded][KP], or null: finish
+    float *out_b;                      // WALK_ITEMS: [splits][s_padded]: sums of factor P, or null
     Finish f;
 };
+
+// rows 0..3 and 8..11 of this lane's column (see at2)
+__device__ __forceinline__ uint4 turned(const char *at)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(at + 256));
+    const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
 
 template <int NS>
 __device__ __forceinline__ v16f product(uint4 a, uint4 b, v16f d)
@@ -486,19 +484,22 @@ constexpr int aside_floats(int KP)
     return sums > bytes ? sums : bytes;
 }
 
-template <int KP, int NS, int MODE>
+// T rows of a stage, in tiles of 32.  For the gradient two stages, each of which also holds 64 rows of sums at the end, fill 512 KP bytes
+// of LDS; the statistics take half of that, for two workgroups a compute unit also at KP = 256.
+constexpr int stage_tiles(int NS, bool grad) { return (NS == 1 ? 2 : 1) * (grad ? 2 : 1); }
+
+template <int KP, int NS, int MODE, bool ROWS>
 __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <= 128) ? 2 : 1) void walk_kernel(WalkParams p)
 {
     typedef typename std::conditional<NS == 2, float, __bf16>::type T;
     constexpr int STEPS = KP / 16;
     constexpr int PART = STEPS * 64;                  // 16-byte pieces of a part of a tile
-    constexpr int SUB = NS == 1 ? 2 : 1;              // tiles of 32 rows a stage
-    constexpr int HALF = PART * NS * SUB;
     constexpr bool GRAD = MODE != WALK_STATS;
-    constexpr int STAGE = HALF * (GRAD ? 2 : 1);
+    constexpr int SUB = stage_tiles(NS, GRAD);
+    constexpr int STAGE = PART * NS * SUB;
     // two stages: one is read while the other arrives (two arrays, so that the compiler sees that they are apart)
     __shared__ uint4 stage0[STAGE], stage1[STAGE];
-    __shared__ float terms0[GRAD ? 128 : 64], terms1[GRAD ? 128 : 64];      // of the stage's T rows: t_term, t_factor
+    __shared__ float terms0[2 * SUB * 32], terms1[2 * SUB * 32];      // of the stage's T rows: t_term, t_factor (a fetch brings 64)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     // workgroups go to the eight XCDs in turn: splits are dealt so that an XCD's L2 sees each part of T from one split only
     int s_block, split;
@@ -519,27 +520,45 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
 #pragma unroll
     for (int q = 0; q < NS; ++q)
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) sf[q][s] = p.s_f1[(s_tile * NS + q) * PART + s * 64 + lane];
+        for (int s = 0; s < STEPS; ++s)
+            sf[q][s] = ROWS ? ((const uint4 *)(p.s_rows + min(s_row, p.s_n - 1) * p.s_ld))[2 * s + h]
+                            : p.s_frag[(s_tile * NS + q) * PART + s * 64 + (lane & 31) * 2 + h];
     const int s_exp = NS == 2 ? p.s_exp[s_tile] : 0;
     const float s_term = p.s_term ? p.s_term[s_row] : 0.f;
 
     v16f acc[GRAD ? KP / 32 : 1] = {};
     float m = -3.402823466e38f, sum = 0.f, b_sum = 0.f;
-    int ref = 140;                                    // exponent of acc (split operands), the least of the tiles so far
+    int ref = 280;                                    // exponent of acc (split operands), the least of the tiles so far
 
     const int first = split * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
+    // this lane's piece of the first product's operand, and its 8 bytes of the second's, which ds_read_tr turns round: 16 lanes read
+    // four rows by 16 columns and get four rows of a column each
+    const int at1 = (lane & 31) * 2 + h;
+    const int at2 = ((lane >> 4 & 1) * 64 + (4 * h + (lane >> 2 & 3)) * 2 + (lane >> 1 & 1)) * 16 + (lane & 1) * 8;
 
     auto fetch_stage = [&](int t, uint4 *to, float *terms) {
-        fetch<HALF>(p.t_f1 + (int64_t)t * PART * NS, to);
-        if (GRAD) fetch<HALF>(p.t_f2 + (int64_t)t * PART * NS, to + HALF);
-        if (wave == 0) fetch_row(p.t_term + (int64_t)t * 32, terms);
-        if (MODE == WALK_GRAD_BASE && wave == 1) fetch_row(p.t_factor + (int64_t)t * 32, terms + 64);
+        if (ROWS) {
+#pragma unroll
+            for (int sub = 0; sub < SUB; ++sub) {
+                const int64_t row = min((int64_t)(t + sub) * 32 + (lane >> 1), p.t_n - 1);     // behind the last: a row whose term is -inf
+                const uint4 *from = (const uint4 *)(p.t_rows + row * p.t_ld) + (lane & 1);
+#pragma unroll
+                for (int s = 0; s < (STEPS + 3) / 4; ++s)
+                    if (STEPS % 4 == 0 || s * 4 + wave < STEPS)
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + (s * 4 + wave) * 2),
+                                                         (__attribute__((address_space(3))) void *)(to + sub * PART + (s * 4 + wave) * 64), 16, 0, 0);
+            }
+        } else {
+            fetch<STAGE>(p.t_frag + (int64_t)t * PART * NS, to);
+        }
+        if (wave < (SUB + 1) / 2) fetch_row(p.t_term + (int64_t)t * 32 + wave * 64, terms + wave * 64);
+        else if (MODE == WALK_ITEMS && wave < SUB) fetch_row(p.t_factor + (int64_t)t * 32 + (wave - SUB / 2) * 64, terms + wave * 64);
     };
     auto compute = [&](int t0, const uint4 *lds, const float *terms) {
-#pragma unroll
+#pragma unroll 2
         for (int sub = 0; sub < SUB; ++sub) {
             const int t = t0 + sub;
-            const uint4 *l1 = lds + sub * PART * NS, *l2 = lds + HALF + sub * PART * NS;
+            const uint4 *l1 = lds + sub * PART * NS;
             float4 tt[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) tt[q] = *(const float4 *)(terms + sub * 32 + 8 * q + 4 * h);
@@ -548,11 +567,11 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
             v16f d = {};
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
-                const uint4 a = l1[s * 64 + lane];
+                const uint4 a = l1[s * 64 + at1];
                 d = product<NS>(a, sf[0][s], d);
                 if (NS == 2) {
                     d = product<NS>(a, sf[NS - 1][s], d);
-                    d = product<NS>(l1[PART + s * 64 + lane], sf[0][s], d);
+                    d = product<NS>(l1[PART + s * 64 + at1], sf[0][s], d);
                 }
             }
             reads_ahead<STEPS * NS, STEPS * (2 * NS - 1)>();
@@ -572,42 +591,45 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                 sum = fmaf(sum, exp2_raw(m - top), add);
                 m = top;
             } else {
-                // split probabilities are scaled to 2^15: fp16 then holds them down to 2^-39; tiles of T with a larger exponent than
-                // the reference take that off here, one with a smaller becomes the reference
-                int up = 0;
+                // split: what enters the second product is scaled to at most 2^15 (probabilities by 2^15, G P by G's exponent), which
+                // fp16 holds down to 2^-39 of that; tiles of T with a larger exponent than the reference take the difference off
+                // here, one with a smaller becomes the reference
+                int up = 0, ge = 0;
                 if (NS == 2) {
-                    const int e = p.t2_exp[t];
+                    ge = MODE == WALK_ITEMS ? p.t_factor_exp[t] : 0;
+                    const int e = p.t_exp[t] + ge;
                     if (e < ref) {
                         const float f = ldexpf(1.f, e - ref);
                         for (int kb = 0; kb < KP / 32; ++kb) acc[kb] *= f;
                         ref = e;
                     }
-                    up = 15 - (e - ref);
+                    up = (MODE == WALK_USERS ? 15 : 0) - (e - ref);
                 }
                 const float add = s_term + (float)up;
                 float P[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) P[r] = exp2_raw(z[r] + add);
-                if (MODE == WALK_GRAD_BASE) {
-                    float b = 0.f;
+                if (MODE == WALK_ITEMS) {
                     float4 tg[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) tg[q] = *(const float4 *)(terms + 64 + sub * 32 + 8 * q + 4 * h);
-                    if (NS == 2 && up < -20) {        // a tile far below the reference: its probabilities as they are
+                    for (int q = 0; q < 4; ++q) tg[q] = *(const float4 *)(terms + SUB * 32 + sub * 32 + 8 * q + 4 * h);
+                    float b = 0.f;
+                    if (NS == 2 && up < -20) {        // a tile far below the reference: its sum for db from the probabilities as they are
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float4 g = tg[r >> 2];
-                            b = fmaf(exp2_raw(z[r] + s_term), (r & 3) == 0 ? g.x : (r & 3) == 1 ? g.y : (r & 3) == 2 ? g.z : g.w, b);
+                        for (int q = 0; q < 4; ++q) {
+                            b = fmaf(exp2_raw(z[4 * q] + s_term), tg[q].x, b); b = fmaf(exp2_raw(z[4 * q + 1] + s_term), tg[q].y, b);
+                            b = fmaf(exp2_raw(z[4 * q + 2] + s_term), tg[q].z, b); b = fmaf(exp2_raw(z[4 * q + 3] + s_term), tg[q].w, b);
                         }
-                        b_sum += b;
-                    } else {
+                    }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        b = fmaf(P[4 * q], tg[q].x, b); b = fmaf(P[4 * q + 1], tg[q].y, b);
-                        b = fmaf(P[4 * q + 2], tg[q].z, b); b = fmaf(P[4 * q + 3], tg[q].w, b);
+                        P[4 * q] *= tg[q].x; P[4 * q + 1] *= tg[q].y; P[4 * q + 2] *= tg[q].z; P[4 * q + 3] *= tg[q].w;
                     }
-                    b_sum += NS == 2 ? ldexpf(b, -up) : b;
+                    if (NS == 1 || up >= -20) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) b += P[r];
                     }
+                    b_sum += NS == 2 ? ldexpf(b, -ge - (up < -20 ? 0 : up)) : b;
                 }
                 uint4 pf[NS][2];
 #pragma unroll
@@ -632,11 +654,12 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                 for (int kb = 0; kb < KP / 32; ++kb)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint4 a = l2[(kb * 2 + e) * 64 + lane];
+                        const char *l2 = (const char *)l1 + at2 + kb * 2048 + e * 512;
+                        const uint4 a = turned(l2);
                         acc[kb] = product<NS>(a, pf[0][e], acc[kb]);
                         if (NS == 2) {
                             acc[kb] = product<NS>(a, pf[NS - 1][e], acc[kb]);
-                            acc[kb] = product<NS>(l2[PART + (kb * 2 + e) * 64 + lane], pf[0][e], acc[kb]);
+                            acc[kb] = product<NS>(turned(l2 + PART * 16), pf[0][e], acc[kb]);
                         }
                     }
             }
@@ -666,7 +689,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
         if (h == 0) { p.out_m[at] = top; p.out_s[at] = sum; }
         return;
     }
-    const float unit = NS == 2 ? ldexpf(1.f, -15 - ref) : 1.f;
+    const float unit = NS == 2 ? ldexpf(1.f, (MODE == WALK_USERS ? -15 : 0) - ref) : 1.f;
     b_sum += __shfl_xor(b_sum, 32);
     if (p.out_acc) {
         if (p.out_b && h == 0) p.out_b[at] = b_sum;
@@ -1061,6 +1084,12 @@ __global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, c
 
 namespace {
 
+// the walks may read both matrices as they lie: bf16, no column missing to a multiple of 32, rows at 16-byte borders
+bool rows_lie(const ifr_catalogue &c)
+{
+    return c.dtype == IFR_BF16 && c.k % 32 == 0 && c.ldx % 8 == 0 && c.ldv % 8 == 0 && (((uintptr_t)c.X | (uintptr_t)c.V) & 15) == 0;
+}
+
 // a workspace as a row of aligned pieces; with base null it only counts
 struct Pieces {
     char *base;
@@ -1095,22 +1124,23 @@ Split split_plan(int64_t s_blocks, int64_t t_tiles, int unit, int64_t resident, 
     return s;
 }
 
-struct Side {                          // one matrix in fragment order
+struct Side {                          // one matrix as the walks read it
     int64_t rows, tiles, padded;       // tiles of 32 rows; padded: rows up to whole S blocks
+    bool lies;                         // bf16 rows of whole, aligned pieces: read as they lie
     int *exps;
-    uint4 *f1, *f2;
+    uint4 *frag;
 };
 
-Side side(Pieces &w, int64_t rows, int KP, int NS, bool want1, bool want2)
+Side side(Pieces &w, const ifr_catalogue &c, bool users)
 {
     Side s;
-    s.rows = rows;
-    s.padded = up(rows, S_ROWS);
+    const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
+    s.rows = users ? c.n : c.n_items;
+    s.padded = up(s.rows, S_ROWS);
     s.tiles = s.padded / 32;
+    s.lies = rows_lie(c);
     s.exps = w.take<int>(NS == 2 ? s.tiles : 0);
-    const int64_t n = s.tiles * NS * (KP / 16) * 64;
-    s.f1 = want1 ? w.take<uint4>(n) : nullptr;
-    s.f2 = want2 ? w.take<uint4>(n) : nullptr;
+    s.frag = w.take<uint4>(s.lies ? 0 : s.tiles * NS * (KP / 16) * 64);
     return s;
 }
 
@@ -1118,7 +1148,7 @@ template <typename T>
 void launch_prepare(const PrepParams &p, int64_t x_tiles, hipStream_t s)
 {
     constexpr int NS = sizeof(T) == 4 ? 2 : 1;
-    hipLaunchKernelGGL((prepare_kernel<T, NS>), dim3((uint32_t)(p.v_tiles + x_tiles)), dim3(256), 32 * (p.KP + 1) * sizeof(float), s, p);
+    hipLaunchKernelGGL((prepare_kernel<T, NS>), dim3((uint32_t)(p.v_blocks + x_tiles)), dim3(256), 32 * (p.KP + 1) * sizeof(float), s, p);
 }
 
 #define IFR_FOR_FACTORS(KP, CALL)                                                                                     \
@@ -1137,7 +1167,9 @@ template <int NS, int MODE>
 void launch_walk(const WalkParams &p, int KP, hipStream_t s)
 {
     const dim3 grid((uint32_t)(p.s_blocks * p.splits));
-#define IFR_WALK(K) hipLaunchKernelGGL((walk_kernel<K, NS, MODE>), grid, dim3(256), 0, s, p)
+#define IFR_WALK(K)                                                                                                   \
+    if (NS == 1 && !p.s_frag) hipLaunchKernelGGL((walk_kernel<K, NS, MODE, NS == 1>), grid, dim3(256), 0, s, p);      \
+    else hipLaunchKernelGGL((walk_kernel<K, NS, MODE, false>), grid, dim3(256), 0, s, p)
     IFR_FOR_FACTORS(KP, IFR_WALK)
 #undef IFR_WALK
 }
@@ -1172,8 +1204,8 @@ ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c)
         return p;
     }
     if (c.dtype != IFR_MXFP4) {
-        p.x = side(w, c.n, KP, NS, true, false);
-        p.v = side(w, c.n_items, KP, NS, true, false);
+        p.x = side(w, c, true);
+        p.v = side(w, c, false);
     }
     if (c.dtype == IFR_MXFP4) {                       // waves walk alone: 16 a compute unit, none with fewer than two tiles
         p.mx_users = c.n > 64 ? 4 : c.n > 32 ? 2 : 1;
@@ -1183,17 +1215,18 @@ ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c)
         p.split.per = (int)((tiles + waves - 1) / waves);
         p.split.count = (int)up((tiles + p.split.per - 1) / p.split.per, 4);
     } else {
-        p.split = split_plan(p.s_padded / S_ROWS, p.t_padded / 32, 2, resident_blocks(KP, NS, WALK_STATS), 0.0);
+        p.split = split_plan(p.s_padded / S_ROWS, p.t_padded / 32, stage_tiles(NS, false), resident_blocks(KP, NS, WALK_STATS), 0.0);
     }
-    p.term = w.take<float>(p.t_padded + 32);
+    p.term = w.take<float>(p.t_padded + 32);         // a fetch brings 64, also where a stage holds 32 rows
     p.out_m = w.take<float>(p.split.count * p.s_padded);
     p.out_s = w.take<float>(p.split.count * p.s_padded);
     return p;
 }
 
 struct BackwardPlan {
-    Side x, v, xg;                     // xg: rows times G, second product of dV
-    float *item_term, *user_term, *G, *acc_x, *acc_v, *acc_b;
+    Side x, v;
+    float *item_term, *user_term, *G, *G_scaled, *acc_x, *acc_v, *acc_b;
+    int *g_exp;
     int32_t *places;
     uint8_t *named;
     int64_t places_padded;
@@ -1205,19 +1238,20 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
     BackwardPlan p = {};
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
     const bool items = dv || db;
-    p.x = side(w, c.n, KP, NS, true, false);
-    p.v = side(w, c.n_items, KP, NS, true, dx);
-    p.xg = side(w, c.n, KP, NS, false, items);
-    p.item_term = w.take<float>(p.v.padded + 32);     // a stage fetches 64 terms, also where it holds 32 rows
-    p.user_term = w.take<float>(p.x.padded + 32);
-    p.G = w.take<float>(p.x.padded + 32);
+    p.x = side(w, c, true);
+    p.v = side(w, c, false);
+    p.item_term = w.take<float>(p.v.padded);
+    p.user_term = w.take<float>(p.x.padded);
+    p.G = w.take<float>(p.x.padded);
+    p.G_scaled = w.take<float>(NS == 2 ? p.x.padded : 0);
+    p.g_exp = w.take<int>(NS == 2 ? p.x.tiles : 0);
     p.places_padded = items ? up(c.n * m, 1024) : 0;
     p.places = w.take<int32_t>(p.places_padded);
     // flags save the search where most groups of 64 items are not named; where the places are as many as the groups, none is saved
     p.named = w.take<uint8_t>(p.places_padded && c.n_items > 64 * c.n * m ? up(p.v.padded / 64, 4) : 0);
-    const int resident = resident_blocks(KP, NS, WALK_GRAD);
-    p.split_x = split_plan(p.x.padded / S_ROWS, p.v.tiles, 2, resident, 0.05);
-    p.split_v = split_plan(p.v.padded / S_ROWS, p.x.tiles, 2, resident, 0.5);
+    const int resident = resident_blocks(KP, NS, WALK_USERS);
+    p.split_x = split_plan(p.x.padded / S_ROWS, p.v.tiles, stage_tiles(NS, true), resident, 0.05);
+    p.split_v = split_plan(p.v.padded / S_ROWS, p.x.tiles, stage_tiles(NS, true), resident, 0.5);
     const bool parts = items && p.split_v.count > 1;
     p.acc_x = w.take<float>(dx ? p.split_x.count * p.x.padded * KP : 0);
     p.acc_v = w.take<float>(parts ? p.split_v.count * p.v.padded * KP : 0);
@@ -1244,22 +1278,32 @@ size_t logprob_backward_workspace(const ifr_catalogue &c, int64_t m, bool want_d
 static PrepParams prepare_sides(const ifr_catalogue &c, const Side &x, const Side &v, float *item_term)
 {
     PrepParams p = {};
-    p.V = c.V; p.X = c.X; p.ldv = c.ldv; p.ldx = c.ldx; p.n_items = c.n_items; p.n = c.n; p.v_tiles = v.tiles;
+    p.V = c.V; p.X = c.X; p.ldv = c.ldv; p.ldx = c.ldx; p.n_items = c.n_items; p.n = c.n;
+    p.v_blocks = v.lies ? (v.padded + 255) / 256 : v.tiles; p.v_padded = v.padded; p.x_padded = x.padded;
     p.k = c.k; p.KP = pad_factors(c.k);
-    p.v_exp = v.exps; p.x_exp = x.exps; p.v_f1 = v.f1; p.v_f2 = v.f2; p.x_f1 = x.f1;
+    p.v_exp = v.exps; p.x_exp = x.exps; p.v_frag = v.frag; p.x_frag = x.frag;
     p.ibase = c.ibase; p.base_unit = (float)(c.scale / LN2); p.item_term = item_term;
     return p;
+}
+
+static void walk_sides(WalkParams &w, const ifr_catalogue &c, const Side &x, const Side &v, bool users_stay)
+{
+    const Side &s = users_stay ? x : v, &t = users_stay ? v : x;
+    w.s_frag = s.frag; w.t_frag = t.frag; w.s_exp = s.exps; w.t_exp = t.exps; w.s_n = s.rows; w.t_n = t.rows;
+    w.s_rows = (const __bf16 *)(users_stay ? c.X : c.V); w.t_rows = (const __bf16 *)(users_stay ? c.V : c.X);
+    w.s_ld = users_stay ? c.ldx : c.ldv; w.t_ld = users_stay ? c.ldv : c.ldx;
+    w.t_tiles = (int)t.tiles; w.s_blocks = (int)(s.padded / S_ROWS); w.s_padded = s.padded;
 }
 
 template <typename T>
 static void forward_typed(const ifr_catalogue &c, const ForwardPlan &p, hipStream_t s)
 {
     constexpr int NS = sizeof(T) == 4 ? 2 : 1;
-    launch_prepare<T>(prepare_sides(c, p.x, p.v, p.term), p.x.tiles, s);
+    launch_prepare<T>(prepare_sides(c, p.x, p.v, p.term), p.x.lies ? 0 : p.x.tiles, s);
     WalkParams w = {};
-    w.s_f1 = p.x.f1; w.t_f1 = p.v.f1; w.t_term = p.term; w.s_exp = p.x.exps; w.t_exp = p.v.exps;
-    w.c = (float)(c.scale / LN2); w.t_tiles = (int)p.v.tiles; w.tiles_per_split = p.split.per; w.splits = p.split.count;
-    w.s_blocks = (int)(p.s_padded / S_ROWS); w.s_padded = p.s_padded;
+    walk_sides(w, c, p.x, p.v, true);
+    w.t_term = p.term;
+    w.c = (float)(c.scale / LN2); w.tiles_per_split = p.split.per; w.splits = p.split.count;
     w.out_m = p.out_m; w.out_s = p.out_s;
     launch_walk<NS, WALK_STATS>(w, pad_factors(c.k), s);
 }
@@ -1346,30 +1390,26 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     PrepParams pp = prepare_sides(c, p.x, p.v, p.item_term);
     pp.lse = g.lse; pp.dlogp = g.dlogp; pp.ids = ids; pp.m = m; pp.ld_ids = ld_ids; pp.ld_dlogp = g.ld_dlogp; pp.places_padded = p.places_padded;
     pp.user_term = p.user_term; pp.G = p.G; pp.places = p.places; pp.named = p.named;
-    pp.g_exp = p.xg.exps; pp.g_f2 = p.xg.f2;
+    pp.G_scaled = p.G_scaled; pp.g_exp = p.g_exp;
     launch_prepare<T>(pp, p.x.tiles, s);
     WalkParams w = {};
     w.c = (float)(c.scale / LN2);
     JoinDx x = {};
     if (g.dX) {
-        w.s_f1 = p.x.f1; w.t_f1 = p.v.f1; w.t_f2 = p.v.f2; w.s_term = p.user_term; w.t_term = p.item_term;
-        w.s_exp = p.x.exps; w.t_exp = w.t2_exp = p.v.exps;
-        w.t_tiles = (int)p.v.tiles; w.tiles_per_split = p.split_x.per; w.splits = p.split_x.count;
-        w.s_blocks = (int)(p.x.padded / S_ROWS); w.s_padded = p.x.padded; w.out_acc = p.acc_x;
-        launch_walk<NS, WALK_GRAD>(w, KP, s);
+        walk_sides(w, c, p.x, p.v, true);
+        w.s_term = p.user_term; w.t_term = p.item_term; w.tiles_per_split = p.split_x.per; w.splits = p.split_x.count; w.out_acc = p.acc_x;
+        launch_walk<NS, WALK_USERS>(w, KP, s);
         x = {p.acc_x, p.G, V, ids, g.dlogp, g.dX, p.x.padded, c.ldv, c.n_items, m, ld_ids, g.ld_dlogp, c.n, g.ld_dx, p.split_x.count, KP, c.k, fours(V, c.ldv), sc,
              (c.n * (KP / 4) + 255) / 256};
     }
     const bool parts = items && p.split_v.count > 1;
     if (items) {
-        w.s_f1 = p.v.f1; w.t_f1 = p.x.f1; w.t_f2 = p.xg.f2; w.s_term = p.item_term; w.t_term = p.user_term;
-        w.s_exp = p.v.exps; w.t_exp = p.x.exps; w.t2_exp = p.xg.exps; w.t_factor = p.G;
-        w.t_tiles = (int)p.x.tiles; w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
-        w.s_blocks = (int)(p.v.padded / S_ROWS); w.s_padded = p.v.padded;
+        walk_sides(w, c, p.x, p.v, false);
+        w.s_term = p.item_term; w.t_term = p.user_term; w.t_factor = NS == 2 ? p.G_scaled : p.G; w.t_factor_exp = p.g_exp;
+        w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
         w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx)};
-        if (g.dibase) launch_walk<NS, WALK_GRAD_BASE>(w, KP, s);
-        else launch_walk<NS, WALK_GRAD>(w, KP, s);
+        launch_walk<NS, WALK_ITEMS>(w, KP, s);
     }
     // the joins as one launch where dX's is short (its workgroups hold the memory of the other's)
     const bool together = parts && x.blocks <= 512;
