@@ -85,13 +85,15 @@ struct PrepParams {
     int *v_exp, *x_exp, *g_exp;
     uint4 *v_frag, *x_frag;
     const float *ibase;
-    float base_unit;                   // item_term = base_unit ibase, -inf behind the last item
+    // terms of split operands are powers of two, to be added to the exponent; those of bf16 operands are in units of <x, v>, to begin
+    // its sum with.  item_term = base_unit ibase, user_term = lse_unit lse; -inf behind the last item and user
+    float base_unit, lse_unit;
     float *item_term;
     // gradient only (lse null otherwise)
     const float *lse, *dlogp;
     const int32_t *ids;
     int64_t m, ld_ids, ld_dlogp, places_padded;
-    float *user_term, *G, *G_scaled;   // -log2(e) lse, -inf behind the last user; the sum of a user's upstream gradients; split: times 2^g_exp
+    float *user_term, *G, *G_scaled;   // G: the sum of a user's upstream gradients; split: also times 2^g_exp
     int32_t *places;                   // the items named in (user, place) order, -1 behind the last place; null: not wanted
     uint8_t *named;                    // [items / 64], cleared before: set where an item is named; or null
 };
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
             if (NS == 2) p.G_scaled[u] = ldexpf(g, e);
             if (NS == 2 && threadIdx.x == 0) p.g_exp[at] = e;
             // no probabilities where lse is -inf: every exponential is 0
-            p.user_term[u] = u < p.n && p.lse[u] != -INFINITY ? -p.lse[u] * LOG2E : -INFINITY;
+            p.user_term[u] = u < p.n && p.lse[u] != -INFINITY ? p.lse[u] * p.lse_unit : -INFINITY;
         }
     }
     if (p.places) {
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(256) void item_terms_kernel(const float *ibase, int
 
 enum { WALK_STATS = 0, WALK_USERS = 1, WALK_ITEMS = 2 };     // lse; the sums of dX (S users, T items); those of dV and db (S items, T users)
 
-// What the gradient of V needs to finish its rows in the kernel that summed them (one split): see finish_rows.
+// What the gradient of V needs to finish its rows in the kernel that summed them (one split): see find_places.
 struct Finish {
     const int32_t *places;             // [n_places, padded to 1024]: items named, in (user, place) order
     const uint8_t *named;              // [n_items / 64]: whether one of 64 items is, or null
@@ -239,7 +241,7 @@ struct WalkParams {
     const uint4 *s_frag, *t_frag;      // null: rows of bf16 as they lie
     const __bf16 *s_rows, *t_rows;
     int64_t s_ld, t_ld, s_n, t_n;
-    const float *s_term, *t_term;      // powers of two added to the score (item_term, user_term of prepare_kernel)
+    const float *s_term, *t_term;      // item_term, user_term of prepare_kernel
     const float *t_factor;             // WALK_ITEMS: G (split: scaled by t_factor_exp)
     const int *s_exp, *t_exp, *t_factor_exp;     // split operands: exponents of their tiles
     float c;                           // scale log2(e)
@@ -322,161 +324,183 @@ __device__ __forceinline__ void load4(const T *row, int c, int k, bool vec, floa
     }
 }
 
-// The last steps of dV for 64 S rows, whose sums lie in LDS as rows[local][KP]: adds g x of every place that names one of the
-// items, scales, rounds and stores.  Each wave looks through a quarter of the places in order and lists those it wants, until its list
-// is full or the quarter is done; the lists are sorted by item.  The groups of threads (four columns a thread) take equal parts of
-// the sorted order, so that an item that everybody names does not fall to one group; an item's first run in a part is set aside and
-// added after the others, in the parts' order.  Nothing depends on scheduling.
-template <typename T, int KP>
-__device__ void finish_rows(const Finish &f, float *rows, float *row_b, uint32_t *list, int *counts, float *aside, int *aside_item, int64_t i0)
+// The last steps of dV: rows of sums lie in LDS as rows[local][KP], 64 at a time; g x of every place that names one of the items is added,
+// the rows are scaled, rounded and stored.  Nothing depends on scheduling.
+//
+// find_places: each wave looks through a quarter of the places and lists those that name one of `count` (at most 128) items, until its
+// list is full or the quarter is done (`step` keeps where it is); the lists are sorted by item.  Returns how many, `more`: come again.
+template <int KP>
+__device__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t *item_of, int64_t i0, int count, int64_t &step, bool &more)
 {
-    constexpr int LIST = list_length(KP), CAP = LIST / 4, EACH = CAP / 64, ROWS = 64;
-    constexpr int COLS = KP / 4;                      // threads of a row
-    constexpr int GROUPS = 256 / COLS;
+    constexpr int LIST = list_length(KP), CAP = LIST / 4, EACH = CAP / 64;
     uint32_t *order = list + LIST;
-    uint8_t *item_of = (uint8_t *)aside;              // free while the lists are made
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int group = tid / COLS, c4 = (tid % COLS) * 4;
-    const bool vec = f.vec_x;
-    const T *X = (const T *)f.X;
     const int64_t steps = (f.n_places + 64 * EACH - 1) / (64 * EACH);          // of a wave, over all places
-    int64_t step = steps * wave / 4;
     const int64_t end = steps * (wave + 1) / 4;
-    bool more = f.n_places > 0 && (!f.named || f.named[i0 >> 6]);
-    while (more) {
-        int held = 0;
-        int32_t id[EACH], next[EACH];
-        auto load = [&](int64_t at, int32_t *to) {
-            const int4 *src = (const int4 *)f.places + at * 64 * (EACH / 4) + lane;
+    if (step < 0) step = steps * wave / 4;
+    int held = 0;
+    int32_t id[EACH], next[EACH];
+    auto load = [&](int64_t at, int32_t *to) {
+        const int4 *src = (const int4 *)f.places + at * 64 * (EACH / 4) + lane;
 #pragma unroll
-            for (int q = 0; q < EACH / 4; ++q) *(int4 *)(to + 4 * q) = src[q * 64];
-        };
-        if (step < end) load(step, id);
-        while (step < end) {
-            if (step + 1 < end) load(step + 1, next);
-            int mine = 0;
+        for (int q = 0; q < EACH / 4; ++q) *(int4 *)(to + 4 * q) = src[q * 64];
+    };
+    if (step < end) load(step, id);
+    while (step < end) {
+        if (step + 1 < end) load(step + 1, next);
+        int mine = 0;
 #pragma unroll
-            for (int q = 0; q < EACH; ++q) {
-                if (id[q] >= f.n_items) id[q] = -1;   // behind the catalogue: no row takes it
-                mine += (uint64_t)((int64_t)id[q] - i0) < (uint64_t)ROWS;
-            }
-            if (__ballot(mine)) {
-                int before = mine;
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int v = __shfl_up(before, o);
-                    if (lane >= o) before += v;
-                }
-                const int all = __shfl(before, 63);
-                if (held + all > CAP) break;          // next time: a step alone always fits
-                before += held - mine;
-                if (mine) {
-#pragma unroll
-                    for (int q = 0; q < EACH; ++q) {
-                        const int64_t local = (int64_t)id[q] - i0;
-                        if ((uint64_t)local < (uint64_t)ROWS) {
-                            item_of[wave * CAP + before] = (uint8_t)local;
-                            list[wave * CAP + before++] = (uint32_t)(step * 64 * EACH + (q >> 2) * 256 + lane * 4 + (q & 3));      // at most 2^32 places
-                        }
-                    }
-                }
-                held += all;
-            }
-            ++step;
-#pragma unroll
-            for (int q = 0; q < EACH; ++q) id[q] = next[q];
+        for (int q = 0; q < EACH; ++q) {
+            if (id[q] >= f.n_items) id[q] = -1;       // behind the catalogue: no row takes it
+            mine += (uint64_t)((int64_t)id[q] - i0) < (uint64_t)count;
         }
-        if (lane == 0) counts[wave] = held;
-        more = __syncthreads_or(step < end);
-        int total = 0, offset = 0;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) offset += counts[w];
-            total += counts[w];
-        }
-        for (int q = lane; q < held; q += 64) order[offset + q] = (uint32_t)item_of[wave * CAP + q] << 12 | (uint32_t)(wave * CAP + q);
-        int size = 1;
-        while (size < total) size <<= 1;
-        for (int q = total + tid; q < size; q += 256) order[q] = ~0u;
-        __syncthreads();
-        for (int w = 2; w <= size; w <<= 1)           // bitonic: keys are unique (item, position)
-            for (int d = w >> 1; d; d >>= 1) {
-                for (int q = tid; q < size / 2; q += 256) {
-                    const int lo = 2 * q - (q & (d - 1)), hi = lo + d;
-                    const uint32_t x = order[lo], y = order[hi];
-                    if ((x > y) == !(lo & w)) { order[lo] = y; order[hi] = x; }
-                }
-                __syncthreads();
+        if (__ballot(mine)) {
+            int before = mine;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(before, o);
+                if (lane >= o) before += v;
             }
-        if (total) {
-            const int part = (total + GROUPS - 1) / GROUPS, from = group * part, to = min(from + part, total);
-            if (group < GROUPS) {
-                if (c4 == 0) aside_item[group] = -1;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                float ab = 0.f;
-                int item = -1, first = -1;
-                auto flush = [&]() {
-                    if (item < 0) return;
-                    if (item == first) {
-                        *(float4 *)(aside + group * KP + c4) = a;
-                        if (c4 == 0) { aside_item[group] = item; aside[GROUPS * KP + group] = ab; }
-                    } else {
-                        float4 *r = (float4 *)(rows + item * KP + c4);
-                        float4 v = *r;
-                        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-                        *r = v;
-                        if (c4 == 0) row_b[item] += ab;
-                    }
-                };
-                for (int q0 = from; q0 < to; q0 += 8) {
-                    float x[8][4], g[8];
-                    int at[8];
+            const int all = __shfl(before, 63);
+            if (held + all > CAP) break;              // next time: a step alone always fits
+            before += held - mine;
+            if (mine) {
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        at[q] = -1;
-                        if (q0 + q < to) {
-                            const uint32_t key = order[q0 + q], place = list[key & 4095], u = place / (uint32_t)f.m;
-                            at[q] = (int)(key >> 12);
-                            g[q] = f.dlogp[(int64_t)u * f.ld_dlogp + (place - u * (uint32_t)f.m)];
-                            load4(X + (int64_t)u * f.ldx, c4, f.k, vec && c4 < f.k, x[q]);
-                        }
+                for (int q = 0; q < EACH; ++q) {
+                    const int64_t local = (int64_t)id[q] - i0;
+                    if ((uint64_t)local < (uint64_t)count) {
+                        item_of[wave * CAP + before] = (uint8_t)local;
+                        list[wave * CAP + before++] = (uint32_t)(step * 64 * EACH + (q >> 2) * 256 + lane * 4 + (q & 3));      // at most 2^32 places
                     }
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        if (at[q] >= 0) {
-                            if (at[q] != item) {
-                                flush();
-                                if (first < 0) first = at[q];
-                                item = at[q];
-                                a = make_float4(0.f, 0.f, 0.f, 0.f);
-                                ab = 0.f;
-                            }
-                            a.x = fmaf(g[q], x[q][0], a.x); a.y = fmaf(g[q], x[q][1], a.y);
-                            a.z = fmaf(g[q], x[q][2], a.z); a.w = fmaf(g[q], x[q][3], a.w);
-                            ab += g[q];
-                        }
                 }
-                flush();
+            }
+            held += all;
+        }
+        ++step;
+#pragma unroll
+        for (int q = 0; q < EACH; ++q) id[q] = next[q];
+    }
+    if (lane == 0) counts[wave] = held;
+    more = __syncthreads_or(step < end);
+    int total = 0, offset = 0;
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) offset += counts[w];
+        total += counts[w];
+    }
+    for (int q = lane; q < held; q += 64) order[offset + q] = (uint32_t)item_of[wave * CAP + q] << 12 | (uint32_t)(wave * CAP + q);
+    int size = 1;
+    while (size < total) size <<= 1;
+    for (int q = total + tid; q < size; q += 256) order[q] = ~0u;
+    __syncthreads();
+    for (int w = 2; w <= size; w <<= 1)               // bitonic: keys are unique (item, position)
+        for (int d = w >> 1; d; d >>= 1) {
+            for (int q = tid; q < size / 2; q += 256) {
+                const int lo = 2 * q - (q & (d - 1)), hi = lo + d;
+                const uint32_t x = order[lo], y = order[hi];
+                if ((x > y) == !(lo & w)) { order[lo] = y; order[hi] = x; }
             }
             __syncthreads();
-            for (int g = 0; g < GROUPS; ++g) {
-                const int item = aside_item[g];
-                if (item < 0) continue;
-                for (int c = tid; c < KP; c += 256) rows[item * KP + c] += aside[g * KP + c];
-                if (tid == 0) row_b[item] += aside[GROUPS * KP + g];
-            }
         }
-        __syncthreads();
+    return total;
+}
+
+// The found places [from, to) in their sorted order, of items whose local number is 64 at a time from `local0`.  The groups of threads
+// (four columns a thread) take equal parts, so that an item that everybody names does not fall to one group; an item's first run in a
+// part is set aside and added after the others, in the parts' order.
+template <typename T, int KP>
+__device__ void add_places(const Finish &f, float *rows, float *row_b, const uint32_t *list, float *aside, int *aside_item, int local0, int from, int to)
+{
+    constexpr int COLS = KP / 4;                      // threads of a row
+    constexpr int GROUPS = 256 / COLS, BATCH = 16;
+    const uint32_t *order = list + list_length(KP);
+    const int tid = threadIdx.x, group = tid / COLS, c4 = (tid % COLS) * 4;
+    if (from >= to) return;
+    const T *X = (const T *)f.X;
+    if (group < GROUPS) {
+        const int part = (to - from + GROUPS - 1) / GROUPS, begin = from + group * part, end = min(begin + part, to);
+        if (c4 == 0) aside_item[group] = -1;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ab = 0.f;
+        int item = -1, first = -1;
+        auto flush = [&]() {
+            if (item < 0) return;
+            if (item == first) {
+                *(float4 *)(aside + group * KP + c4) = a;
+                if (c4 == 0) { aside_item[group] = item; aside[GROUPS * KP + group] = ab; }
+            } else {
+                float4 *r = (float4 *)(rows + item * KP + c4);
+                float4 v = *r;
+                v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+                *r = v;
+                if (c4 == 0) row_b[item] += ab;
+            }
+        };
+        for (int q0 = begin; q0 < end; q0 += BATCH) {
+            float x[BATCH][4], g[BATCH];
+            int at[BATCH];
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q) {
+                at[q] = -1;
+                if (q0 + q < end) {
+                    const uint32_t key = order[q0 + q], place = list[key & 4095], u = place / (uint32_t)f.m;
+                    at[q] = (int)(key >> 12) - local0;
+                    g[q] = f.dlogp[(int64_t)u * f.ld_dlogp + (place - u * (uint32_t)f.m)];
+                    load4(X + (int64_t)u * f.ldx, c4, f.k, f.vec_x && c4 < f.k, x[q]);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q)
+                if (at[q] >= 0) {
+                    if (at[q] != item) {
+                        flush();
+                        if (first < 0) first = at[q];
+                        item = at[q];
+                        a = make_float4(0.f, 0.f, 0.f, 0.f);
+                        ab = 0.f;
+                    }
+                    a.x = fmaf(g[q], x[q][0], a.x); a.y = fmaf(g[q], x[q][1], a.y);
+                    a.z = fmaf(g[q], x[q][2], a.z); a.w = fmaf(g[q], x[q][3], a.w);
+                    ab += g[q];
+                }
+        }
+        flush();
     }
+    __syncthreads();
+    for (int g = 0; g < GROUPS; ++g) {
+        const int item = aside_item[g];
+        if (item < 0) continue;
+        for (int c = tid; c < KP; c += 256) rows[item * KP + c] += aside[g * KP + c];
+        if (tid == 0) row_b[item] += aside[GROUPS * KP + g];
+    }
+    __syncthreads();
+}
+
+// ... where the lists may not hold all of them: in as many rounds as it takes
+template <typename T, int KP>
+__device__ void add_all_places(const Finish &f, float *rows, float *row_b, uint32_t *list, int *counts, float *aside, int *aside_item, int64_t i0)
+{
+    int64_t step = -1;
+    bool more = true;
+    while (more) {
+        const int total = find_places<KP>(f, list, counts, (uint8_t *)aside, i0, 64, step, more);
+        add_places<T, KP>(f, rows, row_b, list, aside, aside_item, 0, 0, total);
+    }
+}
+
+template <typename T, int KP>
+__device__ void store_rows(const Finish &f, const float *rows, const float *row_b, int64_t i0)
+{
     if (f.dV) {
         T *out = (T *)f.dV;
-        for (int i = tid; i < ROWS * KP; i += 256) {
+        for (int i = threadIdx.x; i < 64 * KP; i += 256) {
             const int r = i / KP, c = i - r * KP;
             if (i0 + r < f.n_items && c < f.k) out[(i0 + r) * f.ld_dv + c] = (T)(f.scale * rows[i]);
         }
     }
     if (f.db)
-        for (int r = tid; r < ROWS; r += 256)
+        for (int r = threadIdx.x; r < 64; r += 256)
             if (i0 + r < f.n_items) f.db[i0 + r] = f.scale * row_b[r];
 }
+
 // memory of the sums set aside (one row and one number a group), or a byte for each place of the lists
 constexpr int aside_floats(int KP)
 {
@@ -524,8 +548,9 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
             sf[q][s] = ROWS ? ((const uint4 *)(p.s_rows + min(s_row, p.s_n - 1) * p.s_ld))[2 * s + h]
                             : p.s_frag[(s_tile * NS + q) * PART + s * 64 + (lane & 31) * 2 + h];
     const int s_exp = NS == 2 ? p.s_exp[s_tile] : 0;
-    const float s_term = p.s_term ? p.s_term[s_row] : 0.f;
+    const float s_term = p.s_term ? p.s_term[s_row] * (NS == 1 ? p.c : 1.f) : 0.f;
 
+    const bool want_b = MODE == WALK_ITEMS && (p.out_b || p.f.db);
     v16f acc[GRAD ? KP / 32 : 1] = {};
     float m = -3.402823466e38f, sum = 0.f, b_sum = 0.f;
     int ref = 280;                                    // exponent of acc (split operands), the least of the tiles so far
@@ -565,6 +590,10 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
             float c = p.c;
             if (NS == 2) c = fminf(ldexpf(c, -s_exp - p.t_exp[t]), 3.402823466e38f);
             v16f d = {};
+            if (NS == 1) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) { d[4 * q] = tt[q].x; d[4 * q + 1] = tt[q].y; d[4 * q + 2] = tt[q].z; d[4 * q + 3] = tt[q].w; }
+            }
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 const uint4 a = l1[s * 64 + at1];
@@ -575,21 +604,17 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                 }
             }
             reads_ahead<STEPS * NS, STEPS * (2 * NS - 1)>();
-            float z[16];
+            // the exponent of a score without the S side's part: split c d + term, otherwise c d
+            if (NS == 2) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                z[4 * q] = fmaf(d[4 * q], c, tt[q].x); z[4 * q + 1] = fmaf(d[4 * q + 1], c, tt[q].y);
-                z[4 * q + 2] = fmaf(d[4 * q + 2], c, tt[q].z); z[4 * q + 3] = fmaf(d[4 * q + 3], c, tt[q].w);
+                for (int q = 0; q < 4; ++q) {
+                    d[4 * q] = fmaf(d[4 * q], c, tt[q].x); d[4 * q + 1] = fmaf(d[4 * q + 1], c, tt[q].y);
+                    d[4 * q + 2] = fmaf(d[4 * q + 2], c, tt[q].z); d[4 * q + 3] = fmaf(d[4 * q + 3], c, tt[q].w);
+                }
+                c = 1.f;
             }
             if (MODE == WALK_STATS) {
-                float top = m;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, z[r]);
-                float add = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) add += exp2_raw(z[r] - top);
-                sum = fmaf(sum, exp2_raw(m - top), add);
-                m = top;
+                online(d, c, m, sum);
             } else {
                 // split: what enters the second product is scaled to at most 2^15 (probabilities by 2^15, G P by G's exponent), which
                 // fp16 holds down to 2^-39 of that; tiles of T with a larger exponent than the reference take the difference off
@@ -608,7 +633,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                 const float add = s_term + (float)up;
                 float P[16];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) P[r] = exp2_raw(z[r] + add);
+                for (int r = 0; r < 16; ++r) P[r] = exp2_raw(fmaf(d[r], c, add));
                 if (MODE == WALK_ITEMS) {
                     float4 tg[4];
 #pragma unroll
@@ -617,19 +642,21 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                     if (NS == 2 && up < -20) {        // a tile far below the reference: its sum for db from the probabilities as they are
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            b = fmaf(exp2_raw(z[4 * q] + s_term), tg[q].x, b); b = fmaf(exp2_raw(z[4 * q + 1] + s_term), tg[q].y, b);
-                            b = fmaf(exp2_raw(z[4 * q + 2] + s_term), tg[q].z, b); b = fmaf(exp2_raw(z[4 * q + 3] + s_term), tg[q].w, b);
+                            b = fmaf(exp2_raw(d[4 * q] + s_term), tg[q].x, b); b = fmaf(exp2_raw(d[4 * q + 1] + s_term), tg[q].y, b);
+                            b = fmaf(exp2_raw(d[4 * q + 2] + s_term), tg[q].z, b); b = fmaf(exp2_raw(d[4 * q + 3] + s_term), tg[q].w, b);
                         }
                     }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         P[4 * q] *= tg[q].x; P[4 * q + 1] *= tg[q].y; P[4 * q + 2] *= tg[q].z; P[4 * q + 3] *= tg[q].w;
                     }
-                    if (NS == 1 || up >= -20) {
+                    if (want_b) {
+                        if (NS == 1 || up >= -20) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) b += P[r];
+                            for (int r = 0; r < 16; ++r) b += P[r];
+                        }
+                        b_sum += NS == 2 ? ldexpf(b, -ge - (up < -20 ? 0 : up)) : b;
                     }
-                    b_sum += NS == 2 ? ldexpf(b, -ge - (up < -20 ? 0 : up)) : b;
                 }
                 uint4 pf[NS][2];
 #pragma unroll
@@ -705,6 +732,23 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     static_assert(MODE == WALK_STATS || STAGE * 16 >= 64 * KP * 4, "a stage holds 64 rows of sums");
     static_assert(MODE == WALK_STATS || STAGE * 16 >= list_length(KP) * 8, "a stage holds a list and its order");
     float *rows = (float *)stage0;
+    uint32_t *list = (uint32_t *)stage1;
+    const int64_t i0 = (int64_t)s_block * S_ROWS;
+    const Finish &f = p.f;
+    __syncthreads();
+    bool more = f.n_places > 0 && (!f.named || f.named[i0 >> 6] || f.named[(i0 >> 6) + 1]);
+    const bool any = more;
+    int total = 0, lower = 0;                         // of the sorted order: where the second half's items begin
+    if (any) {
+        int64_t step = -1;
+        total = find_places<KP>(f, list, counts, (uint8_t *)aside, i0, 128, step, more);
+        int hi = total;
+        while (lower < hi) {
+            const int mid = (lower + hi) / 2;
+            if (list[list_length(KP) + mid] >> 12 < 64) lower = mid + 1;
+            else hi = mid;
+        }
+    }
     for (int half = 0; half < 2; ++half) {
         __syncthreads();
         if ((wave >> 1) == half) {
@@ -716,7 +760,9 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
             if (h == 0) row_b[r] = -b_sum;
         }
         __syncthreads();
-        finish_rows<T, KP>(p.f, rows, row_b, (uint32_t *)stage1, counts, aside, aside_item, (int64_t)s_block * S_ROWS + half * 64);
+        if (any && more) add_all_places<T, KP>(f, rows, row_b, list, counts, aside, aside_item, i0 + half * 64);
+        else if (any) add_places<T, KP>(f, rows, row_b, list, aside, aside_item, half * 64, half ? lower : 0, half ? total : lower);
+        store_rows<T, KP>(f, rows, row_b, i0 + half * 64);
     }
 }
 
@@ -1077,7 +1123,8 @@ __global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, c
         row_b[threadIdx.x] = b;
     }
     __syncthreads();
-    finish_rows<T, KP>(f, rows, row_b, list, counts, aside, aside_item, i0);
+    if (f.n_places > 0 && (!f.named || f.named[i0 >> 6])) add_all_places<T, KP>(f, rows, row_b, list, counts, aside, aside_item, i0);
+    store_rows<T, KP>(f, rows, row_b, i0);
 }
 
 // ---------------------------------------------------------------------------- launches
@@ -1282,7 +1329,9 @@ static PrepParams prepare_sides(const ifr_catalogue &c, const Side &x, const Sid
     p.v_blocks = v.lies ? (v.padded + 255) / 256 : v.tiles; p.v_padded = v.padded; p.x_padded = x.padded;
     p.k = c.k; p.KP = pad_factors(c.k);
     p.v_exp = v.exps; p.x_exp = x.exps; p.v_frag = v.frag; p.x_frag = x.frag;
-    p.ibase = c.ibase; p.base_unit = (float)(c.scale / LN2); p.item_term = item_term;
+    p.ibase = c.ibase; p.item_term = item_term;
+    p.base_unit = c.dtype == IFR_F32 ? (float)(c.scale / LN2) : 1.f;
+    p.lse_unit = c.dtype == IFR_F32 ? -LOG2E : (float)(-1.0 / c.scale);
     return p;
 }
 

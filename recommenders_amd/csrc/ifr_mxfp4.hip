@@ -9,6 +9,7 @@ namespace ifr {
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(256) void mx_scores_kernel(MxScoreParams p, int kb,
 #pragma unroll
             for (int i = 0; i < 32 * ROW / 64; ++i) {
                 const int at = i * 64 + lane, row = at / ROW, c = (at - row * ROW) * PIECE;
-                if (row < rows) *(uint4 *)(out + row * p.ld + c) = *(const uint4 *)(strip + row * PITCH + c);
+                if (row < rows) __builtin_nontemporal_store(*(const u4 *)(strip + row * PITCH + c), (u4 *)(out + row * p.ld + c));
             }
         } else {
             for (int row = 0; row < rows; ++row)
