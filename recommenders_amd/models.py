@@ -6,7 +6,9 @@ reference's signatures, return types, exceptions and the three result caches
 (`ranked_items`, `item_scores`, `item_scores_mapped_indices`, recommender.py:160-168, 655-659).
 It can be mixed into the reference's own classes or used through the
 stand-alone `BPR` / `MF` / `WMF` classes below, which take already-trained parameters
-(`init_params=...`, like the reference's `trainable=False` usage; training is out of scope).
+(`init_params=...`, like the reference's `trainable=False` usage; the reference's trainers are out
+of scope).  What those classes learn here -- preferences between slates, rewards of shown slates --
+is in learning.py.
 
 There is no CPU fallback: every score and every ordering comes from libifr.so.  The only host
 work is bookkeeping (id maps, candidate arrays, the all-ties case of an unknown user, whose
@@ -15,6 +17,7 @@ work is bookkeeping (id maps, candidate arrays, the all-ties case of an unknown 
 import numpy as np
 
 from .exception import ScoreException
+from .learning import CatalogueLearningMixin
 
 
 class RecommenderBase:
@@ -313,7 +316,7 @@ class HipScoringMixin:
         return ids.cpu().numpy(), scores.cpu().numpy()
 
 
-class BPR(HipScoringMixin, RecommenderBase):
+class BPR(CatalogueLearningMixin, HipScoringMixin, RecommenderBase):
     """cornac.models.BPR scoring (cornac/models/bpr/recom_bpr.pyx:272-297): s = Bi + V.U[u].
     init_params: {'U': [total_users,k], 'V': [total_items,k], 'Bi': [total_items]}."""
 
@@ -331,6 +334,9 @@ class BPR(HipScoringMixin, RecommenderBase):
     def _hip_factor_params(self):
         bi = self.i_biases if (self.i_biases is not None and self.use_bias) else np.zeros(len(self.i_factors), np.float32)
         return self.u_factors, self.i_factors, None, bi
+
+    def _hip_learned(self):
+        return "u_factors", "i_factors", "i_biases" if self.use_bias and self.i_biases is not None else None
 
     _hip_item_must_be_known = False     # BPR.score never raises (recom_bpr.pyx:290-297)
     _ann_supported = True
@@ -355,7 +361,7 @@ class BPR(HipScoringMixin, RecommenderBase):
         return int(user_idx) % n
 
 
-class MF(HipScoringMixin, RecommenderBase):
+class MF(CatalogueLearningMixin, HipScoringMixin, RecommenderBase):
     """cornac.models.MF scoring (cornac/models/mf/recom_mf.py:254-286):
     s = ((mu + Bi) + Bu[u]) + V.U[u]; an unknown user keeps only mu + Bi."""
 
@@ -385,6 +391,9 @@ class MF(HipScoringMixin, RecommenderBase):
         ibase = (np.float32(self.global_mean) + bi).astype(np.float32)       # fl(mu + Bi), recom_mf.py:276
         return self.u_factors, self.i_factors, bu, ibase
 
+    def _hip_learned(self):             # mu and Bu shift all of a user's scores: no probability depends on them
+        return "u_factors", "i_factors", "i_biases" if self.i_biases is not None else None
+
     def _hip_user_row(self, user_idx):
         if self.knows_user(user_idx):
             return int(user_idx)
@@ -392,7 +401,7 @@ class MF(HipScoringMixin, RecommenderBase):
         return int(user_idx) if self.num_users <= user_idx < self._hip_zero_row else self._hip_zero_row
 
 
-class WMF(HipScoringMixin, RecommenderBase):
+class WMF(CatalogueLearningMixin, HipScoringMixin, RecommenderBase):
     """cornac.models.WMF scoring (cornac/models/wmf/recom_wmf.py:213-239): s = V.U[u];
     unknown users / items raise ScoreException."""
 
@@ -407,6 +416,9 @@ class WMF(HipScoringMixin, RecommenderBase):
 
     def _hip_factor_params(self):
         return self.U, self.V, None, None
+
+    def _hip_learned(self):
+        return "U", "V", None
 
     def _hip_user_row(self, user_idx):
         return int(user_idx) if self.knows_user(user_idx) else -1

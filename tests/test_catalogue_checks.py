@@ -119,3 +119,27 @@ def test_policy_refusals(kw, error, words):
     with pytest.raises(error, match=words):
         _pol(**kw)
     _pol()
+
+
+# ---------------------------------------------------------------- the factor models' checks
+def test_learning_refusals():
+    import numpy as np
+
+    from recommenders_amd.models import BPR
+    m = BPR(k=3, init_params={"U": np.zeros((4, 3), np.float32), "V": np.zeros((5, 3), np.float32), "Bi": np.zeros(5, np.float32)})
+    assert m._hip_users([0, 3, 3]).tolist() == [0, 3, 3] and m._hip_slates([1, -1], 2, "x").shape == (2, 1)
+    for users in ([4], [-1, 0]):
+        with pytest.raises(IndexError, match="user index"):
+            m._hip_users(users)
+    for users in ([[0]], [0.5]):
+        with pytest.raises(ValueError, match="users"):
+            m._hip_users(users)
+    for items in ([[5]], [[-2]]):
+        with pytest.raises(IndexError, match="item index"):
+            m._hip_slates(items, 1, "chosen")
+    with pytest.raises(ValueError, match="chosen"):
+        m._hip_slates([[1], [2]], 1, "chosen")
+    for bad in (dict(batch_size=0), dict(learning_rate=0.0), dict(reg=-1.0), dict(epochs=-1)):
+        with pytest.raises(ValueError, match="batch_size"):
+            list(m._hip_schedule(3, **{**dict(batch_size=2, epochs=1, learning_rate=.1, reg=0.0, seed=0), **bad}))
+    assert sorted(np.concatenate([b for _, b in m._hip_schedule(5, 2, 1, .1, 0.0, 0)]).tolist()) == list(range(5))
