@@ -81,26 +81,27 @@ def _refuse(t, name, dtypes, shape, device):
     raise ValueError(f"{name} requires a gradient: autograd does not see this call, pass {name}.detach() and use the gradients it returns")
 
 
-def _recorded(t):
-    if not t.requires_grad:
-        return False
+def _recorded():
     import torch
     return torch.is_grad_enabled()
 
 
 def _matrix(t, name, dtypes, cols=None, rows=None, device=None):
-    """`t` as a matrix with contiguous rows at least its width apart; ValueError / TypeError where it is not what `name` is."""
+    """(`t`, elements from one row to the next): a matrix with contiguous rows at least its width apart -- a single row reaches as far as it
+    is wide; ValueError / TypeError where it is not what `name` is."""
     try:
         n, w = t.shape
         fine = t.dtype in dtypes and (rows is None or n == rows) and (cols is None or w == cols) and (device is None or t.device == device)
-        n, stride = n, t.stride()
     except (AttributeError, TypeError, ValueError):
         fine = False
-    if not fine or _recorded(t):
+    if not fine or t.requires_grad and _recorded():
         _refuse(t, name, dtypes, (rows, cols), device)
-    if (stride[1] != 1 and w > 1 or stride[0] < w and n > 1) and n * w:
-        t = t.contiguous()
-    return t
+    down, across = t.stride()
+    if across == 1 and down >= w and n > 1:
+        return t, down
+    if (across == 1 or w <= 1) and n <= 1:
+        return t, w
+    return t.contiguous(), w
 
 
 def _vector(t, name, n, device=None):
@@ -108,21 +109,20 @@ def _vector(t, name, n, device=None):
     if t is None:
         return None
     import torch
-    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.shape != (n,) or (device is not None and t.device != device) or _recorded(t):
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.shape != (n,) or (device is not None and t.device != device) or t.requires_grad and _recorded():
         _refuse(t, name, (torch.float32,), (n,), device)
     return t.contiguous()
 
 
-def _row_stride(t):
-    """Elements from one row to the next; a single row reaches as far as it is wide."""
-    if t is None:
-        return 0
-    n, w = t.shape
-    return max(t.stride(0), w) if n > 1 else w
+NONE = (None, 0)
+
+
+def _optional(t, *args):
+    return NONE if t is None else _matrix(t, *args)
 
 
 def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
-    """What the log-probability calls take: (X, V, ids, ibase) ready for the library, or the refusal."""
+    """What the log-probability calls take, ready for the library -- (X, row stride), (V, row stride), (ids, row stride), ibase -- or the refusal."""
     import torch
     if isinstance(X, MxFp4Matrix) != isinstance(V, MxFp4Matrix):
         raise TypeError("X and V must both be tensors or both be MxFp4Matrix")
@@ -132,9 +132,10 @@ def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
         for name, q in (("X", X), ("V", V)):
             if device is not None and q.device != device:
                 raise ValueError(f"{name} is on {q.device}, the scorer on {device}")
+        ldx = ldv = 0
     else:
-        X = _matrix(X, "X", (torch.float32, torch.bfloat16), device=device)
-        V = _matrix(V, "V", (X.dtype,), cols=X.shape[1], device=device)
+        X, ldx = _matrix(X, "X", (torch.float32, torch.bfloat16), device=device)
+        V, ldv = _matrix(V, "V", (X.dtype,), cols=X.shape[1], device=device)
     n, k = X.shape
     n_items = V.shape[0]
     if not 1 <= k <= MAX_FACTORS:
@@ -144,26 +145,21 @@ def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
     scale = float(scale)
     if not 0.0 < scale <= 1e30:
         raise ValueError("scale must be positive")
-    ids = _matrix(ids, "ids", (torch.int32,), rows=n, device=device)
-    return X, V, ids, _vector(ibase, "ibase", n_items, device)
+    return (X, ldx), (V, ldv), _matrix(ids, "ids", (torch.int32,), rows=n, device=device), _vector(ibase, "ibase", n_items, device)
 
 
 def check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, weight, beta, kind, label_smoothing, margin, device=None):
-    """What `preference_loss` takes, ready for the library, or the refusal."""
+    """What `preference_loss` takes, ready for the library -- six (matrix, row stride), weight -- or the refusal."""
     import torch
     f32, masks = (torch.float32,), (torch.bool, torch.uint8)
-    chosen = _matrix(chosen, "chosen", f32, device=device)
-    n = chosen.shape[0]
-    rejected = _matrix(rejected, "rejected", f32, rows=n, device=device)
+    c = _matrix(chosen, "chosen", f32, None, None, device)
+    n, wc = c[0].shape
+    r = _matrix(rejected, "rejected", f32, None, n, device)
+    wr = r[0].shape[1]
     if (ref_chosen is None) != (ref_rejected is None):
         raise ValueError("a reference needs both ref_chosen and ref_rejected")
-    if ref_chosen is not None:
-        ref_chosen = _matrix(ref_chosen, "ref_chosen", f32, rows=n, cols=chosen.shape[1], device=device)
-        ref_rejected = _matrix(ref_rejected, "ref_rejected", f32, rows=n, cols=rejected.shape[1], device=device)
-    if mask_chosen is not None:
-        mask_chosen = _matrix(mask_chosen, "mask_chosen", masks, rows=n, cols=chosen.shape[1], device=device)
-    if mask_rejected is not None:
-        mask_rejected = _matrix(mask_rejected, "mask_rejected", masks, rows=n, cols=rejected.shape[1], device=device)
+    matrices = (c, r, _optional(ref_chosen, "ref_chosen", f32, wc, n, device), _optional(ref_rejected, "ref_rejected", f32, wr, n, device),
+                _optional(mask_chosen, "mask_chosen", masks, wc, n, device), _optional(mask_rejected, "mask_rejected", masks, wr, n, device))
     if kind not in _KINDS:
         raise ValueError("kind must be 'logistic', 'hinge' or 'squared'")
     if not 0.0 < float(beta) <= 1e30:
@@ -174,20 +170,17 @@ def check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, ma
         raise ValueError("label_smoothing needs kind='logistic'")
     if not abs(float(margin)) < 1e30:
         raise ValueError("margin must be finite")
-    return chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, _vector(weight, "weight", n, device)
+    return matrices, _vector(weight, "weight", n, device)
 
 
 def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef, reduction, device=None):
-    """What `policy_loss` takes, ready for the library, or the refusal."""
+    """What `policy_loss` takes, ready for the library -- four (matrix, row stride), advantages, weight -- or the refusal."""
     import torch
     f32 = (torch.float32,)
-    logp = _matrix(logp, "logp", f32, device=device)
-    n, width = logp.shape
-    old_logp = _matrix(old_logp, "old_logp", f32, rows=n, cols=width, device=device)
-    if ref_logp is not None:
-        ref_logp = _matrix(ref_logp, "ref_logp", f32, rows=n, cols=width, device=device)
-    if mask is not None:
-        mask = _matrix(mask, "mask", (torch.bool, torch.uint8), rows=n, cols=width, device=device)
+    x = _matrix(logp, "logp", f32, None, None, device)
+    n, width = x[0].shape
+    matrices = (x, _matrix(old_logp, "old_logp", f32, width, n, device), _optional(ref_logp, "ref_logp", f32, width, n, device),
+                _optional(mask, "mask", (torch.bool, torch.uint8), width, n, device))
     if advantages is None:
         raise TypeError("advantages must be a torch tensor")
     if reduction not in _REDUCTIONS:
@@ -198,7 +191,7 @@ def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, c
         raise ValueError("kl_coef must be finite")
     if kl_coef and ref_logp is None:
         raise ValueError("kl_coef needs ref_logp")
-    return logp, old_logp, _vector(advantages, "advantages", n, device), ref_logp, mask, _vector(weight, "weight", n, device)
+    return matrices, _vector(advantages, "advantages", n, device), _vector(weight, "weight", n, device)
 
 
 class CatalogueOps:
@@ -228,14 +221,14 @@ class CatalogueOps:
         """`X` [n, k] (fp32 or bf16) as an MxFp4Matrix: per block of 32 columns the exponent floor(log2 max|v|) - 2 (at least -127)
         and elements rounded to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 times it, ties to the even code, at most 6."""
         import torch
-        X = _matrix(X, "X", (torch.float32, torch.bfloat16), device=self.device)
+        X, ld = _matrix(X, "X", (torch.float32, torch.bfloat16), None, None, self.device)
         n, k = X.shape
         if k < 1:
             raise ValueError("X must have at least one column")
         kb = (k + 31) // 32
         codes = torch.empty((n, 16 * kb), dtype=torch.uint8, device=self.device)
         scales = torch.empty((n, kb), dtype=torch.uint8, device=self.device)
-        self._check(self._lib.ifr_mxfp4_quantize(self._h, _ptr(X), F32 if X.dtype == torch.float32 else BF16, n, k, _row_stride(X),
+        self._check(self._lib.ifr_mxfp4_quantize(self._h, _ptr(X), F32 if X.dtype == torch.float32 else BF16, n, k, ld,
                                                  _ptr(codes), _ptr(scales), self._stream_of()))
         return MxFp4Matrix._of(codes, scales, k)
 
@@ -244,19 +237,20 @@ class CatalogueOps:
         import torch
         if not isinstance(q, MxFp4Matrix) or q.device != self.device:
             raise ValueError(f"dequantize_mxfp4 takes an MxFp4Matrix on {self.device}")
-        out = self._out(out, q.shape, torch.float32)
-        self._check(self._lib.ifr_mxfp4_dequantize(self._h, _ptr(q.codes), _ptr(q.scales), q.shape[0], q.k, _ptr(out), _row_stride(out),
+        out, ld = self._out(out, q.shape, torch.float32)
+        self._check(self._lib.ifr_mxfp4_dequantize(self._h, _ptr(q.codes), _ptr(q.scales), q.shape[0], q.k, _ptr(out), ld,
                                                    self._stream_of()))
         return out
 
     def _out(self, out, shape, dtype):
+        """(output, row stride)"""
         import torch
         if out is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return torch.empty(shape, dtype=dtype, device=self.device), shape[1]
         if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != self.device or (out.numel() and (
                 out.stride(1) != 1 and out.shape[1] > 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1])):
-            raise ValueError(f"out must be {str(dtype).replace('torch.', '')} {list(shape)} on {self.device} with contiguous rows")
-        return out
+            raise ValueError(f"out must be {_name(dtype)} {list(shape)} on {self.device} with contiguous rows")
+        return out, out.stride(0) if shape[0] > 1 else shape[1]
 
     def score_mxfp4(self, X, V, ubase=None, ibase=None, out=None, dtype=None):
         """Score rows [n, n_items] of a 4-bit model, beside `score_dense`: (ibase + ubase) + <X[u], V[i]>, fp32 sums rounded once to
@@ -275,20 +269,19 @@ class CatalogueOps:
             raise TypeError("score_mxfp4 writes float32 or bfloat16")
         n, n_items = X.shape[0], V.shape[0]
         ubase, ibase = _vector(ubase, "ubase", n, self.device), _vector(ibase, "ibase", n_items, self.device)
-        out = self._out(out, (n, n_items), dtype)
+        out, ld = self._out(out, (n, n_items), dtype)
         self._check(self._lib.ifr_mxfp4_scores(self._h, _ptr(X.codes), _ptr(X.scales), n, _ptr(V.codes), _ptr(V.scales), n_items, X.k, _ptr(ubase),
-                                               _ptr(ibase), _ptr(out), F32 if dtype == torch.float32 else BF16, _row_stride(out), self._stream_of()))
+                                               _ptr(ibase), _ptr(out), F32 if dtype == torch.float32 else BF16, ld, self._stream_of()))
         return out
 
     # ------------------------------------------------------------------ log-probabilities
-    def _catalogue(self, X, V, ibase, scale):
+    def _catalogue(self, X, ldx, V, ldv, ibase, scale):
         import torch
-        mx = isinstance(X, MxFp4Matrix)
         n, k = X.shape
-        if mx:
-            return _lib.Catalogue(X.codes.data_ptr(), V.codes.data_ptr(), X.scales.data_ptr(), V.scales.data_ptr(), _ptr(ibase), n, V.shape[0], 0, 0, k, MXFP4, float(scale))
-        return _lib.Catalogue(X.data_ptr(), V.data_ptr(), None, None, _ptr(ibase), n, V.shape[0], _row_stride(X), _row_stride(V), k,
-                              F32 if X.dtype is torch.float32 else BF16, float(scale))
+        if isinstance(X, MxFp4Matrix):
+            return _lib.Catalogue(X.codes.data_ptr(), V.codes.data_ptr(), X.scales.data_ptr(), V.scales.data_ptr(), _ptr(ibase), n, V.shape[0], 0, 0, k, MXFP4,
+                                  float(scale))
+        return _lib.Catalogue(X.data_ptr(), V.data_ptr(), None, None, _ptr(ibase), n, V.shape[0], ldx, ldv, k, F32 if X.dtype is torch.float32 else BF16, float(scale))
 
     def catalogue_logprob(self, X, V, ids, ibase=None, scale=1.0):
         """(logp [n, m], lse [n]), fp32: logp[u, j] = z[u, ids[u, j]] - lse[u] with z[u, i] = scale * (<X[u], V[i]> + ibase[i]) and
@@ -296,13 +289,13 @@ class CatalogueOps:
         MxFp4Matrix (a frozen model); ids int32 [n, m], negative = an empty place (logp 0; an id past the catalogue gives NaN);
         an ibase of -inf takes an item out.  The n x n_items scores are not stored."""
         import torch
-        X, V, ids, ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
+        (X, ldx), (V, ldv), (ids, ld_ids), ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
         n, m = ids.shape
-        c = self._catalogue(X, V, ibase, scale)
+        c = self._catalogue(X, ldx, V, ldv, ibase, scale)
         logp = torch.empty((n, m), dtype=torch.float32, device=self.device)
         lse = torch.empty((n,), dtype=torch.float32, device=self.device)
         ws, need = self._workspace(self._lib.ifr_catalogue_logprob_workspace, (c.n, c.n_items, c.k, c.dtype), ctypes.byref(c))
-        self._check(self._lib.ifr_catalogue_logprob(self._h, ctypes.byref(c), _ptr(ids), m, _row_stride(ids), _ptr(logp), max(m, 1), _ptr(lse),
+        self._check(self._lib.ifr_catalogue_logprob(self._h, ctypes.byref(c), _ptr(ids), m, ld_ids, _ptr(logp), max(m, 1), _ptr(lse),
                                                     _ptr(ws), need, self._stream_of()))
         return logp, lse
 
@@ -315,9 +308,9 @@ class CatalogueOps:
             raise TypeError("a 4-bit model has no gradient")
         if set(want) - {"X", "V", "ibase"}:
             raise ValueError("want holds 'X', 'V' and 'ibase'")
-        X, V, ids, ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
+        (X, ldx), (V, ldv), (ids, ld_ids), ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
         n, m = ids.shape
-        dlogp = _matrix(dlogp, "dlogp", (torch.float32,), rows=n, cols=m, device=self.device)
+        dlogp, ld_dlogp = _matrix(dlogp, "dlogp", (torch.float32,), m, n, self.device)
         if lse is None:
             raise TypeError("lse must be a torch tensor")
         lse = _vector(lse, "lse", n, self.device)
@@ -325,12 +318,12 @@ class CatalogueOps:
         dX = empty((n, X.shape[1]), dtype=X.dtype, device=self.device) if "X" in want else None
         dV = empty((V.shape[0], V.shape[1]), dtype=V.dtype, device=self.device) if "V" in want else None
         db = empty((V.shape[0],), dtype=torch.float32, device=self.device) if "ibase" in want and ibase is not None else None
-        c = self._catalogue(X, V, ibase, scale)
+        c = self._catalogue(X, ldx, V, ldv, ibase, scale)
         ws, need = self._workspace(self._lib.ifr_catalogue_logprob_backward_workspace, (c.n, c.n_items, c.k, c.dtype, m, dX is None, dV is None, db is None),
                                    ctypes.byref(c), m, int(dX is not None), int(dV is not None), int(db is not None))
-        self._check(self._lib.ifr_catalogue_logprob_backward(self._h, ctypes.byref(c), _ptr(ids), m, _row_stride(ids), _ptr(lse), _ptr(dlogp), _row_stride(dlogp),
-                                                             _ptr(dX), 0 if dX is None else _row_stride(dX), _ptr(dV), 0 if dV is None else _row_stride(dV),
-                                                             _ptr(db), _ptr(ws), need, self._stream_of()))
+        k = X.shape[1]
+        self._check(self._lib.ifr_catalogue_logprob_backward(self._h, ctypes.byref(c), _ptr(ids), m, ld_ids, _ptr(lse), _ptr(dlogp), ld_dlogp, _ptr(dX), k,
+                                                             _ptr(dV), k, _ptr(db), _ptr(ws), need, self._stream_of()))
         return dX, dV, db
 
     # ------------------------------------------------------------------ losses
@@ -341,16 +334,16 @@ class CatalogueOps:
         the rejected slate and Cr, Rr those of a frozen reference.  kind "logistic": log(1 + exp(-h)), smoothed towards the other
         order by label_smoothing; "hinge": max(0, 1 - h); "squared": ((h - 1/2) / beta)^2.  d_chosen and d_rejected are the
         gradients of sum(weight * loss), weight 1 unless given.  Slates of one item with beta = 1 and no reference are BPR's criterion."""
-        chosen, rejected, ref_c, ref_r, mask_c, mask_r, weight = check_preference(
-            chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, weight, beta, kind, label_smoothing, margin, self.device)
-        n = chosen.shape[0]
-        r = PreferenceLoss(chosen.new_empty(n), chosen.new_empty(n), chosen.new_empty(chosen.shape), chosen.new_empty(rejected.shape))
-        p = _lib.Preference(n, chosen.shape[1], rejected.shape[1], _KINDS[kind], int(bool(average)), chosen.data_ptr(), rejected.data_ptr(), _ptr(ref_c),
-                            _ptr(ref_r), _ptr(mask_c), _ptr(mask_r), _ptr(weight), r[0].data_ptr(), r[1].data_ptr(), r[2].data_ptr(), r[3].data_ptr(),
-                            _row_stride(chosen), _row_stride(rejected), _row_stride(ref_c), _row_stride(ref_r), _row_stride(mask_c), _row_stride(mask_r),
-                            chosen.shape[1], rejected.shape[1], float(beta), float(margin), float(label_smoothing))
+        (c, r, rc, rr, mc, mr), weight = check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, weight, beta, kind,
+                                                          label_smoothing, margin, self.device)
+        n, wc = c[0].shape
+        wr = r[0].shape[1]
+        loss, h, d_chosen, d_rejected = c[0].new_empty(n), c[0].new_empty(n), c[0].new_empty((n, wc)), c[0].new_empty((n, wr))
+        p = _lib.Preference(n, wc, wr, _KINDS[kind], 1 if average else 0, c[0].data_ptr(), r[0].data_ptr(), _ptr(rc[0]), _ptr(rr[0]), _ptr(mc[0]), _ptr(mr[0]),
+                            _ptr(weight), loss.data_ptr(), h.data_ptr(), d_chosen.data_ptr(), d_rejected.data_ptr(), c[1], r[1], rc[1], rr[1], mc[1], mr[1],
+                            wc, wr, float(beta), float(margin), float(label_smoothing))
         self._check(self._lib.ifr_preference_loss(self._h, ctypes.byref(p), self._stream_of()))
-        return r
+        return PreferenceLoss(loss, h, d_chosen, d_rejected)
 
     def policy_loss(self, logp, old_logp, advantages, ref_logp=None, mask=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="row", weight=None):
         """PolicyLoss(loss [n], kl [n], clipped int32 [n], d_logp [n, places]) of n rows of choices sampled from an older policy: per
@@ -359,13 +352,13 @@ class CatalogueOps:
         1 ("sum"), 1 / places of the row ("row") or 1 / places of the batch ("batch"); d_logp is the gradient of sum(loss).  kl is the row's
         mean (None without ref_logp), clipped its number of clipped places."""
         import torch
-        logp, old_logp, advantages, ref_logp, mask, weight = check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef,
-                                                                          reduction, self.device)
-        n, width = logp.shape
-        r = PolicyLoss(logp.new_empty(n), None if ref_logp is None else logp.new_empty(n), torch.empty(n, dtype=torch.int32, device=self.device), logp.new_empty((n, width)))
-        p = _lib.Policy(n, width, _REDUCTIONS[reduction], logp.data_ptr(), old_logp.data_ptr(), _ptr(ref_logp), advantages.data_ptr(), _ptr(weight), _ptr(mask),
-                        r[0].data_ptr(), _ptr(r[1]), r[2].data_ptr(), r[3].data_ptr(), _row_stride(logp), _row_stride(old_logp), _row_stride(ref_logp),
-                        _row_stride(mask), width, float(clip_low), float(clip_high), float(kl_coef))
+        (x, old, ref, m), advantages, weight = check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef, reduction, self.device)
+        n, width = x[0].shape
+        loss, kl, d_logp = x[0].new_empty(n), None if ref_logp is None else x[0].new_empty(n), x[0].new_empty((n, width))
+        clipped = torch.empty(n, dtype=torch.int32, device=self.device)
+        p = _lib.Policy(n, width, _REDUCTIONS[reduction], x[0].data_ptr(), old[0].data_ptr(), _ptr(ref[0]), advantages.data_ptr(), _ptr(weight), _ptr(m[0]),
+                        loss.data_ptr(), _ptr(kl), clipped.data_ptr(), d_logp.data_ptr(), x[1], old[1], ref[1], m[1], width, float(clip_low), float(clip_high),
+                        float(kl_coef))
         ws, need = (None, 0) if mask is None or reduction != "batch" else self._workspace(self._lib.ifr_policy_loss_workspace, "policy", ctypes.byref(p))
         self._check(self._lib.ifr_policy_loss(self._h, ctypes.byref(p), _ptr(ws), need, self._stream_of()))
-        return r
+        return PolicyLoss(loss, kl, clipped, d_logp)

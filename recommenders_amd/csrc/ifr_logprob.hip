@@ -234,7 +234,7 @@ struct Finish {
     int64_t n_places, m, ldx, ld_dlogp, ld_dv, n_items;
     int k;
     float scale;
-    int vec_x;                         // rows of X are aligned for loads of four columns, k a multiple of four
+    int vec_x, vec_dv;                 // rows of X, of dV are aligned for four columns at once, k a multiple of four
 };
 
 struct WalkParams {
@@ -491,9 +491,18 @@ __device__ void store_rows(const Finish &f, const float *rows, const float *row_
 {
     if (f.dV) {
         T *out = (T *)f.dV;
-        for (int i = threadIdx.x; i < 64 * KP; i += 256) {
-            const int r = i / KP, c = i - r * KP;
-            if (i0 + r < f.n_items && c < f.k) out[(i0 + r) * f.ld_dv + c] = (T)(f.scale * rows[i]);
+        for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) {
+            const int r = i / (KP / 4), c = (i - r * (KP / 4)) * 4;
+            if (i0 + r >= f.n_items || c >= f.k) continue;
+            const float4 v = *(const float4 *)(rows + r * KP + c);
+            T o[4] = {(T)(f.scale * v.x), (T)(f.scale * v.y), (T)(f.scale * v.z), (T)(f.scale * v.w)};
+            T *to = out + (i0 + r) * f.ld_dv + c;
+            if (f.vec_dv) {
+                __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), o, 4 * sizeof(T));
+            } else {
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < f.k) to[j] = o[j];
+            }
         }
     }
     if (f.db)
@@ -583,6 +592,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
 #pragma unroll 2
         for (int sub = 0; sub < SUB; ++sub) {
             const int t = t0 + sub;
+            if (t >= p.t_tiles) break;                // the stage reaches behind the last row
             const uint4 *l1 = lds + sub * PART * NS;
             float4 tt[4];
 #pragma unroll
@@ -793,8 +803,15 @@ __device__ __forceinline__ uint4 piece(const T *row, int c, int k)
     return o;
 }
 
+// workgroups of direct_kernel a compute unit holds by its registers: the tile, the next one and UT users' operand, and what else there is
+constexpr int direct_resident(int KP, int UT, int size)
+{
+    const int r = (UT + 2) * KP * size / 16 + (size == 4 ? 36 : 60);
+    return r <= 132 ? 4 : r <= 168 ? 3 : r <= 256 ? 2 : 1;
+}
+
 template <typename T, int KP, int UT, bool VEC>
-__global__ __launch_bounds__(256) void direct_kernel(DirectParams p)
+__global__ __launch_bounds__(256, direct_resident(KP, UT, sizeof(T))) void direct_kernel(DirectParams p)
 {
     constexpr int N = 16 / sizeof(T), STEPS = KP / (4 * N);
     __shared__ float lm[4][UT * 16], ls[4][UT * 16];
@@ -1178,14 +1195,14 @@ struct Side {                          // one matrix as the walks read it
     uint4 *frag;
 };
 
-Side side(Pieces &w, const ifr_catalogue &c, bool users)
+Side side(Pieces &w, const ifr_catalogue &c, bool users, bool lies)
 {
     Side s;
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
     s.rows = users ? c.n : c.n_items;
     s.padded = up(s.rows, S_ROWS);
     s.tiles = s.padded / 32;
-    s.lies = rows_lie(c);
+    s.lies = lies;
     s.exps = w.take<int>(NS == 2 ? s.tiles : 0);
     s.frag = w.take<uint4>(s.lies ? 0 : s.tiles * NS * (KP / 16) * 64);
     return s;
@@ -1225,7 +1242,6 @@ int resident_blocks(int KP, int NS, int mode) { return 256 * (mode != WALK_STATS
 
 // Users one pass over V serves (their operand stays in registers: at most 128 of them), and up to how many users the direct kernel is taken.
 int direct_tiles(int KP, int64_t n) { return n <= 16 ? 1 : n <= 32 || KP > 128 ? 2 : 4; }
-constexpr int64_t DIRECT_USERS = 64;
 
 struct ForwardPlan {
     bool direct;
@@ -1236,23 +1252,28 @@ struct ForwardPlan {
     int mx_users;                      // user tiles of a wave, 4-bit model
 };
 
-ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c)
+// The direct kernel is taken for what one pass over V serves.  Beyond, the walk is as fast where V needs no other order (bf16 1 000 000 x
+// 128, 70 users: 64 us) and faster where it does (fp32, 70 users: 415 us by the walk, 458 us in two passes).
+int64_t direct_users(const ifr_catalogue &c) { return 16 * (pad_factors(c.k) > 128 ? 2 : 4); }
+
+ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c, bool lies)
 {
     ForwardPlan p = {};
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
     p.s_padded = up(c.n, S_ROWS);
     p.t_padded = up(c.n_items, S_ROWS);
-    p.direct = c.dtype != IFR_MXFP4 && c.n <= DIRECT_USERS;
+    p.direct = c.dtype != IFR_MXFP4 && c.n <= direct_users(c);
     if (p.direct) {
         const int64_t want = (c.n_items + 63) / 64;
-        p.split.count = (int)(want < 1024 ? want : 1024);      // workgroups of four waves
+        const int64_t most = 256 * direct_resident(KP, direct_tiles(KP, c.n), c.dtype == IFR_F32 ? 4 : 2);      // one round of them
+        p.split.count = (int)(want < most ? want : most);
         p.out_m = w.take<float>(p.split.count * p.s_padded);
         p.out_s = w.take<float>(p.split.count * p.s_padded);
         return p;
     }
     if (c.dtype != IFR_MXFP4) {
-        p.x = side(w, c, true);
-        p.v = side(w, c, false);
+        p.x = side(w, c, true, lies);
+        p.v = side(w, c, false, lies);
     }
     if (c.dtype == IFR_MXFP4) {                       // waves walk alone: 16 a compute unit, none with fewer than two tiles
         p.mx_users = c.n > 64 ? 4 : c.n > 32 ? 2 : 1;
@@ -1280,13 +1301,13 @@ struct BackwardPlan {
     Split split_x, split_v;
 };
 
-BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx, bool dv, bool db)
+BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx, bool dv, bool db, bool lies)
 {
     BackwardPlan p = {};
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
     const bool items = dv || db;
-    p.x = side(w, c, true);
-    p.v = side(w, c, false);
+    p.x = side(w, c, true, lies);
+    p.v = side(w, c, false, lies);
     p.item_term = w.take<float>(p.v.padded);
     p.user_term = w.take<float>(p.x.padded);
     p.G = w.take<float>(p.x.padded);
@@ -1308,18 +1329,21 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
 
 }  // namespace
 
+// The size does not depend on the matrices' addresses and strides: the larger of the two plans.
 size_t logprob_workspace(const ifr_catalogue &c)
 {
-    Pieces w{nullptr};
-    forward_plan(w, c);
-    return w.used;
+    Pieces a{nullptr}, b{nullptr};
+    forward_plan(a, c, false);
+    forward_plan(b, c, true);
+    return a.used > b.used ? a.used : b.used;
 }
 
 size_t logprob_backward_workspace(const ifr_catalogue &c, int64_t m, bool want_dx, bool want_dv, bool want_db)
 {
-    Pieces w{nullptr};
-    backward_plan(w, c, m, want_dx, want_dv, want_db);
-    return w.used;
+    Pieces a{nullptr}, b{nullptr};
+    backward_plan(a, c, m, want_dx, want_dv, want_db, false);
+    backward_plan(b, c, m, want_dx, want_dv, want_db, true);
+    return a.used > b.used ? a.used : b.used;
 }
 
 static PrepParams prepare_sides(const ifr_catalogue &c, const Side &x, const Side &v, float *item_term)
@@ -1341,7 +1365,7 @@ static void walk_sides(WalkParams &w, const ifr_catalogue &c, const Side &x, con
     w.s_frag = s.frag; w.t_frag = t.frag; w.s_exp = s.exps; w.t_exp = t.exps; w.s_n = s.rows; w.t_n = t.rows;
     w.s_rows = (const __bf16 *)(users_stay ? c.X : c.V); w.t_rows = (const __bf16 *)(users_stay ? c.V : c.X);
     w.s_ld = users_stay ? c.ldx : c.ldv; w.t_ld = users_stay ? c.ldv : c.ldx;
-    w.t_tiles = (int)t.tiles; w.s_blocks = (int)(s.padded / S_ROWS); w.s_padded = s.padded;
+    w.t_tiles = (int)((t.rows + 31) / 32); w.s_blocks = (int)(s.padded / S_ROWS); w.s_padded = s.padded;
 }
 
 template <typename T>
@@ -1401,7 +1425,7 @@ int launch_logprob(const ifr_catalogue &c, const int32_t *ids, int64_t m, int64_
                    void *ws, hipStream_t s)
 {
     Pieces w{(char *)ws};
-    const ForwardPlan p = forward_plan(w, c);
+    const ForwardPlan p = forward_plan(w, c, rows_lie(c));
     const int kb = (c.k + 31) / 32;
     if (p.direct) {
         if (c.dtype == IFR_F32) launch_direct<float>(c, p, s);
@@ -1457,7 +1481,7 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
         w.s_term = p.item_term; w.t_term = p.user_term; w.t_factor = NS == 2 ? p.G_scaled : p.G; w.t_factor_exp = p.g_exp;
         w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
-        w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx)};
+        w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx), fours(g.dV, g.ld_dv)};
         launch_walk<NS, WALK_ITEMS>(w, KP, s);
     }
     // the joins as one launch where dX's is short (its workgroups hold the memory of the other's)
@@ -1476,7 +1500,7 @@ int launch_logprob_backward(const ifr_catalogue &c, const int32_t *ids, int64_t 
                             hipStream_t s)
 {
     Pieces w{(char *)ws};
-    const BackwardPlan p = backward_plan(w, c, m, g.dX != nullptr, g.dV != nullptr, g.dibase != nullptr);
+    const BackwardPlan p = backward_plan(w, c, m, g.dX != nullptr, g.dV != nullptr, g.dibase != nullptr, rows_lie(c));
     if (c.dtype == IFR_F32) backward_typed<float>(c, ids, m, ld_ids, g, p, s);
     else backward_typed<__bf16>(c, ids, m, ld_ids, g, p, s);
     return hipGetLastError() == hipSuccess ? 0 : -1;

@@ -10,6 +10,7 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
@@ -79,32 +80,24 @@ __device__ __forceinline__ float mx_scale(uint32_t byte)
     return byte == 255 ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
 }
 
-__device__ __forceinline__ void mx_values8(uint32_t c, float s, float v[8])
-{
-    v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
-    v2f d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
-    v[0] = a[0] * s; v[1] = a[1] * s; v[2] = b[0] * s; v[3] = b[1] * s;
-    v[4] = d[0] * s; v[5] = d[1] * s; v[6] = e[0] * s; v[7] = e[1] * s;
-}
-
+// A lane takes four columns, so that a wave stores 1024 bytes in one piece (past the caches: it is bound by that store).
 template <bool VEC>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, int kb, float *out, int64_t ld)
 {
     const int64_t g = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
-    const int64_t row = g / (kb * 4);
-    const int c8 = (int)(g - row * (kb * 4));
-    if (row >= n) return;
-    float v[8];
-    mx_values8(((const uint32_t *)codes)[row * (kb * 4) + c8], mx_scale(scales[row * kb + (c8 >> 2)]), v);
-    float *o = out + row * ld + (int64_t)c8 * 8;
+    const int64_t row = g / (kb * 8);
+    const int c4 = (int)(g - row * (kb * 8));         // which 4 columns of the row
+    if (row >= n || (int64_t)c4 * 4 >= k) return;
+    const uint32_t c = ((const uint16_t *)codes)[row * (kb * 8) + c4];
+    const float s = mx_scale(scales[row * kb + (c4 >> 3)]);
+    const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+    const f4 v = {a[0] * s, a[1] * s, b[0] * s, b[1] * s};
+    float *o = out + row * ld + (int64_t)c4 * 4;
     if (VEC) {
-        if ((int64_t)c8 * 8 < k) {
-            ((float4 *)o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            ((float4 *)o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        }
+        __builtin_nontemporal_store(v, (f4 *)o);
     } else {
-        for (int j = 0; j < 8; ++j)
-            if ((int64_t)c8 * 8 + j < k) o[j] = v[j];
+        for (int j = 0; j < 4; ++j)
+            if ((int64_t)c4 * 4 + j < k) o[j] = v[j];
     }
 }
 
@@ -213,8 +206,8 @@ int launch_mx_quantize(const void *X, int bf16, int64_t n, int64_t k, int64_t ld
 int launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, float *out, int64_t ld, hipStream_t s)
 {
     const int kb = (int)((k + 31) / 32);
-    const dim3 grid = grid_of((n * kb * 4 + 255) / 256);
-    if (k % 8 == 0 && aligned16(out, ld * 4)) hipLaunchKernelGGL(mx_dequantize_kernel<true>, grid, dim3(256), 0, s, codes, scales, n, k, kb, out, ld);
+    const dim3 grid = grid_of((n * kb * 8 + 255) / 256);
+    if (k % 4 == 0 && aligned16(out, ld * 4)) hipLaunchKernelGGL(mx_dequantize_kernel<true>, grid, dim3(256), 0, s, codes, scales, n, k, kb, out, ld);
     else hipLaunchKernelGGL(mx_dequantize_kernel<false>, grid, dim3(256), 0, s, codes, scales, n, k, kb, out, ld);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
@@ -226,13 +219,14 @@ static void launch_mx_scores_typed(const MxScoreParams &p, int kb, hipStream_t s
     const int vec = aligned16(p.out, p.ld * (int64_t)sizeof(OUT));
     // few scores: 32 items a wave fill the chip; many: 128, which reads X a quarter as often and stores rows of 256 bytes or more
     const bool wide = it * qt >= 16384;
-    const int64_t gx = wide ? (it + 15) / 16 : (it + 3) / 4;
+    constexpr int IT = sizeof(OUT) == 2 ? 8 : 4;
+    const int64_t gx = wide ? (it + 4 * IT - 1) / (4 * IT) : (it + 3) / 4;
     int64_t gy = (4096 + gx - 1) / gx;
     gy = gy < qt ? gy : qt;
     const int64_t per = (qt + gy - 1) / gy;
     gy = (qt + per - 1) / per;
     const dim3 grid((uint32_t)gx, (uint32_t)gy);
-    if (wide) hipLaunchKernelGGL((mx_scores_kernel<STEPS, 4, OUT>), grid, dim3(256), 0, s, p, kb, qt, per, vec);
+    if (wide) hipLaunchKernelGGL((mx_scores_kernel<STEPS, IT, OUT>), grid, dim3(256), 0, s, p, kb, qt, per, vec);
     else hipLaunchKernelGGL((mx_scores_kernel<STEPS, 1, OUT>), grid, dim3(256), 0, s, p, kb, qt, per, vec);
 }
 

@@ -61,7 +61,9 @@ def test_catalogue_device_and_no_grad():
     with torch.no_grad():
         C.check_catalogue(X.clone().requires_grad_(), V, IDS, None, 1.0)
     a = C.check_catalogue(X.t().contiguous().t(), V, IDS[:, :1].expand(4, 5), None, 1.0)
-    assert a[0].stride() == (8, 1) and a[2].is_contiguous()
+    assert a[0][0].stride() == (8, 1) and a[0][1] == 8 and a[2][0].is_contiguous() and a[2][1] == 5
+    assert C.check_catalogue(torch.zeros((4, 20))[:, 3:11], V, IDS, None, 1.0)[0][1] == 20 and C.check_catalogue(X[:1].expand(4, 8), V, IDS, None, 1.0)[0][1] == 8
+    assert C.check_catalogue(torch.zeros((9, 20))[2:3, 3:11], V, IDS[:1], None, 1.0)[0][1] == 8
 
 
 L, R = torch.zeros((4, 3)), torch.zeros((4, 5))

@@ -368,6 +368,17 @@ def test_logprob_strides_and_empty_batches(torch, sc):
     args = (Xw[:, 3:40], Vw[:, 1:38], iw[:, 2:7])
     assert all(torch.equal(a, c) for a, c in zip(sc.catalogue_logprob(*args, ibase=b), want))
     assert all(torch.equal(a, c) for a, c in zip(sc.catalogue_logprob_backward(*args, want[1], dw[:, 1:6], ibase=b), grads))
+    # rows of whole pieces (read as they lie) and the same rows at an odd place (put in order first), in turn
+    X, V, b, ids, dlogp = _case(torch, 150, 300, 64, 5, "bfloat16", True, 24)
+    Xo, Vo = torch.zeros((150, 67), dtype=X.dtype, device="cuda"), torch.zeros((300, 65), dtype=X.dtype, device="cuda")
+    Xo[:, 3:], Vo[:, 1:] = X, V
+    want = sc.catalogue_logprob(X, V, ids, ibase=b)
+    grads = sc.catalogue_logprob_backward(X, V, ids, want[1], dlogp, ibase=b)
+    for args in ((Xo[:, 3:], Vo[:, 1:], ids), (X, Vo[:, 1:], ids), (Xo[:, 3:], V, ids), (X, V, ids)):
+        assert all(torch.equal(a, c) for a, c in zip(sc.catalogue_logprob(*args, ibase=b), want))
+        assert all(torch.equal(a, c) for a, c in zip(sc.catalogue_logprob_backward(*args, want[1], dlogp, ibase=b), grads))
+    X, V, b, ids, _ = _case(torch, 45, 120, 37, 5, "bfloat16", True, 14)
+    want = sc.catalogue_logprob(X, V, ids, ibase=b)
     # one user repeated by a broadcast, ids of another order
     e = sc.catalogue_logprob(X[:1].expand(45, 37), V, ids.t().contiguous().t(), ibase=b)
     assert float((e[1] - want[1][0]).abs().max()) == 0
