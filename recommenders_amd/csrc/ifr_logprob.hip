@@ -212,13 +212,6 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, int64_t n)
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
-// the terms alone, for the 4-bit walk
-__global__ __launch_bounds__(256) void item_terms_kernel(const float *ibase, int64_t n, int64_t padded, float *out)
-{
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < padded) out[i] = i < n ? (ibase ? ibase[i] : 0.f) : -INFINITY;
-}
-
 // ---------------------------------------------------------------------------- the walk
 
 enum { WALK_STATS = 0, WALK_USERS = 1, WALK_ITEMS = 2 };     // lse; the sums of dX (S users, T items); those of dV and db (S items, T users)
@@ -895,7 +888,7 @@ __global__ __launch_bounds__(256, direct_resident(KP, UT, sizeof(T))) void direc
 // the initial value of the sums.  Bound by the exponentials (v_exp_f32 at a quarter of the rate of the rest).
 struct MxWalkParams {
     const uint8_t *xc, *xs, *vc, *vs;
-    const float *base;                 // [t_tiles * 32]: ibase, -inf behind the last item
+    const float *base;                 // ibase or null
     int64_t n, n_items, s_padded;
     int kb, t_tiles, tiles_per_split;
     float c;
@@ -903,7 +896,7 @@ struct MxWalkParams {
 };
 
 template <int STEPS, int UT>
-__global__ __launch_bounds__(256) void walk_mx_kernel(MxWalkParams p)
+__global__ __launch_bounds__(256, STEPS <= 2 ? 3 : 2) void walk_mx_kernel(MxWalkParams p)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
     const int64_t s0 = (int64_t)blockIdx.x * 32 * UT;
@@ -931,6 +924,7 @@ __global__ __launch_bounds__(256) void walk_mx_kernel(MxWalkParams p)
     for (int t = 0; t < UT; ++t) { m[t] = -3.402823466e38f; sum[t] = 0.f; }
     const int split = blockIdx.y * 4 + wave;          // each wave walks items of its own
     const int first = split * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
+    const bool base_vec = p.base && ((uintptr_t)p.base & 15) == 0;
     uint4 a[STEPS];
     int sa[STEPS];
     float4 base[4];
@@ -938,8 +932,19 @@ __global__ __launch_bounds__(256) void walk_mx_kernel(MxWalkParams p)
         const int64_t item = min((int64_t)t * 32 + r, p.n_items - 1);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) block_of(p.vc, p.vs, item, s, &to[s], &scale[s]);
+        if (base_vec && (t + 1) * 32ll <= p.n_items) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) bases[q] = *(const float4 *)(p.base + (int64_t)t * 32 + 8 * q + 4 * h);
+            for (int q = 0; q < 4; ++q) bases[q] = *(const float4 *)(p.base + (int64_t)t * 32 + 8 * q + 4 * h);
+        } else {
+            float b[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int64_t i = (int64_t)t * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                b[e] = i < p.n_items ? (p.base ? p.base[i] : 0.f) : -INFINITY;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) bases[q] = make_float4(b[4 * q], b[4 * q + 1], b[4 * q + 2], b[4 * q + 3]);
+        }
     };
     if (first < last) load(first, a, sa, base);
     for (int t = first; t < last; ++t) {
@@ -1285,7 +1290,7 @@ ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c, bool lies)
     } else {
         p.split = split_plan(p.s_padded / S_ROWS, p.t_padded / 32, stage_tiles(NS, false), resident_blocks(KP, NS, WALK_STATS), 0.0);
     }
-    p.term = w.take<float>(p.t_padded + 32);         // a fetch brings 64, also where a stage holds 32 rows
+    p.term = w.take<float>(c.dtype == IFR_MXFP4 ? 0 : p.t_padded + 32);         // a fetch brings 64, also where a stage holds 32 rows
     p.out_m = w.take<float>(p.split.count * p.s_padded);
     p.out_s = w.take<float>(p.split.count * p.s_padded);
     return p;
@@ -1392,7 +1397,7 @@ static void launch_mx_users(const MxWalkParams &w, int users, dim3 grid, hipStre
 static void launch_mx_walk(const ifr_catalogue &c, const ForwardPlan &p, hipStream_t s)
 {
     const int kb = (c.k + 31) / 32;
-    const MxWalkParams w = {(const uint8_t *)c.X, c.x_scales, (const uint8_t *)c.V, c.v_scales, p.term, c.n, c.n_items, p.s_padded, kb, (int)(p.t_padded / 32),
+    const MxWalkParams w = {(const uint8_t *)c.X, c.x_scales, (const uint8_t *)c.V, c.v_scales, c.ibase, c.n, c.n_items, p.s_padded, kb, (int)((c.n_items + 31) / 32),
                             p.split.per, (float)(c.scale / LN2), p.out_m, p.out_s};
     const dim3 grid((uint32_t)((c.n + 32 * p.mx_users - 1) / (32 * p.mx_users)), (uint32_t)(p.split.count / 4));
     if (kb <= 2) launch_mx_users<1>(w, p.mx_users, grid, s);
@@ -1431,10 +1436,7 @@ int launch_logprob(const ifr_catalogue &c, const int32_t *ids, int64_t m, int64_
         if (c.dtype == IFR_F32) launch_direct<float>(c, p, s);
         else launch_direct<__bf16>(c, p, s);
     } else {
-        if (c.dtype == IFR_MXFP4) {
-            hipLaunchKernelGGL(item_terms_kernel, dim3((uint32_t)((p.t_padded + 255) / 256)), dim3(256), 0, s, c.ibase, c.n_items, p.t_padded, p.term);
-            launch_mx_walk(c, p, s);
-        }
+        if (c.dtype == IFR_MXFP4) launch_mx_walk(c, p, s);
         else if (c.dtype == IFR_F32) forward_typed<float>(c, p, s);
         else forward_typed<__bf16>(c, p, s);
     }

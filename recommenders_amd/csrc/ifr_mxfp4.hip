@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *codes
 // operand) and walks query tiles of 32 (B operand): D[item][query], four neighbouring items of one query a lane and quad, which go
 // through a strip of LDS of the wave's own so that rows are stored in long pieces.  Bound by the store of the scores for k <= 256.
 template <int STEPS, int IT, typename OUT>
-__global__ __launch_bounds__(256) void mx_scores_kernel(MxScoreParams p, int kb, int64_t q_tiles, int64_t q_per_block, int vec)
+__global__ __launch_bounds__(256, 2) void mx_scores_kernel(MxScoreParams p, int kb, int64_t q_tiles, int64_t q_per_block, int vec)
 {
     constexpr int COLS = IT * 32, PITCH = COLS + 16 / sizeof(OUT);      // a row further by one 16-byte piece: fewer bank conflicts
     __shared__ __align__(16) OUT strips[4][32 * PITCH];
