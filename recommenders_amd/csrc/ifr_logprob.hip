@@ -296,8 +296,8 @@ __device__ __forceinline__ void reads_ahead()
     __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
 }
 
-// places a workgroup keeps of those it looks through: their list and its sorted order fit a stage of walk_kernel
-constexpr int list_length(int KP) { return KP >= 128 ? 4096 : KP >= 64 ? 2048 : 1024; }
+// places a workgroup keeps of those it looks through: their users, gradients and sorted order, 12 bytes each, fit a stage of walk_kernel
+constexpr int list_length(int KP) { return KP >= 192 ? 4096 : KP >= 96 ? 2048 : KP >= 64 ? 1024 : 512; }
 
 // four columns of a row, zeros behind its end
 template <typename T>
@@ -326,7 +326,8 @@ template <int KP>
 __device__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t *item_of, int64_t i0, int count, int64_t &step, bool &more)
 {
     constexpr int LIST = list_length(KP), CAP = LIST / 4, EACH = CAP / 64;
-    uint32_t *order = list + LIST;
+    uint32_t *order = list + 2 * LIST;
+    float *gs = (float *)(list + LIST);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t steps = (f.n_places + 64 * EACH - 1) / (64 * EACH);          // of a wave, over all places
     const int64_t end = steps * (wave + 1) / 4;
@@ -334,9 +335,14 @@ __device__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t
     int held = 0;
     int32_t id[EACH], next[EACH];
     auto load = [&](int64_t at, int32_t *to) {
-        const int4 *src = (const int4 *)f.places + at * 64 * (EACH / 4) + lane;
+        if (EACH >= 4) {
+            const int4 *src = (const int4 *)f.places + at * 64 * (EACH / 4) + lane;
 #pragma unroll
-        for (int q = 0; q < EACH / 4; ++q) *(int4 *)(to + 4 * q) = src[q * 64];
+            for (int q = 0; q < EACH / 4; ++q) *(int4 *)(to + 4 * q) = src[q * 64];
+        } else {
+#pragma unroll
+            for (int q = 0; q < EACH; ++q) to[q] = f.places[(at * EACH + q) * 64 + lane];
+        }
     };
     if (step < end) load(step, id);
     while (step < end) {
@@ -361,8 +367,10 @@ __device__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t
                 for (int q = 0; q < EACH; ++q) {
                     const int64_t local = (int64_t)id[q] - i0;
                     if ((uint64_t)local < (uint64_t)count) {
-                        item_of[wave * CAP + before] = (uint8_t)local;
-                        list[wave * CAP + before++] = (uint32_t)(step * 64 * EACH + (q >> 2) * 256 + lane * 4 + (q & 3));      // at most 2^32 places
+                        const int in = EACH >= 4 ? (q >> 2) * 256 + lane * 4 + (q & 3) : q * 64 + lane;
+                        const int to = wave * CAP + before++;
+                        item_of[to] = (uint8_t)local;
+                        list[to] = (uint32_t)(step * 64 * EACH + in);                     // at most 2^32 places
                     }
                 }
             }
@@ -379,7 +387,13 @@ __device__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t
         if (w < wave) offset += counts[w];
         total += counts[w];
     }
-    for (int q = lane; q < held; q += 64) order[offset + q] = (uint32_t)item_of[wave * CAP + q] << 12 | (uint32_t)(wave * CAP + q);
+    for (int q = lane; q < held; q += 64) {           // places to users and gradients, each by one lane
+        const int at = wave * CAP + q;
+        const uint32_t place = list[at], u = place / (uint32_t)f.m;
+        order[offset + q] = (uint32_t)item_of[at] << 12 | (uint32_t)at;
+        list[at] = u;
+        gs[at] = f.dlogp[(int64_t)u * f.ld_dlogp + (place - u * (uint32_t)f.m)];
+    }
     int size = 1;
     while (size < total) size <<= 1;
     for (int q = total + tid; q < size; q += 256) order[q] = ~0u;
@@ -404,7 +418,8 @@ __device__ void add_places(const Finish &f, float *rows, float *row_b, const uin
 {
     constexpr int COLS = KP / 4;                      // threads of a row
     constexpr int GROUPS = 256 / COLS, BATCH = 16;
-    const uint32_t *order = list + list_length(KP);
+    const uint32_t *order = list + 2 * list_length(KP);
+    const float *gs = (const float *)(list + list_length(KP));
     const int tid = threadIdx.x, group = tid / COLS, c4 = (tid % COLS) * 4;
     if (from >= to) return;
     const T *X = (const T *)f.X;
@@ -434,10 +449,10 @@ __device__ void add_places(const Finish &f, float *rows, float *row_b, const uin
             for (int q = 0; q < BATCH; ++q) {
                 at[q] = -1;
                 if (q0 + q < end) {
-                    const uint32_t key = order[q0 + q], place = list[key & 4095], u = place / (uint32_t)f.m;
+                    const uint32_t key = order[q0 + q];
                     at[q] = (int)(key >> 12) - local0;
-                    g[q] = f.dlogp[(int64_t)u * f.ld_dlogp + (place - u * (uint32_t)f.m)];
-                    load4(X + (int64_t)u * f.ldx, c4, f.k, f.vec_x && c4 < f.k, x[q]);
+                    g[q] = gs[key & 4095];
+                    load4(X + (int64_t)list[key & 4095] * f.ldx, c4, f.k, f.vec_x && c4 < f.k, x[q]);
                 }
             }
 #pragma unroll
@@ -733,7 +748,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     __shared__ float row_b[64], aside[aside_floats(KP)];
     __shared__ int counts[4], aside_item[32];
     static_assert(MODE == WALK_STATS || STAGE * 16 >= 64 * KP * 4, "a stage holds 64 rows of sums");
-    static_assert(MODE == WALK_STATS || STAGE * 16 >= list_length(KP) * 8, "a stage holds a list and its order");
+    static_assert(MODE == WALK_STATS || STAGE * 16 >= list_length(KP) * 12, "a stage holds a list and its order");
     float *rows = (float *)stage0;
     uint32_t *list = (uint32_t *)stage1;
     const int64_t i0 = (int64_t)s_block * S_ROWS;
@@ -748,7 +763,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
         int hi = total;
         while (lower < hi) {
             const int mid = (lower + hi) / 2;
-            if (list[list_length(KP) + mid] >> 12 < 64) lower = mid + 1;
+            if (list[2 * list_length(KP) + mid] >> 12 < 64) lower = mid + 1;
             else hi = mid;
         }
     }
@@ -1121,7 +1136,7 @@ template <typename T, int KP>
 __global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, const float *acc_b, int splits, int64_t s_padded, Finish f)
 {
     __shared__ float rows[64 * KP];
-    __shared__ uint32_t list[list_length(KP) * 2];
+    __shared__ uint32_t list[list_length(KP) * 3];
     __shared__ float row_b[64], aside[aside_floats(KP)];
     __shared__ int counts[4], aside_item[32];
     if (blockIdx.x < x.blocks) {
