@@ -410,27 +410,30 @@ __device__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t
     return total;
 }
 
+// threads of a group in add_places: those of a row (four columns each), rounded up so that a wave holds whole groups
+constexpr int group_threads(int KP) { return KP > 128 ? 64 : KP > 64 ? 32 : KP > 32 ? 16 : 8; }
+
 // The found places [from, to) in their sorted order, of items whose local number is 64 at a time from `local0`.  The groups of threads
 // (four columns a thread) take equal parts, so that an item that everybody names does not fall to one group; an item's first run in a
 // part is set aside and added after the others, in the parts' order.
 template <typename T, int KP>
 __device__ void add_places(const Finish &f, float *rows, float *row_b, const uint32_t *list, float *aside, int *aside_item, int local0, int from, int to)
 {
-    constexpr int COLS = KP / 4;                      // threads of a row
-    constexpr int GROUPS = 256 / COLS, BATCH = 16;
+    constexpr int COLS = group_threads(KP), GROUPS = 256 / COLS, BATCH = 16;
     const uint32_t *order = list + 2 * list_length(KP);
     const float *gs = (const float *)(list + list_length(KP));
     const int tid = threadIdx.x, group = tid / COLS, c4 = (tid % COLS) * 4;
     if (from >= to) return;
     const T *X = (const T *)f.X;
-    if (group < GROUPS) {
+    {
         const int part = (to - from + GROUPS - 1) / GROUPS, begin = from + group * part, end = min(begin + part, to);
+        const bool in = c4 < KP, vec = f.vec_x && c4 < f.k;
         if (c4 == 0) aside_item[group] = -1;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         float ab = 0.f;
         int item = -1, first = -1;
         auto flush = [&]() {
-            if (item < 0) return;
+            if (item < 0 || !in) return;
             if (item == first) {
                 *(float4 *)(aside + group * KP + c4) = a;
                 if (c4 == 0) { aside_item[group] = item; aside[GROUPS * KP + group] = ab; }
@@ -443,25 +446,28 @@ __device__ void add_places(const Finish &f, float *rows, float *row_b, const uin
             }
         };
         for (int q0 = begin; q0 < end; q0 += BATCH) {
+            // all keys, then all users, then all rows: sixteen gathers are under way at once
+            uint32_t key[BATCH], u[BATCH];
             float x[BATCH][4], g[BATCH];
-            int at[BATCH];
 #pragma unroll
-            for (int q = 0; q < BATCH; ++q) {
-                at[q] = -1;
-                if (q0 + q < end) {
-                    const uint32_t key = order[q0 + q];
-                    at[q] = (int)(key >> 12) - local0;
-                    g[q] = gs[key & 4095];
-                    load4(X + (int64_t)list[key & 4095] * f.ldx, c4, f.k, f.vec_x && c4 < f.k, x[q]);
-                }
+            for (int q = 0; q < BATCH; ++q) key[q] = order[min(q0 + q, end - 1)];
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q) { u[q] = list[key[q] & 4095]; g[q] = gs[key[q] & 4095]; }
+            if (vec) {
+#pragma unroll
+                for (int q = 0; q < BATCH; ++q) load4(X + (int64_t)u[q] * f.ldx, c4, f.k, true, x[q]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < BATCH; ++q) load4(X + (int64_t)u[q] * f.ldx, c4, f.k, false, x[q]);
             }
 #pragma unroll
             for (int q = 0; q < BATCH; ++q)
-                if (at[q] >= 0) {
-                    if (at[q] != item) {
+                if (q0 + q < end) {
+                    const int at = (int)(key[q] >> 12) - local0;
+                    if (at != item) {
                         flush();
-                        if (first < 0) first = at[q];
-                        item = at[q];
+                        if (first < 0) first = at;
+                        item = at;
                         a = make_float4(0.f, 0.f, 0.f, 0.f);
                         ab = 0.f;
                     }
@@ -521,7 +527,7 @@ __device__ void store_rows(const Finish &f, const float *rows, const float *row_
 // memory of the sums set aside (one row and one number a group), or a byte for each place of the lists
 constexpr int aside_floats(int KP)
 {
-    const int sums = 256 / (KP / 4) * (KP + 1), bytes = list_length(KP) / 4;
+    const int sums = 256 / group_threads(KP) * (KP + 1), bytes = list_length(KP) / 4;
     return sums > bytes ? sums : bytes;
 }
 
