@@ -377,7 +377,7 @@ int ifr_mxfp4_dequantize(ifr_handle h, const uint8_t *codes, const uint8_t *scal
                          void *stream);
 /* Score rows of a 4-bit model, beside ifr_score_dense: out[u][i] = (ibase[i] + ubase[u]) + <X[u], V[i]>, sums in fp32, rounded
  * once to `out_dtype` (IFR_F32 or IFR_BF16).  out: dev [n][ld], ld >= n_items; ibase [n_items], ubase [n]: dev or NULL.
- * 1 <= k <= IFR_MAX_FACTORS, n <= 2^25, 1 <= n_items <= 2^28. */
+ * 1 <= k <= IFR_MAX_FACTORS, n <= 2^23, 1 <= n_items <= 2^28. */
 int ifr_mxfp4_scores(ifr_handle h, const uint8_t *x_codes, const uint8_t *x_scales, int64_t n, const uint8_t *v_codes,
                      const uint8_t *v_scales, int64_t n_items, int k, const float *ubase, const float *ibase, void *out,
                      int out_dtype, int64_t ld, void *stream);
@@ -388,7 +388,7 @@ typedef struct ifr_catalogue {
     const uint8_t *x_scales, *v_scales;   /* IFR_MXFP4: the scales, else NULL                                               */
     const float *ibase;          /* dev [n_items] or NULL; -inf, or what overflows to it as scale ibase log2(e), takes an item out */
     int64_t n, n_items, ldx, ldv;
-    int k, dtype;                /* 1 <= k <= IFR_MAX_FACTORS; n <= 2^25, 1 <= n_items <= 2^28                               */
+    int k, dtype;                /* 1 <= k <= IFR_MAX_FACTORS; n <= 2^23, 1 <= n_items <= 2^28                               */
     double scale;                /* > 0: an inverse temperature                                                             */
 } ifr_catalogue;
 
@@ -403,7 +403,7 @@ int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *i
 /* Its gradient.  dlogp: dev [n][ld_dlogp]; lse as ifr_catalogue_logprob returned it.  With G[u] = the sum of dlogp[u][j] over the
  * places that hold an item and dz[u][i] = sum_j dlogp[u][j] [ids[u][j] = i] - G[u] exp(z[u][i] - lse[u]):
  *   dX = scale dz V, dV = scale dz^T X (both of `dtype`, rows ld_dx / ld_dv apart), dibase = scale sum_u dz (fp32).
- * Any of the three may be NULL.  fp32 or bf16 operands.  No atomics: the same call gives the same bits.  A user whose lse is
+ * Any of the three may be NULL.  A user who names no item takes no part, whatever stands in its row.  fp32 or bf16 operands.  No atomics: the same call gives the same bits.  A user whose lse is
  * -inf (every item taken out) has no probabilities, and only its targets' part of the gradient. */
 int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int64_t m, int want_dx, int want_dv, int want_dibase,
                                              int64_t *bytes);

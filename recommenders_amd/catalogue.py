@@ -12,7 +12,7 @@ from . import _lib
 
 F32, BF16, MXFP4 = 0, 1, 2
 MAX_FACTORS = 256            # IFR_MAX_FACTORS
-MAX_ROWS, MAX_CATALOGUE = 1 << 25, 1 << 28
+MAX_ROWS, MAX_CATALOGUE = 1 << 23, 1 << 28
 
 _KINDS = {"logistic": 0, "hinge": 1, "squared": 2}
 _REDUCTIONS = {"sum": 0, "row": 1, "batch": 2}

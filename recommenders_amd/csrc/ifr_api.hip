@@ -1781,7 +1781,7 @@ int launched(ifr_handle h, int rc, const char *what)
     return rc ? fail(h, IFR_ERR_HIP, std::string(what) + ": launch failed") : IFR_OK;
 }
 
-constexpr int64_t MAX_ROWS = (int64_t)1 << 25, MAX_CATALOGUE = (int64_t)1 << 28, MAX_PLACES = (int64_t)1 << 20, MAX_LIST = (int64_t)1 << 32;
+constexpr int64_t MAX_ROWS = (int64_t)1 << 23, MAX_CATALOGUE = (int64_t)1 << 28, MAX_PLACES = (int64_t)1 << 20, MAX_LIST = (int64_t)1 << 32;
 
 int check_catalogue(ifr_handle h, const char *what, const ifr_catalogue *c)
 {
@@ -1789,7 +1789,7 @@ int check_catalogue(ifr_handle h, const char *what, const ifr_catalogue *c)
     if (!c) return fail(h, IFR_ERR_ARG, w + ": null catalogue");
     if (c->dtype != IFR_F32 && c->dtype != IFR_BF16 && c->dtype != IFR_MXFP4) return fail(h, IFR_ERR_ARG, w + ": unknown dtype");
     if (c->k < 1 || c->k > IFR_MAX_FACTORS) return fail(h, IFR_ERR_ARG, w + ": k must be in [1, 256]");
-    if (c->n < 0 || c->n > MAX_ROWS) return fail(h, IFR_ERR_ARG, w + ": n must be in [0, 2^25]");
+    if (c->n < 0 || c->n > MAX_ROWS) return fail(h, IFR_ERR_ARG, w + ": n must be in [0, 2^23]");
     if (c->n_items < 1 || c->n_items > MAX_CATALOGUE) return fail(h, IFR_ERR_ARG, w + ": n_items must be in [1, 2^28]");
     if (!(c->scale > 0.0) || c->scale > 1e30) return fail(h, IFR_ERR_ARG, w + ": scale must be positive");
     if (c->dtype != IFR_MXFP4 && (c->ldx < c->k || c->ldv < c->k)) return fail(h, IFR_ERR_ARG, w + ": rows shorter than k");

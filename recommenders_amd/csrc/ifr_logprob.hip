@@ -77,7 +77,8 @@ __device__ __forceinline__ void online(const v16f &d, float c, float &m, float &
 // A matrix in the order the walks read it, by tiles of 32 rows, zeros behind the last row and column:
 //   frag [tile][part][KP / 16][row][2][8]: columns 16 s + 8 h + 0..7 of a row are the 16-byte piece 64 s + 2 row + h
 //   exps [tile]: the tile's exponent (split operands); infinities and NaN do not count for it and stay what they are
-// bf16 matrices whose rows are whole, aligned pieces (k = KP) are read as they lie: frag is null then.
+// A bf16 V whose rows are whole, aligned pieces (k = KP) is read as it lies: v_frag is null then, and x_frag where lse is.  For the gradient
+// X is always put in order: users without an item (a batch's padding) become rows of zeros, so that nothing in them reaches dV.
 struct PrepParams {
     const void *V, *X;
     int64_t ldv, ldx, n_items, n, v_blocks, v_padded, x_padded;
@@ -129,6 +130,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
 {
     extern __shared__ float tile[];                   // [32][KP + 1]
     __shared__ float tops[4], sums[256];
+    __shared__ int holds[32];
     const int W = p.KP + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool of_v = blockIdx.x < p.v_blocks;
     const int64_t at = of_v ? blockIdx.x : blockIdx.x - p.v_blocks, r0 = at * 32;
@@ -140,16 +142,31 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
         item_term(at * 256 + threadIdx.x);
         return;
     }
+    if (!of_v && p.lse) {   // G over the places that hold an item: eight threads a user, their sums added in their order
+        const int r = threadIdx.x >> 3;
+        const int64_t u = r0 + r;
+        float g = 0.f;
+        int held = 0;
+        if (u < p.n)
+            for (int64_t j = threadIdx.x & 7; j < p.m; j += 8)
+                if (p.ids[u * p.ld_ids + j] >= 0) { g += p.dlogp[u * p.ld_dlogp + j]; held = 1; }
+        sums[threadIdx.x] = g;
+        for (int o = 4; o; o >>= 1) held |= __shfl_xor(held, o);
+        if ((threadIdx.x & 7) == 0) holds[r] = held;
+        __syncthreads();
+    }
     if (frag) {
         const T *src = (const T *)(of_v ? p.V : p.X);
         const int64_t rows = of_v ? p.n_items : p.n, ld = of_v ? p.ldv : p.ldx;
         float top = 0.f;
-        for (int r = wave; r < 32; r += 4)
+        for (int r = wave; r < 32; r += 4) {
+            const bool in = r0 + r < rows && (of_v || !p.lse || holds[r]);
             for (int c = lane; c < p.KP; c += 64) {
-                const float v = r0 + r < rows && c < p.k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
+                const float v = in && c < p.k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
                 tile[r * W + c] = v;
                 if (NS == 2 && fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
             }
+        }
         if (NS == 2) {
             for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
             if (lane == 0) tops[wave] = top;
@@ -167,16 +184,6 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
         return;
     }
     if (!p.lse) return;
-    {   // G over the places that hold an item: eight threads a user, their sums added in their order
-        const int r = threadIdx.x >> 3;
-        const int64_t u = r0 + r;
-        float g = 0.f;
-        if (u < p.n)
-            for (int64_t j = threadIdx.x & 7; j < p.m; j += 8)
-                if (p.ids[u * p.ld_ids + j] >= 0) g += p.dlogp[u * p.ld_dlogp + j];
-        sums[threadIdx.x] = g;
-    }
-    __syncthreads();
     if (threadIdx.x < 64) {
         const int64_t u = r0 + (threadIdx.x & 31);
         float g = 0.f;
@@ -188,8 +195,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
             p.G[u] = g;
             if (NS == 2) p.G_scaled[u] = ldexpf(g, e);
             if (NS == 2 && threadIdx.x == 0) p.g_exp[at] = e;
-            // no probabilities where lse is -inf: every exponential is 0
-            p.user_term[u] = u < p.n && p.lse[u] != -INFINITY ? p.lse[u] * p.lse_unit : -INFINITY;
+            // no probabilities where lse is -inf, and none that matter where no item is named: every exponential is 0
+            p.user_term[u] = u < p.n && holds[threadIdx.x] && p.lse[u] != -INFINITY ? p.lse[u] * p.lse_unit : -INFINITY;
         }
     }
     if (p.places) {
@@ -231,7 +238,7 @@ struct Finish {
 };
 
 struct WalkParams {
-    const uint4 *s_frag, *t_frag;      // null: rows of bf16 as they lie
+    const uint4 *s_frag, *t_frag;      // null: bf16 rows as they lie
     const __bf16 *s_rows, *t_rows;
     int64_t s_ld, t_ld, s_n, t_n;
     const float *s_term, *t_term;      // item_term, user_term of prepare_kernel
@@ -535,7 +542,8 @@ constexpr int aside_floats(int KP)
 // of LDS; the statistics take half of that, for two workgroups a compute unit also at KP = 256.
 constexpr int stage_tiles(int NS, bool grad) { return (NS == 1 ? 2 : 1) * (grad ? 2 : 1); }
 
-template <int KP, int NS, int MODE, bool ROWS>
+// S_LIES, T_LIES: read as bf16 rows in memory (V; X too for the statistics)
+template <int KP, int NS, int MODE, bool S_LIES, bool T_LIES>
 __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <= 128) ? 2 : 1) void walk_kernel(WalkParams p)
 {
     typedef typename std::conditional<NS == 2, float, __bf16>::type T;
@@ -568,7 +576,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     for (int q = 0; q < NS; ++q)
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
-            sf[q][s] = ROWS ? ((const uint4 *)(p.s_rows + min(s_row, p.s_n - 1) * p.s_ld))[2 * s + h]
+            sf[q][s] = S_LIES ? ((const uint4 *)(p.s_rows + min(s_row, p.s_n - 1) * p.s_ld))[2 * s + h]
                             : p.s_frag[(s_tile * NS + q) * PART + s * 64 + (lane & 31) * 2 + h];
     const int s_exp = NS == 2 ? p.s_exp[s_tile] : 0;
     const float s_term = p.s_term ? p.s_term[s_row] * (NS == 1 ? p.c : 1.f) : 0.f;
@@ -585,7 +593,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     const int at2 = ((lane >> 4 & 1) * 64 + (4 * h + (lane >> 2 & 3)) * 2 + (lane >> 1 & 1)) * 16 + (lane & 1) * 8;
 
     auto fetch_stage = [&](int t, uint4 *to, float *terms) {
-        if (ROWS) {
+        if (T_LIES) {
 #pragma unroll
             for (int sub = 0; sub < SUB; ++sub) {
                 const int64_t row = min((int64_t)(t + sub) * 32 + (lane >> 1), p.t_n - 1);     // behind the last: a row whose term is -inf
@@ -1119,7 +1127,8 @@ __device__ __forceinline__ void join_dx(const JoinDx &p, int64_t block)
         a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
     const float g0 = -p.G[u];
-    float r[4] = {g0 * a.x, g0 * a.y, g0 * a.z, g0 * a.w};
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
+    if (g0 != 0.f) { r[0] = g0 * a.x; r[1] = g0 * a.y; r[2] = g0 * a.z; r[3] = g0 * a.w; }      // (NaN != 0)
 #pragma unroll 4
     for (int64_t j = 0; j < p.m; ++j) {
         const int32_t id = p.ids[u * p.ld_ids + j];
@@ -1257,9 +1266,10 @@ template <int NS, int MODE>
 void launch_walk(const WalkParams &p, int KP, hipStream_t s)
 {
     const dim3 grid((uint32_t)(p.s_blocks * p.splits));
+    const bool lies = !(MODE == WALK_ITEMS ? p.s_frag : p.t_frag);
 #define IFR_WALK(K)                                                                                                   \
-    if (NS == 1 && !p.s_frag) hipLaunchKernelGGL((walk_kernel<K, NS, MODE, NS == 1>), grid, dim3(256), 0, s, p);      \
-    else hipLaunchKernelGGL((walk_kernel<K, NS, MODE, false>), grid, dim3(256), 0, s, p)
+    if (NS == 1 && lies) hipLaunchKernelGGL((walk_kernel<K, NS, MODE, NS == 1 && MODE != WALK_USERS, NS == 1 && MODE != WALK_ITEMS>), grid, dim3(256), 0, s, p); \
+    else hipLaunchKernelGGL((walk_kernel<K, NS, MODE, false, false>), grid, dim3(256), 0, s, p)
     IFR_FOR_FACTORS(KP, IFR_WALK)
 #undef IFR_WALK
 }
@@ -1332,7 +1342,7 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
     BackwardPlan p = {};
     const int KP = pad_factors(c.k), NS = c.dtype == IFR_F32 ? 2 : 1;
     const bool items = dv || db;
-    p.x = side(w, c, true, lies);
+    p.x = side(w, c, true, false);
     p.v = side(w, c, false, lies);
     p.item_term = w.take<float>(p.v.padded);
     p.user_term = w.take<float>(p.x.padded);

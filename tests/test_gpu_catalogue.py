@@ -331,6 +331,30 @@ def test_logprob_masks_and_awkward_places(torch, sc):
     assert torch.isnan(logp[5, 2]) and torch.isnan(logp).sum() == 1
 
 
+@pytest.mark.parametrize("dtype,k", [("float32", 50), ("float32", 128), ("bfloat16", 64), ("bfloat16", 61)])
+def test_a_padded_batch(torch, sc, dtype, k):
+    """Users without an item, with NaN and infinities in their rows, gradients and lse: the others' results are those of a batch without them."""
+    X, V, b, ids, dlogp = _case(torch, 90, 300, k, 4, dtype, True, 31)
+    ids.clamp_(min=0)
+    real = torch.ones(90, dtype=torch.bool, device="cuda")
+    real[5::7] = False
+    want = sc.catalogue_logprob(X[real], V, ids[real], ibase=b)
+    Xp, ip, dp = X.clone(), ids.clone(), dlogp.clone()
+    Xp[~real], ip[~real], dp[~real] = float("nan"), -1, float("nan")
+    Xp[5] = float("inf")
+    logp, lse = sc.catalogue_logprob(Xp, V, ip, ibase=b)
+    assert (logp[~real] == 0).all() and torch.isnan(lse[~real]).all()
+    score, e_lse, _ = _bounds(_reference(torch, X[real], V, b, ids[real], dlogp[real], 1.0), 300, 90, k, 4, dtype)
+    assert float((logp[real] - want[0]).abs().max()) <= 2 * (score + e_lse) and float((lse[real] - want[1]).abs().max()) <= 2 * e_lse
+    dX, dV, db = sc.catalogue_logprob_backward(Xp, V, ip, lse, dp, ibase=b)
+    r = _reference(torch, X[real], V, b, ids[real], dlogp[real], 1.0)
+    assert (dX[~real] == 0).all()
+    for got, ref in ((dX[real], r["dX"]), (dV, r["dV"]), (db, r["db"])):
+        # the norm of the error: a step of 16 bits for operand, probability and result, or 22 bits and the sums' rounding
+        bound = 3 * B if got.dtype == torch.bfloat16 else 2.0 ** -18
+        assert float((got.double() - ref).norm() / ref.norm()) <= bound
+
+
 def test_logprob_nan_stays_in_its_row(torch, sc):
     X, V, b, ids, dlogp = _case(torch, 70, 200, 64, 3, "float32", False, 12)
     ids.clamp_(min=0)
