@@ -75,7 +75,7 @@ __device__ __forceinline__ void online(const v16f &d, float c, float &m, float &
 // ---------------------------------------------------------------------------- preparation
 
 // A matrix in the order the walks read it, by tiles of 32 rows, zeros behind the last row and column:
-//   frag [tile][part][KP / 16][row][2][8]: columns 16 s + 8 h + 0..7 of a row are the 16-byte piece 64 s + 2 row + h
+//   frag [tile][part][KP / 16][64][8]: columns 16 s + 8 h + 0..7 of a row are the 16-byte piece piece_at(s, row, h)
 //   exps [tile]: the tile's exponent (split operands); infinities and NaN do not count for it and stay what they are
 // A bf16 V whose rows are whole, aligned pieces (k = KP) is read as it lies: v_frag is null then, and x_frag where lse is.  For the gradient
 // X is always put in order: users without an item (a batch's padding) become rows of zeros, so that nothing in them reaches dV.
@@ -99,13 +99,23 @@ struct PrepParams {
     uint8_t *named;                    // [items / 64], cleared before: set where an item is named; or null
 };
 
+// Where a tile keeps the piece of columns 16 s + 8 h + 0..7 of a row: a row's two pieces of a step side by side, so that memory is read in
+// 32 bytes; the rows of odd steps and the order of the two are turned so that 16 rows of one h (first product) and four rows of two
+// steps (second product) fall on all 64 banks of LDS.  Without the turns a third of the LDS cycles were conflicts.
+__host__ __device__ constexpr int piece_at(int s, int row, int h)
+{
+    const int r = row ^ (s & 1) * 4;
+    return s * 64 + r * 2 + (h ^ (r >> 3 & 1));
+}
+
 // LDS tile [32][W] -> pieces
 template <int NS>
 __device__ __forceinline__ void store_fragments(const float *tile, int W, int KP, int e, int64_t at, uint4 *f)
 {
     const int per = KP / 16 * 64;                     // 16-byte pieces of one part of a tile
     for (int i = threadIdx.x; i < per; i += 256) {
-        const float *v = tile + ((i >> 1) & 31) * W + (i >> 6) * 16 + (i & 1) * 8;
+        const int step = i >> 6, r = i >> 1 & 31, row = r ^ (step & 1) * 4, h = (i & 1) ^ (r >> 3 & 1);      // piece_at turned round
+        const float *v = tile + row * W + step * 16 + h * 8;
         if (NS == 1) {
             b8 o;
             for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
@@ -253,12 +263,12 @@ struct WalkParams {
     Finish f;
 };
 
-// rows 0..3 and 8..11 of this lane's column (see at2)
-__device__ __forceinline__ uint4 turned(const char *at)
+// two times four rows of this lane's column (see at2 in walk_kernel)
+__device__ __forceinline__ uint4 turned(const char *low, const char *high)
 {
     typedef short s4 __attribute__((ext_vector_type(4)));
-    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
-    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(at + 256));
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)low);
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)high);
     const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
     return make_uint4(a.x, a.y, b.x, b.y);
 }
@@ -577,7 +587,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
             sf[q][s] = S_LIES ? ((const uint4 *)(p.s_rows + min(s_row, p.s_n - 1) * p.s_ld))[2 * s + h]
-                            : p.s_frag[(s_tile * NS + q) * PART + s * 64 + (lane & 31) * 2 + h];
+                            : p.s_frag[(s_tile * NS + q) * PART + piece_at(s, lane & 31, h)];
     const int s_exp = NS == 2 ? p.s_exp[s_tile] : 0;
     const float s_term = p.s_term ? p.s_term[s_row] * (NS == 1 ? p.c : 1.f) : 0.f;
 
@@ -587,17 +597,20 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     int ref = 280;                                    // exponent of acc (split operands), the least of the tiles so far
 
     const int first = split * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
-    // this lane's piece of the first product's operand, and its 8 bytes of the second's, which ds_read_tr turns round: 16 lanes read
-    // four rows by 16 columns and get four rows of a column each
-    const int at1 = (lane & 31) * 2 + h;
-    const int at2 = ((lane >> 4 & 1) * 64 + (4 * h + (lane >> 2 & 3)) * 2 + (lane >> 1 & 1)) * 16 + (lane & 1) * 8;
+    // this lane's pieces of the first product's operand (even and odd steps), and its 8 bytes of the second's, which ds_read_tr turns
+    // round: 16 lanes read four rows by 16 columns and get four rows of a column each (rows 0..7 and 8..15 of a step of 16)
+    const int at1[2] = {piece_at(0, lane & 31, h), piece_at(1, lane & 31, h) - 64};
+    const int row2 = 4 * h + (lane >> 2 & 3), step2 = lane >> 4 & 1, h2 = lane >> 1 & 1;
+    const int at2 = piece_at(step2, row2, h2) * 16 + (lane & 1) * 8, at2_high = piece_at(step2, row2 + 8, h2) * 16 + (lane & 1) * 8;
 
     auto fetch_stage = [&](int t, uint4 *to, float *terms) {
         if (T_LIES) {
 #pragma unroll
             for (int sub = 0; sub < SUB; ++sub) {
-                const int64_t row = min((int64_t)(t + sub) * 32 + (lane >> 1), p.t_n - 1);     // behind the last: a row whose term is -inf
-                const uint4 *from = (const uint4 *)(p.t_rows + row * p.t_ld) + (lane & 1);
+                // steps s of a wave have the parity of the wave; behind the last row: one whose term is -inf
+                const int r = lane >> 1;
+                const int64_t row = min((int64_t)(t + sub) * 32 + (r ^ (wave & 1) * 4), p.t_n - 1);
+                const uint4 *from = (const uint4 *)(p.t_rows + row * p.t_ld) + ((lane & 1) ^ (r >> 3 & 1));
 #pragma unroll
                 for (int s = 0; s < (STEPS + 3) / 4; ++s)
                     if (STEPS % 4 == 0 || s * 4 + wave < STEPS)
@@ -628,11 +641,11 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
             }
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
-                const uint4 a = l1[s * 64 + at1];
+                const uint4 a = l1[s * 64 + at1[s & 1]];
                 d = product<NS>(a, sf[0][s], d);
                 if (NS == 2) {
                     d = product<NS>(a, sf[NS - 1][s], d);
-                    d = product<NS>(l1[PART + s * 64 + at1], sf[0][s], d);
+                    d = product<NS>(l1[PART + s * 64 + at1[s & 1]], sf[0][s], d);
                 }
             }
             reads_ahead<STEPS * NS, STEPS * (2 * NS - 1)>();
@@ -713,12 +726,12 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                 for (int kb = 0; kb < KP / 32; ++kb)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const char *l2 = (const char *)l1 + at2 + kb * 2048 + e * 512;
-                        const uint4 a = turned(l2);
+                        const char *l2 = (const char *)l1 + kb * 2048 + e * 512;
+                        const uint4 a = turned(l2 + at2, l2 + at2_high);
                         acc[kb] = product<NS>(a, pf[0][e], acc[kb]);
                         if (NS == 2) {
                             acc[kb] = product<NS>(a, pf[NS - 1][e], acc[kb]);
-                            acc[kb] = product<NS>(turned(l2 + PART * 16), pf[0][e], acc[kb]);
+                            acc[kb] = product<NS>(turned(l2 + PART * 16 + at2, l2 + PART * 16 + at2_high), pf[0][e], acc[kb]);
                         }
                     }
             }
