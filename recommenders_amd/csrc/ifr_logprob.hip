@@ -231,7 +231,8 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, int64_t n)
 
 // ---------------------------------------------------------------------------- the walk
 
-enum { WALK_STATS = 0, WALK_USERS = 1, WALK_ITEMS = 2 };     // lse; the sums of dX (S users, T items); those of dV and db (S items, T users)
+// lse; the sums of dX (S users, T items); those of dV (S items, T users), and of dV and db
+enum { WALK_STATS = 0, WALK_USERS = 1, WALK_ITEMS = 2, WALK_ITEMS_BASE = 3 };
 
 // What the gradient of V needs to finish its rows in the kernel that summed them (one split): see find_places.
 struct Finish {
@@ -252,14 +253,14 @@ struct WalkParams {
     const __bf16 *s_rows, *t_rows;
     int64_t s_ld, t_ld, s_n, t_n;
     const float *s_term, *t_term;      // item_term, user_term of prepare_kernel
-    const float *t_factor;             // WALK_ITEMS: G (split: scaled by t_factor_exp)
+    const float *t_factor;             // WALK_ITEMS...: G (split: scaled by t_factor_exp)
     const int *s_exp, *t_exp, *t_factor_exp;     // split operands: exponents of their tiles
     float c;                           // scale log2(e)
     int s_blocks, splits, t_tiles, tiles_per_split;
     int64_t s_padded;
     float *out_m, *out_s;              // WALK_STATS: [splits][s_padded]
     float *out_acc;                    // else: [splits][s_padded][KP], or null: finish
-    float *out_b;                      // WALK_ITEMS: [splits][s_padded]: sums of factor P, or null
+    float *out_b;                      // WALK_ITEMS_BASE: [splits][s_padded]: sums of factor P, or null
     Finish f;
 };
 
@@ -591,7 +592,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     const int s_exp = NS == 2 ? p.s_exp[s_tile] : 0;
     const float s_term = p.s_term ? p.s_term[s_row] * (NS == 1 ? p.c : 1.f) : 0.f;
 
-    const bool want_b = MODE == WALK_ITEMS && (p.out_b || p.f.db);
+    constexpr bool ITEMS = MODE == WALK_ITEMS || MODE == WALK_ITEMS_BASE;
     v16f acc[GRAD ? KP / 32 : 1] = {};
     float m = -3.402823466e38f, sum = 0.f, b_sum = 0.f;
     int ref = 280;                                    // exponent of acc (split operands), the least of the tiles so far
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
             fetch<STAGE>(p.t_frag + (int64_t)t * PART * NS, to);
         }
         if (wave < (SUB + 1) / 2) fetch_row(p.t_term + (int64_t)t * 32 + wave * 64, terms + wave * 64);
-        else if (MODE == WALK_ITEMS && wave < SUB) fetch_row(p.t_factor + (int64_t)t * 32 + (wave - SUB / 2) * 64, terms + wave * 64);
+        else if (ITEMS && wave < SUB) fetch_row(p.t_factor + (int64_t)t * 32 + (wave - SUB / 2) * 64, terms + wave * 64);
     };
     auto compute = [&](int t0, const uint4 *lds, const float *terms) {
 #pragma unroll 2
@@ -666,7 +667,7 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                 // here, one with a smaller becomes the reference
                 int up = 0, ge = 0;
                 if (NS == 2) {
-                    ge = MODE == WALK_ITEMS ? p.t_factor_exp[t] : 0;
+                    ge = ITEMS ? p.t_factor_exp[t] : 0;
                     const int e = p.t_exp[t] + ge;
                     if (e < ref) {
                         const float f = ldexpf(1.f, e - ref);
@@ -679,23 +680,26 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
                 float P[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) P[r] = exp2_raw(fmaf(d[r], c, add));
-                if (MODE == WALK_ITEMS) {
+                if (ITEMS) {
                     float4 tg[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) tg[q] = *(const float4 *)(terms + SUB * 32 + sub * 32 + 8 * q + 4 * h);
                     float b = 0.f;
-                    if (NS == 2 && up < -20) {        // a tile far below the reference: its sum for db from the probabilities as they are
+                    if (MODE == WALK_ITEMS_BASE && NS == 2 && up < -20) {        // a tile far below the reference: its sum for db from the probabilities as they are
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             b = fmaf(exp2_raw(d[4 * q] + s_term), tg[q].x, b); b = fmaf(exp2_raw(d[4 * q + 1] + s_term), tg[q].y, b);
                             b = fmaf(exp2_raw(d[4 * q + 2] + s_term), tg[q].z, b); b = fmaf(exp2_raw(d[4 * q + 3] + s_term), tg[q].w, b);
                         }
                     }
+                    {   // products rounded by themselves: dV has the same bits with and without db beside it
+#pragma clang fp contract(off)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        P[4 * q] *= tg[q].x; P[4 * q + 1] *= tg[q].y; P[4 * q + 2] *= tg[q].z; P[4 * q + 3] *= tg[q].w;
+                        for (int q = 0; q < 4; ++q) {
+                            P[4 * q] *= tg[q].x; P[4 * q + 1] *= tg[q].y; P[4 * q + 2] *= tg[q].z; P[4 * q + 3] *= tg[q].w;
+                        }
                     }
-                    if (want_b) {
+                    if (MODE == WALK_ITEMS_BASE) {
                         if (NS == 1 || up >= -20) {
 #pragma unroll
                             for (int r = 0; r < 16; ++r) b += P[r];
@@ -1279,9 +1283,9 @@ template <int NS, int MODE>
 void launch_walk(const WalkParams &p, int KP, hipStream_t s)
 {
     const dim3 grid((uint32_t)(p.s_blocks * p.splits));
-    const bool lies = !(MODE == WALK_ITEMS ? p.s_frag : p.t_frag);
+    const bool lies = !(MODE >= WALK_ITEMS ? p.s_frag : p.t_frag);
 #define IFR_WALK(K)                                                                                                   \
-    if (NS == 1 && lies) hipLaunchKernelGGL((walk_kernel<K, NS, MODE, NS == 1 && MODE != WALK_USERS, NS == 1 && MODE != WALK_ITEMS>), grid, dim3(256), 0, s, p); \
+    if (NS == 1 && lies) hipLaunchKernelGGL((walk_kernel<K, NS, MODE, NS == 1 && MODE != WALK_USERS, NS == 1 && MODE < WALK_ITEMS>), grid, dim3(256), 0, s, p); \
     else hipLaunchKernelGGL((walk_kernel<K, NS, MODE, false, false>), grid, dim3(256), 0, s, p)
     IFR_FOR_FACTORS(KP, IFR_WALK)
 #undef IFR_WALK
@@ -1528,7 +1532,8 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
         w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
         w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx), fours(g.dV, g.ld_dv)};
-        launch_walk<NS, WALK_ITEMS>(w, KP, s);
+        if (g.dibase) launch_walk<NS, WALK_ITEMS_BASE>(w, KP, s);
+        else launch_walk<NS, WALK_ITEMS>(w, KP, s);
     }
     // the joins as one launch where dX's is short (its workgroups hold the memory of the other's)
     const bool together = parts && x.blocks <= 512;
