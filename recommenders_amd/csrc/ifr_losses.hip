@@ -180,8 +180,20 @@ __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP) void preference_kernel(i
 
 namespace {
 
-// threads of a row
-int group_of(int64_t len) { return len <= 64 ? 16 : len <= 2048 ? 64 : len <= 8192 ? 256 : 1024; }
+// Threads of a row, by what a launch takes in units of one trip to memory: rounds of the 8192 waves that the chip holds, times the trips
+// that a row makes (four elements a thread each), six for what a row costs besides, three more where a workgroup has to meet.
+// (16 384 pairs of 500 + 1000: 64 threads 82 us, 256 threads 107 us; 31 455 pairs of 35 + 122: 64 threads 61 us, 16 threads 33 us.)
+int group_of(int64_t len, int64_t n)
+{
+    int best = 16;
+    double least = 0;
+    for (int g = 16; g <= 1024; g *= 4) {
+        const double waves = (double)n * g / 64, rounds = waves <= 8192 ? 1 : waves / 8192;
+        const double cost = rounds * ((double)((len + 4 * g - 1) / (4 * g)) + 6 + (g > 64 ? 3 : 0));
+        if (g == 16 || cost < least) { best = g; least = cost; }
+    }
+    return best;
+}
 
 dim3 grid_of(int64_t n, int group)
 {
@@ -193,7 +205,7 @@ dim3 grid_of(int64_t n, int group)
 
 int launch_preference(const ifr_preference &p, hipStream_t s)
 {
-    const int group = group_of(p.len_chosen > p.len_rejected ? p.len_chosen : p.len_rejected);
+    const int group = group_of(p.len_chosen > p.len_rejected ? p.len_chosen : p.len_rejected, p.n);
     const dim3 grid = grid_of(p.n, group);
     if (group == 16) hipLaunchKernelGGL(preference_kernel<16>, grid, dim3(256), 0, s, p);
     else if (group == 64) hipLaunchKernelGGL(preference_kernel<64>, grid, dim3(256), 0, s, p);
@@ -353,7 +365,7 @@ int launch_policy(const ifr_policy &p, void *ws, hipStream_t s)
     }
     // the clip borders as logarithms, rounded once: log p - log p_old is compared with them
     const float hi = (float)log1p(p.clip_high), lo = (float)log1p(-p.clip_low);
-    const int group = group_of(p.len);
+    const int group = group_of(p.len, p.n);
     const dim3 grid = grid_of(p.n, group);
     if (group == 16) hipLaunchKernelGGL(policy_kernel<16>, grid, dim3(256), 0, s, p, part, n_part, hi, lo);
     else if (group == 64) hipLaunchKernelGGL(policy_kernel<64>, grid, dim3(256), 0, s, p, part, n_part, hi, lo);
