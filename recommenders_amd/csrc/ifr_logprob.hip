@@ -169,12 +169,17 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
         const T *src = (const T *)(of_v ? p.V : p.X);
         const int64_t rows = of_v ? p.n_items : p.n, ld = of_v ? p.ldv : p.ldx;
         float top = 0.f;
-        for (int r = wave; r < 32; r += 4) {
-            const bool in = r0 + r < rows && (of_v || !p.lse || holds[r]);
-            for (int c = lane; c < p.KP; c += 64) {
-                const float v = in && c < p.k ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
-                tile[r * W + c] = v;
-                if (NS == 2 && fabsf(v) < INFINITY) top = fmaxf(top, fabsf(v));
+        for (int c = lane; c < p.KP; c += 64) {
+            float v[8];                               // eight loads under way at once
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int r = wave + 4 * q;
+                v[q] = r0 + r < rows && c < p.k && (of_v || !p.lse || holds[r]) ? as_f32(src[(r0 + r) * ld + c]) : 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                tile[(wave + 4 * q) * W + c] = v[q];
+                if (NS == 2 && fabsf(v[q]) < INFINITY) top = fmaxf(top, fabsf(v[q]));
             }
         }
         if (NS == 2) {
@@ -341,7 +346,7 @@ __device__ __forceinline__ void load4(const T *row, int c, int k, bool vec, floa
 // find_places: each wave looks through a quarter of the places and lists those that name one of `count` (at most 128) items, until its
 // list is full or the quarter is done (`step` keeps where it is); the lists are sorted by item.  Returns how many, `more`: come again.
 template <int KP>
-__device__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t *item_of, int64_t i0, int count, int64_t &step, bool &more)
+__device__ __forceinline__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t *item_of, int64_t i0, int count, int64_t &step, bool &more)
 {
     constexpr int LIST = list_length(KP), CAP = LIST / 4, EACH = CAP / 64;
     uint32_t *order = list + 2 * LIST;
@@ -433,68 +438,51 @@ constexpr int group_threads(int KP) { return KP > 128 ? 64 : KP > 64 ? 32 : KP >
 
 // The found places [from, to) in their sorted order, of items whose local number is 64 at a time from `local0`.  The groups of threads
 // (four columns a thread) take equal parts, so that an item that everybody names does not fall to one group; an item's first run in a
-// part is set aside and added after the others, in the parts' order.
+// part goes to a row set aside, which is added after the others, in the parts' order.  Short code on purpose: it runs once a
+// workgroup, and what it costs is the fetching of its instructions as much as that of the rows.
 template <typename T, int KP>
-__device__ void add_places(const Finish &f, float *rows, float *row_b, const uint32_t *list, float *aside, int *aside_item, int local0, int from, int to)
+__device__ __forceinline__ void add_places(const Finish &f, float *rows, float *row_b, const uint32_t *list, float *aside, int *aside_item, int local0, int from,
+                                           int to)
 {
     constexpr int COLS = group_threads(KP), GROUPS = 256 / COLS, BATCH = 16;
     const uint32_t *order = list + 2 * list_length(KP);
     const float *gs = (const float *)(list + list_length(KP));
     const int tid = threadIdx.x, group = tid / COLS, c4 = (tid % COLS) * 4;
-    if (from >= to) return;
     const T *X = (const T *)f.X;
-    {
-        const int part = (to - from + GROUPS - 1) / GROUPS, begin = from + group * part, end = min(begin + part, to);
-        const bool in = c4 < KP, vec = f.vec_x && c4 < f.k;
-        if (c4 == 0) aside_item[group] = -1;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        float ab = 0.f;
-        int item = -1, first = -1;
-        auto flush = [&]() {
-            if (item < 0 || !in) return;
-            if (item == first) {
-                *(float4 *)(aside + group * KP + c4) = a;
-                if (c4 == 0) { aside_item[group] = item; aside[GROUPS * KP + group] = ab; }
-            } else {
-                float4 *r = (float4 *)(rows + item * KP + c4);
-                float4 v = *r;
-                v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-                *r = v;
-                if (c4 == 0) row_b[item] += ab;
-            }
-        };
-        for (int q0 = begin; q0 < end; q0 += BATCH) {
-            // all keys, then all users, then all rows: sixteen gathers are under way at once
-            uint32_t key[BATCH], u[BATCH];
-            float x[BATCH][4], g[BATCH];
+    const int part = (to - from + GROUPS - 1) / GROUPS, begin = from + group * part, end = min(begin + part, to);
+    const bool in = c4 < KP, vec = f.vec_x && c4 < f.k;
+    const int first = begin < end ? (int)(order[begin] >> 12) - local0 : -1;
+    if (c4 == 0) { aside_item[group] = first; aside[GROUPS * KP + group] = 0.f; }
+    if (in) *(float4 *)(aside + group * KP + c4) = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q0 = begin; q0 < end; q0 += BATCH) {
+        // all keys, then all users, then all rows: sixteen gathers are under way at once
+        uint32_t key[BATCH], u[BATCH];
+        float x[BATCH][4], g[BATCH];
 #pragma unroll
-            for (int q = 0; q < BATCH; ++q) key[q] = order[min(q0 + q, end - 1)];
+        for (int q = 0; q < BATCH; ++q) key[q] = order[min(q0 + q, end - 1)];
 #pragma unroll
-            for (int q = 0; q < BATCH; ++q) { u[q] = list[key[q] & 4095]; g[q] = gs[key[q] & 4095]; }
-            if (vec) {
+        for (int q = 0; q < BATCH; ++q) { u[q] = list[key[q] & 4095]; g[q] = gs[key[q] & 4095]; }
+        if (vec) {
 #pragma unroll
-                for (int q = 0; q < BATCH; ++q) load4(X + (int64_t)u[q] * f.ldx, c4, f.k, true, x[q]);
-            } else {
+            for (int q = 0; q < BATCH; ++q) load4(X + (int64_t)u[q] * f.ldx, c4, f.k, true, x[q]);
+        } else {
 #pragma unroll
-                for (int q = 0; q < BATCH; ++q) load4(X + (int64_t)u[q] * f.ldx, c4, f.k, false, x[q]);
-            }
-#pragma unroll
-            for (int q = 0; q < BATCH; ++q)
-                if (q0 + q < end) {
-                    const int at = (int)(key[q] >> 12) - local0;
-                    if (at != item) {
-                        flush();
-                        if (first < 0) first = at;
-                        item = at;
-                        a = make_float4(0.f, 0.f, 0.f, 0.f);
-                        ab = 0.f;
-                    }
-                    a.x = fmaf(g[q], x[q][0], a.x); a.y = fmaf(g[q], x[q][1], a.y);
-                    a.z = fmaf(g[q], x[q][2], a.z); a.w = fmaf(g[q], x[q][3], a.w);
-                    ab += g[q];
-                }
+            for (int q = 0; q < BATCH; ++q) load4(X + (int64_t)u[q] * f.ldx, c4, f.k, false, x[q]);
         }
-        flush();
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q)
+            if (in && q0 + q < end) {
+                const int at = (int)(key[q] >> 12) - local0;
+                float4 *r = (float4 *)((at == first ? aside + group * KP : rows + at * KP) + c4);
+                float4 v = *r;
+                v.x = fmaf(g[q], x[q][0], v.x); v.y = fmaf(g[q], x[q][1], v.y);
+                v.z = fmaf(g[q], x[q][2], v.z); v.w = fmaf(g[q], x[q][3], v.w);
+                *r = v;
+                if (c4 == 0) {
+                    float *b = at == first ? aside + GROUPS * KP + group : row_b + at;
+                    *b += g[q];
+                }
+            }
     }
     __syncthreads();
     for (int g = 0; g < GROUPS; ++g) {
@@ -506,20 +494,8 @@ __device__ void add_places(const Finish &f, float *rows, float *row_b, const uin
     __syncthreads();
 }
 
-// ... where the lists may not hold all of them: in as many rounds as it takes
 template <typename T, int KP>
-__device__ void add_all_places(const Finish &f, float *rows, float *row_b, uint32_t *list, int *counts, float *aside, int *aside_item, int64_t i0)
-{
-    int64_t step = -1;
-    bool more = true;
-    while (more) {
-        const int total = find_places<KP>(f, list, counts, (uint8_t *)aside, i0, 64, step, more);
-        add_places<T, KP>(f, rows, row_b, list, aside, aside_item, 0, 0, total);
-    }
-}
-
-template <typename T, int KP>
-__device__ void store_rows(const Finish &f, const float *rows, const float *row_b, int64_t i0)
+__device__ __forceinline__ void store_rows(const Finish &f, const float *rows, const float *row_b, int64_t i0)
 {
     if (f.dV) {
         T *out = (T *)f.dV;
@@ -785,33 +761,53 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     const int64_t i0 = (int64_t)s_block * S_ROWS;
     const Finish &f = p.f;
     __syncthreads();
-    bool more = f.n_places > 0 && (!f.named || f.named[i0 >> 6] || f.named[(i0 >> 6) + 1]);
-    const bool any = more;
+    const bool any = f.n_places > 0 && (!f.named || f.named[i0 >> 6] || f.named[(i0 >> 6) + 1]);
+    // the places of all 128 items are found at once; where the lists do not hold them, those of 64 at a time in as many rounds as it takes
+    bool find = any, at_once = true, more = false, fresh = true;
+    int64_t step = -1;
     int total = 0, lower = 0;                         // of the sorted order: where the second half's items begin
-    if (any) {
-        int64_t step = -1;
-        total = find_places<KP>(f, list, counts, (uint8_t *)aside, i0, 128, step, more);
-        int hi = total;
-        while (lower < hi) {
-            const int mid = (lower + hi) / 2;
-            if (list[2 * list_length(KP) + mid] >> 12 < 64) lower = mid + 1;
-            else hi = mid;
+#pragma unroll 1
+    for (int half = 0; half < 2;) {
+        if (fresh) {
+            __syncthreads();
+            if ((wave >> 1) == half) {
+                const int r = (wave & 1) * 32 + (lane & 31);
+                for (int kb = 0; kb < KP / 32; ++kb)
+                    for (int q = 0; q < 4; ++q)
+                        *(float4 *)(rows + r * KP + kb * 32 + 8 * q + 4 * h) =
+                            make_float4(-acc[kb][4 * q] * unit, -acc[kb][4 * q + 1] * unit, -acc[kb][4 * q + 2] * unit, -acc[kb][4 * q + 3] * unit);
+                if (h == 0) row_b[r] = -b_sum;
+            }
+            __syncthreads();
+            fresh = false;
         }
-    }
-    for (int half = 0; half < 2; ++half) {
-        __syncthreads();
-        if ((wave >> 1) == half) {
-            const int r = (wave & 1) * 32 + (lane & 31);
-            for (int kb = 0; kb < KP / 32; ++kb)
-                for (int q = 0; q < 4; ++q)
-                    *(float4 *)(rows + r * KP + kb * 32 + 8 * q + 4 * h) =
-                        make_float4(-acc[kb][4 * q] * unit, -acc[kb][4 * q + 1] * unit, -acc[kb][4 * q + 2] * unit, -acc[kb][4 * q + 3] * unit);
-            if (h == 0) row_b[r] = -b_sum;
+        if (find) {
+            total = find_places<KP>(f, list, counts, (uint8_t *)aside, at_once ? i0 : i0 + half * 64, at_once ? 128 : 64, step, more);
+            if (at_once && more) {
+                at_once = false;
+                step = -1;
+                __syncthreads();
+                continue;
+            }
+            find = false;
+            lower = 0;
+            for (int hi = total; at_once && lower < hi;) {
+                const int mid = (lower + hi) / 2;
+                if (list[2 * list_length(KP) + mid] >> 12 < 64) lower = mid + 1;
+                else hi = mid;
+            }
         }
-        __syncthreads();
-        if (any && more) add_all_places<T, KP>(f, rows, row_b, list, counts, aside, aside_item, i0 + half * 64);
-        else if (any) add_places<T, KP>(f, rows, row_b, list, aside, aside_item, half * 64, half ? lower : 0, half ? total : lower);
+        const int from = at_once && half ? lower : 0, to = at_once && !half ? lower : total;
+        if (from < to) add_places<T, KP>(f, rows, row_b, list, aside, aside_item, at_once ? half * 64 : 0, from, to);
+        if (!at_once && more) {
+            find = true;
+            continue;
+        }
         store_rows<T, KP>(f, rows, row_b, i0 + half * 64);
+        ++half;
+        fresh = true;
+        find = any && !at_once;
+        step = -1;
     }
 }
 
@@ -1192,7 +1188,11 @@ __global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, c
         row_b[threadIdx.x] = b;
     }
     __syncthreads();
-    if (f.n_places > 0 && (!f.named || f.named[i0 >> 6])) add_all_places<T, KP>(f, rows, row_b, list, counts, aside, aside_item, i0);
+    int64_t step = -1;
+    for (bool more = f.n_places > 0 && (!f.named || f.named[i0 >> 6]); more;) {
+        const int total = find_places<KP>(f, list, counts, (uint8_t *)aside, i0, 64, step, more);
+        if (total) add_places<T, KP>(f, rows, row_b, list, aside, aside_item, 0, 0, total);
+    }
     store_rows<T, KP>(f, rows, row_b, i0);
 }
 
