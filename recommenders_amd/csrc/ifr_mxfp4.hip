@@ -103,6 +103,14 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *codes
 
 // ---------------------------------------------------------------------------- product
 
+// what the lanes of a wave wrote to its strip may be read by the others (LDS serves a wave in order: only the compiler has to keep it)
+__device__ __forceinline__ void strip_ready()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Score rows by v_mfma_scale_f32_32x32x64 with both operands in E2M1.  A lane of that instruction holds one block of 32 of one row and
 // that block's scale, which is the layout in memory, so nothing is rearranged.  A wave keeps IT tiles of 32 items in registers (A
 // operand) and walks query tiles of 32 (B operand): D[item][query], four neighbouring items of one query a lane and quad, which go
@@ -144,7 +152,7 @@ __global__ __launch_bounds__(256, 2) void mx_scores_kernel(MxScoreParams p, int 
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) block_of(p.x, q, s, &x[s], &sx[s]);
         const float ub = p.ubase ? p.ubase[q] : 0.f;
-        __builtin_amdgcn_wave_barrier();
+        strip_ready();
 #pragma unroll
         for (int t = 0; t < IT; ++t) {
             v16f d = {0};
@@ -158,7 +166,7 @@ __global__ __launch_bounds__(256, 2) void mx_scores_kernel(MxScoreParams p, int 
                 to[0] = (OUT)v0; to[1] = (OUT)v1; to[2] = (OUT)v2; to[3] = (OUT)v3;
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        strip_ready();
         OUT *out = (OUT *)p.out + qt * 32 * p.ld + i0;
         const int rows = (int)min((int64_t)32, p.x.n - qt * 32);
         if (vec && cols == COLS) {
