@@ -25,6 +25,12 @@ class CatalogueLearningMixin:
             ops = self._hip_ops_engine = HipScorer(self.hip_device)
         return ops
 
+    def hip_invalidate(self):
+        super().hip_invalidate()
+        ops, self._hip_ops_engine = getattr(self, "_hip_ops_engine", None), None
+        if ops is not None:
+            ops.close()
+
     def _hip_parameters(self):
         """(U, V, item biases or None) as new fp32 tensors on the model's GPU."""
         import torch

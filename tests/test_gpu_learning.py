@@ -323,3 +323,13 @@ def test_c_refusals(torch, sc):
 
 def test_models_without_factors_do_not_learn(torch):
     assert not hasattr(EASE(trainable=False, B=np.zeros((3, 3))), "fit_preferences")
+
+
+def test_a_model_that_learned_can_be_copied(torch):
+    """hip_invalidate drops everything on the device, the learning engine too."""
+    import copy
+    m = _model("bpr")[0]
+    m.fit_preferences([0, 1], [3, 4], [5, 6])
+    before = m.log_prob([0], [[3]])
+    m.hip_invalidate()
+    assert np.array_equal(copy.deepcopy(m).log_prob([0], [[3]]), before)
