@@ -360,7 +360,8 @@ int ifr_pad_scores_min(ifr_handle h, float *scores, int64_t n, int64_t ld, void 
  * supplies the GPU and the error text.  They are asynchronous on `stream`, allocate nothing and keep nothing: what they
  * need beside the operands is a workspace of the caller, whose size a ..._workspace call gives (calls that overlap need one
  * each; its contents mean nothing between calls).  All of them may be captured into a HIP graph.  The device that is
- * current in the calling thread is the same after the call.  n = 0 is a call that does nothing. */
+ * current in the calling thread is the same after the call.  n = 0 is a call that does nothing.  An output does not overlap
+ * an operand or another output. */
 
 enum { IFR_F32 = 0, IFR_BF16 = 1, IFR_MXFP4 = 2 };
 
@@ -369,7 +370,7 @@ enum { IFR_F32 = 0, IFR_BF16 = 1, IFR_MXFP4 = 2 };
  * 127 + the exponent of the block's power of two.  The exponent is floor(log2 max|v|) - 2, at least -127; elements are
  * v / 2^exponent rounded to the nearest value, ties to the even code, at most 6 in magnitude.  A block that holds a NaN or an
  * infinity gets scale 255 and stands for NaN.  Columns behind k are zeros.
- * X: dev [n][ld] of `dtype` (IFR_F32 or IFR_BF16), 1 <= k <= ld. */
+ * X: dev [n][ld] of `dtype` (IFR_F32 or IFR_BF16), 1 <= k <= min(ld, 2^20), n <= 2^28. */
 int ifr_mxfp4_quantize(ifr_handle h, const void *X, int dtype, int64_t n, int64_t k, int64_t ld, uint8_t *codes, uint8_t *scales,
                        void *stream);
 /* The values that codes and scales stand for, exactly: out dev [n][ld] fp32, ld >= k. */
@@ -386,15 +387,16 @@ int ifr_mxfp4_scores(ifr_handle h, const uint8_t *x_codes, const uint8_t *x_scal
 typedef struct ifr_catalogue {
     const void *X, *V;           /* dev [n][ldx], [n_items][ldv] of `dtype`; IFR_MXFP4: the codes (ldx, ldv unused)         */
     const uint8_t *x_scales, *v_scales;   /* IFR_MXFP4: the scales, else NULL                                               */
-    const float *ibase;          /* dev [n_items] or NULL; -inf, or what overflows to it as scale ibase log2(e), takes an item out */
+    const float *ibase;          /* dev [n_items] or NULL; -inf, or what overflows to it as scale ibase log2(e), takes an item out
+                                    (its row of V has to be finite all the same: it is multiplied by a probability of zero)   */
     int64_t n, n_items, ldx, ldv;
     int k, dtype;                /* 1 <= k <= IFR_MAX_FACTORS; n <= 2^23, 1 <= n_items <= 2^28                               */
-    double scale;                /* > 0: an inverse temperature                                                             */
+    double scale;                /* 1e-30 ... 1e30: an inverse temperature                                                  */
 } ifr_catalogue;
 
 /* Log-probabilities of items under the softmax over the whole catalogue; the n x n_items scores are never stored.
- * ids: dev [n][ld_ids], m items a user (0 <= m <= 2^20, n m <= 2^32) (a slate; an item may stand in it twice).  A negative id is an empty place: its
- * logp is 0 and nothing flows through it.  An id >= n_items gives NaN.
+ * ids: dev [n][ld_ids], m items a user (0 <= m <= 2^20, n m <= 2^32; a slate, in which an item may stand twice).  A negative id is
+ * an empty place: its logp is 0 and nothing flows through it.  An id >= n_items gives NaN (and counts for G alone below).
  *   lse[u] = log sum_i exp z[u][i] (dev [n] or NULL), logp[u][j] = z[u][ids[u][j]] - lse[u] (dev [n][ld_logp], or NULL where m = 0).
  * Products of fp32 operands keep 22 bits of each operand (more than the sum of k products in fp32 does); sums are fp32. */
 int ifr_catalogue_logprob_workspace(ifr_handle h, const ifr_catalogue *c, int64_t *bytes);
@@ -403,8 +405,9 @@ int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *i
 /* Its gradient.  dlogp: dev [n][ld_dlogp]; lse as ifr_catalogue_logprob returned it.  With G[u] = the sum of dlogp[u][j] over the
  * places that hold an item and dz[u][i] = sum_j dlogp[u][j] [ids[u][j] = i] - G[u] exp(z[u][i] - lse[u]):
  *   dX = scale dz V, dV = scale dz^T X (both of `dtype`, rows ld_dx / ld_dv apart), dibase = scale sum_u dz (fp32).
- * Any of the three may be NULL.  A user who names no item takes no part, whatever stands in its row.  fp32 or bf16 operands.  No atomics: the same call gives the same bits.  A user whose lse is
- * -inf (every item taken out) has no probabilities, and only its targets' part of the gradient. */
+ * Any of the three may be NULL.  fp32 or bf16 operands.  No atomics: the same call gives the same bits.  A user who names no item
+ * takes no part, whatever stands in its row.  A user whose lse is -inf (every item taken out) has no probabilities, and only its
+ * targets' part of the gradient. */
 int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int64_t m, int want_dx, int want_dv, int want_dibase,
                                              int64_t *bytes);
 int ifr_catalogue_logprob_backward(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids,
@@ -423,7 +426,7 @@ enum { IFR_PREFERENCE_LOGISTIC = 0, IFR_PREFERENCE_HINGE = 1, IFR_PREFERENCE_SQU
  * reference and with beta = 1, are BPR's criterion (cornac/models/bpr/recom_bpr.pyx:208-269). */
 typedef struct ifr_preference {
     int64_t n;
-    int32_t len_chosen, len_rejected;            /* places a row, >= 0                                                 */
+    int32_t len_chosen, len_rejected;            /* places a row, 0 ... 2^30                                           */
     int32_t kind, average;
     const float *chosen, *rejected;              /* dev [n][ld]                                                        */
     const float *ref_chosen, *ref_rejected;      /* dev [n][ld], both or none                                          */
@@ -431,7 +434,7 @@ typedef struct ifr_preference {
     const float *weight;                         /* dev [n]: dL/dloss, or NULL: 1                                      */
     float *loss, *h, *d_chosen, *d_rejected;     /* dev [n], [n], [n][ld], [n][ld]; any may be NULL                    */
     int64_t ld_chosen, ld_rejected, ld_ref_chosen, ld_ref_rejected, ld_mask_chosen, ld_mask_rejected, ld_d_chosen, ld_d_rejected;
-    double beta, margin, label_smoothing;        /* beta > 0, 0 <= label_smoothing < 1/2 (logistic only)               */
+    double beta, margin, label_smoothing;        /* beta in [1e-30, 1e30], 0 <= label_smoothing < 1/2 (logistic only)  */
 } ifr_preference;
 int ifr_preference_loss(ifr_handle h, const ifr_preference *p, void *stream);
 
@@ -447,7 +450,7 @@ enum { IFR_POLICY_SUM = 0, IFR_POLICY_ROW = 1, IFR_POLICY_BATCH = 2 };
  * kl[row] = the mean of kl over the row's places; clipped[row] = the number of clipped places.  Rows without a place give 0. */
 typedef struct ifr_policy {
     int64_t n;
-    int32_t len, reduction;
+    int32_t len, reduction;                      /* len: 0 ... 2^30                                                    */
     const float *logp, *old_logp, *ref_logp;     /* dev [n][ld]; ref_logp may be NULL                                  */
     const float *advantages, *weight;            /* dev [n]; weight may be NULL                                        */
     const uint8_t *mask;                         /* dev [n][ld] 0 / 1, or NULL                                         */

@@ -12,7 +12,7 @@ from . import _lib
 
 F32, BF16, MXFP4 = 0, 1, 2
 MAX_FACTORS = 256            # IFR_MAX_FACTORS
-MAX_ROWS, MAX_CATALOGUE = 1 << 23, 1 << 28
+MAX_ROWS, MAX_CATALOGUE, MAX_LENGTH = 1 << 23, 1 << 28, 1 << 30
 
 _KINDS = {"logistic": 0, "hinge": 1, "squared": 2}
 _REDUCTIONS = {"sum": 0, "row": 1, "batch": 2}
@@ -143,8 +143,8 @@ def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
     if n > MAX_ROWS or not 1 <= n_items <= MAX_CATALOGUE:
         raise ValueError(f"at most {MAX_ROWS} rows of X and 1 ... {MAX_CATALOGUE} rows of V")
     scale = float(scale)
-    if not 0.0 < scale <= 1e30:
-        raise ValueError("scale must be positive")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError("scale must be positive, in [1e-30, 1e30]")
     return (X, ldx), (V, ldv), _matrix(ids, "ids", (torch.int32,), rows=n, device=device), _vector(ibase, "ibase", n_items, device)
 
 
@@ -156,14 +156,16 @@ def check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, ma
     n, wc = c[0].shape
     r = _matrix(rejected, "rejected", f32, None, n, device)
     wr = r[0].shape[1]
+    if wc > MAX_LENGTH or wr > MAX_LENGTH:
+        raise ValueError(f"a slate has at most {MAX_LENGTH} places")
     if (ref_chosen is None) != (ref_rejected is None):
         raise ValueError("a reference needs both ref_chosen and ref_rejected")
     matrices = (c, r, _optional(ref_chosen, "ref_chosen", f32, wc, n, device), _optional(ref_rejected, "ref_rejected", f32, wr, n, device),
                 _optional(mask_chosen, "mask_chosen", masks, wc, n, device), _optional(mask_rejected, "mask_rejected", masks, wr, n, device))
     if kind not in _KINDS:
         raise ValueError("kind must be 'logistic', 'hinge' or 'squared'")
-    if not 0.0 < float(beta) <= 1e30:
-        raise ValueError("beta must be positive")
+    if not 1e-30 <= float(beta) <= 1e30:
+        raise ValueError("beta must be positive, in [1e-30, 1e30]")
     if not 0.0 <= float(label_smoothing) < 0.5:
         raise ValueError("label_smoothing must be in [0, 1/2)")
     if label_smoothing and kind != "logistic":
@@ -179,6 +181,8 @@ def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, c
     f32 = (torch.float32,)
     x = _matrix(logp, "logp", f32, None, None, device)
     n, width = x[0].shape
+    if width > MAX_LENGTH:
+        raise ValueError(f"a row has at most {MAX_LENGTH} places")
     matrices = (x, _matrix(old_logp, "old_logp", f32, width, n, device), _optional(ref_logp, "ref_logp", f32, width, n, device),
                 _optional(mask, "mask", (torch.bool, torch.uint8), width, n, device))
     if advantages is None:

@@ -1782,6 +1782,7 @@ int launched(ifr_handle h, int rc, const char *what)
 }
 
 constexpr int64_t MAX_ROWS = (int64_t)1 << 23, MAX_CATALOGUE = (int64_t)1 << 28, MAX_PLACES = (int64_t)1 << 20, MAX_LIST = (int64_t)1 << 32;
+constexpr int32_t MAX_LENGTH = 1 << 30;
 
 int check_catalogue(ifr_handle h, const char *what, const ifr_catalogue *c)
 {
@@ -1791,7 +1792,7 @@ int check_catalogue(ifr_handle h, const char *what, const ifr_catalogue *c)
     if (c->k < 1 || c->k > IFR_MAX_FACTORS) return fail(h, IFR_ERR_ARG, w + ": k must be in [1, 256]");
     if (c->n < 0 || c->n > MAX_ROWS) return fail(h, IFR_ERR_ARG, w + ": n must be in [0, 2^23]");
     if (c->n_items < 1 || c->n_items > MAX_CATALOGUE) return fail(h, IFR_ERR_ARG, w + ": n_items must be in [1, 2^28]");
-    if (!(c->scale > 0.0) || c->scale > 1e30) return fail(h, IFR_ERR_ARG, w + ": scale must be positive");
+    if (!(c->scale >= 1e-30) || c->scale > 1e30) return fail(h, IFR_ERR_ARG, w + ": scale must be positive, in [1e-30, 1e30]");
     if (c->dtype != IFR_MXFP4 && (c->ldx < c->k || c->ldv < c->k)) return fail(h, IFR_ERR_ARG, w + ": rows shorter than k");
     return IFR_OK;
 }
@@ -1926,8 +1927,9 @@ int ifr_preference_loss(ifr_handle h, const ifr_preference *p, void *stream)
         const std::string what = "ifr_preference_loss";
         if (!p) return fail(h, IFR_ERR_ARG, what + ": null argument");
         if (p->n < 0 || p->len_chosen < 0 || p->len_rejected < 0) return fail(h, IFR_ERR_ARG, what + ": negative size");
+        if (p->len_chosen > MAX_LENGTH || p->len_rejected > MAX_LENGTH) return fail(h, IFR_ERR_ARG, what + ": at most 2^30 places a row");
         if (p->kind < IFR_PREFERENCE_LOGISTIC || p->kind > IFR_PREFERENCE_SQUARED) return fail(h, IFR_ERR_ARG, what + ": unknown kind");
-        if (!(p->beta > 0.0) || p->beta > 1e30) return fail(h, IFR_ERR_ARG, what + ": beta must be positive");
+        if (!(p->beta >= 1e-30) || p->beta > 1e30) return fail(h, IFR_ERR_ARG, what + ": beta must be positive, in [1e-30, 1e30]");
         if (!(p->label_smoothing >= 0.0 && p->label_smoothing < 0.5)) return fail(h, IFR_ERR_ARG, what + ": label_smoothing must be in [0, 1/2)");
         if (p->label_smoothing != 0.0 && p->kind != IFR_PREFERENCE_LOGISTIC) return fail(h, IFR_ERR_ARG, what + ": label_smoothing needs the logistic kind");
         if (!(p->margin > -1e30 && p->margin < 1e30)) return fail(h, IFR_ERR_ARG, what + ": margin must be finite");
@@ -1947,6 +1949,7 @@ static int check_policy(ifr_handle h, const std::string &what, const ifr_policy 
 {
     if (!p) return fail(h, IFR_ERR_ARG, what + ": null argument");
     if (p->n < 0 || p->len < 0) return fail(h, IFR_ERR_ARG, what + ": negative size");
+    if (p->len > MAX_LENGTH) return fail(h, IFR_ERR_ARG, what + ": at most 2^30 places a row");
     if (p->reduction < IFR_POLICY_SUM || p->reduction > IFR_POLICY_BATCH) return fail(h, IFR_ERR_ARG, what + ": unknown reduction");
     if (!(p->clip_low >= 0.0 && p->clip_low < 1.0) || !(p->clip_high >= 0.0 && p->clip_high < 1e30))
         return fail(h, IFR_ERR_ARG, what + ": clip_low must be in [0, 1), clip_high at least 0");

@@ -145,3 +145,21 @@ def test_learning_refusals():
         with pytest.raises(ValueError, match="batch_size"):
             list(m._hip_schedule(3, **{**dict(batch_size=2, epochs=1, learning_rate=.1, reg=0.0, seed=0), **bad}))
     assert sorted(np.concatenate([b for _, b in m._hip_schedule(5, 2, 1, .1, 0.0, 0)]).tolist()) == list(range(5))
+
+
+def test_sizes_and_factors_out_of_range():
+    """Rows that the kernels' 32-bit places do not hold, and factors whose reciprocal fp32 does not hold."""
+    wide = torch.empty((1, C.MAX_LENGTH + 1), device="meta")
+    one = torch.empty((1, 1), device="meta")
+    args = (None, None, None, None, None, 0.1, "logistic", 0.0, 0.0)
+    with pytest.raises(ValueError, match="places"):
+        C.check_preference(wide, one, *args)
+    with pytest.raises(ValueError, match="places"):
+        C.check_preference(one, wide, *args)
+    with pytest.raises(ValueError, match="places"):
+        C.check_policy(wide, wide, torch.empty(1, device="meta"), None, None, None, 0.2, 0.2, 0.0, "row")
+    for scale in (1e-31, 1e31, float("nan")):
+        with pytest.raises(ValueError, match="scale must be positive"):
+            C.check_catalogue(X, V, IDS, None, scale)
+    with pytest.raises(ValueError, match="beta must be positive"):
+        C.check_preference(torch.zeros((2, 3)), torch.zeros((2, 3)), None, None, None, None, None, 1e-31, "logistic", 0.0, 0.0)

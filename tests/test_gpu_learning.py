@@ -333,3 +333,21 @@ def test_a_model_that_learned_can_be_copied(torch):
     before = m.log_prob([0], [[3]])
     m.hip_invalidate()
     assert np.array_equal(copy.deepcopy(m).log_prob([0], [[3]]), before)
+
+
+def test_c_refusals_of_sizes_and_factors(torch, sc):
+    from recommenders_amd import _lib
+    x = torch.zeros(64, device="cuda")
+    o, long = x.data_ptr(), (1 << 30) + 1
+    pref = lambda **kw: sc._lib.ifr_preference_loss(sc._h, ctypes.byref(_lib.Preference(**{**dict(n=1, len_chosen=1, len_rejected=1, chosen=o, rejected=o, ld_chosen=1,
+                                                                                             ld_rejected=1, beta=1.0), **kw})), None)
+    pol = lambda **kw: sc._lib.ifr_policy_loss(sc._h, ctypes.byref(_lib.Policy(**{**dict(n=1, len=1, logp=o, old_logp=o, advantages=o, ld_logp=1, ld_old=1), **kw})),
+                                               None, 0, None)
+    c = lambda scale: ctypes.byref(_lib.Catalogue(X=o, V=o, n=1, n_items=1, ldx=8, ldv=8, k=8, dtype=0, scale=scale))
+    need = ctypes.c_int64(0)
+    size = lambda scale: sc._lib.ifr_catalogue_logprob_workspace(sc._h, c(scale), ctypes.byref(need))
+    assert pref() == 0 and pol() == 0 and size(1e-30) == 0 and size(1e30) == 0
+    bad = [pref(len_chosen=long, ld_chosen=long), pref(len_rejected=long, ld_rejected=long), pref(beta=1e-31), pol(len=long, ld_logp=long, ld_old=long),
+           size(1e-31), size(1e31)]
+    assert bad == [-1] * len(bad)
+    torch.cuda.synchronize()
