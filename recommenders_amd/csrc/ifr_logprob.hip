@@ -529,14 +529,18 @@ constexpr int aside_floats(int KP)
 // of LDS; the statistics take half of that, for two workgroups a compute unit also at KP = 256.
 constexpr int stage_tiles(int NS, bool grad) { return (NS == 1 ? 2 : 1) * (grad ? 2 : 1); }
 
+// whether a compute unit holds two workgroups of walk_kernel by its registers
+constexpr bool paired(int KP, int NS, int mode) { return KP * NS <= 256 && (mode == WALK_STATS || KP <= 128); }
+
 // S_LIES, T_LIES: read as bf16 rows in memory (V; X too for the statistics)
 template <int KP, int NS, int MODE, bool S_LIES, bool T_LIES>
-__global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <= 128) ? 2 : 1) void walk_kernel(WalkParams p)
+__global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel(WalkParams p)
 {
     typedef typename std::conditional<NS == 2, float, __bf16>::type T;
     constexpr int STEPS = KP / 16;
     constexpr int PART = STEPS * 64;                  // 16-byte pieces of a part of a tile
-    constexpr bool GRAD = MODE != WALK_STATS;
+    constexpr bool GRAD = MODE != WALK_STATS, PAIRED = paired(KP, NS, MODE);
+    constexpr int ABREAST = NS == 2 && !PAIRED ? 2 : 1;      // blocks of 32 columns whose products alternate
     constexpr int SUB = stage_tiles(NS, GRAD);
     constexpr int STAGE = PART * NS * SUB;
     // two stages: one is read while the other arrives (two arrays, so that the compiler sees that they are apart)
@@ -571,9 +575,8 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
     constexpr bool ITEMS = MODE == WALK_ITEMS || MODE == WALK_ITEMS_BASE;
     v16f acc[GRAD ? KP / 32 : 1] = {};
     float m = -3.402823466e38f, sum = 0.f, b_sum = 0.f;
-    int ref = 280;                                    // exponent of acc (split operands), the least of the tiles so far
-
     const int first = split * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
+    int ref = 280;                                    // exponent of acc (split operands), the least of the tiles so far
     // this lane's pieces of the first product's operand (even and odd steps), and its 8 bytes of the second's, which ds_read_tr turns
     // round: 16 lanes read four rows by 16 columns and get four rows of a column each (rows 0..7 and 8..15 of a step of 16)
     const int at1[2] = {piece_at(0, lane & 31, h), piece_at(1, lane & 31, h) - 64};
@@ -600,120 +603,161 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
         if (wave < (SUB + 1) / 2) fetch_row(p.t_term + (int64_t)t * 32 + wave * 64, terms + wave * 64);
         else if (ITEMS && wave < SUB) fetch_row(p.t_factor + (int64_t)t * 32 + (wave - SUB / 2) * 64, terms + wave * 64);
     };
-    auto compute = [&](int t0, const uint4 *lds, const float *terms) {
-#pragma unroll 2
-        for (int sub = 0; sub < SUB; ++sub) {
-            const int t = t0 + sub;
-            if (t >= p.t_tiles) break;                // the stage reaches behind the last row
-            const uint4 *l1 = lds + sub * PART * NS;
-            float4 tt[4];
+    // The scores of one tile: split c d + term with c of the tile, otherwise the sums begin with the terms.
+    auto scores = [&](const uint4 *l1, const float *tt, float c) {
+        v16f d = {};
+        float4 t4[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) tt[q] = *(const float4 *)(terms + sub * 32 + 8 * q + 4 * h);
-            float c = p.c;
-            if (NS == 2) c = fminf(ldexpf(c, -s_exp - p.t_exp[t]), 3.402823466e38f);
-            v16f d = {};
-            if (NS == 1) {
+        for (int q = 0; q < 4; ++q) t4[q] = *(const float4 *)(tt + 8 * q + 4 * h);
+        if (NS == 1) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) { d[4 * q] = tt[q].x; d[4 * q + 1] = tt[q].y; d[4 * q + 2] = tt[q].z; d[4 * q + 3] = tt[q].w; }
-            }
+            for (int q = 0; q < 4; ++q) { d[4 * q] = t4[q].x; d[4 * q + 1] = t4[q].y; d[4 * q + 2] = t4[q].z; d[4 * q + 3] = t4[q].w; }
+        }
+        // split: two sums in turn, so that no matrix instruction waits for the one before (a wave is alone on its SIMD)
+        v16f other = {};
+        constexpr bool TWO = NS == 2 && GRAD && !PAIRED;
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const uint4 a = l1[s * 64 + at1[s & 1]];
-                d = product<NS>(a, sf[0][s], d);
-                if (NS == 2) {
-                    d = product<NS>(a, sf[NS - 1][s], d);
-                    d = product<NS>(l1[PART + s * 64 + at1[s & 1]], sf[0][s], d);
-                }
-            }
-            reads_ahead<STEPS * NS, STEPS * (2 * NS - 1)>();
-            // the exponent of a score without the S side's part: split c d + term, otherwise c d
+        for (int s = 0; s < STEPS; ++s) {
+            const uint4 a = l1[s * 64 + at1[s & 1]];
+            v16f &d0 = TWO && (s & 1) ? other : d, &d1 = TWO && !(s & 1) ? other : d;
+            d0 = product<NS>(a, sf[0][s], d0);
             if (NS == 2) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    d[4 * q] = fmaf(d[4 * q], c, tt[q].x); d[4 * q + 1] = fmaf(d[4 * q + 1], c, tt[q].y);
-                    d[4 * q + 2] = fmaf(d[4 * q + 2], c, tt[q].z); d[4 * q + 3] = fmaf(d[4 * q + 3], c, tt[q].w);
-                }
-                c = 1.f;
+                d1 = product<NS>(a, sf[NS - 1][s], d1);
+                d0 = product<NS>(l1[PART + s * 64 + at1[s & 1]], sf[0][s], d0);
             }
-            if (MODE == WALK_STATS) {
-                online(d, c, m, sum);
-            } else {
-                // split: what enters the second product is scaled to at most 2^15 (probabilities by 2^15, G P by G's exponent), which
-                // fp16 holds down to 2^-39 of that; tiles of T with a larger exponent than the reference take the difference off
-                // here, one with a smaller becomes the reference
-                int up = 0, ge = 0;
-                if (NS == 2) {
-                    ge = ITEMS ? p.t_factor_exp[t] : 0;
-                    const int e = p.t_exp[t] + ge;
-                    if (e < ref) {
-                        const float f = ldexpf(1.f, e - ref);
-                        for (int kb = 0; kb < KP / 32; ++kb) acc[kb] *= f;
-                        ref = e;
-                    }
-                    up = (MODE == WALK_USERS ? 15 : 0) - (e - ref);
-                }
-                const float add = s_term + (float)up;
-                float P[16];
+        }
+        if (TWO) d += other;
+        if (NS == 2) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) P[r] = exp2_raw(fmaf(d[r], c, add));
-                if (ITEMS) {
-                    float4 tg[4];
+            for (int q = 0; q < 4; ++q) {
+                d[4 * q] = fmaf(d[4 * q], c, t4[q].x); d[4 * q + 1] = fmaf(d[4 * q + 1], c, t4[q].y);
+                d[4 * q + 2] = fmaf(d[4 * q + 2], c, t4[q].z); d[4 * q + 3] = fmaf(d[4 * q + 3], c, t4[q].w);
+            }
+        }
+        return d;
+    };
+    // A stage's tiles (those behind the last row have terms of -inf and add nothing: no branch divides the code, so that the
+    // exponentials of one tile go beside the matrix instructions of the next tile's scores and of the last one's sums).
+    auto compute = [&](const uint4 *lds, const float *terms, const int *t_exps, const int *f_exps) {
+        float c[SUB];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) tg[q] = *(const float4 *)(terms + SUB * 32 + sub * 32 + 8 * q + 4 * h);
-                    float b = 0.f;
-                    if (MODE == WALK_ITEMS_BASE && NS == 2 && up < -20) {        // a tile far below the reference: its sum for db from the probabilities as they are
+        for (int sub = 0; sub < SUB; ++sub) c[sub] = NS == 2 ? fminf(ldexpf(p.c, -s_exp - t_exps[sub]), 3.402823466e38f) : p.c;
+        if (MODE == WALK_STATS) {
+#pragma unroll 2
+            for (int sub = 0; sub < SUB; ++sub) {
+                const v16f d = scores(lds + sub * PART * NS, terms + sub * 32, c[sub]);
+                reads_ahead<STEPS * NS, STEPS * (2 * NS - 1)>();
+                online(d, NS == 2 ? 1.f : c[sub], m, sum);
+            }
+            return;
+        }
+        // split: what enters the second product is scaled to at most 2^15 (probabilities by 2^15, G P by G's exponent), which
+        // fp16 holds down to 2^-39 of that; tiles of T with a larger exponent than the reference take the difference off
+        // here, one with a smaller becomes the reference
+        int up[SUB] = {};
+        bool far = false;
+        if (NS == 2) {
+            int least = ref;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            b = fmaf(exp2_raw(d[4 * q] + s_term), tg[q].x, b); b = fmaf(exp2_raw(d[4 * q + 1] + s_term), tg[q].y, b);
-                            b = fmaf(exp2_raw(d[4 * q + 2] + s_term), tg[q].z, b); b = fmaf(exp2_raw(d[4 * q + 3] + s_term), tg[q].w, b);
-                        }
-                    }
-                    {   // products rounded by themselves: dV has the same bits with and without db beside it
+            for (int sub = 0; sub < SUB; ++sub) least = min(least, t_exps[sub] + (ITEMS ? f_exps[sub] : 0));
+            if (least < ref) {
+                const float f = ldexpf(1.f, least - ref);
+                for (int kb = 0; kb < KP / 32; ++kb) acc[kb] *= f;
+                ref = least;
+            }
+#pragma unroll
+            for (int sub = 0; sub < SUB; ++sub) {
+                up[sub] = (MODE == WALK_USERS ? 15 : 0) - (t_exps[sub] + (ITEMS ? f_exps[sub] : 0) - ref);
+                far |= up[sub] < -20;
+            }
+        }
+        // probabilities of a tile (times G for the items' side), as the operand of the second product
+        struct Operand { uint4 part[NS][2]; };
+        auto probabilities = [&](const v16f &d, int sub) {
+            const float add = s_term + (float)up[sub];
+            float P[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) P[r] = exp2_raw(NS == 2 ? d[r] + add : fmaf(d[r], c[sub], add));
+            if (ITEMS) {
+                {   // products rounded by themselves: dV has the same bits with and without db beside it
 #pragma clang fp contract(off)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            P[4 * q] *= tg[q].x; P[4 * q + 1] *= tg[q].y; P[4 * q + 2] *= tg[q].z; P[4 * q + 3] *= tg[q].w;
-                        }
-                    }
-                    if (MODE == WALK_ITEMS_BASE) {
-                        if (NS == 1 || up >= -20) {
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) b += P[r];
-                        }
-                        b_sum += NS == 2 ? ldexpf(b, -ge - (up < -20 ? 0 : up)) : b;
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 tg = *(const float4 *)(terms + SUB * 32 + sub * 32 + 8 * q + 4 * h);
+                        P[4 * q] *= tg.x; P[4 * q + 1] *= tg.y; P[4 * q + 2] *= tg.z; P[4 * q + 3] *= tg.w;
                     }
                 }
-                uint4 pf[NS][2];
+                if (MODE == WALK_ITEMS_BASE) {
+                    float b = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) b += P[r];
+                    b_sum += NS == 2 ? (up[sub] < -20 ? 0.f : ldexpf(b, -f_exps[sub] - up[sub])) : b;
+                }
+            }
+            Operand o;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (NS == 1) {
+                    b8 v;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = (__bf16)P[8 * e + j];
+                    o.part[0][e] = __builtin_bit_cast(uint4, v);
+                } else {
+                    h8 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        hi[j] = (_Float16)P[8 * e + j];
+                        lo[j] = (_Float16)(P[8 * e + j] - (float)hi[j]);
+                    }
+                    o.part[0][e] = __builtin_bit_cast(uint4, hi);
+                    o.part[NS - 1][e] = __builtin_bit_cast(uint4, lo);
+                }
+            }
+            return o;
+        };
+        // their product with the tile's rows
+        auto add_product = [&](const uint4 *l1, const Operand &o) {
+#pragma unroll
+            for (int kb = 0; kb < KP / 32; kb += ABREAST)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    if (NS == 1) {
-                        b8 o;
+                    uint4 a[ABREAST][NS];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) o[j] = (__bf16)P[8 * e + j];
-                        pf[0][e] = __builtin_bit_cast(uint4, o);
-                    } else {
-                        h8 hi, lo;
+                    for (int j = 0; j < ABREAST; ++j)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            hi[j] = (_Float16)P[8 * e + j];
-                            lo[j] = (_Float16)(P[8 * e + j] - (float)hi[j]);
-                        }
-                        pf[0][e] = __builtin_bit_cast(uint4, hi);
-                        pf[NS - 1][e] = __builtin_bit_cast(uint4, lo);
-                    }
+                        for (int q = 0; q < NS; ++q)
+                            if (kb + j < KP / 32) {
+                                const char *l2 = (const char *)(l1 + q * PART) + (kb + j) * 2048 + e * 512;
+                                a[j][q] = turned(l2 + at2, l2 + at2_high);
+                            }
+#pragma unroll
+                    for (int q = 0; q < 2 * NS - 1; ++q)
+#pragma unroll
+                        for (int j = 0; j < ABREAST; ++j)
+                            if (kb + j < KP / 32) acc[kb + j] = product<NS>(a[j][q >> 1], o.part[q & 1][e], acc[kb + j]);
                 }
+        };
+        v16f next = scores(lds, terms, c[0]);
 #pragma unroll
-                for (int kb = 0; kb < KP / 32; ++kb)
+        for (int sub = 0; sub < SUB; ++sub) {
+            const v16f d = next;
+            if (sub + 1 < SUB) next = scores(lds + (sub + 1) * PART * NS, terms + (sub + 1) * 32, c[sub + 1 < SUB ? sub + 1 : 0]);
+            add_product(lds + sub * PART * NS, probabilities(d, sub));
+        }
+        if (MODE == WALK_ITEMS_BASE && NS == 2 && far) {
+            // tiles far below the reference (seldom): their sums for db from the probabilities as they are
+#pragma unroll 1
+            for (int sub = 0; sub < SUB; ++sub) {
+                if ((sub ? up[SUB - 1] : up[0]) >= -20) continue;
+                const v16f d = scores(lds + sub * PART * NS, terms + sub * 32, sub ? c[SUB - 1] : c[0]);
+                float b = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const char *l2 = (const char *)l1 + kb * 2048 + e * 512;
-                        const uint4 a = turned(l2 + at2, l2 + at2_high);
-                        acc[kb] = product<NS>(a, pf[0][e], acc[kb]);
-                        if (NS == 2) {
-                            acc[kb] = product<NS>(a, pf[NS - 1][e], acc[kb]);
-                            acc[kb] = product<NS>(turned(l2 + PART * 16 + at2, l2 + PART * 16 + at2_high), pf[0][e], acc[kb]);
-                        }
-                    }
+                for (int q = 0; q < 4; ++q) {
+                    const float4 tg = *(const float4 *)(terms + SUB * 32 + sub * 32 + 8 * q + 4 * h);
+                    b = fmaf(exp2_raw(d[4 * q] + s_term), tg.x, b); b = fmaf(exp2_raw(d[4 * q + 1] + s_term), tg.y, b);
+                    b = fmaf(exp2_raw(d[4 * q + 2] + s_term), tg.z, b); b = fmaf(exp2_raw(d[4 * q + 3] + s_term), tg.w, b);
+                }
+                b_sum += ldexpf(b, -(sub ? f_exps[SUB - 1] : f_exps[0]));
             }
         }
     };
@@ -722,15 +766,24 @@ __global__ __launch_bounds__(256, KP * NS <= 256 && (MODE == WALK_STATS || KP <=
         __syncthreads();
     };
 
-    if (first < last) fetch_stage(first, stage0, terms0);
+    // the exponents of a stage's tiles, loaded with it
+    int t_exps[2][SUB] = {}, f_exps[2][SUB] = {};
+    auto fetch_exps = [&](int t, int at) {
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub) {
+            if (NS == 2) t_exps[at][sub] = p.t_exp[t + sub];
+            if (NS == 2 && ITEMS) f_exps[at][sub] = p.t_factor_exp[t + sub];
+        }
+    };
+    if (first < last) { fetch_stage(first, stage0, terms0); fetch_exps(first, 0); }
     for (int t = first; t < last; t += 2 * SUB) {
         arrived();
-        if (t + SUB < last) fetch_stage(t + SUB, stage1, terms1);
-        compute(t, stage0, terms0);
+        if (t + SUB < last) { fetch_stage(t + SUB, stage1, terms1); fetch_exps(t + SUB, 1); }
+        compute(stage0, terms0, t_exps[0], f_exps[0]);
         if (t + SUB >= last) break;
         arrived();
-        if (t + 2 * SUB < last) fetch_stage(t + 2 * SUB, stage0, terms0);
-        compute(t + SUB, stage1, terms1);
+        if (t + 2 * SUB < last) { fetch_stage(t + 2 * SUB, stage0, terms0); fetch_exps(t + 2 * SUB, 0); }
+        compute(stage1, terms1, t_exps[1], f_exps[1]);
     }
 
     const int64_t at = (int64_t)split * p.s_padded + s_row;
@@ -1291,7 +1344,7 @@ void launch_walk(const WalkParams &p, int KP, hipStream_t s)
 #undef IFR_WALK
 }
 
-int resident_blocks(int KP, int NS, int mode) { return 256 * (mode != WALK_STATS && (KP * NS > 256 || KP > 128) ? 1 : 2); }
+int resident_blocks(int KP, int NS, int mode) { return mode == WALK_STATS || paired(KP, NS, mode) ? 512 : 256; }
 
 // Users one pass over V serves (their operand stays in registers: at most 128 of them), and up to how many users the direct kernel is taken.
 int direct_tiles(int KP, int64_t n) { return n <= 16 ? 1 : n <= 32 || KP > 128 ? 2 : 4; }
@@ -1532,8 +1585,8 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
         w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
         w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx), fours(g.dV, g.ld_dv)};
-        if (g.dibase) launch_walk<NS, WALK_ITEMS_BASE>(w, KP, s);
-        else launch_walk<NS, WALK_ITEMS>(w, KP, s);
+        if (NS == 2 || g.dibase) launch_walk<NS, WALK_ITEMS_BASE>(w, KP, s);
+        else launch_walk<1, WALK_ITEMS>(w, KP, s);
     }
     // the joins as one launch where dX's is short (its workgroups hold the memory of the other's)
     const bool together = parts && x.blocks <= 512;
