@@ -438,7 +438,7 @@ constexpr int group_threads(int KP) { return KP > 128 ? 64 : KP > 64 ? 32 : KP >
 
 // The found places [from, to) in their sorted order, of items whose local number is 64 at a time from `local0`.  The groups of threads
 // (four columns a thread) take equal parts, so that an item that everybody names does not fall to one group; an item's first run in a
-// part goes to a row set aside, which is added after the others, in the parts' order.  Short code on purpose: it runs once a
+// part goes to a row set aside, which is added after the others, in the parts' order.  A run is summed in registers.  Short code on purpose: it runs once a
 // workgroup, and what it costs is the fetching of its instructions as much as that of the rows.
 template <typename T, int KP>
 __device__ __forceinline__ void add_places(const Finish &f, float *rows, float *row_b, const uint32_t *list, float *aside, int *aside_item, int local0, int from,
@@ -454,6 +454,14 @@ __device__ __forceinline__ void add_places(const Finish &f, float *rows, float *
     const int first = begin < end ? (int)(order[begin] >> 12) - local0 : -1;
     if (c4 == 0) { aside_item[group] = first; aside[GROUPS * KP + group] = 0.f; }
     if (in) *(float4 *)(aside + group * KP + c4) = make_float4(0.f, 0.f, 0.f, 0.f);
+    int cur = -1;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum_b = 0.f;
+    auto row_of = [&](int at) { return at == first ? aside + group * KP : rows + at * KP; };
+    auto flush = [&]() {
+        *(float4 *)(row_of(cur) + c4) = sum;
+        if (c4 == 0) *(cur == first ? aside + GROUPS * KP + group : row_b + cur) += sum_b;
+    };
     for (int q0 = begin; q0 < end; q0 += BATCH) {
         // all keys, then all users, then all rows: sixteen gathers are under way at once
         uint32_t key[BATCH], u[BATCH];
@@ -473,17 +481,18 @@ __device__ __forceinline__ void add_places(const Finish &f, float *rows, float *
         for (int q = 0; q < BATCH; ++q)
             if (in && q0 + q < end) {
                 const int at = (int)(key[q] >> 12) - local0;
-                float4 *r = (float4 *)((at == first ? aside + group * KP : rows + at * KP) + c4);
-                float4 v = *r;
-                v.x = fmaf(g[q], x[q][0], v.x); v.y = fmaf(g[q], x[q][1], v.y);
-                v.z = fmaf(g[q], x[q][2], v.z); v.w = fmaf(g[q], x[q][3], v.w);
-                *r = v;
-                if (c4 == 0) {
-                    float *b = at == first ? aside + GROUPS * KP + group : row_b + at;
-                    *b += g[q];
+                if (at != cur) {
+                    if (cur >= 0) flush();
+                    cur = at;
+                    sum = *(const float4 *)(row_of(at) + c4);
+                    sum_b = 0.f;
                 }
+                sum.x = fmaf(g[q], x[q][0], sum.x); sum.y = fmaf(g[q], x[q][1], sum.y);
+                sum.z = fmaf(g[q], x[q][2], sum.z); sum.w = fmaf(g[q], x[q][3], sum.w);
+                sum_b += g[q];
             }
     }
+    if (in && cur >= 0) flush();
     __syncthreads();
     for (int g = 0; g < GROUPS; ++g) {
         const int item = aside_item[g];
