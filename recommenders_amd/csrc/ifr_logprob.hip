@@ -35,6 +35,8 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.6931471805599453;
 constexpr int S_ROWS = 128;            // S rows of a workgroup: 4 waves of 32
+constexpr int64_t DEAL_FROM = 65536;
+constexpr int BUCKETS = 64, CHUNK = 4096;      // of places: see deal_kernel
 constexpr int64_t MAX_GRID = 1 << 22;  // workgroups of 256 in one launch (the grid counts work items in 32 bits)
 
 int pad_factors(int k) { return (k + 31) / 32 * 32; }
@@ -234,6 +236,106 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, int64_t n)
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
+// Places in the order of 64 buckets of items (whole S blocks each), so that a workgroup that finishes rows of dV looks through its
+// bucket's only.  A stable counting sort: a workgroup takes 4096 places, a thread 16 neighbouring ones, and each (bucket, thread) has a
+// byte of its own in LDS, so no order depends on scheduling.  Empty places and those behind the catalogue are left out.
+struct Deal {
+    const int32_t *places;
+    int64_t chunks, n_items, bucket_items;
+    uint32_t *counts;                  // [BUCKETS][chunks], then their exclusive sums
+    uint32_t *bounds;                  // [BUCKETS + 1]
+    int32_t *to;                       // the items again, -1 up to the next 1024
+    uint32_t *place_of;
+};
+
+template <bool WRITE>
+__global__ __launch_bounds__(256) void deal_kernel(Deal d)
+{
+    __shared__ uint32_t held[64 * 64];                // [bucket][thread], bytes
+    uint8_t *mine = (uint8_t *)held + threadIdx.x;
+    const int64_t chunk = blockIdx.x, at = chunk * CHUNK + threadIdx.x * 16;
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) held[i] = 0;
+    int32_t id[16];
+    uint8_t bucket[16];
+    for (int q = 0; q < 16; q += 4) *(int4 *)(id + q) = *(const int4 *)(d.places + at + q);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const bool in = id[q] >= 0 && id[q] < d.n_items;
+        bucket[q] = in ? (uint8_t)(id[q] / (int32_t)d.bucket_items) : 255;
+        if (in) ++mine[bucket[q] * 256];
+    }
+    __syncthreads();
+    // four threads a bucket, 64 of the bytes each
+    const int b = threadIdx.x >> 2, quarter = threadIdx.x & 3;
+    uint32_t sum = 0;
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t w = held[b * 64 + quarter * 16 + i];
+        sum += (w & 255) + (w >> 8 & 255) + (w >> 16 & 255) + (w >> 24);
+    }
+    uint32_t before = 0, all = sum;
+    for (int o = 1; o < 4; ++o) {
+        const uint32_t other = __shfl_xor(sum, o);
+        all += other;
+        if ((quarter ^ o) < quarter) before += other;
+    }
+    if (!WRITE) {
+        if (quarter == 0) d.counts[b * d.chunks + chunk] = all;
+        return;
+    }
+    // where the places of each thread and bucket go: sixteen bits beside the chunk's begin
+    __shared__ uint16_t first[64 * 256];
+    uint32_t run = before;
+    for (int i = 0; i < 64; ++i) {
+        first[b * 256 + quarter * 64 + i] = (uint16_t)run;
+        run += ((const uint8_t *)held)[b * 256 + quarter * 64 + i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+        if (bucket[q] != 255) {
+            const uint32_t to = d.counts[bucket[q] * d.chunks + chunk] + first[bucket[q] * 256 + threadIdx.x]++;
+            d.to[to] = id[q];
+            d.place_of[to] = (uint32_t)(at + q);
+        }
+    if (chunk == 0) {
+        const uint32_t total = d.bounds[BUCKETS];
+        for (uint32_t i = total + threadIdx.x; i < (total + 1023) / 1024 * 1024; i += 256) d.to[i] = -1;
+    }
+}
+
+// exclusive sums of the counts, one workgroup
+__global__ __launch_bounds__(1024) void deal_sums_kernel(Deal d)
+{
+    __shared__ uint32_t waves[16];
+    const int64_t all = BUCKETS * d.chunks;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t carry = 0;
+    for (int64_t i0 = 0; i0 < all; i0 += 1024) {
+        const int64_t i = i0 + threadIdx.x;
+        const uint32_t v = i < all ? d.counts[i] : 0;
+        uint32_t sum = v;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t other = __shfl_up(sum, o);
+            if (lane >= o) sum += other;
+        }
+        if (lane == 63) waves[wave] = sum;
+        __syncthreads();
+        uint32_t before = carry;
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) before += waves[w];
+            carry += waves[w];
+        }
+        before += sum - v;
+        if (i < all) {
+            d.counts[i] = before;
+            if (i % d.chunks == 0) d.bounds[i / d.chunks] = before;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) d.bounds[BUCKETS] = carry;
+}
+
 // ---------------------------------------------------------------------------- the walk
 
 // lse; the sums of dX (S users, T items); those of dV (S items, T users), and of dV and db
@@ -247,6 +349,9 @@ struct Finish {
     const float *dlogp;
     void *dV;                          // [n_items][ld_dv] or null
     float *db;                         // [n_items] or null
+    const uint32_t *place_of;          // places dealt into buckets: the number of each, or null: as they are
+    const uint32_t *bounds;            // [BUCKETS + 1]: a bucket's first place
+    int64_t bucket_items;              // items of a bucket
     int64_t n_places, m, ldx, ld_dlogp, ld_dv, n_items;
     int k;
     float scale;
@@ -352,9 +457,14 @@ __device__ __forceinline__ int find_places(const Finish &f, uint32_t *list, int 
     uint32_t *order = list + 2 * LIST;
     float *gs = (float *)(list + LIST);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t steps = (f.n_places + 64 * EACH - 1) / (64 * EACH);          // of a wave, over all places
-    const int64_t end = steps * (wave + 1) / 4;
-    if (step < 0) step = steps * wave / 4;
+    int64_t begin = 0, steps = (f.n_places + 64 * EACH - 1) / (64 * EACH);     // of a wave, over all places or the bucket's
+    if (f.place_of) {                                 // what lies beside them in the first and last step names other items
+        const int64_t b = i0 / f.bucket_items;
+        begin = f.bounds[b] / (64 * EACH);
+        steps = (f.bounds[b + 1] + 64 * EACH - 1) / (64 * EACH) - begin;
+    }
+    const int64_t end = begin + steps * (wave + 1) / 4;
+    if (step < 0) step = begin + steps * wave / 4;
     int held = 0;
     int32_t id[EACH], next[EACH];
     auto load = [&](int64_t at, int32_t *to) {
@@ -412,7 +522,7 @@ __device__ __forceinline__ int find_places(const Finish &f, uint32_t *list, int 
     }
     for (int q = lane; q < held; q += 64) {           // places to users and gradients, each by one lane
         const int at = wave * CAP + q;
-        const uint32_t place = list[at], u = place / (uint32_t)f.m;
+        const uint32_t place = f.place_of ? f.place_of[list[at]] : list[at], u = place / (uint32_t)f.m;
         order[offset + q] = (uint32_t)item_of[at] << 12 | (uint32_t)at;
         list[at] = u;
         gs[at] = f.dlogp[(int64_t)u * f.ld_dlogp + (place - u * (uint32_t)f.m)];
@@ -1413,8 +1523,12 @@ struct BackwardPlan {
     int32_t *places;
     uint8_t *named;
     int64_t places_padded;
+    Deal deal;                         // places dealt into buckets, or places null
     Split split_x, split_v;
 };
+
+// Places are dealt into buckets where the workgroups' looking through all of them would take longer than the dealing.
+bool deals(const ifr_catalogue &c, int64_t m, bool items) { return items && c.n * m >= DEAL_FROM && c.n * m < (int64_t)1 << 31 && c.n_items >= 16 * S_ROWS; }
 
 BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx, bool dv, bool db, bool lies)
 {
@@ -1428,8 +1542,19 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
     p.G = w.take<float>(p.x.padded);
     p.G_scaled = w.take<float>(NS == 2 ? p.x.padded : 0);
     p.g_exp = w.take<int>(NS == 2 ? p.x.tiles : 0);
-    p.places_padded = items ? up(c.n * m, 1024) : 0;
+    p.places_padded = items ? up(c.n * m, CHUNK) : 0;
     p.places = w.take<int32_t>(p.places_padded);
+    if (deals(c, m, items)) {
+        Deal &d = p.deal;
+        d.chunks = p.places_padded / CHUNK;
+        d.n_items = c.n_items;
+        d.bucket_items = up(up(c.n_items, S_ROWS) / S_ROWS, BUCKETS) / BUCKETS * S_ROWS;
+        d.counts = w.take<uint32_t>(BUCKETS * d.chunks);
+        d.bounds = w.take<uint32_t>(BUCKETS + 1);
+        d.to = w.take<int32_t>(p.places_padded);
+        d.place_of = w.take<uint32_t>(p.places_padded);
+        d.places = p.places;
+    }
     // flags save the search where most groups of 64 items are not named; where the places are as many as the groups, none is saved
     p.named = w.take<uint8_t>(p.places_padded && c.n_items > 64 * c.n * m ? up(p.v.padded / 64, 4) : 0);
     const int resident = resident_blocks(KP, NS, WALK_USERS);
@@ -1577,6 +1702,12 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     pp.user_term = p.user_term; pp.G = p.G; pp.places = p.places; pp.named = p.named;
     pp.G_scaled = p.G_scaled; pp.g_exp = p.g_exp;
     launch_prepare<T>(pp, p.x.tiles, s);
+    const bool dealt = deals(c, m, items);
+    if (dealt) {
+        hipLaunchKernelGGL(deal_kernel<false>, dim3((uint32_t)p.deal.chunks), dim3(256), 0, s, p.deal);
+        hipLaunchKernelGGL(deal_sums_kernel, dim3(1), dim3(1024), 0, s, p.deal);
+        hipLaunchKernelGGL(deal_kernel<true>, dim3((uint32_t)p.deal.chunks), dim3(256), 0, s, p.deal);
+    }
     WalkParams w = {};
     w.c = (float)(c.scale / LN2);
     JoinDx x = {};
@@ -1593,7 +1724,7 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
         w.s_term = p.item_term; w.t_term = p.user_term; w.t_factor = NS == 2 ? p.G_scaled : p.G; w.t_factor_exp = p.g_exp;
         w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
-        w.f = {p.places, p.named, X, g.dlogp, g.dV, g.dibase, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx), fours(g.dV, g.ld_dv)};
+        w.f = {dealt ? p.deal.to : p.places, p.named, X, g.dlogp, g.dV, g.dibase, dealt ? p.deal.place_of : nullptr, p.deal.bounds, p.deal.bucket_items, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx), fours(g.dV, g.ld_dv)};
         if (NS == 2 || g.dibase) launch_walk<NS, WALK_ITEMS_BASE>(w, KP, s);
         else launch_walk<1, WALK_ITEMS>(w, KP, s);
     }

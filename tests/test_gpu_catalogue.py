@@ -254,6 +254,27 @@ def test_logprob_gradient_of_items_that_everybody_names(torch, sc, n, items, k, 
     assert all(torch.equal(a, c) for a, c in zip(got, again))
 
 
+@pytest.mark.parametrize("n,items,k,m", [(700, 5000, 33, 100), (4100, 2048, 64, 16), (1100, 9000, 130, 64), (70000, 2111, 32, 1)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_logprob_gradient_of_many_places(torch, sc, n, items, k, m, dtype):
+    """Places enough to be dealt into buckets first: one item in half of them, empty ones, catalogues of 16 to 71 blocks of 128 rows."""
+    X, V, b, ids, dlogp = _case(torch, n, items, k, m, dtype, True, 21, spread=0.2)
+    g = _gen(torch, 22)
+    pick = torch.rand((n, m), generator=g, device="cuda")
+    ids = torch.where(pick < 0.5, torch.full_like(ids, items // 2), torch.where(pick < 0.6, torch.full_like(ids, items - 1), ids))
+    dlogp /= n
+    _, lse = sc.catalogue_logprob(X, V, ids, ibase=b)
+    r = _reference(torch, X, V, b, ids, dlogp, 1.0)
+    got = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp, ibase=b)
+    # the norm of the error: rounding of the result, operands and probabilities in 16 bits (their errors are independent and add up
+    # like at most sqrt(3) steps), or 22 bits and up to n m additions of one item's places, errors again independent
+    bound = 3 * B if dtype == "bfloat16" else 8 * 2.0 ** -22 + math.sqrt(n * m) * U
+    for a, ref in zip(got, (r["dX"], r["dV"], r["db"])):
+        assert float((a.double() - ref).norm() / ref.norm()) <= (bound if a.dtype != torch.float32 or dtype == "float32" else 2.0 ** -18 + math.sqrt(n * m) * U)
+    again = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp, ibase=b)
+    assert all(torch.equal(a, c) for a, c in zip(got, again))
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_logprob_parts_that_are_not_wanted(torch, sc, dtype):
     X, V, b, ids, dlogp = _case(torch, 50, 300, 70, 3, dtype, True, 5)
