@@ -135,8 +135,9 @@ __device__ __forceinline__ void store_fragments(const float *tile, int W, int KP
     }
 }
 
-// Everything the walks read, a workgroup a tile of 32 rows of V (or 256 of its terms, where it needs no other order) or X.
-// Memory-bound: one read, one write.
+// Everything the walks read, a workgroup a tile of 32 rows of V (or 256 of its terms, where it needs no other order) or X.  One read, one
+// write, through LDS since a piece is eight columns of one row; short, so bound by the latency of its loads (eight under way a thread).
+// fp32 2048 + 26 744 rows of 200: 14 us (23 MB in, 26 MB out).
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
 {
@@ -238,7 +239,8 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, int64_t n)
 
 // Places in the order of 64 buckets of items (whole S blocks each), so that a workgroup that finishes rows of dV looks through its
 // bucket's only.  A stable counting sort: a workgroup takes 4096 places, a thread 16 neighbouring ones, and each (bucket, thread) has a
-// byte of its own in LDS, so no order depends on scheduling.  Empty places and those behind the catalogue are left out.
+// byte of its own in LDS, so no order depends on scheduling.  Empty places and those behind the catalogue are left out.  Latency-bound:
+// three short launches.
 struct Deal {
     const int32_t *places;
     int64_t chunks, n_items, bucket_items;
@@ -652,6 +654,16 @@ constexpr int stage_tiles(int NS, bool grad) { return (NS == 1 ? 2 : 1) * (grad 
 constexpr bool paired(int KP, int NS, int mode) { return KP * NS <= 256 && (mode == WALK_STATS || KP <= 128); }
 
 // S_LIES, T_LIES: read as bf16 rows in memory (V; X too for the statistics)
+//
+// Bound by the matrix instructions together with what does not fit beside them: 16 exponentials a lane and tile (a quarter of the rate of
+// the rest), the conversion of P to 16 bits, and the clock under their load (bf16 2048 x 1 000 000 x 128, sums of dX: 942 us, the
+// same instructions on rows of zeros 745 us).  A tile is 32 rows as the 32 x 32 instructions have it: 16 x 16 ones would read LDS twice as
+// often for the same products.  128 S rows a workgroup: their operand (KP / 16 registers of 4 a part) and the sums of 32 x KP a wave
+// fill the registers, so that a compute unit holds two workgroups up to 256 columns in all parts and one beyond; LDS serves four waves
+// with one stage.  Sizes and what they measured (matrix unit busy, of the SIMDs' cycles):
+//   bf16 2048 x 1 000 000 x 128: lse 0.66 ms (45 %), sums of dX 1.01 ms (60 %), dV finished 1.29 ms under the profiler (45 %)
+//   fp32 2048 x 26 744 x 200: lse 71 us (62 %), sums of dX 165 us (47 %), dV and db finished 266 us (38 %)
+// = 1.57 PFLOP in 2.6 ms for the bf16 step, where a large product of the library reaches 1206 TFLOP/s.
 template <int KP, int NS, int MODE, bool S_LIES, bool T_LIES>
 __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel(WalkParams p)
 {
@@ -986,7 +998,9 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
 // The statistics for few users, straight from V as it lies in memory: a wave takes 16 items at a time, its lanes 16 rows by four
 // pieces of 16 bytes, which are the A operands of the 16 x 16 instructions (fp32: 16x16x4, a piece feeds four of them; bf16: 16x16x32).
 // The order of the factors is the same in X's operand, so it does not matter.  V is read once for 16 UT users, the next tile's rows
-// are on their way while one is computed: HBM-bound.
+// are on their way while one is computed: HBM-bound (fp32, one user x 1 000 000 x 128: 512 MB in 100 us, 5.1 TB/s; a sum over as much by
+// the library 3.95 TB/s).  The first form, the walk after V had been put in its
+// order, took 1650 us for this call.
 struct DirectParams {
     const void *X, *V;
     const float *ibase;
@@ -1099,7 +1113,9 @@ __global__ __launch_bounds__(256, direct_resident(KP, UT, sizeof(T))) void direc
 
 // The same statistics from 4-bit operands: a lane of the instruction holds one block of 32 of a row and its scale, as it lies in
 // memory.  A wave keeps UT tiles of 32 users (B operand) and walks item tiles of 32, the next one's codes on their way; the bases are
-// the initial value of the sums.  Bound by the exponentials (v_exp_f32 at a quarter of the rate of the rest).
+// the initial value of the sums.  Bound by the exponentials (v_exp_f32 at a quarter of the rate of the rest) and the maxima and sums
+// beside them: 2048 x 125 000 x 128 in 63 us, 256 M exponentials at 26 us of issue, the vector unit busy in 88 % of the cycles.  Four user
+// tiles a wave: one item tile's loads and scales serve 128 users (the first form had one and took 145 us).
 struct MxWalkParams {
     const uint8_t *xc, *xs, *vc, *vs;
     const float *base;                 // ibase or null
@@ -1246,7 +1262,7 @@ __device__ __forceinline__ float dot_share<Mx>(const Targets &t, int64_t u, int6
 }
 
 // A workgroup a user: lse from the splits, then logp of the named items, 16 lanes a place (the score as one fp32 sum over the
-// factors).  Bound by the latency of its gathers.
+// factors).  Bound by the latency of its gathers (2048 users x 20 places, 200 columns: 9 us).
 template <typename T>
 __global__ __launch_bounds__(256) void targets_kernel(Targets t)
 {
@@ -1285,7 +1301,8 @@ __global__ __launch_bounds__(256) void targets_kernel(Targets t)
     }
 }
 
-// dX = scale (sum over the places of g v - G acc): four columns a thread
+// dX = scale (sum over the places of g v - G acc): four columns a thread, so that a user's row of V is read in long pieces.  Bound by the
+// splits' sums and the gathers of V (2048 x 200, 20 places, 16 splits: 16 us, 46 MB).
 struct JoinDx {
     const float *acc, *G;
     const void *V;
@@ -1331,7 +1348,8 @@ __device__ __forceinline__ void join_dx(const JoinDx &p, int64_t block)
 template <typename T>
 __global__ __launch_bounds__(256) void join_dx_kernel(JoinDx p) { join_dx<T>(p, blockIdx.x); }
 
-// dV and db where the walk was split: the splits' sums of 64 items, then the same last steps.  The first x.blocks workgroups do dX.
+// dV and db where the walk was split (few items, many users): the splits' sums of 64 items, then the same last steps.  The first x.blocks
+// workgroups do dX: one launch for both, since each is a few microseconds.  Latency-bound.
 template <typename T, int KP>
 __global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, const float *acc_b, int splits, int64_t s_padded, Finish f)
 {
@@ -1393,7 +1411,8 @@ struct Pieces {
 };
 
 // Splits of the T axis: the count with the shortest plan, in stages: rounds of resident workgroups times (a split's stages + what a
-// workgroup costs besides), plus what joining costs where there is more than one.
+// workgroup costs besides, about four), plus what joining costs where there is more than one.  2048 users x 26 744 items leave 16
+// workgroups without a split of dX and take 16 splits; dV's 209 workgroups take none, since five (two rounds and a join) cost more.
 struct Split { int count, per; };
 
 Split split_plan(int64_t s_blocks, int64_t t_tiles, int unit, int64_t resident, double join)
@@ -1527,7 +1546,8 @@ struct BackwardPlan {
     Split split_x, split_v;
 };
 
-// Places are dealt into buckets where the workgroups' looking through all of them would take longer than the dealing.
+// Places are dealt into buckets where the workgroups' looking through all of them takes longer than the dealing: with 524 288 places and
+// 100 000 items dV takes 757 us dealt and 1056 us as they are, with 40 960 and 26 744 items 272 and 264 us.
 bool deals(const ifr_catalogue &c, int64_t m, bool items) { return items && c.n * m >= DEAL_FROM && c.n * m < (int64_t)1 << 31 && c.n_items >= 16 * S_ROWS; }
 
 BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx, bool dv, bool db, bool lies)

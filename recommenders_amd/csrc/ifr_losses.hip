@@ -113,7 +113,8 @@ __device__ __forceinline__ void preference_of(const ifr_preference &p, float h, 
 
 }  // namespace
 
-// A group of threads a pair: the sums of both slates in 64 bits (without a reference the two are large and near each other), the loss, and
+// A group of threads a pair (16 384 pairs of 500 + 1000 with masks and a reference, 319 MB: 77 us, 4.1 TB/s; 64 pairs of 10 + 10: 8 us under the
+// profiler, all latency): the sums of both slates in 64 bits (without a reference the two are large and near each other), the loss, and
 // the gradient, which is one number per slate.
 template <int GROUP>
 __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP) void preference_kernel(ifr_preference p)
@@ -266,6 +267,8 @@ __global__ __launch_bounds__(256) void policy_count_kernel(ifr_policy p, int64_t
     if (threadIdx.x == 0) part[blockIdx.x] = total;
 }
 
+// A group of threads a row; the count of the row's places comes first where the scale needs it (the mask alone is read twice, from the caches).
+// 4096 rows of 8191, 570 MB: 133 us, 4.3 TB/s, where a copy reaches 4.73; before it 7.5 us for the count of the batch's places.
 template <int GROUP>
 __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP) void policy_kernel(ifr_policy p, const int64_t *part, int n_part, float hi, float lo)
 {
