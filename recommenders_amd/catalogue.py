@@ -201,8 +201,8 @@ def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, c
 class CatalogueOps:
     """The catalogue operators of `HipScorer` (engine.py), which supplies `_lib`, `_h`, `device` and `_check`."""
 
-    def _workspace(self, fn, key, *args):
-        """(workspace, bytes) of a call; `key`: the sizes its length depends on, remembered."""
+    def _workspace(self, like, fn, key, *args):
+        """(workspace where `like` lies, bytes) of a call; `key`: the sizes its length depends on, remembered."""
         import torch
         known = self.__dict__.setdefault("_workspace_bytes", {})
         need = known.get(key)
@@ -213,7 +213,7 @@ class CatalogueOps:
             if len(known) >= 256:
                 known.clear()
             known[key] = need
-        return torch.empty(max(1, need), dtype=torch.uint8, device=self.device), need
+        return like.new_empty(max(1, need), dtype=torch.uint8), need
 
     def _stream_of(self):
         """The current stream's handle (the call behind torch.cuda.current_stream, without the object around it)."""
@@ -230,8 +230,8 @@ class CatalogueOps:
         if k < 1:
             raise ValueError("X must have at least one column")
         kb = (k + 31) // 32
-        codes = torch.empty((n, 16 * kb), dtype=torch.uint8, device=self.device)
-        scales = torch.empty((n, kb), dtype=torch.uint8, device=self.device)
+        codes = X.new_empty((n, 16 * kb), dtype=torch.uint8)
+        scales = X.new_empty((n, kb), dtype=torch.uint8)
         self._check(self._lib.ifr_mxfp4_quantize(self._h, _ptr(X), F32 if X.dtype == torch.float32 else BF16, n, k, ld,
                                                  _ptr(codes), _ptr(scales), self._stream_of()))
         return MxFp4Matrix._of(codes, scales, k)
@@ -241,16 +241,15 @@ class CatalogueOps:
         import torch
         if not isinstance(q, MxFp4Matrix) or q.device != self.device:
             raise ValueError(f"dequantize_mxfp4 takes an MxFp4Matrix on {self.device}")
-        out, ld = self._out(out, q.shape, torch.float32)
+        out, ld = self._out(out, q.shape, torch.float32, q.codes)
         self._check(self._lib.ifr_mxfp4_dequantize(self._h, _ptr(q.codes), _ptr(q.scales), q.shape[0], q.k, _ptr(out), ld,
                                                    self._stream_of()))
         return out
 
-    def _out(self, out, shape, dtype):
+    def _out(self, out, shape, dtype, like):
         """(output, row stride)"""
-        import torch
         if out is None:
-            return torch.empty(shape, dtype=dtype, device=self.device), shape[1]
+            return like.new_empty(shape, dtype=dtype), shape[1]
         if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != self.device or (out.numel() and (
                 out.stride(1) != 1 and out.shape[1] > 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1])):
             raise ValueError(f"out must be {_name(dtype)} {list(shape)} on {self.device} with contiguous rows")
@@ -273,7 +272,7 @@ class CatalogueOps:
             raise TypeError("score_mxfp4 writes float32 or bfloat16")
         n, n_items = X.shape[0], V.shape[0]
         ubase, ibase = _vector(ubase, "ubase", n, self.device), _vector(ibase, "ibase", n_items, self.device)
-        out, ld = self._out(out, (n, n_items), dtype)
+        out, ld = self._out(out, (n, n_items), dtype, V.codes)
         self._check(self._lib.ifr_mxfp4_scores(self._h, _ptr(X.codes), _ptr(X.scales), n, _ptr(V.codes), _ptr(V.scales), n_items, X.k, _ptr(ubase),
                                                _ptr(ibase), _ptr(out), F32 if dtype == torch.float32 else BF16, ld, self._stream_of()))
         return out
@@ -296,9 +295,8 @@ class CatalogueOps:
         (X, ldx), (V, ldv), (ids, ld_ids), ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
         n, m = ids.shape
         c = self._catalogue(X, ldx, V, ldv, ibase, scale)
-        logp = torch.empty((n, m), dtype=torch.float32, device=self.device)
-        lse = torch.empty((n,), dtype=torch.float32, device=self.device)
-        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_workspace, (c.n, c.n_items, c.k, c.dtype), ctypes.byref(c))
+        logp, lse = ids.new_empty((n, m), dtype=torch.float32), ids.new_empty(n, dtype=torch.float32)
+        ws, need = self._workspace(ids, self._lib.ifr_catalogue_logprob_workspace, (c.n, c.n_items, c.k, c.dtype), ctypes.byref(c))
         self._check(self._lib.ifr_catalogue_logprob(self._h, ctypes.byref(c), _ptr(ids), m, ld_ids, _ptr(logp), max(m, 1), _ptr(lse),
                                                     _ptr(ws), need, self._stream_of()))
         return logp, lse
@@ -318,12 +316,11 @@ class CatalogueOps:
         if lse is None:
             raise TypeError("lse must be a torch tensor")
         lse = _vector(lse, "lse", n, self.device)
-        empty = torch.empty if n else torch.zeros
-        dX = empty((n, X.shape[1]), dtype=X.dtype, device=self.device) if "X" in want else None
-        dV = empty((V.shape[0], V.shape[1]), dtype=V.dtype, device=self.device) if "V" in want else None
-        db = empty((V.shape[0],), dtype=torch.float32, device=self.device) if "ibase" in want and ibase is not None else None
+        dX = X.new_empty(X.shape) if "X" in want else None
+        dV = (V.new_empty if n else V.new_zeros)(V.shape) if "V" in want else None
+        db = (ibase.new_empty if n else ibase.new_zeros)(V.shape[0]) if "ibase" in want and ibase is not None else None
         c = self._catalogue(X, ldx, V, ldv, ibase, scale)
-        ws, need = self._workspace(self._lib.ifr_catalogue_logprob_backward_workspace, (c.n, c.n_items, c.k, c.dtype, m, dX is None, dV is None, db is None),
+        ws, need = self._workspace(ids, self._lib.ifr_catalogue_logprob_backward_workspace, (c.n, c.n_items, c.k, c.dtype, m, dX is None, dV is None, db is None),
                                    ctypes.byref(c), m, int(dX is not None), int(dV is not None), int(db is not None))
         k = X.shape[1]
         self._check(self._lib.ifr_catalogue_logprob_backward(self._h, ctypes.byref(c), _ptr(ids), m, ld_ids, _ptr(lse), _ptr(dlogp), ld_dlogp, _ptr(dX), k,
@@ -359,10 +356,10 @@ class CatalogueOps:
         (x, old, ref, m), advantages, weight = check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef, reduction, self.device)
         n, width = x[0].shape
         loss, kl, d_logp = x[0].new_empty(n), None if ref_logp is None else x[0].new_empty(n), x[0].new_empty((n, width))
-        clipped = torch.empty(n, dtype=torch.int32, device=self.device)
+        clipped = x[0].new_empty(n, dtype=torch.int32)
         p = _lib.Policy(n, width, _REDUCTIONS[reduction], x[0].data_ptr(), old[0].data_ptr(), _ptr(ref[0]), advantages.data_ptr(), _ptr(weight), _ptr(m[0]),
                         loss.data_ptr(), _ptr(kl), clipped.data_ptr(), d_logp.data_ptr(), x[1], old[1], ref[1], m[1], width, float(clip_low), float(clip_high),
                         float(kl_coef))
-        ws, need = (None, 0) if mask is None or reduction != "batch" else self._workspace(self._lib.ifr_policy_loss_workspace, "policy", ctypes.byref(p))
+        ws, need = (None, 0) if mask is None or reduction != "batch" else self._workspace(clipped, self._lib.ifr_policy_loss_workspace, "policy", ctypes.byref(p))
         self._check(self._lib.ifr_policy_loss(self._h, ctypes.byref(p), _ptr(ws), need, self._stream_of()))
         return PolicyLoss(loss, kl, clipped, d_logp)
