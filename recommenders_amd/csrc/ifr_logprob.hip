@@ -443,7 +443,10 @@ __device__ __forceinline__ void load4(const T *row, int c, int k, bool vec, floa
             v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
         }
     } else {
-        for (int j = 0; j < 4; ++j) v[j] = c + j < k ? as_f32(row[c + j]) : 0.f;
+        for (int j = 0; j < 4; ++j) {                 // no branch: the last column again behind it
+            const float a = as_f32(row[min(c + j, k - 1)]);
+            v[j] = c + j < k ? a : 0.f;
+        }
     }
 }
 
@@ -606,9 +609,9 @@ __device__ __forceinline__ void add_places(const Finish &f, float *rows, float *
     }
     if (in && cur >= 0) flush();
     __syncthreads();
-    for (int g = 0; g < GROUPS; ++g) {
+    const int used = (to - from + part - 1) / part;   // groups that had places
+    for (int g = 0; g < used; ++g) {
         const int item = aside_item[g];
-        if (item < 0) continue;
         for (int c = tid; c < KP; c += 256) rows[item * KP + c] += aside[g * KP + c];
         if (tid == 0) row_b[item] += aside[GROUPS * KP + g];
     }
