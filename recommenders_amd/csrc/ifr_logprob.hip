@@ -453,21 +453,23 @@ __device__ __forceinline__ void load4(const T *row, int c, int k, bool vec, floa
 // The last steps of dV: rows of sums lie in LDS as rows[local][KP], 64 at a time; g x of every place that names one of the items is added,
 // the rows are scaled, rounded and stored.  Nothing depends on scheduling.
 //
-// find_places: each wave looks through a quarter of the places and lists those that name one of `count` (at most 128) items, until its
-// list is full or the quarter is done (`step` keeps where it is); the lists are sorted by item.  Returns how many, `more`: come again.
+// find_places: each wave looks through a quarter of the places [from, to) -- those of the users that the workgroup walked -- and lists
+// those that name one of `count` (at most 128) items, until its list is full or the quarter is done (`step` keeps where it is); the
+// lists are sorted by item.  Returns how many, `more`: come again.
 template <int KP>
-__device__ __forceinline__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t *item_of, int64_t i0, int count, int64_t &step, bool &more)
+__device__ __forceinline__ int find_places(const Finish &f, uint32_t *list, int *counts, uint8_t *item_of, int64_t i0, int count, int64_t from, int64_t to,
+                                           int64_t &step, bool &more)
 {
     constexpr int LIST = list_length(KP), CAP = LIST / 4, EACH = CAP / 64;
     uint32_t *order = list + 2 * LIST;
     float *gs = (float *)(list + LIST);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int64_t begin = 0, steps = (f.n_places + 64 * EACH - 1) / (64 * EACH);     // of a wave, over all places or the bucket's
     if (f.place_of) {                                 // what lies beside them in the first and last step names other items
         const int64_t b = i0 / f.bucket_items;
-        begin = f.bounds[b] / (64 * EACH);
-        steps = (f.bounds[b + 1] + 64 * EACH - 1) / (64 * EACH) - begin;
+        from = f.bounds[b] / (64 * EACH) * (64 * EACH);
+        to = (f.bounds[b + 1] + 64 * EACH - 1) / (64 * EACH) * (64 * EACH);
     }
+    const int64_t begin = from / (64 * EACH), steps = (to + 64 * EACH - 1) / (64 * EACH) - begin;
     const int64_t end = begin + steps * (wave + 1) / 4;
     if (step < 0) step = begin + steps * wave / 4;
     int held = 0;
@@ -486,9 +488,14 @@ __device__ __forceinline__ int find_places(const Finish &f, uint32_t *list, int 
     while (step < end) {
         if (step + 1 < end) load(step + 1, next);
         int mine = 0;
+        const bool edge = step * 64 * EACH < from || (step + 1) * 64 * EACH > to;
 #pragma unroll
         for (int q = 0; q < EACH; ++q) {
             if (id[q] >= f.n_items) id[q] = -1;       // behind the catalogue: no row takes it
+            if (edge) {
+                const int64_t at = step * 64 * EACH + (EACH >= 4 ? (q >> 2) * 256 + lane * 4 + (q & 3) : q * 64 + lane);
+                if (at < from || at >= to) id[q] = -1;
+            }
             mine += (uint64_t)((int64_t)id[q] - i0) < (uint64_t)count;
         }
         if (__ballot(mine)) {
@@ -618,24 +625,27 @@ __device__ __forceinline__ void add_places(const Finish &f, float *rows, float *
     __syncthreads();
 }
 
+// four columns of a row of dV
+template <typename T>
+__device__ __forceinline__ void store4(const Finish &f, int64_t i, int c, float4 v)
+{
+    if (!f.dV || i >= f.n_items || c >= f.k) return;
+    T o[4] = {(T)(f.scale * v.x), (T)(f.scale * v.y), (T)(f.scale * v.z), (T)(f.scale * v.w)};
+    T *to = (T *)f.dV + i * f.ld_dv + c;
+    if (f.vec_dv) {
+        __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), o, 4 * sizeof(T));
+    } else {
+        for (int j = 0; j < 4; ++j)
+            if (c + j < f.k) to[j] = o[j];
+    }
+}
+
 template <typename T, int KP>
 __device__ __forceinline__ void store_rows(const Finish &f, const float *rows, const float *row_b, int64_t i0)
 {
-    if (f.dV) {
-        T *out = (T *)f.dV;
-        for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) {
-            const int r = i / (KP / 4), c = (i - r * (KP / 4)) * 4;
-            if (i0 + r >= f.n_items || c >= f.k) continue;
-            const float4 v = *(const float4 *)(rows + r * KP + c);
-            T o[4] = {(T)(f.scale * v.x), (T)(f.scale * v.y), (T)(f.scale * v.z), (T)(f.scale * v.w)};
-            T *to = out + (i0 + r) * f.ld_dv + c;
-            if (f.vec_dv) {
-                __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), o, 4 * sizeof(T));
-            } else {
-                for (int j = 0; j < 4; ++j)
-                    if (c + j < f.k) to[j] = o[j];
-            }
-        }
+    for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) {
+        const int r = i / (KP / 4), c = (i - r * (KP / 4)) * 4;
+        store4<T>(f, i0 + r, c, *(const float4 *)(rows + r * KP + c));
     }
     if (f.db)
         for (int r = threadIdx.x; r < 64; r += 256)
@@ -930,15 +940,15 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
     }
     const float unit = NS == 2 ? ldexpf(1.f, (MODE == WALK_USERS ? -15 : 0) - ref) : 1.f;
     b_sum += __shfl_xor(b_sum, 32);
-    if (p.out_acc) {
-        if (p.out_b && h == 0) p.out_b[at] = b_sum;
+    if (MODE == WALK_USERS) {
         for (int kb = 0; kb < KP / 32; ++kb)
             for (int q = 0; q < 4; ++q)
                 *(float4 *)(p.out_acc + at * KP + kb * 32 + 8 * q + 4 * h) =
                     make_float4(acc[kb][4 * q] * unit, acc[kb][4 * q + 1] * unit, acc[kb][4 * q + 2] * unit, acc[kb][4 * q + 3] * unit);
         return;
     }
-    // one split: the rows are finished here, 64 a time (waves 0 and 1, then 2 and 3), their sums in the first stage's memory
+    // dV: the places of the users walked are added here, to 64 rows a time (waves 0 and 1, then 2 and 3) whose sums lie in the first stage's
+    // memory; one split finishes the rows, more leave parts of the gradient for join_kernel
     __shared__ float row_b[64], aside[aside_floats(KP)];
     __shared__ int counts[4], aside_item[32];
     static_assert(MODE == WALK_STATS || STAGE * 16 >= 64 * KP * 4, "a stage holds 64 rows of sums");
@@ -948,7 +958,8 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
     const int64_t i0 = (int64_t)s_block * S_ROWS;
     const Finish &f = p.f;
     __syncthreads();
-    const bool any = f.n_places > 0 && (!f.named || f.named[i0 >> 6] || f.named[(i0 >> 6) + 1]);
+    const int64_t from_place = first * 32ll * f.m, to_place = min(last * 32ll * f.m, f.n_places);
+    const bool any = from_place < to_place && (!f.named || f.named[i0 >> 6] || f.named[(i0 >> 6) + 1]);
     // the places of all 128 items are found at once; where the lists do not hold them, those of 64 at a time in as many rounds as it takes
     bool find = any, at_once = true, more = false, fresh = true;
     int64_t step = -1;
@@ -969,7 +980,7 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             fresh = false;
         }
         if (find) {
-            total = find_places<KP>(f, list, counts, (uint8_t *)aside, at_once ? i0 : i0 + half * 64, at_once ? 128 : 64, step, more);
+            total = find_places<KP>(f, list, counts, (uint8_t *)aside, at_once ? i0 : i0 + half * 64, at_once ? 128 : 64, from_place, to_place, step, more);
             if (at_once && more) {
                 at_once = false;
                 step = -1;
@@ -990,7 +1001,13 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             find = true;
             continue;
         }
-        store_rows<T, KP>(f, rows, row_b, i0 + half * 64);
+        if (p.out_acc) {
+            const int64_t to_row = (int64_t)split * p.s_padded + i0 + half * 64;
+            for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) ((float4 *)(p.out_acc + to_row * KP))[i] = ((const float4 *)rows)[i];
+            if (p.out_b && threadIdx.x < 64) p.out_b[to_row + threadIdx.x] = row_b[threadIdx.x];
+        } else {
+            store_rows<T, KP>(f, rows, row_b, i0 + half * 64);
+        }
         ++half;
         fresh = true;
         find = any && !at_once;
@@ -1315,7 +1332,7 @@ struct JoinDx {
     int64_t s_padded, ldv, n_items, m, ld_ids, ld_dlogp, n, ld_dx;
     int splits, KP, k, vec_v;
     float scale;
-    int64_t blocks;                    // workgroups it takes
+    int64_t blocks;                    // workgroups it takes (none without dX)
 };
 
 template <typename T>
@@ -1351,42 +1368,30 @@ __device__ __forceinline__ void join_dx(const JoinDx &p, int64_t block)
 template <typename T>
 __global__ __launch_bounds__(256) void join_dx_kernel(JoinDx p) { join_dx<T>(p, blockIdx.x); }
 
-// dV and db where the walk was split (few items, many users): the splits' sums of 64 items, then the same last steps.  The first x.blocks
+// dV and db where the walk was split (few items, many users): the sum of the splits' parts, four columns a thread.  The first x.blocks
 // workgroups do dX: one launch for both, since each is a few microseconds.  Latency-bound.
-template <typename T, int KP>
-__global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, const float *acc_b, int splits, int64_t s_padded, Finish f)
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(JoinDx x, const float *acc, const float *acc_b, int splits, int64_t s_padded, int KP, Finish f)
 {
-    __shared__ float rows[64 * KP];
-    __shared__ uint32_t list[list_length(KP) * 3];
-    __shared__ float row_b[64], aside[aside_floats(KP)];
-    __shared__ int counts[4], aside_item[32];
     if (blockIdx.x < x.blocks) {
         join_dx<T>(x, blockIdx.x);
         return;
     }
-    const int64_t i0 = (blockIdx.x - x.blocks) * 64;
-    for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int64_t at = (blockIdx.x - x.blocks) * 256ll + threadIdx.x, i = at / (KP / 4);
+    const int c = (int)(at - i * (KP / 4)) * 4;
+    if (i >= f.n_items) return;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int q = 0; q < splits; ++q) {
-            const float4 v = ((const float4 *)(acc + ((int64_t)q * s_padded + i0) * KP))[i];
-            a.x -= v.x; a.y -= v.y; a.z -= v.z; a.w -= v.w;
-        }
-        ((float4 *)rows)[i] = a;
+    for (int q = 0; q < splits; ++q) {
+        const float4 v = *(const float4 *)(acc + ((int64_t)q * s_padded + i) * KP + c);
+        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
-    if (threadIdx.x < 64) {
+    store4<T>(f, i, c, a);
+    if (c == 0 && f.db) {
         float b = 0.f;
-        if (acc_b)
-            for (int q = 0; q < splits; ++q) b -= acc_b[(int64_t)q * s_padded + i0 + threadIdx.x];
-        row_b[threadIdx.x] = b;
+        for (int q = 0; q < splits; ++q) b += acc_b[(int64_t)q * s_padded + i];
+        f.db[i] = f.scale * b;
     }
-    __syncthreads();
-    int64_t step = -1;
-    for (bool more = f.n_places > 0 && (!f.named || f.named[i0 >> 6]); more;) {
-        const int total = find_places<KP>(f, list, counts, (uint8_t *)aside, i0, 64, step, more);
-        if (total) add_places<T, KP>(f, rows, row_b, list, aside, aside_item, 0, 0, total);
-    }
-    store_rows<T, KP>(f, rows, row_b, i0);
 }
 
 // ---------------------------------------------------------------------------- launches
@@ -1418,14 +1423,14 @@ struct Pieces {
 // workgroups without a split of dX and take 16 splits; dV's 209 workgroups take none, since five (two rounds and a join) cost more.
 struct Split { int count, per; };
 
-Split split_plan(int64_t s_blocks, int64_t t_tiles, int unit, int64_t resident, double join)
+Split split_plan(int64_t s_blocks, int64_t t_tiles, int unit, int64_t resident, double join, double places = 0.0)
 {
     const int64_t stages = (t_tiles + unit - 1) / unit;
     int64_t best = 1;
     double best_cost = 0;
     for (int64_t c = 1; c <= stages && c <= 4096; c = c < 16 ? c + 1 : c + c / 8) {
         const int64_t per = (stages + c - 1) / c;
-        const double cost = (double)((s_blocks * c + resident - 1) / resident) * ((double)per + 4.0) + (c > 1 ? join * (double)c : 0.0);
+        const double cost = (double)((s_blocks * c + resident - 1) / resident) * ((double)per + 4.0 + places / (double)(s_blocks * c)) + (c > 1 ? join * (double)c : 0.0);
         if (c == 1 || cost < best_cost) { best = c; best_cost = cost; }
     }
     Split s;
@@ -1567,7 +1572,14 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
     p.g_exp = w.take<int>(NS == 2 ? p.x.tiles : 0);
     p.places_padded = items ? up(c.n * m, CHUNK) : 0;
     p.places = w.take<int32_t>(p.places_padded);
-    if (deals(c, m, items)) {
+    // flags save the search where most groups of 64 items are not named; where the places are as many as the groups, none is saved
+    p.named = w.take<uint8_t>(p.places_padded && c.n_items > 64 * c.n * m ? up(p.v.padded / 64, 4) : 0);
+    const int resident = resident_blocks(KP, NS, WALK_USERS);
+    p.split_x = split_plan(p.x.padded / S_ROWS, p.v.tiles, stage_tiles(NS, true), resident, 0.05);
+    // a hundred places take about as long as a stage, and so do the parts of a hundred blocks, written and read again
+    const int64_t v_blocks = p.v.padded / S_ROWS;
+    p.split_v = split_plan(v_blocks, p.x.tiles, stage_tiles(NS, true), resident, 0.1 + 0.01 * (double)v_blocks, items ? 0.01 * (double)(c.n * m) : 0.0);
+    if (p.split_v.count == 1 && deals(c, m, items)) {
         Deal &d = p.deal;
         d.chunks = p.places_padded / CHUNK;
         d.n_items = c.n_items;
@@ -1578,11 +1590,6 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
         d.place_of = w.take<uint32_t>(p.places_padded);
         d.places = p.places;
     }
-    // flags save the search where most groups of 64 items are not named; where the places are as many as the groups, none is saved
-    p.named = w.take<uint8_t>(p.places_padded && c.n_items > 64 * c.n * m ? up(p.v.padded / 64, 4) : 0);
-    const int resident = resident_blocks(KP, NS, WALK_USERS);
-    p.split_x = split_plan(p.x.padded / S_ROWS, p.v.tiles, stage_tiles(NS, true), resident, 0.05);
-    p.split_v = split_plan(p.v.padded / S_ROWS, p.x.tiles, stage_tiles(NS, true), resident, 0.5);
     const bool parts = items && p.split_v.count > 1;
     p.acc_x = w.take<float>(dx ? p.split_x.count * p.x.padded * KP : 0);
     p.acc_v = w.take<float>(parts ? p.split_v.count * p.v.padded * KP : 0);
@@ -1725,7 +1732,7 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     pp.user_term = p.user_term; pp.G = p.G; pp.places = p.places; pp.named = p.named;
     pp.G_scaled = p.G_scaled; pp.g_exp = p.g_exp;
     launch_prepare<T>(pp, p.x.tiles, s);
-    const bool dealt = deals(c, m, items);
+    const bool dealt = p.deal.chunks > 0;
     if (dealt) {
         hipLaunchKernelGGL(deal_kernel<false>, dim3((uint32_t)p.deal.chunks), dim3(256), 0, s, p.deal);
         hipLaunchKernelGGL(deal_sums_kernel, dim3(1), dim3(1024), 0, s, p.deal);
@@ -1751,15 +1758,10 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
         if (NS == 2 || g.dibase) launch_walk<NS, WALK_ITEMS_BASE>(w, KP, s);
         else launch_walk<1, WALK_ITEMS>(w, KP, s);
     }
-    // the joins as one launch where dX's is short (its workgroups hold the memory of the other's)
-    const bool together = parts && x.blocks <= 512;
-    if (g.dX && !together) hipLaunchKernelGGL((join_dx_kernel<T>), dim3((uint32_t)x.blocks), dim3(256), 0, s, x);
+    if (g.dX && !parts) hipLaunchKernelGGL((join_dx_kernel<T>), dim3((uint32_t)x.blocks), dim3(256), 0, s, x);
     if (parts) {
-        if (!together) x.blocks = 0;
-        const dim3 grid((uint32_t)(x.blocks + p.v.padded / 64));
-#define IFR_JOIN(K) hipLaunchKernelGGL((join_kernel<T, K>), grid, dim3(256), 0, s, x, p.acc_v, p.acc_b, p.split_v.count, p.v.padded, w.f)
-        IFR_FOR_FACTORS(KP, IFR_JOIN)
-#undef IFR_JOIN
+        const dim3 grid((uint32_t)(x.blocks + (c.n_items * (KP / 4) + 255) / 256));
+        hipLaunchKernelGGL((join_kernel<T>), grid, dim3(256), 0, s, x, p.acc_v, p.acc_b, p.split_v.count, p.v.padded, KP, w.f);
     }
 }
 

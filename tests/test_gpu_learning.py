@@ -351,3 +351,36 @@ def test_c_refusals_of_sizes_and_factors(torch, sc):
            size(1e-31), size(1e31)]
     assert bad == [-1] * len(bad)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_captured_gradient_of_many_places_replays(torch, sc, dtype):
+    """Batches whose places are dealt into buckets: one graph, batches of many and of no places in turn, every replay the eager call's bits."""
+    n, items, k, m = 1100, 4096, 40, 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    X, V = ((torch.randn((r, k), generator=g, device="cuda") * .3).to(getattr(torch, dtype)) for r in (n, items))
+
+    def batch(lowest, highest):
+        ids = torch.randint(lowest, highest, (n, m), generator=g, device="cuda", dtype=torch.int32)
+        d = torch.randn((n, m), generator=g, device="cuda") / n
+        return ids, d, sc.catalogue_logprob(X, V, ids)[1]
+
+    held = [t.clone() for t in batch(-1, items)]
+    call = lambda ids, d, lse: sc.catalogue_logprob_backward(X, V, ids, lse, d)[:2]
+    call(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(*held)
+    # every item; 128 of the last ones alone; empty places alone; half of them empty; behind the catalogue too
+    for lowest, highest in ((0, items), (items - 128, items), (-1, 0), (-items, items), (0, 2 * items)):
+        fresh = batch(lowest, highest)
+        for t, f in zip(held, fresh):
+            t.copy_(f)
+        graph.replay()
+        want = call(*fresh)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(out, want))
+        if highest == 0:
+            assert not want[0].any() and not want[1].any()
