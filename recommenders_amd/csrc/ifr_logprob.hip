@@ -960,23 +960,43 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
     __syncthreads();
     const int64_t from_place = first * 32ll * f.m, to_place = min(last * 32ll * f.m, f.n_places);
     const bool any = from_place < to_place && (!f.named || f.named[i0 >> 6] || f.named[(i0 >> 6) + 1]);
+    auto lay = [&](int half) {                        // the sums of 64 items
+        __syncthreads();
+        if ((wave >> 1) == half) {
+            const int r = (wave & 1) * 32 + (lane & 31);
+            for (int kb = 0; kb < KP / 32; ++kb)
+                for (int q = 0; q < 4; ++q)
+                    *(float4 *)(rows + r * KP + kb * 32 + 8 * q + 4 * h) =
+                        make_float4(-acc[kb][4 * q] * unit, -acc[kb][4 * q + 1] * unit, -acc[kb][4 * q + 2] * unit, -acc[kb][4 * q + 3] * unit);
+            if (h == 0) row_b[r] = -b_sum;
+        }
+        __syncthreads();
+    };
+    auto leave = [&](int half) {
+        if (p.out_acc) {
+            const int64_t to_row = (int64_t)split * p.s_padded + i0 + half * 64;
+            for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) ((float4 *)(p.out_acc + to_row * KP))[i] = ((const float4 *)rows)[i];
+            if (p.out_b && threadIdx.x < 64) p.out_b[to_row + threadIdx.x] = row_b[threadIdx.x];
+        } else {
+            store_rows<T, KP>(f, rows, row_b, i0 + half * 64);
+        }
+    };
+    if (!any) {                                       // nothing to add: no register is put aside for it
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            lay(half);
+            leave(half);
+        }
+        return;
+    }
     // the places of all 128 items are found at once; where the lists do not hold them, those of 64 at a time in as many rounds as it takes
-    bool find = any, at_once = true, more = false, fresh = true;
+    bool find = true, at_once = true, more = false, fresh = true;
     int64_t step = -1;
     int total = 0, lower = 0;                         // of the sorted order: where the second half's items begin
 #pragma unroll 1
     for (int half = 0; half < 2;) {
         if (fresh) {
-            __syncthreads();
-            if ((wave >> 1) == half) {
-                const int r = (wave & 1) * 32 + (lane & 31);
-                for (int kb = 0; kb < KP / 32; ++kb)
-                    for (int q = 0; q < 4; ++q)
-                        *(float4 *)(rows + r * KP + kb * 32 + 8 * q + 4 * h) =
-                            make_float4(-acc[kb][4 * q] * unit, -acc[kb][4 * q + 1] * unit, -acc[kb][4 * q + 2] * unit, -acc[kb][4 * q + 3] * unit);
-                if (h == 0) row_b[r] = -b_sum;
-            }
-            __syncthreads();
+            lay(half);
             fresh = false;
         }
         if (find) {
@@ -1001,16 +1021,10 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             find = true;
             continue;
         }
-        if (p.out_acc) {
-            const int64_t to_row = (int64_t)split * p.s_padded + i0 + half * 64;
-            for (int i = threadIdx.x; i < 64 * KP / 4; i += 256) ((float4 *)(p.out_acc + to_row * KP))[i] = ((const float4 *)rows)[i];
-            if (p.out_b && threadIdx.x < 64) p.out_b[to_row + threadIdx.x] = row_b[threadIdx.x];
-        } else {
-            store_rows<T, KP>(f, rows, row_b, i0 + half * 64);
-        }
+        leave(half);
         ++half;
         fresh = true;
-        find = any && !at_once;
+        find = !at_once;
         step = -1;
     }
 }
