@@ -674,9 +674,9 @@ constexpr bool paired(int KP, int NS, int mode) { return KP * NS <= 256 && (mode
 // often for the same products.  128 S rows a workgroup: their operand (KP / 16 registers of 4 a part) and the sums of 32 x KP a wave
 // fill the registers, so that a compute unit holds two workgroups up to 256 columns in all parts and one beyond; LDS serves four waves
 // with one stage.  Sizes and what they measured (matrix unit busy, of the SIMDs' cycles):
-//   bf16 2048 x 1 000 000 x 128: lse 0.66 ms (45 %), sums of dX 1.01 ms (60 %), dV finished 1.29 ms under the profiler (45 %)
-//   fp32 2048 x 26 744 x 200: lse 71 us (62 %), sums of dX 165 us (47 %), dV and db finished 266 us (38 %)
-// = 1.57 PFLOP in 2.6 ms for the bf16 step, where a large product of the library reaches 1206 TFLOP/s.
+//   bf16 2048 x 1 000 000 x 128: lse 0.70 ms (45 %), sums of dX 1.02 ms (62 %), dV finished 1.37 ms (44 %), all under the profiler
+//   fp32 2048 x 26 744 x 200: lse 73 us (62 %), sums of dX 170 us (47 %), dV and db finished 259 us (38 %)
+// = 2.6 PFLOP with the recomputed scores in 2.6 - 2.8 ms for the bf16 step, where a large product of the library reaches 1206 TFLOP/s.
 template <int KP, int NS, int MODE, bool S_LIES, bool T_LIES>
 __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel(WalkParams p)
 {
@@ -1569,7 +1569,7 @@ struct BackwardPlan {
 };
 
 // Places are dealt into buckets where the workgroups' looking through all of them takes longer than the dealing: with 524 288 places and
-// 100 000 items dV takes 757 us dealt and 1056 us as they are, with 40 960 and 26 744 items 272 and 264 us.
+// 100 000 items dV takes 743 us dealt and 1056 us as they are, with 40 960 and 26 744 items 272 and 264 us.
 bool deals(const ifr_catalogue &c, int64_t m, bool items) { return items && c.n * m >= DEAL_FROM && c.n * m < (int64_t)1 << 31 && c.n_items >= 16 * S_ROWS; }
 
 BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx, bool dv, bool db, bool lies)
