@@ -681,6 +681,7 @@ template <int KP, int NS, int MODE, bool S_LIES, bool T_LIES>
 __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel(WalkParams p)
 {
     typedef typename std::conditional<NS == 2, float, __bf16>::type T;
+    typedef typename std::conditional<NS == 2, _Float16, __bf16>::type E;
     constexpr int STEPS = KP / 16;
     constexpr int PART = STEPS * 64;                  // 16-byte pieces of a part of a tile
     constexpr bool GRAD = MODE != WALK_STATS, PAIRED = paired(KP, NS, MODE);
@@ -815,8 +816,10 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
                 far |= up[sub] < -20;
             }
         }
-        // probabilities of a tile (times G for the items' side), as the operand of the second product
-        struct Operand { uint4 part[NS][2]; };
+        // probabilities of a tile (times G for the items' side), as the operand of the second product: two parts in either type, since a
+        // gradient is the difference of this product and the named items' rows, and only what P keeps is left of a user who is nearly
+        // sure of its item.  bf16: hi + lo is off by at most 2^-16 of P, and near 1 by 2^-8 of 1 - P (one part lost such rows whole)
+        struct Operand { uint4 part[2][2]; };
         auto probabilities = [&](const v16f &d, int sub) {
             const float add = s_term + (float)up[sub];
             float P[16];
@@ -841,25 +844,18 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             Operand o;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                if (NS == 1) {
-                    b8 v;
+                typename std::conditional<NS == 1, b8, h8>::type hi, lo;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = (__bf16)P[8 * e + j];
-                    o.part[0][e] = __builtin_bit_cast(uint4, v);
-                } else {
-                    h8 hi, lo;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        hi[j] = (_Float16)P[8 * e + j];
-                        lo[j] = (_Float16)(P[8 * e + j] - (float)hi[j]);
-                    }
-                    o.part[0][e] = __builtin_bit_cast(uint4, hi);
-                    o.part[NS - 1][e] = __builtin_bit_cast(uint4, lo);
+                for (int j = 0; j < 8; ++j) {
+                    hi[j] = (E)P[8 * e + j];
+                    lo[j] = (E)(P[8 * e + j] - (float)hi[j]);
                 }
+                o.part[0][e] = __builtin_bit_cast(uint4, hi);
+                o.part[1][e] = __builtin_bit_cast(uint4, lo);
             }
             return o;
         };
-        // their product with the tile's rows
+        // their product with the tile's rows: hi hi, hi lo and, where the rows have two parts, lo hi
         auto add_product = [&](const uint4 *l1, const Operand &o) {
 #pragma unroll
             for (int kb = 0; kb < KP / 32; kb += ABREAST)
@@ -875,7 +871,7 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
                                 a[j][q] = turned(l2 + at2, l2 + at2_high);
                             }
 #pragma unroll
-                    for (int q = 0; q < 2 * NS - 1; ++q)
+                    for (int q = 0; q < NS + 1; ++q)
 #pragma unroll
                         for (int j = 0; j < ABREAST; ++j)
                             if (kb + j < KP / 32) acc[kb + j] = product<NS>(a[j][q >> 1], o.part[q & 1][e], acc[kb + j]);
