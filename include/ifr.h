@@ -407,8 +407,9 @@ int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *i
  *   dX = scale dz V, dV = scale dz^T X (both of `dtype`, rows ld_dx / ld_dv apart), dibase = scale sum_u dz (fp32).
  * Any of the three may be NULL.  fp32 or bf16 operands.  No atomics: the same call gives the same bits.  A user who names no item
  * takes no part, whatever stands in its row.  A user whose lse is -inf (every item taken out) has no probabilities, and only its
- * targets' part of the gradient.  Probabilities (times G) enter the products with bf16 operands in two bf16 parts, off by at most 2^-16 of
- * themselves and by 2^-8 of their distance from 1. */
+ * targets' part of the gradient.  Probabilities (times G) enter the products in two parts: with bf16 operands
+ * off by at most 2^-16 of themselves and by 2^-8 of their distance from 1, with fp32 ones by 2^-22 of themselves or 2^-39 of the largest of
+ * the 32 neighbouring terms of a user's (an item's) sum. */
 int ifr_catalogue_logprob_backward_workspace(ifr_handle h, const ifr_catalogue *c, int64_t m, int want_dx, int want_dv, int want_dibase,
                                              int64_t *bytes);
 int ifr_catalogue_logprob_backward(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids,

@@ -85,7 +85,7 @@ struct PrepParams {
     const void *V, *X;
     int64_t ldv, ldx, n_items, n, v_blocks, v_padded, x_padded;
     int k, KP;
-    int *v_exp, *x_exp, *g_exp;
+    int *v_exp, *x_exp;
     uint4 *v_frag, *x_frag;
     const float *ibase;
     // terms of split operands are powers of two, to be added to the exponent; those of bf16 operands are in units of <x, v>, to begin
@@ -96,7 +96,7 @@ struct PrepParams {
     const float *lse, *dlogp;
     const int32_t *ids;
     int64_t m, ld_ids, ld_dlogp, places_padded;
-    float *user_term, *G, *G_scaled;   // G: the sum of a user's upstream gradients; split: also times 2^g_exp
+    float *user_term, *G;              // G: the sum of a user's upstream gradients
     int32_t *places;                   // the items named in (user, place) order, -1 behind the last place; null: not wanted
     uint8_t *named;                    // [items / 64], cleared before: set where an item is named; or null
 };
@@ -202,20 +202,13 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
         return;
     }
     if (!p.lse) return;
-    if (threadIdx.x < 64) {
-        const int64_t u = r0 + (threadIdx.x & 31);
+    if (threadIdx.x < 32) {
+        const int64_t u = r0 + threadIdx.x;
         float g = 0.f;
-        for (int q = 0; q < 8; ++q) g += sums[(threadIdx.x & 31) * 8 + q];
-        float top = fabsf(g) < INFINITY ? fabsf(g) : 0.f;
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const int e = split_exponent(top);
-        if (threadIdx.x < 32) {
-            p.G[u] = g;
-            if (NS == 2) p.G_scaled[u] = ldexpf(g, e);
-            if (NS == 2 && threadIdx.x == 0) p.g_exp[at] = e;
-            // no probabilities where lse is -inf, and none that matter where no item is named: every exponential is 0
-            p.user_term[u] = u < p.n && holds[threadIdx.x] && p.lse[u] != -INFINITY ? p.lse[u] * p.lse_unit : -INFINITY;
-        }
+        for (int q = 0; q < 8; ++q) g += sums[threadIdx.x * 8 + q];
+        p.G[u] = g;
+        // no probabilities where lse is -inf, and none that matter where no item is named: every exponential is 0
+        p.user_term[u] = u < p.n && holds[threadIdx.x] && p.lse[u] != -INFINITY ? p.lse[u] * p.lse_unit : -INFINITY;
     }
     if (p.places) {
         const int64_t all = p.n * p.m;
@@ -365,8 +358,8 @@ struct WalkParams {
     const __bf16 *s_rows, *t_rows;
     int64_t s_ld, t_ld, s_n, t_n;
     const float *s_term, *t_term;      // item_term, user_term of prepare_kernel
-    const float *t_factor;             // WALK_ITEMS...: G (split: scaled by t_factor_exp)
-    const int *s_exp, *t_exp, *t_factor_exp;     // split operands: exponents of their tiles
+    const float *t_factor;             // WALK_ITEMS...: G
+    const int *s_exp, *t_exp;          // split operands: exponents of their tiles
     float c;                           // scale log2(e)
     int s_blocks, splits, t_tiles, tiles_per_split;
     int64_t s_padded;
@@ -721,7 +714,6 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
     v16f acc[GRAD ? KP / 32 : 1] = {};
     float m = -3.402823466e38f, sum = 0.f, b_sum = 0.f;
     const int first = split * p.tiles_per_split, last = min(first + p.tiles_per_split, p.t_tiles);
-    int ref = 280;                                    // exponent of acc (split operands), the least of the tiles so far
     // this lane's pieces of the first product's operand (even and odd steps), and its 8 bytes of the second's, which ds_read_tr turns
     // round: 16 lanes read four rows by 16 columns and get four rows of a column each (rows 0..7 and 8..15 of a step of 16)
     const int at1[2] = {piece_at(0, lane & 31, h), piece_at(1, lane & 31, h) - 64};
@@ -783,10 +775,13 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
     };
     // A stage's tiles (those behind the last row have terms of -inf and add nothing: no branch divides the code, so that the
     // exponentials of one tile go beside the matrix instructions of the next tile's scores and of the last one's sums).
-    auto compute = [&](const uint4 *lds, const float *terms, const int *t_exps, const int *f_exps) {
-        float c[SUB];
+    auto compute = [&](const uint4 *lds, const float *terms, const int *t_exps) {
+        float c[SUB], unit[SUB];
 #pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) c[sub] = NS == 2 ? fminf(ldexpf(p.c, -s_exp - t_exps[sub]), 3.402823466e38f) : p.c;
+        for (int sub = 0; sub < SUB; ++sub) {
+            c[sub] = NS == 2 ? fminf(ldexpf(p.c, -s_exp - t_exps[sub]), 3.402823466e38f) : p.c;
+            unit[sub] = NS == 2 ? ldexpf(1.f, -t_exps[sub]) : 1.f;
+        }
         if (MODE == WALK_STATS) {
 #pragma unroll 2
             for (int sub = 0; sub < SUB; ++sub) {
@@ -796,35 +791,17 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             }
             return;
         }
-        // split: what enters the second product is scaled to at most 2^15 (probabilities by 2^15, G P by G's exponent), which
-        // fp16 holds down to 2^-39 of that; tiles of T with a larger exponent than the reference take the difference off
-        // here, one with a smaller becomes the reference
-        int up[SUB] = {};
-        bool far = false;
-        if (NS == 2) {
-            int least = ref;
-#pragma unroll
-            for (int sub = 0; sub < SUB; ++sub) least = min(least, t_exps[sub] + (ITEMS ? f_exps[sub] : 0));
-            if (least < ref) {
-                const float f = ldexpf(1.f, least - ref);
-                for (int kb = 0; kb < KP / 32; ++kb) acc[kb] *= f;
-                ref = least;
-            }
-#pragma unroll
-            for (int sub = 0; sub < SUB; ++sub) {
-                up[sub] = (MODE == WALK_USERS ? 15 : 0) - (t_exps[sub] + (ITEMS ? f_exps[sub] : 0) - ref);
-                far |= up[sub] < -20;
-            }
-        }
         // probabilities of a tile (times G for the items' side), as the operand of the second product: two parts in either type, since a
         // gradient is the difference of this product and the named items' rows, and only what P keeps is left of a user who is nearly
         // sure of its item.  bf16: hi + lo is off by at most 2^-16 of P, and near 1 by 2^-8 of 1 - P (one part lost such rows whole)
-        struct Operand { uint4 part[2][2]; };
+        // fp32: 22 bits, or an absolute step of 2^-39 of the largest of a S row's 32 elements.  That power of two is the tile's and the row's
+        // own, taken off where the tile's product is added to the sums in fp32, so that neither an unlikely item nor one beside a user of
+        // large G loses bits
+        struct Operand { uint4 part[2][2]; float back; };
         auto probabilities = [&](const v16f &d, int sub) {
-            const float add = s_term + (float)up[sub];
             float P[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) P[r] = exp2_raw(NS == 2 ? d[r] + add : fmaf(d[r], c[sub], add));
+            for (int r = 0; r < 16; ++r) P[r] = exp2_raw(NS == 2 ? d[r] + s_term : fmaf(d[r], c[sub], s_term));
             if (ITEMS) {
                 {   // products rounded by themselves: dV has the same bits with and without db beside it
 #pragma clang fp contract(off)
@@ -838,10 +815,23 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
                     float b = 0.f;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) b += P[r];
-                    b_sum += NS == 2 ? (up[sub] < -20 ? 0.f : ldexpf(b, -f_exps[sub] - up[sub])) : b;
+                    b_sum += b;
                 }
             }
             Operand o;
+            o.back = 1.f;
+            if (NS == 2) {
+                // the S row's 32 elements (16 here, 16 in lane + or - 32) by the power of two that brings the largest to [2^14, 2^15)
+                float top = fabsf(P[0]);
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(P[r]));
+                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                const uint32_t field = max(max((uint32_t)both[0], (uint32_t)both[1]) >> 23, 15u);
+                const float up = __uint_as_float((268u - field) << 23);
+                o.back = __uint_as_float((field - 14u) << 23) * unit[sub];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) P[r] *= up;
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 typename std::conditional<NS == 1, b8, h8>::type hi, lo;
@@ -858,7 +848,8 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         // their product with the tile's rows: hi hi, hi lo and, where the rows have two parts, lo hi
         auto add_product = [&](const uint4 *l1, const Operand &o) {
 #pragma unroll
-            for (int kb = 0; kb < KP / 32; kb += ABREAST)
+            for (int kb = 0; kb < KP / 32; kb += ABREAST) {
+                v16f part[ABREAST] = {};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint4 a[ABREAST][NS];
@@ -874,8 +865,19 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
                     for (int q = 0; q < NS + 1; ++q)
 #pragma unroll
                         for (int j = 0; j < ABREAST; ++j)
-                            if (kb + j < KP / 32) acc[kb + j] = product<NS>(a[j][q >> 1], o.part[q & 1][e], acc[kb + j]);
+                            if (kb + j < KP / 32) {
+                                v16f &to = NS == 2 ? part[j] : acc[kb + j];
+                                to = product<NS>(a[j][q >> 1], o.part[q & 1][e], to);
+                            }
                 }
+                if (NS == 2) {
+#pragma unroll
+                    for (int j = 0; j < ABREAST; ++j)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (kb + j < KP / 32) acc[kb + j][r] = fmaf(part[j][r], o.back, acc[kb + j][r]);
+                }
+            }
         };
         v16f next = scores(lds, terms, c[0]);
 #pragma unroll
@@ -884,22 +886,6 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             if (sub + 1 < SUB) next = scores(lds + (sub + 1) * PART * NS, terms + (sub + 1) * 32, c[sub + 1 < SUB ? sub + 1 : 0]);
             add_product(lds + sub * PART * NS, probabilities(d, sub));
         }
-        if (MODE == WALK_ITEMS_BASE && NS == 2 && far) {
-            // tiles far below the reference (seldom): their sums for db from the probabilities as they are
-#pragma unroll 1
-            for (int sub = 0; sub < SUB; ++sub) {
-                if ((sub ? up[SUB - 1] : up[0]) >= -20) continue;
-                const v16f d = scores(lds + sub * PART * NS, terms + sub * 32, sub ? c[SUB - 1] : c[0]);
-                float b = 0.f;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float4 tg = *(const float4 *)(terms + SUB * 32 + sub * 32 + 8 * q + 4 * h);
-                    b = fmaf(exp2_raw(d[4 * q] + s_term), tg.x, b); b = fmaf(exp2_raw(d[4 * q + 1] + s_term), tg.y, b);
-                    b = fmaf(exp2_raw(d[4 * q + 2] + s_term), tg.z, b); b = fmaf(exp2_raw(d[4 * q + 3] + s_term), tg.w, b);
-                }
-                b_sum += ldexpf(b, -(sub ? f_exps[SUB - 1] : f_exps[0]));
-            }
-        }
     };
     auto arrived = [&]() {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -907,23 +893,22 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
     };
 
     // the exponents of a stage's tiles, loaded with it
-    int t_exps[2][SUB] = {}, f_exps[2][SUB] = {};
+    int t_exps[2][SUB] = {};
     auto fetch_exps = [&](int t, int at) {
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
             if (NS == 2) t_exps[at][sub] = p.t_exp[t + sub];
-            if (NS == 2 && ITEMS) f_exps[at][sub] = p.t_factor_exp[t + sub];
         }
     };
     if (first < last) { fetch_stage(first, stage0, terms0); fetch_exps(first, 0); }
     for (int t = first; t < last; t += 2 * SUB) {
         arrived();
         if (t + SUB < last) { fetch_stage(t + SUB, stage1, terms1); fetch_exps(t + SUB, 1); }
-        compute(stage0, terms0, t_exps[0], f_exps[0]);
+        compute(stage0, terms0, t_exps[0]);
         if (t + SUB >= last) break;
         arrived();
         if (t + 2 * SUB < last) { fetch_stage(t + 2 * SUB, stage0, terms0); fetch_exps(t + 2 * SUB, 0); }
-        compute(stage1, terms1, t_exps[1], f_exps[1]);
+        compute(stage1, terms1, t_exps[1]);
     }
 
     const int64_t at = (int64_t)split * p.s_padded + s_row;
@@ -934,13 +919,12 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         if (h == 0) { p.out_m[at] = top; p.out_s[at] = sum; }
         return;
     }
-    const float unit = NS == 2 ? ldexpf(1.f, (MODE == WALK_USERS ? -15 : 0) - ref) : 1.f;
     b_sum += __shfl_xor(b_sum, 32);
     if (MODE == WALK_USERS) {
         for (int kb = 0; kb < KP / 32; ++kb)
             for (int q = 0; q < 4; ++q)
                 *(float4 *)(p.out_acc + at * KP + kb * 32 + 8 * q + 4 * h) =
-                    make_float4(acc[kb][4 * q] * unit, acc[kb][4 * q + 1] * unit, acc[kb][4 * q + 2] * unit, acc[kb][4 * q + 3] * unit);
+                    make_float4(acc[kb][4 * q], acc[kb][4 * q + 1], acc[kb][4 * q + 2], acc[kb][4 * q + 3]);
         return;
     }
     // dV: the places of the users walked are added here, to 64 rows a time (waves 0 and 1, then 2 and 3) whose sums lie in the first stage's
@@ -963,7 +947,7 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             for (int kb = 0; kb < KP / 32; ++kb)
                 for (int q = 0; q < 4; ++q)
                     *(float4 *)(rows + r * KP + kb * 32 + 8 * q + 4 * h) =
-                        make_float4(-acc[kb][4 * q] * unit, -acc[kb][4 * q + 1] * unit, -acc[kb][4 * q + 2] * unit, -acc[kb][4 * q + 3] * unit);
+                        make_float4(-acc[kb][4 * q], -acc[kb][4 * q + 1], -acc[kb][4 * q + 2], -acc[kb][4 * q + 3]);
             if (h == 0) row_b[r] = -b_sum;
         }
         __syncthreads();
@@ -1555,8 +1539,7 @@ ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c, bool lies)
 
 struct BackwardPlan {
     Side x, v;
-    float *item_term, *user_term, *G, *G_scaled, *acc_x, *acc_v, *acc_b;
-    int *g_exp;
+    float *item_term, *user_term, *G, *acc_x, *acc_v, *acc_b;
     int32_t *places;
     uint8_t *named;
     int64_t places_padded;
@@ -1578,8 +1561,6 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
     p.item_term = w.take<float>(p.v.padded);
     p.user_term = w.take<float>(p.x.padded);
     p.G = w.take<float>(p.x.padded);
-    p.G_scaled = w.take<float>(NS == 2 ? p.x.padded : 0);
-    p.g_exp = w.take<int>(NS == 2 ? p.x.tiles : 0);
     p.places_padded = items ? up(c.n * m, CHUNK) : 0;
     p.places = w.take<int32_t>(p.places_padded);
     // flags save the search where most groups of 64 items are not named; where the places are as many as the groups, none is saved
@@ -1740,7 +1721,6 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     PrepParams pp = prepare_sides(c, p.x, p.v, p.item_term);
     pp.lse = g.lse; pp.dlogp = g.dlogp; pp.ids = ids; pp.m = m; pp.ld_ids = ld_ids; pp.ld_dlogp = g.ld_dlogp; pp.places_padded = p.places_padded;
     pp.user_term = p.user_term; pp.G = p.G; pp.places = p.places; pp.named = p.named;
-    pp.G_scaled = p.G_scaled; pp.g_exp = p.g_exp;
     launch_prepare<T>(pp, p.x.tiles, s);
     const bool dealt = p.deal.chunks > 0;
     if (dealt) {
@@ -1761,7 +1741,7 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     const bool parts = items && p.split_v.count > 1;
     if (items) {
         walk_sides(w, c, p.x, p.v, false);
-        w.s_term = p.item_term; w.t_term = p.user_term; w.t_factor = NS == 2 ? p.G_scaled : p.G; w.t_factor_exp = p.g_exp;
+        w.s_term = p.item_term; w.t_term = p.user_term; w.t_factor = p.G;
         w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
         w.f = {dealt ? p.deal.to : p.places, p.named, X, g.dlogp, g.dV, g.dibase, dealt ? p.deal.place_of : nullptr, p.deal.bounds, p.deal.bucket_items, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx), fours(g.dV, g.ld_dv)};

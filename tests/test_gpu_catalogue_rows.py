@@ -107,3 +107,43 @@ def test_gradient_of_confident_users(torch, sc, n, items, k, dtype):
     assert _within(dX, r.dX, r.t_dX).all() and _within(dV, r.dV, r.t_dV).all()
 
 
+@pytest.mark.parametrize("n,items,k", [(70, 300, 64), (33, 500, 200), (300, 200, 33)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_gradient_of_unlikely_items(torch, sc, n, items, k, dtype):
+    """Items that nobody names and that have a probability of about 2^-87: their rows of dV keep the precision of the others'."""
+    g = _gen(torch, n)
+    dt = getattr(torch, dtype)
+    X, V = (torch.randn((n, k), generator=g, device="cuda") * 0.3).to(dt), (torch.randn((items, k), generator=g, device="cuda") * 0.3).to(dt)
+    b = torch.randn(items, generator=g, device="cuda")
+    b[40:90] = -60.0
+    ids = torch.randint(100, items, (n, 3), generator=g, device="cuda", dtype=torch.int32)
+    dlogp = torch.randn((n, 3), generator=g, device="cuda")
+    r = Exact(torch, X, V, b, ids, dlogp, 1.0, 3 * 2.0 ** -22, 2.0 ** -16 if dtype == "bfloat16" else 2.0 ** -21)
+    _, lse = sc.catalogue_logprob(X, V, ids, ibase=b)
+    dX, dV, db = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp, ibase=b)
+    assert 0 < float(r.dV[40:90].abs().max()) < 1e-20
+    assert float((r.t_dV[40:90].norm(dim=1) / r.dV[40:90].norm(dim=1)).median()) < 0.05
+    assert _within(dX, r.dX, r.t_dX).all() and _within(dV, r.dV, r.t_dV).all() and _within(db, r.db, r.t_db).all()
+
+
+@pytest.mark.parametrize("n,items,k", [(70, 300, 64), (40, 257, 200)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_gradient_beside_a_user_of_large_gradient(torch, sc, n, items, k, dtype):
+    """One user's upstream gradient is 2^30 times the others', and all of its probability lies on one item: rows of dV of the other items,
+    and the other users' rows of dX, are as precise as without it."""
+    g = _gen(torch, n + 1)
+    dt = getattr(torch, dtype)
+    X, V = (torch.randn((n, k), generator=g, device="cuda") * 0.3), (torch.randn((items, k), generator=g, device="cuda") * 0.3).to(dt)
+    X[3] = V[50].float() * (160 / float(V[50].float().norm() ** 2))
+    X = X.to(dt)
+    ids = torch.randint(60, items, (n, 3), generator=g, device="cuda", dtype=torch.int32)
+    dlogp = torch.randn((n, 3), generator=g, device="cuda")
+    ids[3], dlogp[3] = 50, dlogp[3] * 2.0 ** 30
+    r = Exact(torch, X, V, None, ids, dlogp, 1.0, 3 * 2.0 ** -22, 2.0 ** -16 if dtype == "bfloat16" else 2.0 ** -21)
+    _, lse = sc.catalogue_logprob(X, V, ids)
+    dX, dV, _ = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp)
+    others = torch.arange(items, device="cuda") != 50
+    assert float((r.t_dV.norm(dim=1) / r.dV.norm(dim=1))[others].median()) < 0.05
+    assert _within(dX, r.dX, r.t_dX).all() and _within(dV, r.dV, r.t_dV).all()
+
+
