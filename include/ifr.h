@@ -388,7 +388,8 @@ typedef struct ifr_catalogue {
     const void *X, *V;           /* dev [n][ldx], [n_items][ldv] of `dtype`; IFR_MXFP4: the codes (ldx, ldv unused)         */
     const uint8_t *x_scales, *v_scales;   /* IFR_MXFP4: the scales, else NULL                                               */
     const float *ibase;          /* dev [n_items] or NULL; -inf, or what overflows to it as scale ibase log2(e), takes an item out
-                                    (its row of V has to be finite all the same: it is multiplied by a probability of zero)   */
+                                    (its row of V, and that row's products with the users', have to be finite all the same: a probability of
+                                    zero multiplies them)                                                                   */
     int64_t n, n_items, ldx, ldv;
     int k, dtype;                /* 1 <= k <= IFR_MAX_FACTORS; n <= 2^23, 1 <= n_items <= 2^28                               */
     double scale;                /* 1e-30 ... 1e30: an inverse temperature                                                  */
@@ -398,7 +399,9 @@ typedef struct ifr_catalogue {
  * ids: dev [n][ld_ids], m items a user (0 <= m <= 2^20, n m <= 2^32; a slate, in which an item may stand twice).  A negative id is
  * an empty place: its logp is 0 and nothing flows through it.  An id >= n_items gives NaN (and counts for G alone below).
  *   lse[u] = log sum_i exp z[u][i] (dev [n] or NULL), logp[u][j] = z[u][ids[u][j]] - lse[u] (dev [n][ld_logp], or NULL where m = 0).
- * Products of fp32 operands keep 22 bits of each operand (more than the sum of k products in fp32 does); sums are fp32. */
+ * Products of fp32 operands keep 22 bits of each element, and 2^-39 of its row's largest magnitude of one that is more than 2^17 times smaller
+ * than that (a row whose largest is below 2^-111 counts as zeros); neither depends on other rows.  Few users are multiplied in fp32 itself.
+ * Sums are fp32. */
 int ifr_catalogue_logprob_workspace(ifr_handle h, const ifr_catalogue *c, int64_t *bytes);
 int ifr_catalogue_logprob(ifr_handle h, const ifr_catalogue *c, const int32_t *ids, int64_t m, int64_t ld_ids, float *logp,
                           int64_t ld_logp, float *lse, void *ws, int64_t ws_bytes, void *stream);

@@ -11,9 +11,9 @@
 // between lanes, and the block of probabilities already is the B operand of the second product, whose contraction runs over t in
 // the order the block's registers hold (t = 16 c + 8 (j / 4) + 4 (lane / 32) + j % 4 for element j of step c).
 //
-// Operands in 16 bits: bf16 as it is.  fp32 is split into two fp16 parts after scaling each tile of 32 rows by the power of two that
-// brings its largest magnitude to [2^14, 2^15): hi + lo keeps 22 bits of values near the maximum and an absolute step of 2^-39 of
-// the maximum below, and three products (hi hi, hi lo, lo hi) leave out lo lo, at most 2^-22 of a term.  Three fp16 products at 16
+// Operands in 16 bits: bf16 as it is.  fp32 is split into two fp16 parts after scaling each row by the power of two that
+// brings its largest magnitude to [2^14, 2^15): hi + lo keeps 22 bits of values down to 2^-17 of the row's maximum and an absolute step of
+// 2^-39 of the maximum below, and three products (hi hi, hi lo, lo hi) leave out lo lo, at most 2^-22 of a term.  Three fp16 products at 16
 // times the rate of the fp32 matrix instruction cost a fifth of it.
 #include <hip/hip_runtime.h>
 
@@ -47,8 +47,8 @@ __device__ __forceinline__ float as_f32(__bf16 v) { return (float)v; }
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// exponent e with max * 2^e in [2^14, 2^15) for a finite maximum (a subnormal one counts as 2^-126: scaled to at most 2^14, which is as
-// exact); a tile of zeros gets the largest, so that it never is the reference of a sum
+// exponent e with max * 2^e in [2^14, 2^15) for a row's largest finite magnitude (a subnormal one counts as 2^-126: scaled to at most 2^14, which is as
+// exact), a row of zeros too
 __device__ __forceinline__ int split_exponent(float top)
 {
     const uint32_t m = __float_as_uint(top);
@@ -78,14 +78,14 @@ __device__ __forceinline__ void online(const v16f &d, float c, float &m, float &
 
 // A matrix in the order the walks read it, by tiles of 32 rows, zeros behind the last row and column:
 //   frag [tile][part][KP / 16][64][8]: columns 16 s + 8 h + 0..7 of a row are the 16-byte piece piece_at(s, row, h)
-//   exps [tile]: the tile's exponent (split operands); infinities and NaN do not count for it and stay what they are
+//   units [row]: 2^(-24 - e) of the row's exponent e (split operands); infinities and NaN do not count for it and stay what they are
 // A bf16 V whose rows are whole, aligned pieces (k = KP) is read as it lies: v_frag is null then, and x_frag where lse is.  For the gradient
 // X is always put in order: users without an item (a batch's padding) become rows of zeros, so that nothing in them reaches dV.
 struct PrepParams {
     const void *V, *X;
     int64_t ldv, ldx, n_items, n, v_blocks, v_padded, x_padded;
     int k, KP;
-    int *v_exp, *x_exp;
+    float *v_unit, *x_unit;
     uint4 *v_frag, *x_frag;
     const float *ibase;
     // terms of split operands are powers of two, to be added to the exponent; those of bf16 operands are in units of <x, v>, to begin
@@ -96,7 +96,7 @@ struct PrepParams {
     const float *lse, *dlogp;
     const int32_t *ids;
     int64_t m, ld_ids, ld_dlogp, places_padded;
-    float *user_term, *G;              // G: the sum of a user's upstream gradients
+    float *user_term, *G, *G_scaled;   // G: the sum of a user's upstream gradients; split: also times 2^24
     int32_t *places;                   // the items named in (user, place) order, -1 behind the last place; null: not wanted
     uint8_t *named;                    // [items / 64], cleared before: set where an item is named; or null
 };
@@ -112,7 +112,7 @@ __host__ __device__ constexpr int piece_at(int s, int row, int h)
 
 // LDS tile [32][W] -> pieces
 template <int NS>
-__device__ __forceinline__ void store_fragments(const float *tile, int W, int KP, int e, int64_t at, uint4 *f)
+__device__ __forceinline__ void store_fragments(const float *tile, int W, int KP, const int *e, int64_t at, uint4 *f)
 {
     const int per = KP / 16 * 64;                     // 16-byte pieces of one part of a tile
     for (int i = threadIdx.x; i < per; i += 256) {
@@ -125,7 +125,7 @@ __device__ __forceinline__ void store_fragments(const float *tile, int W, int KP
         } else {
             h8 hi, lo;
             for (int j = 0; j < 8; ++j) {
-                const float x = ldexpf(v[j], e);
+                const float x = ldexpf(v[j], e[row]);
                 hi[j] = (_Float16)x;
                 lo[j] = (_Float16)(x - (float)hi[j]);
             }
@@ -142,8 +142,8 @@ template <typename T, int NS>
 __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
 {
     extern __shared__ float tile[];                   // [32][KP + 1]
-    __shared__ float tops[4], sums[256];
-    __shared__ int holds[32];
+    __shared__ float sums[256];
+    __shared__ int exps[32], holds[32];
     const int W = p.KP + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool of_v = blockIdx.x < p.v_blocks;
     const int64_t at = of_v ? blockIdx.x : blockIdx.x - p.v_blocks, r0 = at * 32;
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
     if (frag) {
         const T *src = (const T *)(of_v ? p.V : p.X);
         const int64_t rows = of_v ? p.n_items : p.n, ld = of_v ? p.ldv : p.ldx;
-        float top = 0.f;
+        float top[8] = {};
         for (int c = lane; c < p.KP; c += 64) {
             float v[8];                               // eight loads under way at once
 #pragma unroll
@@ -182,20 +182,27 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 tile[(wave + 4 * q) * W + c] = v[q];
-                if (NS == 2 && fabsf(v[q]) < INFINITY) top = fmaxf(top, fabsf(v[q]));
+                if (NS == 2 && fabsf(v[q]) < INFINITY) top[q] = fmaxf(top[q], fabsf(v[q]));
             }
         }
         if (NS == 2) {
-            for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-            if (lane == 0) tops[wave] = top;
+            // eight rows at once: a lane gives half of what it holds to the lane that keeps those rows, until eight lanes hold one row
+#pragma unroll
+            for (int w = 4, o = 32; w; w >>= 1, o >>= 1)
+#pragma unroll
+                for (int q = 0; q < w; ++q) {
+                    const float give = lane & o ? top[q] : top[q + w], keep = lane & o ? top[q + w] : top[q];
+                    top[q] = fmaxf(keep, __shfl_xor(give, o));
+                }
+            for (int o = 4; o; o >>= 1) top[0] = fmaxf(top[0], __shfl_xor(top[0], o));
+            if ((lane & 7) == 0) {
+                const int r = wave + 4 * (lane >> 3), e = split_exponent(top[0]);
+                exps[r] = e;
+                (of_v ? p.v_unit : p.x_unit)[r0 + r] = ldexpf(1.f, -24 - e);
+            }
         }
         __syncthreads();
-        int e = 0;
-        if (NS == 2) {
-            e = split_exponent(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-            if (threadIdx.x == 0) (of_v ? p.v_exp : p.x_exp)[at] = e;
-        }
-        store_fragments<NS>(tile, W, p.KP, e, at, frag);
+        store_fragments<NS>(tile, W, p.KP, exps, at, frag);
     }
     if (of_v) {
         if (threadIdx.x < 32) item_term(r0 + threadIdx.x);
@@ -207,6 +214,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
         float g = 0.f;
         for (int q = 0; q < 8; ++q) g += sums[threadIdx.x * 8 + q];
         p.G[u] = g;
+        if (NS == 2) p.G_scaled[u] = g * 16777216.f;
         // no probabilities where lse is -inf, and none that matter where no item is named: every exponential is 0
         p.user_term[u] = u < p.n && holds[threadIdx.x] && p.lse[u] != -INFINITY ? p.lse[u] * p.lse_unit : -INFINITY;
     }
@@ -358,8 +366,8 @@ struct WalkParams {
     const __bf16 *s_rows, *t_rows;
     int64_t s_ld, t_ld, s_n, t_n;
     const float *s_term, *t_term;      // item_term, user_term of prepare_kernel
-    const float *t_factor;             // WALK_ITEMS...: G
-    const int *s_exp, *t_exp;          // split operands: exponents of their tiles
+    const float *t_factor;             // WALK_ITEMS...: G (split: times 2^24)
+    const float *s_unit, *t_unit;      // split operands: powers of two of their rows
     float c;                           // scale log2(e)
     int s_blocks, splits, t_tiles, tiles_per_split;
     int64_t s_padded;
@@ -683,7 +691,9 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
     constexpr int STAGE = PART * NS * SUB;
     // two stages: one is read while the other arrives (two arrays, so that the compiler sees that they are apart)
     __shared__ uint4 stage0[STAGE], stage1[STAGE];
-    __shared__ float terms0[2 * SUB * 32], terms1[2 * SUB * 32];      // of the stage's T rows: t_term, t_factor (a fetch brings 64)
+    // of the stage's T rows: t_term, t_factor, t_unit (a fetch brings 64)
+    constexpr int ROWS = SUB * 32 < 64 ? 64 : SUB * 32;
+    __shared__ __align__(16) float terms0[(NS + 1) * ROWS], terms1[(NS + 1) * ROWS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     // workgroups go to the eight XCDs in turn: splits are dealt so that an XCD's L2 sees each part of T from one split only
     int s_block, split;
@@ -707,7 +717,9 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         for (int s = 0; s < STEPS; ++s)
             sf[q][s] = S_LIES ? ((const uint4 *)(p.s_rows + min(s_row, p.s_n - 1) * p.s_ld))[2 * s + h]
                             : p.s_frag[(s_tile * NS + q) * PART + piece_at(s, lane & 31, h)];
-    const int s_exp = NS == 2 ? p.s_exp[s_tile] : 0;
+    // split: a score is scale log2(e) 2^-(e_s + e_t) of a product; the T row's part leaves 2^24 to the S row's, so that a product of a T row's
+    // parts (below 2^38) times its own power of two stays below 2^127 whatever the row holds
+    const float s_unit = NS == 2 ? fminf(p.c * (p.s_unit[s_row] * 16777216.f) * 16777216.f, 3.402823466e38f) : 1.f;
     const float s_term = p.s_term ? p.s_term[s_row] * (NS == 1 ? p.c : 1.f) : 0.f;
 
     constexpr bool ITEMS = MODE == WALK_ITEMS || MODE == WALK_ITEMS_BASE;
@@ -737,11 +749,13 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         } else {
             fetch<STAGE>(p.t_frag + (int64_t)t * PART * NS, to);
         }
-        if (wave < (SUB + 1) / 2) fetch_row(p.t_term + (int64_t)t * 32 + wave * 64, terms + wave * 64);
-        else if (ITEMS && wave < SUB) fetch_row(p.t_factor + (int64_t)t * 32 + (wave - SUB / 2) * 64, terms + wave * 64);
+        constexpr int EACH = ROWS / 64;
+        if (wave < EACH) fetch_row(p.t_term + (int64_t)t * 32 + wave * 64, terms + wave * 64);
+        else if (ITEMS && wave < 2 * EACH) fetch_row(p.t_factor + (int64_t)t * 32 + (wave - EACH) * 64, terms + wave * 64);
+        else if (NS == 2 && wave == 2) fetch_row(p.t_unit + (int64_t)t * 32, terms + 2 * ROWS);
     };
-    // The scores of one tile: split c d + term with c of the tile, otherwise the sums begin with the terms.
-    auto scores = [&](const uint4 *l1, const float *tt, float c) {
+    // The scores of one tile: split (d t_unit) s_unit + term, otherwise the sums begin with the terms.
+    auto scores = [&](const uint4 *l1, const float *tt) {
         v16f d = {};
         float4 t4[4];
 #pragma unroll
@@ -767,27 +781,22 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         if (NS == 2) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                d[4 * q] = fmaf(d[4 * q], c, t4[q].x); d[4 * q + 1] = fmaf(d[4 * q + 1], c, t4[q].y);
-                d[4 * q + 2] = fmaf(d[4 * q + 2], c, t4[q].z); d[4 * q + 3] = fmaf(d[4 * q + 3], c, t4[q].w);
+                const float4 u4 = *(const float4 *)(tt + 2 * ROWS + 8 * q + 4 * h);
+                d[4 * q] = fmaf(d[4 * q] * u4.x, s_unit, t4[q].x); d[4 * q + 1] = fmaf(d[4 * q + 1] * u4.y, s_unit, t4[q].y);
+                d[4 * q + 2] = fmaf(d[4 * q + 2] * u4.z, s_unit, t4[q].z); d[4 * q + 3] = fmaf(d[4 * q + 3] * u4.w, s_unit, t4[q].w);
             }
         }
         return d;
     };
     // A stage's tiles (those behind the last row have terms of -inf and add nothing: no branch divides the code, so that the
     // exponentials of one tile go beside the matrix instructions of the next tile's scores and of the last one's sums).
-    auto compute = [&](const uint4 *lds, const float *terms, const int *t_exps) {
-        float c[SUB], unit[SUB];
-#pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) {
-            c[sub] = NS == 2 ? fminf(ldexpf(p.c, -s_exp - t_exps[sub]), 3.402823466e38f) : p.c;
-            unit[sub] = NS == 2 ? ldexpf(1.f, -t_exps[sub]) : 1.f;
-        }
+    auto compute = [&](const uint4 *lds, const float *terms) {
         if (MODE == WALK_STATS) {
 #pragma unroll 2
             for (int sub = 0; sub < SUB; ++sub) {
-                const v16f d = scores(lds + sub * PART * NS, terms + sub * 32, c[sub]);
+                const v16f d = scores(lds + sub * PART * NS, terms + sub * 32);
                 reads_ahead<STEPS * NS, STEPS * (2 * NS - 1)>();
-                online(d, NS == 2 ? 1.f : c[sub], m, sum);
+                online(d, NS == 2 ? 1.f : p.c, m, sum);
             }
             return;
         }
@@ -801,13 +810,13 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         auto probabilities = [&](const v16f &d, int sub) {
             float P[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) P[r] = exp2_raw(NS == 2 ? d[r] + s_term : fmaf(d[r], c[sub], s_term));
+            for (int r = 0; r < 16; ++r) P[r] = exp2_raw(NS == 2 ? d[r] + s_term : fmaf(d[r], p.c, s_term));
             if (ITEMS) {
                 {   // products rounded by themselves: dV has the same bits with and without db beside it
 #pragma clang fp contract(off)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const float4 tg = *(const float4 *)(terms + SUB * 32 + sub * 32 + 8 * q + 4 * h);
+                        const float4 tg = *(const float4 *)(terms + ROWS + sub * 32 + 8 * q + 4 * h);
                         P[4 * q] *= tg.x; P[4 * q + 1] *= tg.y; P[4 * q + 2] *= tg.z; P[4 * q + 3] *= tg.w;
                     }
                 }
@@ -821,14 +830,20 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             Operand o;
             o.back = 1.f;
             if (NS == 2) {
-                // the S row's 32 elements (16 here, 16 in lane + or - 32) by the power of two that brings the largest to [2^14, 2^15)
+                // times the T rows' powers of two (their parts are scaled by the inverse); then the S row's 32 elements (16 here, 16 in
+                // lane + or - 32) by the power of two that brings the largest to [2^14, 2^15)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 u4 = *(const float4 *)(terms + 2 * ROWS + sub * 32 + 8 * q + 4 * h);
+                    P[4 * q] *= u4.x; P[4 * q + 1] *= u4.y; P[4 * q + 2] *= u4.z; P[4 * q + 3] *= u4.w;
+                }
                 float top = fabsf(P[0]);
 #pragma unroll
                 for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(P[r]));
                 const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                 const uint32_t field = max(max((uint32_t)both[0], (uint32_t)both[1]) >> 23, 15u);
                 const float up = __uint_as_float((268u - field) << 23);
-                o.back = __uint_as_float((field - 14u) << 23) * unit[sub];
+                o.back = __uint_as_float((field - 14u) << 23);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) P[r] *= up;
             }
@@ -879,11 +894,11 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
                 }
             }
         };
-        v16f next = scores(lds, terms, c[0]);
+        v16f next = scores(lds, terms);
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
             const v16f d = next;
-            if (sub + 1 < SUB) next = scores(lds + (sub + 1) * PART * NS, terms + (sub + 1) * 32, c[sub + 1 < SUB ? sub + 1 : 0]);
+            if (sub + 1 < SUB) next = scores(lds + (sub + 1) * PART * NS, terms + (sub + 1) * 32);
             add_product(lds + sub * PART * NS, probabilities(d, sub));
         }
     };
@@ -892,23 +907,15 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         __syncthreads();
     };
 
-    // the exponents of a stage's tiles, loaded with it
-    int t_exps[2][SUB] = {};
-    auto fetch_exps = [&](int t, int at) {
-#pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) {
-            if (NS == 2) t_exps[at][sub] = p.t_exp[t + sub];
-        }
-    };
-    if (first < last) { fetch_stage(first, stage0, terms0); fetch_exps(first, 0); }
+    if (first < last) fetch_stage(first, stage0, terms0);
     for (int t = first; t < last; t += 2 * SUB) {
         arrived();
-        if (t + SUB < last) { fetch_stage(t + SUB, stage1, terms1); fetch_exps(t + SUB, 1); }
-        compute(stage0, terms0, t_exps[0]);
+        if (t + SUB < last) fetch_stage(t + SUB, stage1, terms1);
+        compute(stage0, terms0);
         if (t + SUB >= last) break;
         arrived();
-        if (t + 2 * SUB < last) { fetch_stage(t + 2 * SUB, stage0, terms0); fetch_exps(t + 2 * SUB, 0); }
-        compute(stage1, terms1, t_exps[1]);
+        if (t + 2 * SUB < last) fetch_stage(t + 2 * SUB, stage0, terms0);
+        compute(stage1, terms1);
     }
 
     const int64_t at = (int64_t)split * p.s_padded + s_row;
@@ -919,12 +926,14 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         if (h == 0) { p.out_m[at] = top; p.out_s[at] = sum; }
         return;
     }
-    b_sum += __shfl_xor(b_sum, 32);
+    // split: G, and with it the sum for db, is 2^24 times itself, and the T rows' powers of two are 2^-24 of themselves
+    b_sum = (b_sum + __shfl_xor(b_sum, 32)) * (NS == 2 ? 1.f / 16777216.f : 1.f);
     if (MODE == WALK_USERS) {
+        constexpr float UNIT = NS == 2 ? 16777216.f : 1.f;
         for (int kb = 0; kb < KP / 32; ++kb)
             for (int q = 0; q < 4; ++q)
                 *(float4 *)(p.out_acc + at * KP + kb * 32 + 8 * q + 4 * h) =
-                    make_float4(acc[kb][4 * q], acc[kb][4 * q + 1], acc[kb][4 * q + 2], acc[kb][4 * q + 3]);
+                    make_float4(acc[kb][4 * q] * UNIT, acc[kb][4 * q + 1] * UNIT, acc[kb][4 * q + 2] * UNIT, acc[kb][4 * q + 3] * UNIT);
         return;
     }
     // dV: the places of the users walked are added here, to 64 rows a time (waves 0 and 1, then 2 and 3) whose sums lie in the first stage's
@@ -1436,7 +1445,7 @@ Split split_plan(int64_t s_blocks, int64_t t_tiles, int unit, int64_t resident, 
 struct Side {                          // one matrix as the walks read it
     int64_t rows, tiles, padded;       // tiles of 32 rows; padded: rows up to whole S blocks
     bool lies;                         // bf16 rows of whole, aligned pieces: read as they lie
-    int *exps;
+    float *units;
     uint4 *frag;
 };
 
@@ -1448,7 +1457,7 @@ Side side(Pieces &w, const ifr_catalogue &c, bool users, bool lies)
     s.padded = up(s.rows, S_ROWS);
     s.tiles = s.padded / 32;
     s.lies = lies;
-    s.exps = w.take<int>(NS == 2 ? s.tiles : 0);
+    s.units = w.take<float>(NS == 2 ? s.padded + 32 : 0);      // a fetch brings 64, also where a stage holds 32 rows
     s.frag = w.take<uint4>(s.lies ? 0 : s.tiles * NS * (KP / 16) * 64);
     return s;
 }
@@ -1539,7 +1548,7 @@ ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c, bool lies)
 
 struct BackwardPlan {
     Side x, v;
-    float *item_term, *user_term, *G, *acc_x, *acc_v, *acc_b;
+    float *item_term, *user_term, *G, *G_scaled, *acc_x, *acc_v, *acc_b;
     int32_t *places;
     uint8_t *named;
     int64_t places_padded;
@@ -1561,6 +1570,7 @@ BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx
     p.item_term = w.take<float>(p.v.padded);
     p.user_term = w.take<float>(p.x.padded);
     p.G = w.take<float>(p.x.padded);
+    p.G_scaled = w.take<float>(NS == 2 ? p.x.padded : 0);
     p.places_padded = items ? up(c.n * m, CHUNK) : 0;
     p.places = w.take<int32_t>(p.places_padded);
     // flags save the search where most groups of 64 items are not named; where the places are as many as the groups, none is saved
@@ -1613,7 +1623,7 @@ static PrepParams prepare_sides(const ifr_catalogue &c, const Side &x, const Sid
     p.V = c.V; p.X = c.X; p.ldv = c.ldv; p.ldx = c.ldx; p.n_items = c.n_items; p.n = c.n;
     p.v_blocks = v.lies ? (v.padded + 255) / 256 : v.tiles; p.v_padded = v.padded; p.x_padded = x.padded;
     p.k = c.k; p.KP = pad_factors(c.k);
-    p.v_exp = v.exps; p.x_exp = x.exps; p.v_frag = v.frag; p.x_frag = x.frag;
+    p.v_unit = v.units; p.x_unit = x.units; p.v_frag = v.frag; p.x_frag = x.frag;
     p.ibase = c.ibase; p.item_term = item_term;
     p.base_unit = c.dtype == IFR_F32 ? (float)(c.scale / LN2) : 1.f;
     p.lse_unit = c.dtype == IFR_F32 ? -LOG2E : (float)(-1.0 / c.scale);
@@ -1623,7 +1633,7 @@ static PrepParams prepare_sides(const ifr_catalogue &c, const Side &x, const Sid
 static void walk_sides(WalkParams &w, const ifr_catalogue &c, const Side &x, const Side &v, bool users_stay)
 {
     const Side &s = users_stay ? x : v, &t = users_stay ? v : x;
-    w.s_frag = s.frag; w.t_frag = t.frag; w.s_exp = s.exps; w.t_exp = t.exps; w.s_n = s.rows; w.t_n = t.rows;
+    w.s_frag = s.frag; w.t_frag = t.frag; w.s_unit = s.units; w.t_unit = t.units; w.s_n = s.rows; w.t_n = t.rows;
     w.s_rows = (const __bf16 *)(users_stay ? c.X : c.V); w.t_rows = (const __bf16 *)(users_stay ? c.V : c.X);
     w.s_ld = users_stay ? c.ldx : c.ldv; w.t_ld = users_stay ? c.ldv : c.ldx;
     w.t_tiles = (int)((t.rows + 31) / 32); w.s_blocks = (int)(s.padded / S_ROWS); w.s_padded = s.padded;
@@ -1720,7 +1730,7 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     }
     PrepParams pp = prepare_sides(c, p.x, p.v, p.item_term);
     pp.lse = g.lse; pp.dlogp = g.dlogp; pp.ids = ids; pp.m = m; pp.ld_ids = ld_ids; pp.ld_dlogp = g.ld_dlogp; pp.places_padded = p.places_padded;
-    pp.user_term = p.user_term; pp.G = p.G; pp.places = p.places; pp.named = p.named;
+    pp.user_term = p.user_term; pp.G = p.G; pp.G_scaled = p.G_scaled; pp.places = p.places; pp.named = p.named;
     launch_prepare<T>(pp, p.x.tiles, s);
     const bool dealt = p.deal.chunks > 0;
     if (dealt) {
@@ -1741,7 +1751,7 @@ static void backward_typed(const ifr_catalogue &c, const int32_t *ids, int64_t m
     const bool parts = items && p.split_v.count > 1;
     if (items) {
         walk_sides(w, c, p.x, p.v, false);
-        w.s_term = p.item_term; w.t_term = p.user_term; w.t_factor = p.G;
+        w.s_term = p.item_term; w.t_term = p.user_term; w.t_factor = NS == 2 ? p.G_scaled : p.G;
         w.tiles_per_split = p.split_v.per; w.splits = p.split_v.count;
         w.out_acc = parts ? p.acc_v : nullptr; w.out_b = p.acc_b;
         w.f = {dealt ? p.deal.to : p.places, p.named, X, g.dlogp, g.dV, g.dibase, dealt ? p.deal.place_of : nullptr, p.deal.bounds, p.deal.bucket_items, c.n * m, m, c.ldx, g.ld_dlogp, g.ld_dv, c.n_items, c.k, sc, fours(X, c.ldx), fours(g.dV, g.ld_dv)};

@@ -147,3 +147,40 @@ def test_gradient_beside_a_user_of_large_gradient(torch, sc, n, items, k, dtype)
     assert _within(dX, r.dX, r.t_dX).all() and _within(dV, r.dV, r.t_dV).all()
 
 
+@pytest.mark.parametrize("n,items,k", [(90, 300, 50), (40, 310, 200), (130, 257, 128), (600, 90, 33)])
+@pytest.mark.parametrize("large", [2.0 ** 24, 2.0 ** 40, 2.0 ** 60])
+def test_large_rows_leave_their_neighbours_alone(torch, sc, n, items, k, large):
+    """fp32: a user, an item that is taken out and a padding user whose rows are far larger than their neighbours', and an item that is large
+    only where every user has a zero: the other users and items keep their precision."""
+    g = _gen(torch, n + k)
+    X, V = torch.randn((n, k), generator=g, device="cuda") * 0.3, torch.randn((items, k), generator=g, device="cuda") * 0.3
+    b = torch.randn(items, generator=g, device="cuda")
+    ids = torch.randint(12, items, (n, 3), generator=g, device="cuda", dtype=torch.int32)
+    dlogp = torch.randn((n, 3), generator=g, device="cuda")
+    X[7] *= large
+    V[11] *= large
+    b[11] = -math.inf
+    X[20], ids[20] = large, -1
+    X[:, k - 1] = 0
+    with_item = V.clone()
+    with_item[45] = 0
+    with_item[45, k - 1] = large
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[7] = rest[20] = False
+    for v in (V, with_item):
+        r = Exact(torch, X, v, b, ids, dlogp, 1.0, 3 * 2.0 ** -22, 2.0 ** -21)
+        logp, lse = sc.catalogue_logprob(X, v, ids, ibase=b)
+        assert float(r.e_lse[rest].max()) < 2e-3
+        assert _within(lse, r.lse, r.e_lse)[rest].all() and _within(logp, r.logp, r.e_logp)[rest].all()
+    logp, lse = sc.catalogue_logprob(X, V, ids, ibase=b)
+    r = Exact(torch, X, V, b, ids, dlogp, 1.0, 3 * 2.0 ** -22, 2.0 ** -21)
+    dX, dV, db = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp, ibase=b)
+    assert (dX[20] == 0).all() and _within(dX, r.dX, r.t_dX)[rest].all()
+    # the large user's own part lies on the items that it names and on its likeliest ones
+    clear = torch.ones(items, dtype=torch.bool, device="cuda")
+    clear[ids[7].long()] = False
+    clear[(X[7].double() @ V.double().t() + b.double()).topk(3).indices] = False
+    assert float((r.t_dV.norm(dim=1) / r.dV.norm(dim=1).clamp(min=1e-12))[clear].median()) < 0.01
+    assert _within(dV, r.dV, r.t_dV)[clear].all() and _within(db, r.db, r.t_db)[clear].all()
+
+
