@@ -360,6 +360,6 @@ class CatalogueOps:
         p = _lib.Policy(n, width, _REDUCTIONS[reduction], x[0].data_ptr(), old[0].data_ptr(), _ptr(ref[0]), advantages.data_ptr(), _ptr(weight), _ptr(m[0]),
                         loss.data_ptr(), _ptr(kl), clipped.data_ptr(), d_logp.data_ptr(), x[1], old[1], ref[1], m[1], width, float(clip_low), float(clip_high),
                         float(kl_coef))
-        ws, need = (None, 0) if mask is None or reduction != "batch" else self._workspace(clipped, self._lib.ifr_policy_loss_workspace, "policy", ctypes.byref(p))
+        ws, need = (None, 0) if mask is None or reduction != "batch" else self._workspace(clipped, self._lib.ifr_policy_loss_workspace, ("policy", not p.mask), ctypes.byref(p))
         self._check(self._lib.ifr_policy_loss(self._h, ctypes.byref(p), _ptr(ws), need, self._stream_of()))
         return PolicyLoss(loss, kl, clipped, d_logp)

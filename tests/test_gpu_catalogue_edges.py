@@ -1,0 +1,41 @@
+"""GPU tests of the catalogue operators at the edges of what they take: empty batches before full ones, factors and scales near the ends
+of their ranges, the tile forms of large batches.  U = 2^-24 is half a step of fp32 relative to the value, B = 2^-8 of bf16."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+U, B = 2.0 ** -24, 2.0 ** -8
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch
+
+
+@pytest.fixture(scope="module")
+def sc(torch):
+    from recommenders_amd import HipScorer
+    return HipScorer(0)
+
+
+def _gen(torch, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+@pytest.mark.parametrize("n,width", [(0, 5), (3, 0), (0, 0)])
+def test_policy_batch_after_an_empty_one(torch, n, width):
+    """A scorer whose first call with a mask and the batch's mean has no place takes full batches afterwards."""
+    from recommenders_amd import HipScorer
+    sc = HipScorer(0)
+    empty = torch.zeros((n, width), device="cuda")
+    p = sc.policy_loss(empty, empty, torch.ones(n, device="cuda"), mask=torch.ones((n, width), dtype=torch.bool, device="cuda"), reduction="batch")
+    assert p.loss.shape == (n,) and (p.loss == 0).all() and p.d_logp.shape == (n, width)
+    logp = torch.zeros((2, 3), device="cuda")
+    mask = torch.tensor([[True, True, False], [True, False, False]], device="cuda")
+    p = sc.policy_loss(logp, logp, torch.tensor([3.0, 6.0], device="cuda"), mask=mask, reduction="batch")
+    assert p.loss.tolist() == [-2.0, -2.0] and p.d_logp.tolist() == [[-1.0, -1.0, 0.0], [-2.0, 0.0, 0.0]]
+    sc.close()
