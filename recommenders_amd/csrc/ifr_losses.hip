@@ -93,9 +93,11 @@ __device__ __forceinline__ float sigmoid(float x)
     return (x >= 0.f ? 1.f : e) / (1.f + e);
 }
 
-// loss and its slope in h (a NaN in h stays one: fmaxf would drop it)
-__device__ __forceinline__ void preference_of(const ifr_preference &p, float h, float *loss, float *slope)
+// loss, and slope times factor = its slope in h times beta (a NaN in h stays one: fmaxf would drop it).  Squared: the slope 2 (h - 1/2) / beta^2
+// leaves fp32 where beta is far from 1, its product with beta does not
+__device__ __forceinline__ void preference_of(const ifr_preference &p, float h, float *loss, float *slope, float *factor)
 {
+    *factor = (float)p.beta;
     if (h != h) { *loss = h; *slope = h; return; }
     if (p.kind == IFR_PREFERENCE_LOGISTIC) {
         const float e = (float)p.label_smoothing;
@@ -107,7 +109,8 @@ __device__ __forceinline__ void preference_of(const ifr_preference &p, float h, 
     } else {
         const float b = (float)p.beta, d = (h - 0.5f) / b;
         *loss = d * d;
-        *slope = 2.f * d / b;
+        *slope = 2.f * d;
+        *factor = 1.f;
     }
 }
 
@@ -153,9 +156,9 @@ __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP) void preference_kernel(i
             count[side] = p.average ? max(group_sum<GROUP>(c, ldsn), 1) : 1;
         }
         const float h = (float)(p.beta * (sum[0] / count[0] - sum[1] / count[1]) - p.margin);
-        float loss, slope;
-        preference_of(p, h, &loss, &slope);
-        const float g = (p.weight ? p.weight[row] : 1.f) * slope * (float)p.beta;
+        float loss, slope, factor;
+        preference_of(p, h, &loss, &slope, &factor);
+        const float g = (p.weight ? p.weight[row] : 1.f) * slope * factor;
         if (me == 0) {
             if (p.loss) p.loss[row] = loss;
             if (p.h) p.h[row] = h;

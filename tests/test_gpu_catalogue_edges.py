@@ -39,3 +39,15 @@ def test_policy_batch_after_an_empty_one(torch, n, width):
     p = sc.policy_loss(logp, logp, torch.tensor([3.0, 6.0], device="cuda"), mask=mask, reduction="batch")
     assert p.loss.tolist() == [-2.0, -2.0] and p.d_logp.tolist() == [[-1.0, -1.0, 0.0], [-2.0, 0.0, 0.0]]
     sc.close()
+
+
+@pytest.mark.parametrize("beta", [1e-30, 1e-25, 1e-10, 1.0, 1e25, 1e30])
+def test_squared_preference_over_the_range_of_beta(torch, sc, beta):
+    """d loss / dh times beta is 2 (h - 1/2) / beta, which fp32 holds where the factors 2 (h - 1/2) / beta^2 and beta leave it."""
+    D = torch.tensor([[0.0], [1.0], [-3.0], [1e-3]], device="cuda")
+    p = sc.preference_loss(D, torch.zeros_like(D), beta=beta, kind="squared")
+    h = (beta * D.double()[:, 0])
+    # h rounds to fp32 (and to a multiple of 2^-149), then a difference, a quotient and a product
+    want = 2 * (h - 0.5) / beta
+    tol = 8 * U * want.abs() + 2 * (U * h.abs() + 2.0 ** -149) / beta
+    assert ((p.d_chosen.double()[:, 0] - want).abs() <= tol).all() and torch.equal(p.d_rejected, -p.d_chosen)
