@@ -1248,9 +1248,10 @@ struct Targets {
     float *lse, *logp;
 };
 
-__device__ __forceinline__ float mx_unit(uint32_t byte)
+// e times the two scales' powers of two at once (one alone may leave fp32); NaN where a scale stands for it
+__device__ __forceinline__ float mx_scaled(float e, int a, int b)
 {
-    return byte == 255 ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+    return a == 255 || b == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(e, a + b - 254);
 }
 
 // lane l of 16: its share of <x, v>
@@ -1279,7 +1280,7 @@ __device__ __forceinline__ float dot_share<Mx>(const Targets &t, int64_t u, int6
         const v2f a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 2), b2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 2);
         const v2f a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a, 1.0f, 3), b3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b, 1.0f, 3);
         const float e = a0[0] * b0[0] + a0[1] * b0[1] + a1[0] * b1[0] + a1[1] * b1[1] + a2[0] * b2[0] + a2[1] * b2[1] + a3[0] * b3[0] + a3[1] * b3[1];
-        d += e * mx_unit(t.xs[u * t.kb + (c >> 2)]) * mx_unit(t.vs[id * t.kb + (c >> 2)]);
+        d += mx_scaled(e, t.xs[u * t.kb + (c >> 2)], t.vs[id * t.kb + (c >> 2)]);
     }
     return d;
 }

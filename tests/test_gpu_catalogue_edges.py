@@ -51,3 +51,22 @@ def test_squared_preference_over_the_range_of_beta(torch, sc, beta):
     want = 2 * (h - 0.5) / beta
     tol = 8 * U * want.abs() + 2 * (U * h.abs() + 2.0 ** -149) / beta
     assert ((p.d_chosen.double()[:, 0] - want).abs() <= tol).all() and torch.equal(p.d_rejected, -p.d_chosen)
+
+
+@pytest.mark.parametrize("up,down", [(118, 118), (124, 124), (126, 120)])
+def test_logprob_of_4bit_rows_whose_scales_cancel(torch, sc, up, down):
+    """Users near the top of fp32 and items as far below 1: scores are ordinary numbers, and so is every log-probability."""
+    g = _gen(torch, up)
+    X, V = torch.randn((5, 96), generator=g, device="cuda") * 0.3, torch.randn((70, 96), generator=g, device="cuda") * 0.3
+    ids = torch.randint(0, 70, (5, 4), generator=g, device="cuda", dtype=torch.int32)
+    xq, vq = sc.quantize_mxfp4(X * 2.0 ** up), sc.quantize_mxfp4(V * 2.0 ** -down)
+    scale = 2.0 ** (down - up)
+    logp, lse = sc.catalogue_logprob(xq, vq, ids, scale=scale)
+    x, v = sc.dequantize_mxfp4(xq).double(), sc.dequantize_mxfp4(vq).double()
+    z, room = scale * x @ v.t(), float((scale * x.abs() @ v.abs().t()).max())
+    want = torch.logsumexp(z, 1)
+    # exact products, at most 96 additions in fp32, and the roundings of scale, exponent (twice |z| and |lse|), v_exp_f32 and the sum of 70
+    score = 100 * U * room
+    e_lse = score + 6 * U * (float(z.abs().max()) + float(want.abs().max()) + 8) + 2.0 ** -21 + 99 * U
+    assert float((lse.double() - want).abs().max()) <= e_lse
+    assert float((logp.double() - (z.gather(1, ids.long()) - want[:, None])).abs().max()) <= score + 2 * e_lse
