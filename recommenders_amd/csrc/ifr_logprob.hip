@@ -83,7 +83,7 @@ __device__ __forceinline__ void online(const v16f &d, float c, float &m, float &
 // X is always put in order: users without an item (a batch's padding) become rows of zeros, so that nothing in them reaches dV.
 struct PrepParams {
     const void *V, *X;
-    int64_t ldv, ldx, n_items, n, v_blocks, v_padded, x_padded;
+    int64_t ldv, ldx, n_items, n, v_blocks, v_padded;
     int k, KP;
     float *v_unit, *x_unit;
     uint4 *v_frag, *x_frag;
@@ -1622,7 +1622,7 @@ static PrepParams prepare_sides(const ifr_catalogue &c, const Side &x, const Sid
 {
     PrepParams p = {};
     p.V = c.V; p.X = c.X; p.ldv = c.ldv; p.ldx = c.ldx; p.n_items = c.n_items; p.n = c.n;
-    p.v_blocks = v.lies ? (v.padded + 255) / 256 : v.tiles; p.v_padded = v.padded; p.x_padded = x.padded;
+    p.v_blocks = v.lies ? (v.padded + 255) / 256 : v.tiles; p.v_padded = v.padded;
     p.k = c.k; p.KP = pad_factors(c.k);
     p.v_unit = v.units; p.x_unit = x.units; p.v_frag = v.frag; p.x_frag = x.frag;
     p.ibase = c.ibase; p.item_term = item_term;

@@ -39,8 +39,6 @@ class CatalogueLearningMixin:
         for name in self._hip_learned():
             a = None if name is None else getattr(self, name)
             out.append(None if a is None else torch.tensor(np.asarray(a, np.float32), device=dev))
-        if out[0] is None or out[1] is None:
-            raise RuntimeError(f"{self.name} has no factors: pass init_params")
         return out
 
     def _hip_frozen(self, parameters, precision):
@@ -68,6 +66,8 @@ class CatalogueLearningMixin:
 
     # ------------------------------------------------------------------ checks
     def _hip_users(self, users):
+        if any(getattr(self, name) is None for name in self._hip_learned()[:2]):
+            raise RuntimeError(f"{self.name} has no factors: pass init_params")
         u = np.asarray(users)
         n = len(getattr(self, self._hip_learned()[0]))
         if u.ndim != 1 or u.dtype.kind not in "iu":
