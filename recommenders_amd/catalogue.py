@@ -4,7 +4,8 @@ softmax over the whole catalogue with their gradient, and the preference and pol
 Operands are torch tensors on the scorer's GPU; a tensor whose last dimension is not contiguous is copied, any row stride is
 taken as it is.  Every call runs on the GPU's current stream, allocates its outputs and its workspace there with torch's
 allocator (so it can be captured into a graph) and does not synchronise.  Gradients are results of their own, not of autograd:
-tensors that require one are refused while autograd records."""
+tensors that require one are refused while autograd records, those with a tangent always (torch.no_grad does not stop
+forward-mode differentiation)."""
 import ctypes
 from collections import namedtuple
 
@@ -86,6 +87,17 @@ def _recorded():
     return torch.is_grad_enabled()
 
 
+def _refuse_tangents(**tensors):
+    """ValueError if one of them carries a tangent of forward-mode differentiation."""
+    import torch
+    ad = torch.autograd.forward_ad
+    if ad._current_level < 0:                    # no level is open
+        return
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} carries a tangent: forward-mode differentiation does not see this call, pass the primal of unpack_dual({name})")
+
+
 def _matrix(t, name, dtypes, cols=None, rows=None, device=None):
     """(`t`, elements from one row to the next): a matrix with contiguous rows at least its width apart -- a single row reaches as far as it
     is wide; ValueError / TypeError where it is not what `name` is."""
@@ -124,6 +136,7 @@ def _optional(t, *args):
 def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
     """What the log-probability calls take, ready for the library -- (X, row stride), (V, row stride), (ids, row stride), ibase -- or the refusal."""
     import torch
+    _refuse_tangents(X=X, V=V, ibase=ibase)
     if isinstance(X, MxFp4Matrix) != isinstance(V, MxFp4Matrix):
         raise TypeError("X and V must both be tensors or both be MxFp4Matrix")
     if isinstance(X, MxFp4Matrix):
@@ -151,6 +164,7 @@ def check_catalogue(X, V, ids, ibase, scale, device=None, extra=()):
 def check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, mask_rejected, weight, beta, kind, label_smoothing, margin, device=None):
     """What `preference_loss` takes, ready for the library -- six (matrix, row stride), weight -- or the refusal."""
     import torch
+    _refuse_tangents(chosen=chosen, rejected=rejected, ref_chosen=ref_chosen, ref_rejected=ref_rejected, weight=weight)
     f32, masks = (torch.float32,), (torch.bool, torch.uint8)
     c = _matrix(chosen, "chosen", f32, None, None, device)
     n, wc = c[0].shape
@@ -178,6 +192,7 @@ def check_preference(chosen, rejected, ref_chosen, ref_rejected, mask_chosen, ma
 def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, clip_high, kl_coef, reduction, device=None):
     """What `policy_loss` takes, ready for the library -- four (matrix, row stride), advantages, weight -- or the refusal."""
     import torch
+    _refuse_tangents(logp=logp, old_logp=old_logp, advantages=advantages, ref_logp=ref_logp, weight=weight)
     f32 = (torch.float32,)
     x = _matrix(logp, "logp", f32, None, None, device)
     n, width = x[0].shape
@@ -196,6 +211,16 @@ def check_policy(logp, old_logp, advantages, ref_logp, mask, weight, clip_low, c
     if kl_coef and ref_logp is None:
         raise ValueError("kl_coef needs ref_logp")
     return matrices, _vector(advantages, "advantages", n, device), _vector(weight, "weight", n, device)
+
+
+def _refuse_out(out):
+    """TypeError / ValueError where `out` is not a tensor, or one whose history would not know of what is written."""
+    import torch
+    if not isinstance(out, torch.Tensor):
+        raise TypeError("out must be a torch tensor")
+    if out.requires_grad and _recorded():
+        raise ValueError("out requires a gradient: autograd does not see this call")
+    _refuse_tangents(out=out)
 
 
 class CatalogueOps:
@@ -225,6 +250,7 @@ class CatalogueOps:
         """`X` [n, k] (fp32 or bf16) as an MxFp4Matrix: per block of 32 columns the exponent floor(log2 max|v|) - 2 (at least -127)
         and elements rounded to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 times it, ties to the even code, at most 6."""
         import torch
+        _refuse_tangents(X=X)
         X, ld = _matrix(X, "X", (torch.float32, torch.bfloat16), None, None, self.device)
         n, k = X.shape
         if k < 1:
@@ -250,6 +276,7 @@ class CatalogueOps:
         """(output, row stride)"""
         if out is None:
             return like.new_empty(shape, dtype=dtype), shape[1]
+        _refuse_out(out)
         if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != self.device or (out.numel() and (
                 out.stride(1) != 1 and out.shape[1] > 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1])):
             raise ValueError(f"out must be {_name(dtype)} {list(shape)} on {self.device} with contiguous rows")
@@ -267,6 +294,9 @@ class CatalogueOps:
             raise ValueError(f"score_mxfp4: at most {MAX_FACTORS} factors, {MAX_ROWS} rows of X, 1 ... {MAX_CATALOGUE} rows of V")
         if X.device != self.device or V.device != self.device:
             raise ValueError(f"X and V must be on {self.device}")
+        _refuse_tangents(ubase=ubase, ibase=ibase)
+        if out is not None:
+            _refuse_out(out)
         dtype = torch.float32 if dtype is None and out is None else out.dtype if dtype is None else dtype
         if dtype not in (torch.float32, torch.bfloat16):
             raise TypeError("score_mxfp4 writes float32 or bfloat16")
@@ -312,6 +342,7 @@ class CatalogueOps:
             raise ValueError("want holds 'X', 'V' and 'ibase'")
         (X, ldx), (V, ldv), (ids, ld_ids), ibase = check_catalogue(X, V, ids, ibase, scale, self.device)
         n, m = ids.shape
+        _refuse_tangents(lse=lse, dlogp=dlogp)
         dlogp, ld_dlogp = _matrix(dlogp, "dlogp", (torch.float32,), m, n, self.device)
         if lse is None:
             raise TypeError("lse must be a torch tensor")

@@ -1,7 +1,11 @@
 """CPU tests of what the catalogue operators and the factor models refuse, before any library call."""
 import numpy as np
 import pytest
+import torch
+from torch.autograd import forward_ad
 
+from recommenders_amd import MxFp4Matrix
+from recommenders_amd import catalogue as C
 from recommenders_amd.models import BPR, MF, WMF
 
 
@@ -11,3 +15,74 @@ def test_models_without_factors(model):
         for call in (lambda: m.log_prob([0], [[0]]), lambda: m.fit_preferences([0], [[0]], [[1]]), lambda: m.fit_policy([0], [[0]], [1.0])):
             with pytest.raises(RuntimeError, match="has no factors: pass init_params"):
                 call()
+
+
+X, V, IDS = torch.zeros((4, 8)), torch.zeros((9, 8)), torch.zeros((4, 2), dtype=torch.int32)
+L, R = torch.zeros((4, 3)), torch.zeros((4, 5))
+
+
+def _dual(t):
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+def _ops():
+    ops = C.CatalogueOps()                       # every refusal here comes before the library is called
+    ops.device = torch.device("cpu")
+    return ops
+
+
+def _mx(n, k):
+    kb = (k + 31) // 32
+    return MxFp4Matrix(torch.zeros((n, 16 * kb), dtype=torch.uint8), torch.zeros((n, kb), dtype=torch.uint8), k)
+
+
+def _pref(**kw):
+    a = dict(chosen=L, rejected=R, ref_chosen=L, ref_rejected=R, mask_chosen=None, mask_rejected=None, weight=torch.ones(4), beta=0.1, kind="logistic",
+             label_smoothing=0.0, margin=0.0)
+    a.update(kw)
+    return C.check_preference(**a)
+
+
+def _pol(**kw):
+    a = dict(logp=L, old_logp=L, advantages=torch.zeros(4), ref_logp=L, mask=None, weight=torch.ones(4), clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="row")
+    a.update(kw)
+    return C.check_policy(**a)
+
+
+@pytest.mark.parametrize("name,call", [
+    ("X", lambda: C.check_catalogue(_dual(X), V, IDS, None, 1.0)),
+    ("V", lambda: C.check_catalogue(X, _dual(V), IDS, None, 1.0)),
+    ("ibase", lambda: C.check_catalogue(X, V, IDS, _dual(torch.zeros(9)), 1.0)),
+    ("ibase", lambda: C.check_catalogue(_mx(4, 8), _mx(9, 8), IDS, _dual(torch.zeros(9)), 1.0)),
+    ("lse", lambda: _ops().catalogue_logprob_backward(X, V, IDS, _dual(torch.zeros(4)), torch.zeros((4, 2)))),
+    ("dlogp", lambda: _ops().catalogue_logprob_backward(X, V, IDS, torch.zeros(4), _dual(torch.zeros((4, 2))))),
+    ("X", lambda: _ops().quantize_mxfp4(_dual(X))),
+    ("ubase", lambda: _ops().score_mxfp4(_mx(4, 8), _mx(9, 8), ubase=_dual(torch.zeros(4)))),
+    ("ibase", lambda: _ops().score_mxfp4(_mx(4, 8), _mx(9, 8), ibase=_dual(torch.zeros(9)))),
+    ("out", lambda: _ops().score_mxfp4(_mx(4, 8), _mx(9, 8), out=_dual(torch.zeros((4, 9))))),
+    ("out", lambda: _ops().dequantize_mxfp4(_mx(4, 8), out=_dual(torch.zeros((4, 8))))),
+    ("chosen", lambda: _pref(chosen=_dual(L))), ("rejected", lambda: _pref(rejected=_dual(R))), ("ref_chosen", lambda: _pref(ref_chosen=_dual(L))),
+    ("ref_rejected", lambda: _pref(ref_rejected=_dual(R))), ("weight", lambda: _pref(weight=_dual(torch.ones(4)))),
+    ("logp", lambda: _pol(logp=_dual(L))), ("old_logp", lambda: _pol(old_logp=_dual(L))), ("ref_logp", lambda: _pol(ref_logp=_dual(L))),
+    ("advantages", lambda: _pol(advantages=_dual(torch.ones(4)))), ("weight", lambda: _pol(weight=_dual(torch.ones(4)))),
+])
+def test_tangents_are_refused(name, call):
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match=f"^{name} carries a tangent"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match=f"^{name} carries a tangent"):
+            call()
+        C.check_catalogue(X, V, IDS, torch.zeros(9), 1.0), _pref(), _pol()         # an open level alone is no reason
+        C.check_catalogue(forward_ad.unpack_dual(_dual(X)).primal, V, IDS, None, 1.0)
+
+
+@pytest.mark.parametrize("call", [lambda out: _ops().score_mxfp4(_mx(4, 8), _mx(9, 8), out=out), lambda out: _ops().dequantize_mxfp4(_mx(4, 9), out=out)])
+def test_outputs_are_checked(call):
+    for out in (np.zeros((4, 9), np.float32), [0.0], 1.0):
+        with pytest.raises(TypeError, match="out must be a torch tensor"):
+            call(out)
+    with pytest.raises(ValueError, match="out requires a gradient"):
+        call(torch.zeros((4, 9), requires_grad=True))
+    for out in (torch.zeros((4, 8)), torch.zeros((9, 4)).t(), torch.zeros((4, 1)).expand(4, 9)):
+        with pytest.raises(ValueError, match="out must be float32"):
+            call(out)
