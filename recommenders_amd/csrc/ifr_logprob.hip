@@ -830,12 +830,13 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             Operand o;
             o.back = 1.f;
             if (NS == 2) {
-                // times the T rows' powers of two (their parts are scaled by the inverse); then the S row's 32 elements (16 here, 16 in
+                // times the T rows' powers of two, 2^-e (their parts are scaled by the inverse; G brings the 2^24 that they leave out); then the S row's 32 elements (16 here, 16 in
                 // lane + or - 32) by the power of two that brings the largest to [2^14, 2^15)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
+                    constexpr float REST = ITEMS ? 1.f : 16777216.f;
                     const float4 u4 = *(const float4 *)(terms + 2 * ROWS + sub * 32 + 8 * q + 4 * h);
-                    P[4 * q] *= u4.x; P[4 * q + 1] *= u4.y; P[4 * q + 2] *= u4.z; P[4 * q + 3] *= u4.w;
+                    P[4 * q] *= u4.x * REST; P[4 * q + 1] *= u4.y * REST; P[4 * q + 2] *= u4.z * REST; P[4 * q + 3] *= u4.w * REST;
                 }
                 float top = fabsf(P[0]);
 #pragma unroll
@@ -926,14 +927,13 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         if (h == 0) { p.out_m[at] = top; p.out_s[at] = sum; }
         return;
     }
-    // split: G, and with it the sum for db, is 2^24 times itself, and the T rows' powers of two are 2^-24 of themselves
+    // split: G, and with it the sum for db, is 2^24 times itself
     b_sum = (b_sum + __shfl_xor(b_sum, 32)) * (NS == 2 ? 1.f / 16777216.f : 1.f);
     if (MODE == WALK_USERS) {
-        constexpr float UNIT = NS == 2 ? 16777216.f : 1.f;
         for (int kb = 0; kb < KP / 32; ++kb)
             for (int q = 0; q < 4; ++q)
                 *(float4 *)(p.out_acc + at * KP + kb * 32 + 8 * q + 4 * h) =
-                    make_float4(acc[kb][4 * q] * UNIT, acc[kb][4 * q + 1] * UNIT, acc[kb][4 * q + 2] * UNIT, acc[kb][4 * q + 3] * UNIT);
+                    make_float4(acc[kb][4 * q], acc[kb][4 * q + 1], acc[kb][4 * q + 2], acc[kb][4 * q + 3]);
         return;
     }
     // dV: the places of the users walked are added here, to 64 rows a time (waves 0 and 1, then 2 and 3) whose sums lie in the first stage's

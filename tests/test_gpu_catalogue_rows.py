@@ -184,3 +184,17 @@ def test_large_rows_leave_their_neighbours_alone(torch, sc, n, items, k, large):
     assert _within(dV, r.dV, r.t_dV)[clear].all() and _within(db, r.db, r.t_db)[clear].all()
 
 
+@pytest.mark.parametrize("n,items,k", [(90, 300, 50), (40, 200, 200)])
+@pytest.mark.parametrize("spread", [1e-32, 1e-28, 1e-24, 1e28, 1e30])
+def test_magnitudes_far_from_one(torch, sc, n, items, k, spread):
+    """fp32 items far from 1 and users as far on the other side: ordinary scores, and every row with the precision of one near 1."""
+    g = _gen(torch, n)
+    X, V = torch.randn((n, k), generator=g, device="cuda") * 0.3 / spread, torch.randn((items, k), generator=g, device="cuda") * 0.3 * spread
+    ids = torch.randint(0, items, (n, 3), generator=g, device="cuda", dtype=torch.int32)
+    dlogp = torch.randn((n, 3), generator=g, device="cuda")
+    r = Exact(torch, X, V, None, ids, dlogp, 1.0, 3 * 2.0 ** -22, 2.0 ** -21)
+    logp, lse = sc.catalogue_logprob(X, V, ids)
+    assert _within(lse, r.lse, r.e_lse).all() and _within(logp, r.logp, r.e_logp).all()
+    dX, dV, _ = sc.catalogue_logprob_backward(X, V, ids, lse, dlogp)
+    assert _within(dX, r.dX, r.t_dX).all() and _within(dV, r.dV, r.t_dV).all()
+    assert float((r.t_dX.norm(dim=1) / r.dX.norm(dim=1)).median()) < 0.02 and float((r.t_dV.norm(dim=1) / r.dV.norm(dim=1)).median()) < 0.02
