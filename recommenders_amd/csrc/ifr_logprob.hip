@@ -777,7 +777,11 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
                 d0 = product<NS>(l1[PART + s * 64 + at1[s & 1]], sf[0][s], d0);
             }
         }
-        if (TWO) d += other;
+        if (TWO) {
+            d += other;
+            // the scaling stays behind the products: moved between them it took 512 registers and spilled (224 columns: sums of dX 204 us, so 182)
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (NS == 2) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
