@@ -70,3 +70,23 @@ def test_logprob_of_4bit_rows_whose_scales_cancel(torch, sc, up, down):
     e_lse = score + 6 * U * (float(z.abs().max()) + float(want.abs().max()) + 8) + 2.0 ** -21 + 99 * U
     assert float((lse.double() - want).abs().max()) <= e_lse
     assert float((logp.double() - (z.gather(1, ids.long()) - want[:, None])).abs().max()) <= score + 2 * e_lse
+
+
+@pytest.mark.parametrize("n,items", [(513, 32800), (700, 24001), (1030, 16404)])
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("k", [33, 200])
+def test_scores_of_a_large_batch(torch, sc, n, items, out, k):
+    """Enough tiles of 32 x 32 for the form that keeps 128 or 256 items a wave; rows at 16-byte borders and others, widths that end inside a tile."""
+    g = _gen(torch, n + k)
+    X, V = torch.randn((n, k), generator=g, device="cuda"), torch.randn((items, k), generator=g, device="cuda") * 0.1
+    ib, ub = torch.randn(items, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+    xq, vq = sc.quantize_mxfp4(X), sc.quantize_mxfp4(V)
+    x, v = sc.dequantize_mxfp4(xq).double(), sc.dequantize_mxfp4(vq).double()
+    ref = x @ v.t() + ib.double() + ub.double()[:, None]
+    # k products (exact) and two bases: at most k + 2 additions in fp32, then one rounding to the output's type
+    tol = (k + 2) * U * (x.abs() @ v.abs().t() + ib.double().abs() + ub.double().abs()[:, None]) + (B * (1 + 1e-3) * ref.abs() if out == "bfloat16" else 0) + 1e-30
+    s = sc.score_mxfp4(xq, vq, ubase=ub, ibase=ib, dtype=getattr(torch, out))
+    assert ((s.double() - ref).abs() <= tol).all()
+    wide = torch.full((n, items + 5), 5.0, dtype=s.dtype, device="cuda")
+    sc.score_mxfp4(xq, vq, ubase=ub, ibase=ib, out=wide[:, :items])
+    assert torch.equal(wide[:, :items], s) and (wide[:, items:] == 5).all()
