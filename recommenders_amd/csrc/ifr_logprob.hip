@@ -137,7 +137,7 @@ __device__ __forceinline__ void store_fragments(const float *tile, int W, int KP
 
 // Everything the walks read, a workgroup a tile of 32 rows of V (or 256 of its terms, where it needs no other order) or X.  One read, one
 // write, through LDS since a piece is eight columns of one row; short, so bound by the latency of its loads (eight under way a thread).
-// fp32 2048 + 26 744 rows of 200: 14 us (23 MB in, 26 MB out).
+// fp32 2048 + 26 744 rows of 200: 16 us (23 MB in, 26 MB out).
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void prepare_kernel(PrepParams p)
 {
@@ -670,14 +670,16 @@ constexpr bool paired(int KP, int NS, int mode) { return KP * NS <= 256 && (mode
 // S_LIES, T_LIES: read as bf16 rows in memory (V; X too for the statistics)
 //
 // Bound by the matrix instructions together with what does not fit beside them: 16 exponentials a lane and tile (a quarter of the rate of
-// the rest), the conversion of P to 16 bits, and the clock under their load (bf16 2048 x 1 000 000 x 128, sums of dX: 942 us, the
-// same instructions on rows of zeros 745 us).  A tile is 32 rows as the 32 x 32 instructions have it: 16 x 16 ones would read LDS twice as
+// the rest), the conversion of P to two parts of 16 bits, with fp32 operands the scaling of P and of each tile's product (600 vector
+// instructions a wave and tile of 224 columns beside 84 matrix ones), and the clock under their load (bf16 2048 x 1 000 000 x 128, sums of
+// dX: 1350 us, the same instructions on rows of zeros 1010 us).  A tile is 32 rows as the 32 x 32 instructions have it: 16 x 16 ones would read LDS twice as
 // often for the same products.  128 S rows a workgroup: their operand (KP / 16 registers of 4 a part) and the sums of 32 x KP a wave
 // fill the registers, so that a compute unit holds two workgroups up to 256 columns in all parts and one beyond; LDS serves four waves
 // with one stage.  Sizes and what they measured (matrix unit busy, of the SIMDs' cycles):
-//   bf16 2048 x 1 000 000 x 128: lse 0.70 ms (45 %), sums of dX 1.02 ms (62 %), dV finished 1.37 ms (44 %), all under the profiler
-//   fp32 2048 x 26 744 x 200: lse 73 us (62 %), sums of dX 170 us (47 %), dV and db finished 259 us (38 %)
-// = 2.6 PFLOP with the recomputed scores in 2.6 - 2.8 ms for the bf16 step, where a large product of the library reaches 1206 TFLOP/s.
+//   bf16 2048 x 1 000 000 x 128: lse 0.66 ms (45 %), sums of dX 1.38 ms (66 %), dV finished 1.66 ms (52 %), all under the profiler
+//   fp32 2048 x 26 744 x 200: lse 71 us (62 %), sums of dX 185 us (42 %), dV and db finished 289 us (34 %)
+// = 3.7 PFLOP with the recomputed scores and both parts of P in 3.3 - 3.5 ms for the bf16 step, where a large product of the library
+// reaches 1206 TFLOP/s.  (P in one part took 2.6 ms, and lost the gradient of users who are sure of their item.)
 template <int KP, int NS, int MODE, bool S_LIES, bool T_LIES>
 __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel(WalkParams p)
 {
@@ -806,7 +808,7 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
         }
         // probabilities of a tile (times G for the items' side), as the operand of the second product: two parts in either type, since a
         // gradient is the difference of this product and the named items' rows, and only what P keeps is left of a user who is nearly
-        // sure of its item.  bf16: hi + lo is off by at most 2^-16 of P, and near 1 by 2^-8 of 1 - P (one part lost such rows whole)
+        // sure of its item.  bf16: hi + lo is off by at most 2^-16 of P, and near 1 by 2^-8 of 1 - P (one part lost such rows whole).
         // fp32: 22 bits, or an absolute step of 2^-39 of the largest of a S row's 32 elements.  That power of two is the tile's and the row's
         // own, taken off where the tile's product is added to the sums in fp32, so that neither an unlikely item nor one beside a user of
         // large G loses bits
@@ -834,8 +836,8 @@ __global__ __launch_bounds__(256, paired(KP, NS, MODE) ? 2 : 1) void walk_kernel
             Operand o;
             o.back = 1.f;
             if (NS == 2) {
-                // times the T rows' powers of two, 2^-e (their parts are scaled by the inverse; G brings the 2^24 that they leave out); then the S row's 32 elements (16 here, 16 in
-                // lane + or - 32) by the power of two that brings the largest to [2^14, 2^15)
+                // times the T rows' powers of two, 2^-e (their parts are scaled by the inverse; G brings the 2^24 that they leave out); then
+                // the S row's 32 elements (16 here, 16 in lane + or - 32) by the power of two that brings the largest to [2^14, 2^15)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     constexpr float REST = ITEMS ? 1.f : 16777216.f;
@@ -1513,7 +1515,7 @@ struct ForwardPlan {
 };
 
 // The direct kernel is taken for what one pass over V serves.  Beyond, the walk is as fast where V needs no other order (bf16 1 000 000 x
-// 128, 70 users: 64 us) and faster where it does (fp32, 70 users: 415 us by the walk, 458 us in two passes).
+// 128, 70 users: 66 us, 113 us in two passes) and faster where it does (fp32, 70 users: 374 us by the walk, 460 us in two passes).
 int64_t direct_users(const ifr_catalogue &c) { return 16 * (pad_factors(c.k) > 128 ? 2 : 4); }
 
 ForwardPlan forward_plan(Pieces &w, const ifr_catalogue &c, bool lies)
@@ -1562,7 +1564,7 @@ struct BackwardPlan {
 };
 
 // Places are dealt into buckets where the workgroups' looking through all of them takes longer than the dealing: with 524 288 places and
-// 100 000 items dV takes 743 us dealt and 1056 us as they are, with 40 960 and 26 744 items 272 and 264 us.
+// 100 000 items dV takes 838 us dealt and 1164 us as they are, with 81 920 and 26 744 items 333 and 335 us.
 bool deals(const ifr_catalogue &c, int64_t m, bool items) { return items && c.n * m >= DEAL_FROM && c.n * m < (int64_t)1 << 31 && c.n_items >= 16 * S_ROWS; }
 
 BackwardPlan backward_plan(Pieces &w, const ifr_catalogue &c, int64_t m, bool dx, bool dv, bool db, bool lies)
